@@ -65,6 +65,25 @@ class StepArgs(C.Structure):
                 ("emb_update", C.c_uint32), ("emb_lr", C.c_float), ("sample_seed", C.c_uint64)]
 
 
+class EmbedArgs(C.Structure):
+    """`aideen_embed_args`."""
+    _fields_ = [("dtype", C.c_uint32), ("n_tokens", C.c_uint32), ("dim", C.c_uint32), ("vocab", C.c_uint32),
+                ("scale", C.c_float), ("accumulate", C.c_uint32), ("table_ld", C.c_int64), ("rows_ld", C.c_int64)]
+
+
+class LayerNormArgs(C.Structure):
+    """`aideen_layer_norm_args`."""
+    _fields_ = [("dtype", C.c_uint32), ("rows", C.c_uint32), ("dim", C.c_uint32), ("eps", C.c_float),
+                ("x_ld", C.c_int64), ("y_ld", C.c_int64), ("dx_ld", C.c_int64)]
+
+
+class LinearCeArgs(C.Structure):
+    """`aideen_linear_ce_args`."""
+    _fields_ = [("dtype", C.c_uint32), ("rows", C.c_uint32), ("dim", C.c_uint32), ("vocab", C.c_uint32),
+                ("reduction", C.c_uint32), ("x_ld", C.c_int64), ("w_ld", C.c_int64), ("dx_ld", C.c_int64),
+                ("dw_ld", C.c_int64)]
+
+
 _LIB = None
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libaideen_b200.so")
 
@@ -108,6 +127,18 @@ _SIGS = {
     "aideen_device_ptr": (_P, [_P, C.c_int]),
     "aideen_adjoint_noalloc": (C.c_int, [_P, _P, _P, _P, _P, C.c_uint32, C.c_uint32, C.c_uint32,
                                          C.c_uint32, C.c_float, C.c_uint32, _P, _P, _P, _P]),
+    "aideen_operator_error": (C.c_char_p, []),
+    "aideen_operator_check": (C.c_int, [_P]),
+    "aideen_embed": (C.c_int, [C.POINTER(EmbedArgs), _P, _P, _P, _P]),
+    "aideen_embed_grad_workspace": (C.c_int, [C.POINTER(EmbedArgs), C.POINTER(C.c_size_t)]),
+    "aideen_embed_grad": (C.c_int, [C.POINTER(EmbedArgs), _P, _P, _P, _P, C.c_size_t, _P]),
+    "aideen_layer_norm": (C.c_int, [C.POINTER(LayerNormArgs), _P, _P, _P, _P, _P, _P, _P]),
+    "aideen_layer_norm_grad_workspace": (C.c_int, [C.POINTER(LayerNormArgs), C.POINTER(C.c_size_t)]),
+    "aideen_layer_norm_grad": (C.c_int, [C.POINTER(LayerNormArgs), _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
+    "aideen_linear_ce_workspace": (C.c_int, [C.POINTER(LinearCeArgs), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
+    "aideen_linear_ce": (C.c_int, [C.POINTER(LinearCeArgs), _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
+    "aideen_linear_ce_grad": (C.c_int, [C.POINTER(LinearCeArgs), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t,
+                                        _P]),
     "aideen_gemm_selftest": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                        C.POINTER(C.c_float), C.POINTER(C.c_float), C.POINTER(C.c_float)]),
     "aideen_comm_unique_id": (C.c_int, [_P]),

@@ -1,0 +1,259 @@
+"""Operators on the caller's CUDA tensors: embedding lookup, layer
+normalisation and the cross entropy of a linear head, each with its gradient.
+
+They stand beside `GpuDeqBackend` (which owns the DEQ block's buffers) for the
+token side of a model whose tensors the caller holds: torch tensors in float32,
+bfloat16 or float16.  Every call goes through `libaideen_b200.so`
+(include/aideen_b200.h has the formulas and the rules on ids and targets);
+there is no CPU fallback.  Work is queued on torch's current stream of the
+tensors' device, outputs and scratch memory come from torch's allocator, and
+nothing waits, so every call can be captured into a CUDA graph.  Arguments that
+cannot be served raise `AideenError` before anything is launched.
+
+A matrix may have any row stride as long as its last dimension is contiguous
+and its leading dimensions share one stride; 16-byte aligned rows are fastest.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from .backend import AideenError, EmbedArgs, LayerNormArgs, LinearCeArgs, load_library
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_REDUCTIONS = {"mean": 0, "sum": 1}
+
+
+def _check(rc: int, what: str):
+    if rc != 0:
+        raise AideenError(f"{what}: status {rc}: {load_library().aideen_operator_error().decode()}")
+
+
+def _tensor(t, what: str, name: str, like=None, dtype=None):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise AideenError(f"{what}: {name} must be a CUDA tensor")
+    if dtype is not None:
+        if t.dtype != dtype:
+            raise AideenError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+    elif t.dtype not in _DTYPES:
+        raise AideenError(f"{what}: {name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if like is not None and t.device != like.device:
+        raise AideenError(f"{what}: {name} is on {t.device}, not on {like.device}")
+    return t
+
+
+def _rows(t, what: str, name: str):
+    """(rows, dim, row stride) of a matrix with any number of leading dimensions."""
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise AideenError(f"{what}: {name} needs a last dimension of at least 1")
+    dim = t.shape[-1]
+    if t.dim() == 1:
+        return 1, dim, dim
+    if t.dim() > 2:
+        try:
+            t = t.view(-1, dim)
+        except RuntimeError:
+            raise AideenError(f"{what}: {name}'s leading dimensions have no common row stride") from None
+    n = t.shape[0]
+    if dim > 1 and t.stride(1) != 1:
+        raise AideenError(f"{what}: {name}'s last dimension is not contiguous")
+    ld = t.stride(0) if n > 1 else dim
+    if ld < dim:
+        raise AideenError(f"{what}: {name}'s rows overlap")
+    return n, dim, ld
+
+
+def _vector(t, what: str, name: str, n: int, like, dtype=None):
+    if t is None:
+        return None
+    _tensor(t, what, name, like, dtype or like.dtype)
+    if t.numel() != n or not t.is_contiguous():
+        raise AideenError(f"{what}: {name} must be contiguous with {n} elements")
+    return t.data_ptr()
+
+
+def _out(t, what: str, name: str, shape, like):
+    """A given output, checked, or a new one."""
+    if t is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    _tensor(t, what, name, like, like.dtype)
+    if tuple(t.shape) != tuple(shape):
+        raise AideenError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def _launch(device, what: str, fn, *args):
+    """One call on torch's current stream of `device`, with that device current."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc != 0:
+        _check(rc, what)
+
+
+def _scratch(nbytes: int, device):
+    # torch's blocks start on 512 bytes; the library asks for 256
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def check(device=None):
+    """Wait for torch's current stream and raise if a bounded wait of an
+    operator ran out on the device since the last check."""
+    with torch.cuda.device(device):
+        _check(load_library().aideen_operator_check(torch.cuda.current_stream().cuda_stream), "check")
+
+
+# ---- embedding -------------------------------------------------------------
+def _ids(ids, what: str, like, name: str = "ids"):
+    _tensor(ids, what, name, like, torch.int32)
+    if not ids.is_contiguous():
+        raise AideenError(f"{what}: {name} must be contiguous")
+    return ids.data_ptr()
+
+
+def embed(ids, table, scale: float = 1.0, out=None):
+    """`scale * table[ids]` (ids int32, any shape; table [vocab, dim]); an id
+    outside [0, vocab) gives a row of zeros."""
+    what = "embed"
+    _tensor(table, what, "table")
+    if table.dim() != 2:
+        raise AideenError(f"{what}: table must be [vocab, dim]")
+    vocab, dim, ld = _rows(table, what, "table")
+    ip = _ids(ids, what, table)
+    out = _out(out, what, "out", (*ids.shape, dim), table)
+    n = ids.numel()
+    old = _rows(out, what, "out")[2] if n else dim
+    a = EmbedArgs(_DTYPES[table.dtype], n, dim, vocab, scale, 0, ld, old)
+    _launch(table.device, what, load_library().aideen_embed, C.byref(a), ip, table.data_ptr(), out.data_ptr())
+    return out
+
+
+def embed_grad(ids, dout, vocab: int, scale: float = 1.0, into=None):
+    """Gradient of `embed` by its table: [vocab, dim], or added to `into` (only
+    rows that occur in `ids` are touched then) and `into` returned."""
+    what = "embed_grad"
+    _tensor(dout, what, "dout")
+    ip = _ids(ids, what, dout)
+    if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape:
+        raise AideenError(f"{what}: dout must have ids' shape and one more dimension")
+    dim, n = dout.shape[-1], ids.numel()
+    rld = _rows(dout, what, "dout")[2] if n else dim
+    grad = _out(into, what, "into", (vocab, dim), dout)
+    gld = _rows(grad, what, "into")[2]
+    a = EmbedArgs(_DTYPES[dout.dtype], n, dim, vocab, scale, int(into is not None), gld, rld)
+    lib, size = load_library(), C.c_size_t()
+    _check(lib.aideen_embed_grad_workspace(C.byref(a), C.byref(size)), what)
+    ws = _scratch(size.value, dout.device)
+    _launch(dout.device, what, lib.aideen_embed_grad, C.byref(a), ip, dout.data_ptr(), grad.data_ptr(), ws.data_ptr(),
+            size.value)
+    return grad
+
+
+# ---- layer normalisation ----------------------------------------------------
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
+    """(y, mean, rstd): each row of x (its last dimension) normalised; mean and
+    rstd are float32 with x's leading shape, for `layer_norm_grad`."""
+    what = "layer_norm"
+    _tensor(x, what, "x")
+    n, dim, xld = _rows(x, what, "x")
+    wp, bp = _vector(weight, what, "weight", dim, x), _vector(bias, what, "bias", dim, x)
+    y = _out(out, what, "out", x.shape, x)
+    yld = _rows(y, what, "out")[2]
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    a = LayerNormArgs(_DTYPES[x.dtype], n, dim, eps, xld, yld, 0)
+    _launch(x.device, what, load_library().aideen_layer_norm, C.byref(a), x.data_ptr(), wp, bp, y.data_ptr(),
+            mean.data_ptr(), rstd.data_ptr())
+    return y, mean, rstd
+
+
+def layer_norm_grad(dy, x, weight, mean, rstd, want=("x", "weight", "bias")):
+    """(dx, dweight, dbias) from the forward's x, mean and rstd; weight may be
+    None (1).  `want` names the gradients to form; the others are None."""
+    what = "layer_norm_grad"
+    _tensor(x, what, "x")
+    _tensor(dy, what, "dy", x, x.dtype)
+    if dy.shape != x.shape:
+        raise AideenError(f"{what}: dy and x differ in shape")
+    n, dim, xld = _rows(x, what, "x")
+    yld = _rows(dy, what, "dy")[2]
+    wp = _vector(weight, what, "weight", dim, x)
+    mp = _vector(mean, what, "mean", n, x, torch.float32)
+    rp = _vector(rstd, what, "rstd", n, x, torch.float32)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if "x" in want else None
+    dw = torch.empty(dim, dtype=x.dtype, device=x.device) if "weight" in want else None
+    db = torch.empty(dim, dtype=x.dtype, device=x.device) if "bias" in want else None
+    a = LayerNormArgs(_DTYPES[x.dtype], n, dim, 0.0, xld, yld, dim)
+    lib, size, ws = load_library(), C.c_size_t(), None
+    if dw is not None or db is not None:
+        with torch.cuda.device(x.device):  # the size depends on the device's SM count
+            _check(lib.aideen_layer_norm_grad_workspace(C.byref(a), C.byref(size)), what)
+        ws = _scratch(size.value, x.device)
+    _launch(x.device, what, lib.aideen_layer_norm_grad, C.byref(a), dy.data_ptr(), x.data_ptr(), wp, mp, rp,
+            None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+            None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), size.value)
+    return dx, dw, db
+
+
+# ---- cross entropy of a linear head -----------------------------------------
+def _ce_args(what, x, weight, targets, bias, reduction):
+    _tensor(x, what, "x")
+    _tensor(weight, what, "weight", x, x.dtype)
+    if reduction not in _REDUCTIONS:
+        raise AideenError(f"{what}: reduction must be 'mean' or 'sum'")
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise AideenError(f"{what}: weight must be [vocab, {x.shape[-1]}]")
+    tp = _ids(targets, what, x, "targets")
+    if targets.shape != x.shape[:-1]:
+        raise AideenError(f"{what}: targets must have x's leading shape")
+    n, dim, xld = _rows(x, what, "x")
+    if n == 0:
+        xld = dim
+    vocab, _, wld = _rows(weight, what, "weight")
+    bp = _vector(bias, what, "bias", vocab, x)
+    return LinearCeArgs(_DTYPES[x.dtype], n, dim, vocab, _REDUCTIONS[reduction], xld, wld, dim, dim), tp, bp
+
+
+def linear_ce(x, weight, targets, bias=None, reduction: str = "mean"):
+    """(loss [1], row_loss, lse) of the cross entropy of `x @ weight.T + bias`
+    against int32 targets; the logits are not kept.  Rows whose target lies
+    outside [0, vocab) are not counted (row_loss and lse 0)."""
+    what = "linear_ce"
+    a, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)
+    lib, size = load_library(), C.c_size_t()
+    with torch.cuda.device(x.device):
+        _check(lib.aideen_linear_ce_workspace(C.byref(a), C.byref(size), None), what)
+    loss = torch.empty(1, dtype=torch.float32, device=x.device)
+    row_loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    lse = torch.empty_like(row_loss)
+    ws = _scratch(size.value, x.device)
+    _launch(x.device, what, lib.aideen_linear_ce, C.byref(a), x.data_ptr(), weight.data_ptr(), bp, tp,
+            loss.data_ptr(), row_loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size.value)
+    return loss, row_loss, lse
+
+
+def linear_ce_grad(x, weight, targets, lse, bias=None, dloss=None, reduction: str = "mean",
+                   want=("x", "weight", "bias")):
+    """(dx, dweight, dbias) of `dloss * loss` from `linear_ce`'s lse (same bias
+    and reduction); dloss is a float32 tensor of one element or None (1).
+    `want` names the gradients to form; the others, and dbias without a bias,
+    are None."""
+    what = "linear_ce_grad"
+    a, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)
+    lp = _vector(lse, what, "lse", a.rows, x, torch.float32)
+    gp = _vector(dloss, what, "dloss", 1, x, torch.float32)
+    lib, size = load_library(), C.c_size_t()
+    with torch.cuda.device(x.device):
+        _check(lib.aideen_linear_ce_workspace(C.byref(a), None, C.byref(size)), what)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if "x" in want else None
+    dw = torch.empty((a.vocab, a.dim), dtype=x.dtype, device=x.device) if "weight" in want else None
+    db = torch.empty(a.vocab, dtype=x.dtype, device=x.device) if "bias" in want and bias is not None else None
+    ws = _scratch(size.value, x.device)
+    _launch(x.device, what, lib.aideen_linear_ce_grad, C.byref(a), x.data_ptr(), weight.data_ptr(), bp, tp, lp, gp,
+            None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+            None if db is None else db.data_ptr(), ws.data_ptr(), size.value)
+    return dx, dw, db

@@ -324,6 +324,119 @@ int aideen_adjoint_noalloc(const float *hstar, const float *branch, const float 
                            uint32_t anderson_m, float *v_out, float *gpre_out, float *ns_grad_out,
                            void *stream);
 
+/* ---- operators on caller-owned device tensors (no counterpart in the reference) --
+ * The token side of a language model around the DEQ block, for callers that
+ * hold their own tensors: embedding lookup, layer normalisation and the
+ * cross entropy of a linear head, each with its gradient.  Like
+ * aideen_adjoint_noalloc they need no context and allocate nothing:
+ *
+ *   - every tensor pointer is a device pointer on the current device, aligned to
+ *     its element type; matrices are row-major with the given row stride (`_ld`,
+ *     in elements, at least the row's length; rows must not overlap).  Outputs
+ *     must not overlap inputs or each other.
+ *   - scratch memory is the caller's: a *_workspace function gives its size for
+ *     the same arguments, the pointer is 256-byte aligned, and its contents
+ *     need no initialisation and mean nothing between calls.  Calls that overlap
+ *     on the GPU (other streams, graphs replayed side by side) need one each.
+ *   - work is queued on `stream` (a cudaStream_t) and not waited for; every call
+ *     may be captured into a CUDA graph.
+ *   - arguments are checked before anything is launched: AIDEEN_E_INVALID, and
+ *     aideen_operator_error() says why.  The *_workspace functions make the
+ *     checks that need no pointers and touch no GPU.
+ *   - results do not depend on timing: the same call gives the same bits.
+ *
+ * dtype is the type of every tensor but ids, targets, statistics and losses
+ * (int32 and float32).  Sums, statistics and products are accumulated in
+ * float32 and rounded to dtype once, where a result is stored, except where
+ * aideen_linear_ce_grad says otherwise. */
+enum { AIDEEN_F32 = 0, AIDEEN_BF16 = 1, AIDEEN_F16 = 2 };
+
+/* Reason of the calling thread's last AIDEEN_E_INVALID / AIDEEN_E_CUDA from an
+ * operator ("" if none). */
+const char *aideen_operator_error(void);
+/* Wait for `stream`, then report whether a bounded device-side wait of an
+ * operator ran out on the current device since the last check
+ * (AIDEEN_E_TIMEOUT: outputs since then are invalid).  Not during capture. */
+int aideen_operator_check(void *stream);
+
+/* Embedding lookup: out[n] = scale * table[ids[n]]; an id outside [0, vocab)
+ * gives a row of zeros. */
+typedef struct aideen_embed_args {
+  uint32_t dtype;
+  uint32_t n_tokens;     /* 0 is allowed */
+  uint32_t dim;          /* >= 1 */
+  uint32_t vocab;        /* >= 1 */
+  float scale;
+  uint32_t accumulate;   /* gradient only: 1 = add to table_grad, 0 = write all of it */
+  int64_t table_ld;      /* row stride of table / table_grad [vocab][dim] */
+  int64_t rows_ld;       /* row stride of out / dout [n_tokens][dim] */
+} aideen_embed_args;
+int aideen_embed(const aideen_embed_args *args, const int32_t *ids, const void *table, void *out,
+                 void *stream);
+/* Its gradient: table_grad[v] (+)= scale * sum of dout[n] over the tokens n
+ * with ids[n] == v, ids outside [0, vocab) left out.  The tokens are sorted by
+ * id (stably), so each row is one float32 sum in a fixed order.  With
+ * accumulate = 1 only rows that occur are read and written (a head that shares
+ * the table adds its gradient this way); else every row is written, zeros where
+ * an id does not occur. */
+int aideen_embed_grad_workspace(const aideen_embed_args *args, size_t *bytes);
+int aideen_embed_grad(const aideen_embed_args *args, const int32_t *ids, const void *dout,
+                      void *table_grad, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Layer normalisation of each row: y = (x - mean) * rstd * weight + bias with
+ * rstd = 1 / sqrt(var + eps).  weight, bias [dim] may be NULL (1 and 0); mean
+ * and rstd [rows] may be NULL when the gradient is not needed. */
+typedef struct aideen_layer_norm_args {
+  uint32_t dtype;
+  uint32_t rows;         /* 0 is allowed */
+  uint32_t dim;          /* >= 1 */
+  float eps;             /* >= 0 */
+  int64_t x_ld;          /* row stride of x */
+  int64_t y_ld;          /* row stride of y, and of dy in the gradient */
+  int64_t dx_ld;         /* row stride of dx (gradient only) */
+} aideen_layer_norm_args;
+int aideen_layer_norm(const aideen_layer_norm_args *args, const void *x, const void *weight,
+                      const void *bias, void *y, float *mean, float *rstd, void *stream);
+/* Its gradient from the forward's x, mean and rstd.  dx, dweight and dbias may
+ * be NULL where they are not wanted (not all three). */
+int aideen_layer_norm_grad_workspace(const aideen_layer_norm_args *args, size_t *bytes);
+int aideen_layer_norm_grad(const aideen_layer_norm_args *args, const void *dy, const void *x,
+                           const void *weight, const float *mean, const float *rstd, void *dx,
+                           void *dweight, void *dbias, void *workspace, size_t workspace_bytes,
+                           void *stream);
+
+/* Softmax cross entropy of a linear head, without keeping the logits
+ * z = x W^T + bias:  lse[n] = log sum_v exp z[n][v],  row_loss[n] = lse[n] -
+ * z[n][targets[n]],  loss = sum of row_loss / (counted rows, at least 1), or the
+ * plain sum.  A row whose target is outside [0, vocab) is not counted: its
+ * row_loss and lse are 0, and what its x holds reaches no result. */
+enum { AIDEEN_CE_MEAN = 0, AIDEEN_CE_SUM = 1 };
+typedef struct aideen_linear_ce_args {
+  uint32_t dtype;
+  uint32_t rows;         /* 0 is allowed */
+  uint32_t dim;          /* >= 1 */
+  uint32_t vocab;        /* >= 1 */
+  uint32_t reduction;    /* AIDEEN_CE_* */
+  int64_t x_ld, w_ld;    /* row strides of x [rows][dim] and W [vocab][dim] */
+  int64_t dx_ld, dw_ld;  /* row strides of dx and dW (gradient only) */
+} aideen_linear_ce_args;
+/* Workspace of the loss and of the gradient (either pointer may be NULL). */
+int aideen_linear_ce_workspace(const aideen_linear_ce_args *args, size_t *loss_bytes, size_t *grad_bytes);
+/* bias [vocab], loss [1], row_loss [rows] and lse [rows] may be NULL (not all of
+ * the last three). */
+int aideen_linear_ce(const aideen_linear_ce_args *args, const void *x, const void *w, const void *bias,
+                     const int32_t *targets, float *loss, float *row_loss, float *lse, void *workspace,
+                     size_t workspace_bytes, void *stream);
+/* Gradient of dloss * loss (dloss: a device float, NULL = 1) from the loss
+ * call's lse; the same bias.  The logits are formed again in pieces of the
+ * vocabulary.  dx, dw and dbias may be NULL where they are not wanted (not all
+ * three).  dx rows that are not counted are zero.  In 16 bits, softmax - onehot
+ * is rounded to dtype before its two products (its relative error there is that
+ * of one rounding); dx, dW and dbias are rounded once more when stored. */
+int aideen_linear_ce_grad(const aideen_linear_ce_args *args, const void *x, const void *w, const void *bias,
+                          const int32_t *targets, const float *lse, const float *dloss, void *dx, void *dw,
+                          void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- diagnostics (no counterpart in the reference) --------------------------
  * Runs a tcgen05 3xTF32 GEMM and the CUDA-core fp32 GEMM on the same seeded
  * device operands (C = op(A) op(B), row-major, `batch` independent problems)

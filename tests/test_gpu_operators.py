@@ -1,0 +1,531 @@
+"""Operators on caller-owned tensors against plain float64 formulas, at the sizes
+and masks where they can go wrong.
+
+Tolerances are worst-case rounding bounds, element by element, written from the
+operation counts: U32 = 2^-24 is half a step of float32, U[t] of the stored
+type, TINY[t] half of the smallest number it can hold, and a float32 sum of k
+terms is off by at most k U32 sum |terms| (2 k U32 where the tensor cores add,
+which may cut instead of round)."""
+import pytest
+import torch
+
+from aideen_b200 import operators as K
+from aideen_b200.backend import AideenError
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+U32 = 2.0 ** -24
+U = {t: torch.finfo(t).eps / 2 for t in TYPES}
+TINY = {F32: 2.0 ** -149, BF16: 2.0 ** -134, F16: 2.0 ** -25}
+
+
+def rand(gen, *shape, dtype=F32, std=1.0, mean=0.0):
+    return (torch.randn(*shape, generator=gen, device="cuda") * std + mean).to(dtype)
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def close(got, want, bound):
+    """|got - want| <= bound everywhere (float64)."""
+    assert got.shape == want.shape
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound.clamp(min=1e-300)).max())
+
+
+def strided(t, pad):
+    """The same values with a row stride of `pad` more elements."""
+    if pad == 0:
+        return t
+    big = torch.full((t.shape[0], t.shape[1] + pad), float("nan"), dtype=t.dtype, device=t.device)
+    big[:, :t.shape[1]] = t
+    return big[:, :t.shape[1]]
+
+
+# ---- embedding -------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,dim,vocab,pad", [(1, 512, 100, 0), (0, 8, 5, 0), (7, 1, 3, 0), (65, 33, 50, 0),
+                                              (300, 1024, 64, 8), (129, 264, 1000, 3)])
+def test_embed(dtype, n, dim, vocab, pad):
+    g = gen(n + dim)
+    table = strided(rand(g, vocab, dim, dtype=dtype), pad)
+    ids = torch.randint(-2, vocab + 2, (n,), generator=g, device="cuda", dtype=torch.int32)
+    out = strided(torch.zeros(n, dim, dtype=dtype, device="cuda"), pad)
+    got = K.embed(ids, table, scale=2.3, out=out)
+    assert got is out
+    inside = (ids >= 0) & (ids < vocab)
+    scale = float(torch.tensor(2.3, dtype=F32))
+    want = torch.where(inside[:, None], table.double()[ids.clamp(0, vocab - 1).long()] * scale, 0.0)
+    close(got, want, (U[dtype] + U32) * (1 + U[dtype]) * want.abs() + TINY[dtype])
+
+
+def embed_grad_reference(ids, dout, vocab, scale):
+    """(sum, sum of magnitudes, counts) per id in float64."""
+    keep = ((ids >= 0) & (ids < vocab)).nonzero()[:, 0]
+    at, rows = ids[keep].long(), dout.double()[keep] * scale
+    zero = torch.zeros(vocab, dout.shape[1], dtype=torch.float64, device="cuda")
+    count = torch.zeros(vocab, dtype=torch.float64, device="cuda")
+    count.index_add_(0, at, torch.ones_like(at, dtype=torch.float64))
+    return zero.clone().index_add_(0, at, rows), zero.clone().index_add_(0, at, rows.abs()), count
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,dim,vocab,kind", [
+    (1, 512, 300, "any"), (0, 16, 5, "any"), (9, 1, 1, "any"), (257, 40, 7, "any"), (1000, 33, 70000, "any"),
+    (4096, 64, 50257, "zipf"), (16384, 8, 3, "one"), (16385, 24, 257, "zipf"), (40001, 16, 65536, "zipf"),
+    (513, 32, 256, "outside"), (32 * 8 * 32 + 5, 8, 255, "runs")])
+@pytest.mark.parametrize("into", [False, True])
+def test_embed_grad(dtype, n, dim, vocab, kind, into):
+    g = gen(n + dim + vocab)
+    if kind == "any":
+        ids = torch.randint(-1, vocab + 1, (n,), generator=g, device="cuda")
+    elif kind == "zipf":
+        ids = ((vocab + 1.0) ** torch.rand(n, generator=g, device="cuda", dtype=torch.float64)).long() - 1
+    elif kind == "one":
+        ids = torch.full((n,), 1, device="cuda")
+    elif kind == "outside":  # nothing is inside
+        ids = torch.where(torch.rand(n, generator=g, device="cuda") < 0.5, -1, vocab)
+    else:  # runs that end exactly on tile borders
+        ids = torch.arange(n, device="cuda") // 64 % vocab
+    ids = ids.int()
+    dout = rand(g, n, dim, dtype=dtype)
+    outside = (ids < 0) | (ids >= vocab)
+    dout[outside] = float("nan")  # reaches no result
+    scale = 0.5
+    old = rand(g, vocab, dim, dtype=dtype)
+    old[vocab // 2] = float("inf")
+    grad = old.clone() if into else None
+    got = K.embed_grad(ids, dout, vocab, scale=scale, into=grad)
+    want, mag, count = embed_grad_reference(ids, dout, vocab, scale)
+    if into:
+        assert got is grad
+        untouched = count == 0
+        assert torch.equal(got[untouched], old[untouched])
+        want = torch.where(untouched[:, None], 0.0, want + old.double())
+        got = torch.where(untouched[:, None], torch.zeros_like(got), got)
+        live = torch.isfinite(want)
+        assert torch.equal(torch.isfinite(got), live)
+        want, got = torch.where(live, want, 0.0), torch.where(live, got, torch.zeros_like(got))
+    sums = (count[:, None] + 2) * U32 * mag + 2 * U32 * want.abs()
+    close(got, want, sums + U[dtype] * (want.abs() + sums) + TINY[dtype])
+    if not into:
+        assert torch.equal(got, K.embed_grad(ids, dout, vocab, scale=scale))  # the same bits
+
+
+def test_embed_grad_strides_and_shapes():
+    g = gen(5)
+    ids = torch.randint(0, 40, (3, 50), generator=g, device="cuda", dtype=torch.int32)
+    wide = rand(g, 3, 50, 48, dtype=BF16)
+    dout = wide[:, :, :40]  # one row stride over both leading dimensions
+    big = torch.full((40, 56), 7.0, dtype=BF16, device="cuda")
+    K.embed_grad(ids, dout, 40, into=big[:, :40].zero_())
+    want, mag, count = embed_grad_reference(ids.reshape(-1), dout.reshape(-1, 40), 40, 1.0)
+    sums = (count[:, None] + 2) * U32 * mag
+    close(big[:, :40], want, sums + U[BF16] * (want.abs() + sums) + TINY[BF16])
+    assert bool((big[:, 40:] == 7).all())  # behind the rows nothing is written
+
+
+# ---- layer normalisation ----------------------------------------------------
+def norm_reference(x, w, b, eps):
+    x = x.double()
+    mean = x.mean(1, keepdim=True)
+    xc = x - mean
+    var = (xc * xc).mean(1, keepdim=True)
+    rstd = 1 / (var + eps).sqrt()
+    y = xc * rstd
+    if w is not None:
+        y = y * w.double()
+    if b is not None:
+        y = y + b.double()
+    return x, mean, xc, var, rstd, y
+
+
+# longest chain of additions in a row's sum: per lane, over the lanes and warps,
+# and the strided sums of the longest rows
+def chain(dim):
+    return 64 + dim // 1024
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,pad", [(1, 512, 0), (0, 8, 0), (3, 1, 0), (33, 100, 0), (5, 128, 0), (70, 1000, 0),
+                                           (9, 1024, 8), (17, 513, 3), (4, 4096, 0), (3, 8192, 0), (2, 8200, 0),
+                                           (2, 20011, 0), (1025, 64, 0)])
+@pytest.mark.parametrize("affine", [True, False])
+def test_layer_norm(dtype, rows, dim, pad, affine):
+    g = gen(rows + dim)
+    x = strided(rand(g, rows, dim, dtype=dtype, std=1.7, mean=3.0), pad)
+    w = rand(g, dim, dtype=dtype, std=0.1, mean=1.0) if affine else None
+    b = rand(g, dim, dtype=dtype, std=0.1) if affine else None
+    eps = 1e-5
+    y, mean, rstd = K.layer_norm(x, w, b, eps=eps)
+    xd, m, xc, var, r, want = norm_reference(x, w, b, eps)
+    c = chain(dim)
+    dm = c * U32 * xd.abs().mean(1, keepdim=True) + U32 * m.abs() + 1e-30
+    close(mean[:, None], m, dm)
+    # the variance is taken about the computed mean: off by dm^2, and by the rounding of the differences
+    dvar = (c + 4) * U32 * var + dm * dm + 2 * U32 * xc.abs().mean(1, keepdim=True) * (xd.abs().amax(1, keepdim=True) if rows else 0)
+    rel_r = 0.5 * dvar / (var + eps) + 4 * U32
+    close(rstd[:, None], r, r * rel_r * (1 + rel_r))
+    wd = w.double().abs() if affine else 1.0
+    dy = wd * (r * (dm + 2 * U32 * xc.abs()) + (xc * r).abs() * (rel_r + 2 * U32)) * 1.01 + 2 * U32 * want.abs()
+    close(y, want, dy + U[dtype] * (want.abs() + dy) + TINY[dtype])
+
+
+def test_layer_norm_constant_and_extreme_rows():
+    # a constant row: variance 0, y is the bias; rows with Inf or NaN spoil only themselves
+    x = torch.full((4, 96), 3.0, device="cuda")
+    x[1, 5], x[2, 7] = float("inf"), float("nan")
+    b = torch.linspace(-1, 1, 96, device="cuda")
+    y, mean, rstd = K.layer_norm(x, None, b)
+    assert torch.equal(y[0], b) and torch.equal(y[3], b)
+    assert float(mean[0]) == 3.0 and abs(float(rstd[0]) - 1e-5 ** -0.5) < 1e-4 * 1e-5 ** -0.5
+    assert bool(torch.isnan(y[1:3]).all())
+    # large values: squares stay in range as long as the variance does
+    big = torch.tensor([[1e18, -1e18, 2e18, 0.0]], device="cuda")
+    y, _, _ = K.layer_norm(big, eps=0.0)
+    want = norm_reference(big, None, None, 0.0)[5]
+    close(y, want, 40 * U32 * (want.abs() + 1))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,pad", [(1, 512, 0), (0, 8, 0), (3, 1, 0), (2, 33, 0), (257, 100, 0), (2048, 512, 0),
+                                           (70, 1000, 8), (601, 1024, 0), (17, 513, 3), (40, 2048, 0), (9, 4096, 0),
+                                           (5, 8192, 0), (70, 9001, 0)])
+@pytest.mark.parametrize("affine", [True, False])
+def test_layer_norm_grad(dtype, rows, dim, pad, affine):
+    g = gen(rows + dim + 1)
+    x = strided(rand(g, rows, dim, dtype=dtype, std=1.7, mean=0.3), pad)
+    dy = strided(rand(g, rows, dim, dtype=dtype), pad)
+    w = rand(g, dim, dtype=dtype, std=0.1, mean=1.0) if affine else None
+    _, m, _, _, r, _ = norm_reference(x, None, None, 1e-5)
+    mean, rstd = m[:, 0].float(), r[:, 0].float()
+    dx, dw, db = K.layer_norm_grad(dy, x, w, mean, rstd)
+    md, rd = mean.double()[:, None], rstd.double()[:, None]
+    xh = (x.double() - md) * rd
+    gd = dy.double() * (w.double() if affine else 1.0)
+    c1, c2 = gd.mean(1, keepdim=True), (gd * xh).mean(1, keepdim=True)
+    want = rd * (gd - c1 - xh * c2)
+    c = chain(dim) + 4
+    e1, e2 = c * U32 * gd.abs().mean(1, keepdim=True), (c + 4) * U32 * (gd * xh).abs().mean(1, keepdim=True)
+    e = rd * (e1 + xh.abs() * e2 + 6 * U32 * (gd.abs() + c1.abs() + (xh * c2).abs())) * 1.01
+    close(dx, want, e + U[dtype] * (want.abs() + e) + TINY[dtype])
+    for got, terms in ((dw, dy.double() * xh), (db, dy.double())):
+        s = terms.sum(0)
+        e = (rows + 16) * U32 * terms.abs().sum(0)
+        close(got, s, e + U[dtype] * (s.abs() + e) + TINY[dtype])
+    again = K.layer_norm_grad(dy, x, w, mean, rstd)
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again))
+    # the parts alone are the same as together
+    assert torch.equal(K.layer_norm_grad(dy, x, w, mean, rstd, want=("x",))[0], dx)
+    only = K.layer_norm_grad(dy, x, w, mean, rstd, want=("bias",))
+    assert only[0] is None and only[1] is None and torch.equal(only[2], db)
+
+
+# ---- cross entropy of a linear head -----------------------------------------
+def ce_reference(x, w, b, tg, reduction, dloss, dtype):
+    """Results in float64 and their bounds."""
+    n, d = x.shape
+    v = w.shape[0]
+    wd = w.double()
+    keep = ((tg >= 0) & (tg < v)).nonzero()[:, 0]
+    xd, t = x.double()[keep], tg[keep].long()
+    z = xd @ wd.t()
+    # d products and additions, the bias, the shift of the exponent
+    ez = 2 * (d + 16) * U32 * (xd.abs() @ wd.abs().t())
+    if b is not None:
+        z = z + b.double()
+        ez = ez + 2 * U32 * b.double().abs()
+    ez = ez + 4 * U32 * torch.where(torch.isfinite(z), z.abs(), 0.0)
+    lse = torch.logsumexp(z, 1)
+    # sums of exponentials: each 8 units off, a few hundred additions at most in a chain
+    elz = ez.masked_fill(~torch.isfinite(z), 0.0).amax(1) + 600 * U32 + 4 * U32 * lse.abs()
+    rows = lse - z.gather(1, t[:, None])[:, 0]
+    erows = elz + ez.gather(1, t[:, None])[:, 0] + 4 * U32 * (lse.abs() + rows.abs())
+    count = max(1, keep.numel()) if reduction == "mean" else 1
+    c = dloss / count
+    p = (z - lse[:, None]).exp()
+    G = p.clone()
+    G[torch.arange(keep.numel(), device="cuda"), t] -= 1
+    eG = p * torch.expm1((ez + elz[:, None] + 8 * U32).clamp(max=10)) + 2 * U32
+    if dtype != F32:
+        eG = eG + U[dtype] * (G.abs() + eG) + (2.0 ** -36 if dtype == F16 else 0.0)
+    full = lambda rows_, width: torch.zeros(n, *width, dtype=torch.float64, device="cuda").index_copy_(0, keep, rows_)  # noqa: E731
+    dx = c * (G @ wd)
+    edx = abs(c) * (eG @ wd.abs() + 2 * (v + 16) * U32 * (G.abs() @ wd.abs())) + 4 * U32 * dx.abs()
+    dw = c * (G.t() @ xd)
+    k = keep.numel()
+    edw = abs(c) * (eG.t() @ xd.abs() + 2 * (k + 16) * U32 * (G.abs().t() @ xd.abs())) + 4 * U32 * dw.abs()
+    db = c * G.sum(0)
+    edb = abs(c) * (eG.sum(0) + 2 * (k + 16) * U32 * G.abs().sum(0)) + 4 * U32 * db.abs()
+    loss = rows.sum() / count
+    eloss = erows.sum() / count + (n + 8) * U32 * rows.abs().sum() / count
+    return dict(loss=(loss.reshape(1), eloss.reshape(1)), rows=(full(rows, ()), full(erows, ())),
+                lse=(full(lse, ()), full(elz, ())), dx=(full(dx, (d,)), full(edx, (d,))), dw=(dw, edw), db=(db, edb))
+
+
+def ce_check(x, w, b, tg, reduction="mean", dloss=1.0):
+    dtype = x.dtype
+    loss, rows, lse = K.linear_ce(x, w, tg, bias=b, reduction=reduction)
+    dl = None if dloss == 1.0 else torch.full((1,), dloss, device="cuda")
+    dx, dw, db = K.linear_ce_grad(x, w, tg, lse, bias=b, dloss=dl, reduction=reduction)
+    K.check(x.device)
+    ref = ce_reference(x, w, b, tg, reduction, dloss, dtype)
+    for got, name in ((loss, "loss"), (rows, "rows"), (lse, "lse")):
+        close(got, ref[name][0], ref[name][1] + 1e-30)
+    for got, name in ((dx, "dx"), (dw, "dw")) + (((db, "db"),) if b is not None else ()):
+        want, e = ref[name]
+        close(got, want, e + U[dtype] * (want.abs() + e) + TINY[dtype])
+    assert (db is None) == (b is None)
+    return loss, rows, lse, dx, dw, db
+
+
+def ce_inputs(seed, rows, dim, vocab, dtype, bias, ignored=0.0, pad=0, spread=3.0):
+    g = gen(seed)
+    x = strided(rand(g, rows, dim, dtype=dtype), pad)
+    w = strided(rand(g, vocab, dim, dtype=dtype, std=spread / dim ** 0.5), pad)
+    b = rand(g, vocab, dtype=dtype, std=0.5) if bias else None
+    tg = torch.randint(0, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    if ignored:
+        tg[torch.rand(rows, generator=g, device="cuda") < ignored] = -100
+    return x, w, b, tg
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,vocab,bias,ignored,pad", [
+    (1, 512, 1000, True, 0.0, 0), (1, 1, 1, False, 0.0, 0), (2, 7, 2, True, 0.0, 0), (5, 16, 65, True, 0.3, 0),
+    (127, 64, 255, False, 0.0, 0), (128, 128, 256, True, 0.0, 0), (129, 65, 257, True, 0.5, 0),
+    (300, 250, 1030, True, 0.1, 3), (257, 96, 4999, False, 0.2, 8), (640, 512, 777, True, 0.0, 0),
+    (3, 1024, 9001, True, 0.0, 0), (1025, 40, 513, True, 0.9, 0)])
+def test_linear_ce(dtype, rows, dim, vocab, bias, ignored, pad):
+    x, w, b, tg = ce_inputs(rows + dim, rows, dim, vocab, dtype, bias, ignored, pad)
+    dloss = 512.0 if dtype == F16 else 1.0
+    first = ce_check(x, w, b, tg, dloss=dloss)
+    again = ce_check(x, w, b, tg, dloss=dloss)
+    for p, q in zip(first, again):
+        assert p is q is None or torch.equal(p, q)  # the same bits
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_ce_at_the_training_vocabulary(dtype):
+    x, w, b, tg = ce_inputs(3, 200, 512, 50257, dtype, True, 0.1)
+    ce_check(x, w, b, tg, reduction="sum", dloss=0.25 if dtype != F16 else 8.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_ce_rows_that_are_not_counted_reach_nothing(dtype):
+    x, w, b, tg = ce_inputs(9, 150, 72, 300, dtype, True)
+    tg[10:30], tg[149], tg[0] = -1, 300, -2147483648
+    clean = K.linear_ce(x, w, tg, bias=b)
+    grads = K.linear_ce_grad(x, w, tg, clean[2], bias=b)
+    bad = x.clone()
+    bad[10:20], bad[20:30], bad[149], bad[0] = float("nan"), float("inf"), float("nan"), -float("inf")
+    loss, rows, lse = K.linear_ce(bad, w, tg, bias=b)
+    for p, q in zip((loss, rows, lse), clean):
+        assert torch.equal(p, q)
+    for p, q in zip(K.linear_ce_grad(bad, w, tg, lse, bias=b), grads):
+        assert torch.equal(p, q)
+    out = (tg < 0) | (tg >= 300)
+    assert bool((rows[out] == 0).all()) and bool((lse[out] == 0).all()) and bool((grads[0][out] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [0, 1, 130])
+def test_linear_ce_without_counted_rows(dtype, rows):
+    x, w, b, tg = ce_inputs(4, rows, 64, 300, dtype, True)
+    tg.fill_(-1)
+    x.fill_(float("nan"))
+    loss, row_loss, lse = K.linear_ce(x, w, tg, bias=b)
+    dx, dw, db = K.linear_ce_grad(x, w, tg, lse, bias=b)
+    assert float(loss) == 0.0
+    for t in (row_loss, lse, dx, dw, db):
+        assert bool((t == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_ce_masked_vocabulary(dtype):
+    """A bias of -Inf (or the type's lowest value) takes entries out of the softmax."""
+    x, w, b, tg = ce_inputs(6, 140, 64, 600, dtype, True)
+    dead = torch.arange(600, device="cuda") % 3 == 1
+    dead[256:512] = True  # a whole tile among them
+    tg = torch.where(dead[tg.long()], torch.full_like(tg, 2), tg)
+    low = -float("inf") if dtype != BF16 else torch.finfo(dtype).min
+    b[dead] = low
+    loss, rows, lse = K.linear_ce(x, w, tg, bias=b)
+    dx, dw, db = K.linear_ce_grad(x, w, tg, lse, bias=b)
+    keep = (~dead).nonzero()[:, 0]
+    back = torch.zeros(600, dtype=torch.int32, device="cuda")
+    back[keep] = torch.arange(keep.numel(), device="cuda", dtype=torch.int32)
+    ref = ce_reference(x, w[keep], b[keep], back[tg.long()], "mean", 1.0, dtype)
+    for got, name in ((loss, "loss"), (rows, "rows"), (lse, "lse")):
+        close(got, ref[name][0], ref[name][1])
+    for got, name in ((dx, "dx"), (dw[keep], "dw"), (db[keep], "db")):
+        want, e = ref[name]
+        close(got, want, e + U[dtype] * (want.abs() + e) + TINY[dtype])
+    assert bool((dw[dead] == 0).all()) and bool((db[dead] == 0).all())
+
+
+def test_linear_ce_nonfinite_rows_spoil_only_themselves():
+    x, w, b, tg = ce_inputs(8, 64, 32, 100, F32, True)
+    x[5, 3], x[9, 1] = float("nan"), float("inf")
+    _, rows, lse = K.linear_ce(x, w, tg, bias=b)
+    dx, _, _ = K.linear_ce_grad(x, w, tg, lse, bias=b)
+    spoilt = torch.zeros(64, dtype=torch.bool, device="cuda")
+    spoilt[5] = spoilt[9] = True
+    assert torch.equal(~torch.isfinite(rows), spoilt)
+    assert torch.equal(~torch.isfinite(dx).all(1), spoilt)
+    # a vocabulary with nothing in it: no probability to give
+    rows = K.linear_ce(x[:4], w, tg[:4], bias=torch.full_like(b, -float("inf")))[1]
+    assert not bool(torch.isfinite(rows).any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_ce_peaked_rows(dtype):
+    """Large logits: the softmax is all but one-hot, the loss near zero or large."""
+    x, w, b, tg = ce_inputs(12, 100, 64, 700, dtype, False, spread=40.0)
+    tg[::2] = (x[::2].double() @ w.double().t()).argmax(1).int()
+    ce_check(x, w, b, tg, dloss=64.0)
+
+
+def test_linear_ce_parts_alone():
+    x, w, b, tg = ce_inputs(2, 70, 48, 333, BF16, True, 0.2)
+    _, _, lse = K.linear_ce(x, w, tg, bias=b)
+    whole = K.linear_ce_grad(x, w, tg, lse, bias=b)
+    for i, name in enumerate(("x", "weight", "bias")):
+        part = K.linear_ce_grad(x, w, tg, lse, bias=b, want=(name,))
+        assert torch.equal(part[i], whole[i]) and sum(p is not None for p in part) == 1
+
+
+# ---- streams, graphs, devices ------------------------------------------------
+def model(ids, tg, table, lw, lb, hb):
+    """Embedding, norm and tied head; loss and the gradients of every leaf."""
+    s = table.shape[1] ** 0.5
+    e = K.embed(ids, table, scale=s)
+    y, mean, rstd = K.layer_norm(e, lw, lb)
+    loss, _, lse = K.linear_ce(y, table, tg, bias=hb)
+    dy, dtable, dhb = K.linear_ce_grad(y, table, tg, lse, bias=hb)
+    de, dlw, dlb = K.layer_norm_grad(dy, e, lw, mean, rstd)
+    K.embed_grad(ids, de, table.shape[0], scale=s, into=dtable)
+    return loss, dtable, dlw, dlb, dhb
+
+
+def model_inputs(seed, dtype, n=192, dim=72, vocab=530):
+    g = gen(seed)
+    ids = torch.randint(0, vocab, (2, n // 2), generator=g, device="cuda", dtype=torch.int32)
+    tg = torch.randint(0, vocab, (2, n // 2), generator=g, device="cuda", dtype=torch.int32)
+    tg[0, :7] = -1
+    return (ids, tg, rand(g, vocab, dim, dtype=dtype, std=0.25), rand(g, dim, dtype=dtype, std=0.1, mean=1.0),
+            rand(g, dim, dtype=dtype, std=0.1), rand(g, vocab, dtype=dtype, std=0.3))
+
+
+def model_reference(ids, tg, table, lw, lb, hb):
+    leaves = [t.double().requires_grad_() for t in (table, lw, lb, hb)]
+    t, w, b, h = leaves
+    e = t[ids.long()] * t.shape[1] ** 0.5
+    y = (e - e.mean(-1, keepdim=True)) / (e.var(-1, unbiased=False, keepdim=True) + 1e-5).sqrt() * w + b
+    z = (y @ t.t() + h).log_softmax(-1)
+    keep = tg >= 0
+    loss = -(z.gather(-1, tg.clamp(min=0).long()[..., None])[..., 0] * keep).sum() / keep.sum()
+    return loss, torch.autograd.grad(loss, leaves)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_model_of_them_together(dtype):
+    """Each of the five stages rounds its output once, and each gradient passes
+    at most eight roundings of relative size U on the way to its leaf; in the
+    2-norm they add as independent errors at worst linearly, doubled for the
+    reuse of the rounded values in the products' other operand."""
+    inputs = model_inputs(1, dtype)
+    got = model(*inputs)
+    loss, want = model_reference(*inputs)
+    tol = 16 * U[dtype] + 1000 * U32
+    assert abs(float(got[0]) - float(loss)) <= tol * float(loss)
+    for g, w in zip(got[1:], want):
+        assert float((g.double() - w).norm()) <= tol * float(w.norm())
+
+
+def test_the_models_gradient_against_differences():
+    """Central differences of the float64 loss along random directions, at a step
+    of 1e-4: off by h^2 times a third derivative of a few times the loss, far
+    below the float32 results' 1e-4 relative."""
+    inputs = model_inputs(2, F32)
+    grads = model(*inputs)[1:]
+    g = gen(3)
+    for i, grad in enumerate(grads):
+        d = torch.randn(grad.shape, generator=g, device="cuda", dtype=torch.float64)
+        h = 1e-4
+
+        def at(step):
+            moved = [t.double() for t in inputs[2:]]
+            moved[i] = moved[i] + step * d
+            return float(model_reference(inputs[0], inputs[1], *moved)[0])
+        want = (at(h) - at(-h)) / (2 * h)
+        got = float((grad.double() * d).sum())
+        assert abs(got - want) <= 1e-4 * float(grad.double().norm() * d.norm()), (i, got, want)
+
+
+def test_streams_and_captured_graphs():
+    """The same bits on a side stream and from graphs replayed side by side, with
+    inputs that change between replays."""
+    sets = [model_inputs(s, BF16) for s in (11, 12, 13)]
+    want = [model(*s) for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = model(*sets[1])
+    side.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want[1]))
+    graphs, outs, ins = [], [], []
+    for k in range(2):
+        s = [t.clone() for t in sets[k]]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o = model(*s)
+        graphs.append(graph), outs.append(o), ins.append(s)
+    for k in range(2):  # other inputs than at capture
+        for dst, src in zip(ins[k], sets[k + 1]):
+            dst.copy_(src)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                graphs[k].replay()
+    torch.cuda.synchronize()
+    K.check()
+    for k in range(2):
+        assert all(torch.equal(p, q) for p, q in zip(outs[k], want[k + 1]))
+
+
+def test_python_refusals():
+    t = torch.zeros(4, 8, device="cuda")
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    bad = [lambda: K.embed(i.long(), t), lambda: K.embed(i, t.double()), lambda: K.embed(i, t.t()),
+           lambda: K.embed(i, t, out=torch.zeros(4, 9, device="cuda")), lambda: K.embed(i.cpu(), t),
+           lambda: K.embed_grad(i[:3], t, 5), lambda: K.embed_grad(i, t, 0),
+           lambda: K.embed_grad(i, t, 5, into=torch.zeros(5, 8, device="cuda", dtype=BF16)),
+           lambda: K.layer_norm(t, torch.zeros(7, device="cuda")), lambda: K.layer_norm(t, t[:, 0]),
+           lambda: K.layer_norm(t, eps=-1.0), lambda: K.layer_norm(t.half(), torch.zeros(8, device="cuda")),
+           lambda: K.layer_norm(torch.zeros(2, 4, 8, device="cuda").transpose(0, 1)),
+           lambda: K.layer_norm_grad(t, t, None, i, i), lambda: K.layer_norm_grad(t[:2], t, None, t[:, 0], t[:, 0]),
+           lambda: K.layer_norm_grad(t, t, None, t[0, :4], t[0, :4], want=()),
+           lambda: K.linear_ce(t, torch.zeros(5, 7, device="cuda"), i), lambda: K.linear_ce(t, t, i[:2]),
+           lambda: K.linear_ce(t, t, i, reduction="none"), lambda: K.linear_ce(t, t.half(), i),
+           lambda: K.linear_ce_grad(t, t, i, t[:, 0]), lambda: K.linear_ce_grad(t, t, i, t[0, :4], want=())]
+    for call in bad:
+        with pytest.raises(AideenError):
+            call()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_tensors_on_another_device_than_the_current_one():
+    a = model_inputs(21, BF16)
+    want = model(*a)
+    with torch.cuda.device(0):
+        got = model(*[t.to("cuda:1") for t in a])
+    assert all(torch.equal(p, q.to("cuda:0")) for p, q in zip(want, got))

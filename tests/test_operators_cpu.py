@@ -1,0 +1,139 @@
+"""Refusals of the operators on caller-owned tensors: every bad argument is
+turned down on the host, with a reason, before anything is launched (no GPU is
+needed, and the addresses below are never touched)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from aideen_b200 import backend, operators
+from aideen_b200.backend import AideenError, EmbedArgs, LayerNormArgs, LinearCeArgs
+
+OK, INVALID = 0, 1
+P = 1 << 20  # an aligned address that stands for a device pointer
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return backend.load_library()
+
+
+def embed_args(**kw):
+    a = dict(dtype=0, n_tokens=4, dim=8, vocab=10, scale=1.0, accumulate=0, table_ld=8, rows_ld=8)
+    a.update(kw)
+    return EmbedArgs(**a)
+
+
+def norm_args(**kw):
+    a = dict(dtype=0, rows=4, dim=8, eps=1e-5, x_ld=8, y_ld=8, dx_ld=8)
+    a.update(kw)
+    return LayerNormArgs(**a)
+
+
+def ce_args(**kw):
+    a = dict(dtype=0, rows=4, dim=8, vocab=10, reduction=0, x_ld=8, w_ld=8, dx_ld=8, dw_ld=8)
+    a.update(kw)
+    return LinearCeArgs(**a)
+
+
+def refused(lib, rc, word):
+    assert rc == INVALID
+    why = lib.aideen_operator_error().decode()
+    assert word in why, why
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(dtype=3), "dtype"), (dict(dim=0), "dim"), (dict(vocab=0), "vocab"), (dict(vocab=1 << 31), "vocab"),
+    (dict(n_tokens=(1 << 30) + 1), "tokens"), (dict(accumulate=2), "accumulate"), (dict(table_ld=7), "stride"),
+    (dict(rows_ld=-8), "stride")])
+def test_embed_refuses_bad_arguments(lib, bad, word):
+    a = embed_args(**bad)
+    n = C.c_size_t()
+    refused(lib, lib.aideen_embed(C.byref(a), P, P, P, None), word)
+    refused(lib, lib.aideen_embed_grad_workspace(C.byref(a), C.byref(n)), word)
+    refused(lib, lib.aideen_embed_grad(C.byref(a), P, P, P, P, 1 << 20, None), word)
+
+
+def test_embed_refuses_bad_pointers(lib):
+    a, n = embed_args(), C.c_size_t()
+    refused(lib, lib.aideen_embed(None, P, P, P, None), "null")
+    refused(lib, lib.aideen_embed(C.byref(a), None, P, P, None), "null")
+    refused(lib, lib.aideen_embed(C.byref(a), P, P + 2, P, None), "aligned")
+    refused(lib, lib.aideen_embed(C.byref(a), P + 1, P, P, None), "aligned")
+    assert lib.aideen_embed_grad_workspace(C.byref(a), C.byref(n)) == OK and n.value > 0
+    refused(lib, lib.aideen_embed_grad(C.byref(a), P, P, None, P, n.value, None), "null")
+    refused(lib, lib.aideen_embed_grad(C.byref(a), P, P, P, P, n.value - 1, None), "workspace")
+    refused(lib, lib.aideen_embed_grad(C.byref(a), P, P, P, P + 16, n.value, None), "workspace")
+    refused(lib, lib.aideen_embed_grad(C.byref(a), P, P, P, None, 0, None), "workspace")
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(dtype=9), "dtype"), (dict(dim=0), "dim"), (dict(rows=(1 << 30) + 1), "rows"), (dict(eps=-1.0), "eps"),
+    (dict(eps=float("nan")), "eps"), (dict(x_ld=7), "stride"), (dict(y_ld=0), "stride")])
+def test_layer_norm_refuses_bad_arguments(lib, bad, word):
+    a, n = norm_args(**bad), C.c_size_t()
+    refused(lib, lib.aideen_layer_norm(C.byref(a), P, P, P, P, P, P, None), word)
+    refused(lib, lib.aideen_layer_norm_grad_workspace(C.byref(a), C.byref(n)), word)
+    refused(lib, lib.aideen_layer_norm_grad(C.byref(a), P, P, P, P, P, P, P, P, P, 1 << 20, None), word)
+
+
+def test_layer_norm_refuses_bad_pointers(lib):
+    a, n = norm_args(), C.c_size_t()
+    refused(lib, lib.aideen_layer_norm(C.byref(a), None, P, P, P, P, P, None), "null")
+    refused(lib, lib.aideen_layer_norm(C.byref(a), P, P + 1, P, P, P, P, None), "aligned")
+    assert lib.aideen_layer_norm_grad_workspace(C.byref(a), C.byref(n)) == OK and n.value > 0
+    grad = lib.aideen_layer_norm_grad
+    refused(lib, grad(C.byref(a), P, P, P, P, P, None, None, None, P, n.value, None), "no output")
+    refused(lib, grad(C.byref(a), P, P, P, None, P, P, P, P, P, n.value, None), "null")
+    refused(lib, grad(C.byref(a), P, P, P, P, P, P, P, P, P, n.value - 1, None), "workspace")
+    refused(lib, grad(C.byref(norm_args(dx_ld=3)), P, P, P, P, P, P, P, P, P, n.value, None), "stride")
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(dtype=3), "dtype"), (dict(dim=0), "dim"), (dict(vocab=0), "vocab"), (dict(rows=(1 << 24) + 1), "rows"),
+    (dict(reduction=2), "reduction"), (dict(x_ld=7), "stride"), (dict(w_ld=7), "stride")])
+def test_linear_ce_refuses_bad_arguments(lib, bad, word):
+    a, n, m = ce_args(**bad), C.c_size_t(), C.c_size_t()
+    refused(lib, lib.aideen_linear_ce_workspace(C.byref(a), C.byref(n), C.byref(m)), word)
+    refused(lib, lib.aideen_linear_ce(C.byref(a), P, P, P, P, P, P, P, P, 1 << 30, None), word)
+    refused(lib, lib.aideen_linear_ce_grad(C.byref(a), P, P, P, P, P, P, P, P, P, P, 1 << 30, None), word)
+
+
+def test_linear_ce_refuses_bad_pointers(lib):
+    a, n, m = ce_args(), C.c_size_t(), C.c_size_t()
+    assert lib.aideen_linear_ce_workspace(C.byref(a), C.byref(n), C.byref(m)) == OK and n.value and m.value
+    loss, grad = lib.aideen_linear_ce, lib.aideen_linear_ce_grad
+    refused(lib, loss(C.byref(a), P, P, P, P, None, None, None, P, n.value, None), "no output")
+    refused(lib, loss(C.byref(a), P, None, P, P, P, P, P, P, n.value, None), "null")
+    refused(lib, loss(C.byref(a), P, P + 2, P, P, P, P, P, P, n.value, None), "aligned")
+    refused(lib, loss(C.byref(a), P, P, P, P, P, P, P, P, n.value - 1, None), "workspace")
+    refused(lib, grad(C.byref(a), P, P, P, P, P, P, None, None, None, P, m.value, None), "no output")
+    refused(lib, grad(C.byref(a), P, P, P, P, None, P, P, P, P, P, m.value, None), "null")
+    refused(lib, grad(C.byref(a), P, P, P, P, P, P, P, P, P, P, m.value - 1, None), "workspace")
+    refused(lib, grad(C.byref(ce_args(dw_ld=7)), P, P, P, P, P, P, P, P, P, P, m.value, None), "stride")
+    refused(lib, grad(C.byref(ce_args(dx_ld=7)), P, P, P, P, P, P, P, P, P, P, m.value, None), "stride")
+
+
+def test_workspaces_grow_with_the_sizes_and_stay_below_the_logits(lib):
+    """The point of the pieces: at the training shard's size the gradient's
+    workspace is a fraction of the float32 logits, and it stops growing with the
+    vocabulary."""
+    def grad_bytes(vocab, rows=16384):
+        m = C.c_size_t()
+        a = ce_args(dtype=1, rows=rows, dim=512, vocab=vocab, x_ld=512, w_ld=512)
+        assert lib.aideen_linear_ce_workspace(C.byref(a), None, C.byref(m)) == OK
+        return m.value
+    assert grad_bytes(50257) < 16384 * 50257 * 4 / 4
+    assert grad_bytes(200000) < 1.5 * grad_bytes(50257)
+
+
+@pytest.mark.parametrize("call", [
+    lambda t, i: operators.embed(i, t),
+    lambda t, i: operators.embed_grad(i, t, 4),
+    lambda t, i: operators.layer_norm(t),
+    lambda t, i: operators.layer_norm_grad(t, t, None, t, t),
+    lambda t, i: operators.linear_ce(t, t, i),
+    lambda t, i: operators.linear_ce_grad(t, t, i, t)])
+def test_host_tensors_are_refused(call):
+    with pytest.raises(AideenError, match="CUDA tensor"):
+        call(torch.zeros(4, 8), torch.zeros(4, dtype=torch.int32))
