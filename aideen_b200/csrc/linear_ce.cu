@@ -5,237 +5,826 @@
 //   G = softmax(z) - onehot(t)  (0 where the row is not counted)
 //   dx = c G W,  dW = c G^T x,  db = c sum_n G,   c = dloss / counted rows
 //
-// CUDA-core form: 64 x 64 tiles of z through shared memory.  The loss keeps a
-// running maximum and sum per row and vocabulary slice; the gradient forms G for
-// a piece of the vocabulary at a time and multiplies it.
+// Steps:
+//   stage   counted rows of x are gathered to the front (a padded row costs no
+//           product and its contents reach nothing) as 16-bit operands; float32
+//           is split into three bfloat16 pieces that add up to it exactly.
+//   stats   z tile by tile on the tensor cores; the epilogue keeps a running
+//           maximum and sum per row and stores nothing else.
+//   rows    joins the partial statistics, forms z[n][t[n]] as a plain dot product.
+//   pieces  (gradient) for each piece of the vocabulary: z again, G into a
+//           16-bit buffer of one piece, then one launch for both products with G.
+//
+// Tensor-core kernel (ce_mma_kernel): a persistent grid of CTA pairs, each on
+// 256 x 256 tiles (tcgen05.mma cta_group::2: every CTA holds 128 rows of the
+// accumulator and loads half of either operand).  Per CTA: warp 0 streams 64-deep
+// slices by TMA into a ring of five 32 KB stages, warp 1 of the leading CTA
+// issues the MMAs into one of two 256-column accumulators in tensor memory, and
+// warps 2..9 drain the other one.  float32 operands take six products of their
+// pieces (all but those below 2^-24), the small ones first.
+// Bound: the tensor cores (2 N V d for the loss, 6 N V d for the gradient).
+//
+// Every wait is bounded; a wait that runs out sets an error word, issues nothing
+// further, lets its copies land, frees the tensor memory and returns.
+#include <cuda.h>
+
 #include "common.cuh"
 #include "operators.cuh"
+#include "tc_common.cuh"
 
 namespace aideen {
 namespace {
 
 __device__ unsigned int g_ce_timeout;
 
-constexpr int kTile = 64, kStep = 16;
-constexpr int kPiece = 4096;  // vocabulary columns of G held at a time
-constexpr int kSlices = 64;   // vocabulary slices of the loss
+constexpr int kTileM = 256, kTileN = 256, kBlockK = 64;
+constexpr int kStages = 5, kHalfBytes = 128 * kBlockK * 2, kStageBytes = 2 * kHalfBytes;
+constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
+constexpr int kBoxBytes = 4096;  // 32 rows of 128 bytes
+constexpr uint32_t kWaitLimit = 1u << 24;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// float16 keeps softmax - onehot times 2^12: probabilities down to 2^-26 stay
+// normal numbers, and the largest magnitude is 2^12
+constexpr float kHalfScale = 4096.f;
+constexpr size_t kSmemBytes = (size_t)kStages * kStageBytes + kEpiWarps * 2 * kBoxBytes + 2 * kTileN * 4 + 256;
 
-struct CeArgs {
-  const void *x, *w, *b;
-  const int32_t *tg;
-  const float *lse;
-  long x_ld, w_ld;
-  int rows, dim, vocab;
+enum { kStats = 0, kPiece = 1, kProducts = 2 };
+
+struct MmaArgs {
+  const int *count;   // counted rows
+  int vocab, dim;
+  int planes;         // 16-bit pieces per operand element: 1, or 3 for float32
+  uint32_t idesc;     // operand types of the instruction descriptor
+  // kStats, kPiece: vocabulary tiles [0, tiles_n) from column v0 on
+  int v0, tiles_n;
+  const void *bias;
+  uint32_t dtype;     // of bias, dW
+  float2 *stats;      // kStats: [slot][2][256] (maximum, sum) in base 2
+  const float *lse2;  // kPiece: compacted rows' lse in base 2
+  const int32_t *tgt; // and their targets
+  float g_scale;
+  // kProducts
+  int bn;             // columns of an output tile: 128 or 256
+  int tiles_d;        // of dim
+  int piece_k;        // 64-deep slices of the piece
+  int tiles_v;        // dW tiles of the piece (0: dW not wanted)
+  int splits;         // K splits of dx (0: dx not wanted)
+  int first;          // first piece: dx slabs are written, not added to
+  int dw_tma;         // dW can be stored by TMA
+  void *dw;
+  long dw_ld;
+  const float *dloss;
+  int mean;
 };
 
-__device__ __forceinline__ bool counted(int32_t t, int vocab) { return t >= 0 && t < vocab; }
+__device__ __forceinline__ float grad_scale(const float *dloss, const int *count, int mean) {
+  return (dloss ? *dloss : 1.f) / (mean ? fmaxf((float)*count, 1.f) : 1.f);
+}
 
-// acc[i][j] = sum_k A(m0 + 4 ty + i, k) B(n0 + 4 tx + j, k); fa / fb give 0 outside.
-template <typename FA, typename FB>
-__device__ __forceinline__ void tile_product(FA fa, FB fb, int K, float (&acc)[4][4], float (*sa)[kTile + 1],
-                                             float (*sb)[kTile + 1]) {
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-  for (int k0 = 0; k0 < K; k0 += kStep) {
-    for (int i = threadIdx.x; i < kTile * kStep; i += 256) {
-      sa[i % kStep][i / kStep] = k0 + i % kStep < K ? fa(i / kStep, k0 + i % kStep) : 0.f;
-      sb[i % kStep][i / kStep] = k0 + i % kStep < K ? fb(i / kStep, k0 + i % kStep) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kStep; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][4 * ty + i], sb[k][4 * tx + j], acc[i][j]);
-    __syncthreads();
+// ---- pair-of-CTAs primitives ------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of the leading CTA's copy of a shared-memory object.
+__device__ __forceinline__ uint32_t leader_addr(const void *p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+__device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
   }
+  return false;
+}
+// Load into this CTA's shared memory; the bytes are counted on `bar` of the
+// leading CTA.
+__device__ __forceinline__ void pair_load(void *dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void pair_mma(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+      "l"(da), "l"(db), "r"(idesc), "r"(accumulate));
+}
+// Arrives on `bar` of both CTAs once every MMA issued so far is done.
+__device__ __forceinline__ void pair_commit(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void remote_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+      "%28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <typename T>
-__device__ __forceinline__ void logits_tile(const CeArgs &a, int m0, int n0, float (&acc)[4][4],
-                                            float (*sa)[kTile + 1], float (*sb)[kTile + 1]) {
-  const T *x = static_cast<const T *>(a.x), *w = static_cast<const T *>(a.w), *b = static_cast<const T *>(a.b);
-  tile_product(
-      [&](int m, int k) { return m0 + m < a.rows ? op_load<T>(x[(long)(m0 + m) * a.x_ld + k]) : 0.f; },
-      [&](int n, int k) { return n0 + n < a.vocab ? op_load<T>(w[(long)(n0 + n) * a.w_ld + k]) : 0.f; }, a.dim, acc,
-      sa, sb);
-  const int tx = threadIdx.x & 15;
-  if (b) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float bv = n0 + 4 * tx + j < a.vocab ? op_load<T>(b[n0 + 4 * tx + j]) : 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i][j] += bv;
+// Products of pieces in the order they are added: (A piece, B piece).
+__device__ __forceinline__ void product_pair(int planes, int j, int &pa, int &pb) {
+  if (planes == 1) { pa = pb = 0; return; }
+  // lo*hi, hi*lo, mid*mid, mid*hi, hi*mid, hi*hi
+  constexpr uint32_t A = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
+  constexpr uint32_t B = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+  pa = (A >> (2 * j)) & 3;
+  pb = (B >> (2 * j)) & 3;
+}
+
+// One output tile of a launch.
+struct Unit {
+  int m, n;      // tile coordinates (rows of 256, columns of kTileN or bn)
+  int kb0, nkb;  // 64-deep slices
+  int dw;        // kProducts: 1 = dW tile, 0 = dx tile
+  int z;         // dx: split
+};
+
+// Units of one pair.  kStats and kPiece: a contiguous share of the (row tile,
+// vocabulary tile) order, so that a pair stays on one row tile.  kProducts: dW tiles,
+// then dx tiles, dealt out round robin.
+template <int MODE>
+struct Units {
+  long next, end, step;
+  int tiles_n, k_dim, k_rows;
+  const MmaArgs &a;
+  int count;
+  __device__ __forceinline__ Units(const MmaArgs &args, int cnt) : a(args), count(cnt) {
+    const long pairs = gridDim.x >> 1, p = blockIdx.x >> 1;
+    // without a counted row one tile of zeros still writes dW
+    const int tiles_m = max(1, (count + kTileM - 1) / kTileM);
+    k_dim = (a.dim + kBlockK - 1) / kBlockK;
+    k_rows = max(1, (count + kBlockK - 1) / kBlockK);
+    tiles_n = a.tiles_n;
+    if (MODE == kProducts) {
+      next = p;
+      end = (long)a.tiles_v * a.tiles_d + (long)tiles_m * a.tiles_d * a.splits;
+      step = pairs;
+    } else {
+      const long total = (long)tiles_m * tiles_n;
+      next = p * total / pairs;
+      end = (p + 1) * total / pairs;
+      step = 1;
     }
   }
-}
-
-__device__ __forceinline__ void merge(float &m, float &s, float m2, float s2) {
-  const float mm = fmaxf(m, m2);
-  if (mm == -INFINITY) { s += s2; return; }
-  s = s * expf(m - mm) + s2 * expf(m2 - mm);
-  m = mm;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) ce_stats_kernel(const CeArgs a, float2 *part, float *picked) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  __shared__ float2 st[kTile][16];
-  const int m0 = blockIdx.x * kTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float m[4], s[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { m[i] = -INFINITY; s[i] = 0.f; }
-  for (int n0 = blockIdx.y * kTile; n0 < a.vocab; n0 += kTile * gridDim.y) {
-    float acc[4][4];
-    logits_tile<T>(a, m0, n0, acc, sa, sb);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = m0 + 4 * ty + i;
-      const int t = row < a.rows ? a.tg[row] : -1;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int col = n0 + 4 * tx + j;
-        if (col >= a.vocab) continue;
-        merge(m[i], s[i], acc[i][j], isinf(acc[i][j]) && acc[i][j] < 0 ? 0.f : 1.f);
-        if (col == t) picked[row] = acc[i][j];
+  __device__ __forceinline__ bool get(Unit &u) {
+    do {
+      if (next >= end) return false;
+      at(u);
+      next += step;
+    } while (u.nkb == 0);  // a short last piece may leave a split nothing
+    return true;
+  }
+  __device__ __forceinline__ void at(Unit &u) const {
+    if (MODE != kProducts) {
+      u.m = (int)(next / tiles_n);
+      u.n = (int)(next % tiles_n);
+      u.kb0 = 0;
+      u.nkb = k_dim;
+      u.dw = u.z = 0;
+    } else {
+      const long nw = (long)a.tiles_v * a.tiles_d;
+      if (next < nw) {
+        u.dw = 1;
+        u.m = (int)(next / a.tiles_d);
+        u.n = (int)(next % a.tiles_d);
+        u.kb0 = 0;
+        u.nkb = k_rows;
+        u.z = 0;
+      } else {
+        const long i = next - nw;
+        u.dw = 0;
+        u.n = (int)(i % a.tiles_d);
+        u.z = (int)(i / a.tiles_d % a.splits);
+        u.m = (int)(i / a.tiles_d / a.splits);
+        u.kb0 = (int)((long)u.z * a.piece_k / a.splits);
+        u.nkb = (int)((long)(u.z + 1) * a.piece_k / a.splits) - u.kb0;
       }
     }
   }
+};
+
+// Writes 32 columns of a lane's row (two calls fill a box of 64 16-bit columns).
+template <typename T>
+__device__ __forceinline__ void box_put16(unsigned char *box, int lane, int half, const float (&v)[32]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) st[4 * ty + i][tx] = make_float2(m[i], s[i]);
+  for (int k = 0; k < 4; ++k) {
+    OpVec<T, 8> x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.v[i] = op_store<T>(v[8 * k + i]);
+    *reinterpret_cast<OpVec<T, 8> *>(box + lane * 128 + (((half * 4 + k) ^ (lane & 7)) * 16)) = x;
+  }
+}
+__device__ __forceinline__ void box_put32(unsigned char *box, int lane, const float (&v)[32]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    *reinterpret_cast<float4 *>(box + lane * 128 + ((k ^ (lane & 7)) * 16)) =
+        make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+}
+
+// One warp's two staging boxes: take() gives the one whose last store has been
+// read, send() hands it to TMA.
+struct Boxes {
+  unsigned char *base;
+  int n = 0;
+  __device__ __forceinline__ unsigned char *take(int lane) {
+    unsigned char *b = base + (n & 1) * kBoxBytes;
+    if (lane == 0) bulk_wait_read<1>();
+    __syncwarp();
+    return b;
+  }
+  __device__ __forceinline__ void send(int lane, const CUtensorMap *map, const unsigned char *box, int x, int y, int z,
+                                       bool add) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      if (add) tma_reduce_add_3d(map, box, x, y, z);
+      else tma_store_3d(map, box, x, y, z);
+      bulk_commit();
+    }
+    ++n;
+  }
+};
+
+struct Maps {
+  CUtensorMap a, b;    // kStats, kPiece: x and W by rows.  kProducts, dx: G by rows, W by columns
+  CUtensorMap a2, b2;  // kProducts, dW: G by columns, x by columns
+  CUtensorMap c, c2;   // stores: kPiece: G.  kProducts: dx slabs, dW
+};
+
+template <int MODE, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    ce_mma_kernel(const __grid_constant__ Maps maps, const MmaArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char *sm = smem_raw;
+  if (smem_u32(sm) & 1023) {  // the swizzled tiles need it; the same in every CTA
+    if (threadIdx.x == 0) atomicCAS(&g_ce_timeout, 0u, 1u);
+    return;
+  }
+  unsigned char *boxes = sm + kStages * kStageBytes;
+  float *sbias = reinterpret_cast<float *>(boxes + kEpiWarps * 2 * kBoxBytes);  // [2][kTileN]
+  uint64_t *full = reinterpret_cast<uint64_t *>(sbias + 2 * kTileN);
+  uint64_t *empty = full + kStages;
+  uint64_t *tfull = empty + kStages;
+  uint64_t *tempty = tfull + 2;
+  uint64_t *done = tempty + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
+  uint32_t *err = tmem_slot + 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  const int count = *a.count;
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 2 * kEpiWarps);
+    }
+    mbar_init(done, 1);
+    *err = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(2u * kTileN));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (threadIdx.x < kTile && m0 + threadIdx.x < a.rows) {
-    float mm = -INFINITY, ss = 0.f;
-    for (int k = 0; k < 16; ++k) merge(mm, ss, st[threadIdx.x][k].x, st[threadIdx.x][k].y);
-    part[(size_t)blockIdx.y * a.rows + m0 + threadIdx.x] = make_float2(mm, ss);
+  cluster_barrier();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  const int products = a.planes == 1 ? 1 : 6;
+  const int bn = MODE == kProducts ? a.bn : kTileN;  // columns of a tile; either CTA loads half
+  Units<MODE> units(a, count);
+  Unit u;
+
+  if (warp == 0) {
+    if (lane == 0) {  // ---------------- loads
+      uint32_t it = 0;
+      bool ok = true;
+      const uint32_t bytes = 2u * (kHalfBytes + bn / 2 * kBlockK * 2);  // of both CTAs
+      while (ok && units.get(u)) {
+        const int m0 = u.m * kTileM + (int)rank * 128, n0 = u.n * bn + (int)rank * (bn / 2);
+        for (int j = 0; j < products && ok; ++j) {
+          int pa, pb;
+          product_pair(a.planes, j, pa, pb);
+          for (int kb = 0; kb < u.nkb; ++kb, ++it) {
+            const int s = it % kStages;
+            if (it >= (uint32_t)kStages && !wait_bounded(&empty[s], ((it / kStages) - 1) & 1)) { ok = false; break; }
+            if (*(volatile uint32_t *)err) { ok = false; break; }
+            unsigned char *sa = sm + s * kStageBytes, *sb = sa + kHalfBytes;
+            const uint32_t bar = leader_addr(&full[s]);
+            if (rank == 0) mbar_expect_tx(&full[s], bytes);
+            const int k0 = (u.kb0 + kb) * kBlockK;
+            if (MODE != kProducts) {
+              pair_load(sa, &maps.a, bar, k0, m0, pa);
+              pair_load(sb, &maps.b, bar, k0, a.v0 + n0, pb);
+            } else if (u.dw) {
+              for (int c = 0; c < 2; ++c) pair_load(sa + c * 8192, &maps.a2, bar, m0 + 64 * c, k0, pa);
+              for (int c = 0; c < bn / 128; ++c) pair_load(sb + c * 8192, &maps.b2, bar, n0 + 64 * c, k0, pb);
+            } else {
+              pair_load(sa, &maps.a, bar, k0, m0, pa);
+              for (int c = 0; c < bn / 128; ++c) pair_load(sb + c * 8192, &maps.b, bar, n0 + 64 * c, a.v0 + k0, pb);
+            }
+          }
+        }
+      }
+      if (!ok) atomicExch(err, 1u);
+      // every stage's last use is over (its arrival has landed here) before this CTA may leave
+      for (uint32_t j = it > (uint32_t)kStages ? it - kStages : 0; j < it && ok; ++j)
+        if (!wait_bounded(&empty[j % kStages], (j / kStages) & 1)) { ok = false; atomicExch(err, 1u); }
+      if (!ok && rank == 0) {  // let the copies in flight land
+        for (uint32_t j = it > (uint32_t)kStages ? it - kStages : 0; j < it; ++j)
+          wait_bounded(&full[j % kStages], (j / kStages) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {  // ---------------- MMAs
+      uint32_t it = 0;
+      int j = 0;
+      bool ok = true;
+      for (; ok && units.get(u); ++j) {
+        const int acc = j & 1;
+        if (j >= 2 && !wait_bounded(&tempty[acc], ((j >> 1) - 1) & 1)) { ok = false; break; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        // rows by 64: 128-byte rows, 8-row groups 1024 apart; columns by 64: blocks of 64
+        // columns 8192 apart, 8-row groups 1024 apart
+        const bool acol = MODE == kProducts && u.dw, bcol = MODE == kProducts;
+        const uint32_t idesc = a.idesc | (acol ? 1u << 15 : 0u) | (bcol ? 1u << 16 : 0u) | (uint32_t)(bn >> 3) << 17 |
+                               (uint32_t)(kTileM >> 4) << 24;
+        const uint32_t lbo_a = acol ? 8192u : 16u, lbo_b = bcol ? 8192u : 16u;
+        const uint32_t ka = acol ? 2048u : 32u, kb_ = bcol ? 2048u : 32u;  // 16 deep
+        const uint32_t d = tmem + (uint32_t)acc * kTileN;
+        const int total = products * u.nkb;
+        for (int k = 0; k < total; ++k, ++it) {
+          const int s = it % kStages;
+          if (!wait_bounded(&full[s], (it / kStages) & 1) || *(volatile uint32_t *)err) { ok = false; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          unsigned char *sa = sm + s * kStageBytes, *sb = sa + kHalfBytes;
+#pragma unroll
+          for (int q = 0; q < kBlockK / 16; ++q)
+            pair_mma(d, sdesc(sa + q * ka, lbo_a, 1024u, 2u), sdesc(sb + q * kb_, lbo_b, 1024u, 2u), idesc,
+                     k > 0 || q > 0 ? 1u : 0u);
+          pair_commit(&empty[s]);
+        }
+        if (!ok) break;
+        pair_commit(&tfull[acc]);
+      }
+      if (!ok) atomicExch(err, 1u);
+      pair_commit(done);
+      wait_bounded(done, 0);  // every MMA of the pair is over
+    }
+  } else {  // ---------------- epilogue: lanes are accumulator rows
+    const int q = warp & 3, half = (warp - 2) >> 2;  // tensor-memory lane quarter, half of the columns
+    const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16);
+    Boxes box{boxes + (warp - 2) * 2 * kBoxBytes};
+    const int etid = tid - 64;
+    int j = 0, last_m = -1;
+    float run_m = -INFINITY, run_s = 0.f;  // kStats: this row's statistics over the pair's tiles
+    float lse2 = 0.f;
+    int32_t tgt = -1;
+    const float scale = MODE == kProducts ? grad_scale(a.dloss, a.count, a.mean) / a.g_scale : 0.f;
+    auto flush = [&]() {
+      if (last_m < 0) return;
+      const size_t slot = (size_t)(blockIdx.x >> 1) + last_m;
+      a.stats[(slot * 2 + half) * kTileM + rank * 128 + q * 32 + lane] = make_float2(run_m, run_s);
+    };
+    bool dead = false;  // a wait ran out: keep the barriers below in step, touch nothing
+    for (; units.get(u); ++j) {
+      const int acc = j & 1;
+      const float *sb = sbias + acc * kTileN;
+      if (MODE != kProducts) {
+        // this tile's bias in base 2 (-Inf behind the vocabulary); the buffer's last
+        // reader passed the barrier of the tile before
+        const int v = a.v0 + u.n * kTileN + etid;
+        float b = -INFINITY;
+        if (v < a.vocab) b = a.bias ? op_load<T>(static_cast<const T *>(a.bias)[v]) * kLog2e : 0.f;
+        sbias[acc * kTileN + etid] = b;
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+        if (u.m != last_m) {
+          if (MODE == kStats) {
+            flush();
+            run_m = -INFINITY;
+            run_s = 0.f;
+          } else {
+            const int row = u.m * kTileM + (int)rank * 128 + q * 32 + lane;
+            lse2 = row < count ? a.lse2[row] : INFINITY;  // rows behind the last: G = 0
+            tgt = row < count ? a.tgt[row] : -1;
+          }
+          last_m = u.m;
+        }
+      }
+      if (!dead && (!wait_bounded(&tfull[acc], (j >> 1) & 1) || *(volatile uint32_t *)err)) {
+        atomicExch(err, 1u);
+        dead = true;
+      }
+      if (__any_sync(0xffffffffu, dead)) {
+        dead = true;
+        continue;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int hcols = bn / 2;  // this warp's columns
+      const uint32_t t0 = lane_addr + (uint32_t)(acc * kTileN + half * hcols);
+      const int row0 = u.m * kTileM + (int)rank * 128 + q * 32;
+      auto release = [&]() {  // the accumulator has been read: hand it back
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) remote_arrive(leader_addr(&tempty[acc]));
+      };
+      if (MODE == kStats) {
+#pragma unroll 1
+        for (int c = 0; c < hcols; c += 32) {
+          float v[32];
+          tmem_load32(t0 + c, v);
+          if (c + 32 == hcols) release();
+          const float4 *b4 = reinterpret_cast<const float4 *>(sb + half * hcols + c);
+          float top = run_m;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 b = b4[k];
+            v[4 * k] = fmaf(v[4 * k], kLog2e, b.x);
+            v[4 * k + 1] = fmaf(v[4 * k + 1], kLog2e, b.y);
+            v[4 * k + 2] = fmaf(v[4 * k + 2], kLog2e, b.z);
+            v[4 * k + 3] = fmaf(v[4 * k + 3], kLog2e, b.w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, v[4 * k + i]);
+          }
+          const float ref = top == -INFINITY ? 0.f : top;  // nothing but -Inf so far
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            s0 += exp2_fast(v[k] - ref);
+            s1 += exp2_fast(v[k + 1] - ref);
+          }
+          run_s = run_s * exp2_fast(run_m - ref) + (s0 + s1);
+          run_m = top;
+        }
+      } else if (MODE == kPiece) {
+        const int n0 = u.n * kTileN + half * hcols;
+#pragma unroll 1
+        for (int c = 0; c < hcols; c += 64) {
+          float v[2][32];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            tmem_load32(t0 + c + 32 * h, v[h]);
+            const float4 *b4 = reinterpret_cast<const float4 *>(sb + half * hcols + c + 32 * h);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float4 b = b4[k];
+              v[h][4 * k] = exp2_fast(fmaf(v[h][4 * k], kLog2e, b.x - lse2));
+              v[h][4 * k + 1] = exp2_fast(fmaf(v[h][4 * k + 1], kLog2e, b.y - lse2));
+              v[h][4 * k + 2] = exp2_fast(fmaf(v[h][4 * k + 2], kLog2e, b.z - lse2));
+              v[h][4 * k + 3] = exp2_fast(fmaf(v[h][4 * k + 3], kLog2e, b.w - lse2));
+            }
+          }
+          if (c + 64 == hcols) release();
+          const int at = tgt - (a.v0 + n0 + c);  // the target's column among these 64
+          if (__any_sync(0xffffffffu, at >= 0 && at < 64)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (32 * h + k == at) v[h][k] -= 1.f;
+          }
+          if constexpr (sizeof(T) == 2) {
+            if (a.g_scale != 1.f) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int k = 0; k < 32; ++k) v[h][k] *= a.g_scale;
+            }
+            unsigned char *bx = box.take(lane);
+            box_put16<T>(bx, lane, 0, v[0]);
+            box_put16<T>(bx, lane, 1, v[1]);
+            box.send(lane, &maps.c, bx, n0 + c, row0, 0, false);
+          } else {
+            for (int p = 0; p < 3; ++p) {
+              unsigned char *bx = box.take(lane);
+              box_put16<__nv_bfloat16>(bx, lane, 0, v[0]);
+              box_put16<__nv_bfloat16>(bx, lane, 1, v[1]);
+              box.send(lane, &maps.c, bx, n0 + c, row0, p, false);
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int k = 0; k < 32; ++k) v[h][k] -= __bfloat162float(__float2bfloat16_rn(v[h][k]));
+            }
+          }
+        }
+      } else {
+        const int n0 = u.n * bn + half * hcols;
+#pragma unroll 1
+        for (int c = 0; c < hcols; c += 64) {
+          float v[2][32];
+          tmem_load32(t0 + c, v[0]);
+          tmem_load32(t0 + c + 32, v[1]);
+          if (c + 64 == hcols) release();
+          const int col = n0 + c;
+          if (u.dw) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[h][k] *= scale;
+            const int vrow = a.v0 + row0;
+            if (!a.dw_tma) {
+              if (vrow + lane < a.vocab) {
+                T *o = static_cast<T *>(a.dw) + (long)(vrow + lane) * a.dw_ld;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                  for (int k = 0; k < 32; ++k)
+                    if (col + 32 * h + k < a.dim) o[col + 32 * h + k] = op_store<T>(v[h][k]);
+              }
+            } else if constexpr (sizeof(T) == 2) {
+              if (col < a.dim && vrow < a.vocab) {
+                unsigned char *bx = box.take(lane);
+                box_put16<T>(bx, lane, 0, v[0]);
+                box_put16<T>(bx, lane, 1, v[1]);
+                box.send(lane, &maps.c2, bx, col, vrow, 0, false);
+              }
+            } else {
+              for (int h = 0; h < 2; ++h) {
+                if (col + 32 * h >= a.dim || vrow >= a.vocab) continue;
+                unsigned char *bx = box.take(lane);
+                box_put32(bx, lane, h ? v[1] : v[0]);
+                box.send(lane, &maps.c2, bx, col + 32 * h, vrow, 0, false);
+              }
+            }
+          } else {
+            for (int h = 0; h < 2; ++h) {
+              if (col + 32 * h >= a.dim) continue;
+              unsigned char *bx = box.take(lane);
+              box_put32(bx, lane, h ? v[1] : v[0]);
+              box.send(lane, &maps.c, bx, col + 32 * h, row0, u.z, !a.first);
+            }
+          }
+        }
+      }
+    }
+    if (MODE == kStats) flush();
+    if (lane == 0) bulk_wait<0>();  // stores complete before the shared memory goes away
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (tid == 0 && *(volatile uint32_t *)err) atomicCAS(&g_ce_timeout, 0u, 1u);
+  __syncwarp();
+  cluster_barrier();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * kTileN));
+  cluster_barrier();
+}
+
+// ---- staging ----------------------------------------------------------------
+__device__ __forceinline__ bool counted(int32_t t, int vocab) { return t >= 0 && t < vocab; }
+
+// Position of every counted row among them (-1: not counted), and their number.
+// One CTA: 8 targets per thread and turn.
+__global__ void __launch_bounds__(1024) ce_index_kernel(const int32_t *__restrict__ tg, long n, int vocab,
+                                                        int32_t *slot, int *count) {
+  __shared__ int wsum[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  for (long i0 = 0; i0 < n; i0 += 8192) {
+    const long i = i0 + threadIdx.x * 8;
+    int flag[8], mine = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      flag[k] = i + k < n && counted(tg[i + k], vocab);
+      mine += flag[k];
+    }
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) before += wsum[w];
+      all += wsum[w];
+    }
+    int at = base + before + x - mine;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (i + k < n) slot[i + k] = flag[k] ? at : -1;
+      at += flag[k];
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = base;
+}
+
+// Splits v into bfloat16 pieces (one piece: itself rounded, exact for 16-bit input).
+template <typename T>
+__device__ __forceinline__ void put_pieces(uint16_t *dst, size_t plane, float v) {
+  if constexpr (sizeof(T) == 2) {
+    reinterpret_cast<T *>(dst)[0] = op_store<T>(v);
+  } else {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const __nv_bfloat16 b = __float2bfloat16_rn(v);
+      reinterpret_cast<__nv_bfloat16 *>(dst)[p * plane] = b;
+      v -= __bfloat162float(b);
+    }
   }
 }
 
-__global__ void ce_rows_kernel(const CeArgs a, const float2 *part, int slices, const float *picked, float *row_loss,
-                               float *lse) {
-  const int n = blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= a.rows) return;
-  float l = 0.f, z = 0.f;
-  if (counted(a.tg[n], a.vocab)) {
-    float m = -INFINITY, s = 0.f;
-    for (int k = 0; k < slices; ++k) merge(m, s, part[(size_t)k * a.rows + n].x, part[(size_t)k * a.rows + n].y);
-    l = m + logf(s);
-    z = picked[n];
+// x rows to their slots, zeros behind the last up to a whole tile (one at least); with lse the
+// compacted targets and base-2 lse.  One warp per row.
+template <typename T>
+__global__ void ce_stage_rows_kernel(const T *__restrict__ x, long x_ld, const int32_t *__restrict__ tg,
+                                     const int32_t *__restrict__ slot, const int *__restrict__ count, long rows, int dim,
+                                     int pitch, size_t plane, uint16_t *xc, const float *__restrict__ lse, float *lse2,
+                                     int32_t *tgt) {
+  const int lane = threadIdx.x & 31;
+  const long n = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (n < rows) {
+    const int at = slot[n];
+    if (at < 0) return;
+    uint16_t *o = xc + (size_t)at * pitch;
+    for (int c = lane; c < dim; c += 32) put_pieces<T>(o + c, plane, op_load<T>(x[n * x_ld + c]));
+    if (lse && lane == 0) {
+      lse2[at] = lse[n] * kLog2e;
+      tgt[at] = tg[n];
+    }
+  } else {
+    const int c0 = *count;
+    const long at = c0 + (n - rows);
+    if (at >= max(1, (c0 + kTileM - 1) / kTileM) * kTileM) return;
+    uint16_t *o = xc + (size_t)at * pitch;
+    for (int c = lane; c < dim; c += 32) put_pieces<T>(o + c, plane, 0.f);
   }
-  row_loss[n] = l - z;
-  if (lse) lse[n] = l;
 }
 
-// loss = sum of the rows (fixed order), and the number of counted rows.
-__global__ void __launch_bounds__(1024) ce_loss_kernel(const CeArgs a, const float *row_loss, int mean, float *loss,
-                                                       float *count) {
+// W (any stride and alignment) as 16-bit operands.
+template <typename T>
+__global__ void ce_stage_w_kernel(const T *__restrict__ w, long w_ld, long vocab, int dim, int pitch, size_t plane,
+                                  uint16_t *wc) {
+  const int lane = threadIdx.x & 31;
+  const long v = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (v >= vocab) return;
+  uint16_t *o = wc + (size_t)v * pitch;
+  for (int c = lane; c < dim; c += 32) put_pieces<T>(o + c, plane, op_load<T>(w[v * w_ld + c]));
+}
+
+// ---- joins -------------------------------------------------------------------
+__device__ __forceinline__ void merge2(float &m, float &s, float m2, float s2) {
+  const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
+  s = s * exp2f(m - ref) + s2 * exp2f(m2 - ref);
+  m = top;
+}
+
+// One warp per row: the pairs' partial statistics of its tile, and its target's logit.
+template <typename T>
+__global__ void ce_rows_kernel(const T *__restrict__ x, long x_ld, const T *__restrict__ w, long w_ld,
+                               const T *__restrict__ bias, const int32_t *__restrict__ tg,
+                               const int32_t *__restrict__ slot, const int *__restrict__ count, long rows, int dim,
+                               int tiles_n, int pairs, const float2 *__restrict__ stats, float *row_loss, float *lse) {
+  const int lane = threadIdx.x & 31;
+  const long n = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (n >= rows) return;
+  const int at = slot[n];
+  if (at < 0) {
+    if (lane == 0) {
+      row_loss[n] = 0.f;
+      if (lse) lse[n] = 0.f;
+    }
+    return;
+  }
+  const long t = tg[n];
+  float dot = 0.f;
+  for (int c = lane; c < dim; c += 32) dot = fmaf(op_load<T>(x[n * x_ld + c]), op_load<T>(w[t * w_ld + c]), dot);
+  dot = warp_sum(dot);
+  // pairs that worked on this row tile (see Units): pair of tile i = ((i + 1) pairs - 1) / total
+  const long m = at / kTileM, total = (long)((*count + kTileM - 1) / kTileM) * tiles_n;
+  const long p0 = ((m * tiles_n + 1) * pairs - 1) / total, p1 = ((m + 1) * tiles_n * pairs - 1) / total;
+  float top = -INFINITY, sum = 0.f;
+  for (long i = lane; i < 2 * (p1 - p0 + 1); i += 32) {
+    const long p = p0 + i / 2;
+    if (p * total / pairs == (p + 1) * total / pairs) continue;  // fewer tiles than pairs: this one had none
+    const float2 v = stats[((size_t)(p + m) * 2 + i % 2) * kTileM + at % kTileM];
+    merge2(top, sum, v.x, v.y);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, top, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
+    merge2(top, sum, m2, s2);
+  }
+  if (lane == 0) {
+    const float l = (top + log2f(sum)) * kLn2;
+    if (lse) lse[n] = l;
+    row_loss[n] = l - (dot + (bias ? op_load<T>(bias[t]) : 0.f));
+  }
+}
+
+// loss: the rows' sum in a fixed order.
+__global__ void __launch_bounds__(1024) ce_loss_kernel(const float *__restrict__ row_loss, long rows,
+                                                       const int *__restrict__ count, int mean, float *loss) {
   __shared__ float red[2 * 8 * 32];
   BlockReducer br(red);
-  float v[2] = {0.f, 0.f};
-  for (int n = threadIdx.x; n < a.rows; n += 1024) {
-    if (row_loss) v[0] += row_loss[n];
-    v[1] += counted(a.tg[n], a.vocab) ? 1.f : 0.f;
-  }
-  br.sum<2>(v);
-  if (threadIdx.x == 0) {
-    if (loss) *loss = mean ? v[0] / fmaxf(v[1], 1.f) : v[0];
-    if (count) *count = v[1];
-  }
+  float v[1] = {0.f};
+  for (long n = threadIdx.x; n < rows; n += 1024) v[0] += row_loss[n];
+  br.sum<1>(v);
+  if (threadIdx.x == 0) *loss = mean ? v[0] / fmaxf((float)*count, 1.f) : v[0];
 }
 
+// dx: the splits' slabs added in order, scaled, back to the rows' places.
 template <typename T>
-__global__ void __launch_bounds__(256) ce_piece_kernel(const CeArgs a, int v0, float *G) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const int m0 = blockIdx.x * kTile, n0 = v0 + blockIdx.y * kTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4];
-  logits_tile<T>(a, m0, n0, acc, sa, sb);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = m0 + 4 * ty + i;
-    if (row >= a.rows) continue;
-    const int t = a.tg[row];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = n0 + 4 * tx + j;
-      float g = 0.f;
-      if (counted(t, a.vocab) && col < a.vocab) g = expf(acc[i][j] - a.lse[row]) - (col == t ? 1.f : 0.f);
-      if (col - v0 < kPiece) G[(size_t)row * kPiece + col - v0] = g;
-    }
+__global__ void ce_dx_kernel(const float *__restrict__ slab, size_t slab_stride, int splits, int pitch,
+                             const int32_t *__restrict__ slot, long rows, int dim, const float *__restrict__ dloss,
+                             const int *__restrict__ count, int mean, float inv_g, T *dx, long dx_ld) {
+  const int lane = threadIdx.x & 31;
+  const long n = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (n >= rows) return;
+  const int at = slot[n];
+  const float c = grad_scale(dloss, count, mean) * inv_g;
+  for (int i = lane; i < dim; i += 32) {
+    float s = 0.f;
+    if (at >= 0)
+      for (int k = 0; k < splits; ++k) s += slab[k * slab_stride + (size_t)at * pitch + i];
+    dx[n * dx_ld + i] = op_store<T>(c * s);
   }
 }
 
-// dx += G W over this piece.
+// db of a piece: column sums of G, 64 columns per CTA, the warps' sums added in order.
 template <typename T>
-__global__ void __launch_bounds__(256) ce_dx_kernel(const CeArgs a, int v0, const float *G, float *dx, int first) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const int m0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const T *w = static_cast<const T *>(a.w);
-  const int K = min(kPiece, a.vocab - v0);
-  float acc[4][4];
-  tile_product([&](int m, int k) { return m0 + m < a.rows ? G[(size_t)(m0 + m) * kPiece + k] : 0.f; },
-               [&](int n, int k) { return n0 + n < a.dim ? op_load<T>(w[(long)(v0 + k) * a.w_ld + n0 + n]) : 0.f; },
-               K, acc, sa, sb);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = m0 + 4 * ty + i, col = n0 + 4 * tx + j;
-      if (row >= a.rows || col >= a.dim) continue;
-      float *p = dx + (size_t)row * a.dim + col;
-      *p = first ? acc[i][j] : *p + acc[i][j];
+__global__ void __launch_bounds__(1024) ce_db_kernel(const uint16_t *__restrict__ G, long pitch, size_t plane, int planes,
+                                                     const int *__restrict__ count, int v0, int vocab,
+                                                     const float *__restrict__ dloss, int mean, float inv_g, T *db) {
+  __shared__ float sh[32][65];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = *count;
+  float s0 = 0.f, s1 = 0.f;
+  using G2 = OpVec<uint16_t, 2>;
+  for (int p = planes - 1; p >= 0; --p) {
+#pragma unroll 8
+    for (int n = warp; n < rows; n += 32) {
+      const G2 g = *reinterpret_cast<const G2 *>(G + p * plane + (size_t)n * pitch + blockIdx.x * 64 + 2 * lane);
+      if constexpr (sizeof(T) == 2) {
+        s0 += op_load<T>(reinterpret_cast<const T &>(g.v[0]));
+        s1 += op_load<T>(reinterpret_cast<const T &>(g.v[1]));
+      } else {
+        s0 += __bfloat162float(reinterpret_cast<const __nv_bfloat16 &>(g.v[0]));
+        s1 += __bfloat162float(reinterpret_cast<const __nv_bfloat16 &>(g.v[1]));
+      }
     }
+  }
+  sh[warp][2 * lane] = s0;
+  sh[warp][2 * lane + 1] = s1;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int v = v0 + blockIdx.x * 64 + threadIdx.x;
+    if (v >= vocab) return;
+    float s = 0.f;
+    for (int w = 0; w < 32; ++w) s += sh[w][threadIdx.x];
+    db[v] = op_store<T>(grad_scale(dloss, count, mean) * inv_g * s);
+  }
 }
 
-__device__ __forceinline__ float ce_scale(const float *dloss, const float *count, int mean) {
-  return (dloss ? *dloss : 1.f) / (mean ? fmaxf(*count, 1.f) : 1.f);
-}
-
-template <typename T>
-__global__ void ce_dx_store_kernel(const CeArgs a, const float *acc, const float *dloss, const float *count, int mean,
-                                   T *dx, long ld) {
-  const float c = ce_scale(dloss, count, mean);
-  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < (size_t)a.rows * a.dim;
-       i += (size_t)gridDim.x * blockDim.x)
-    dx[(long)(i / a.dim) * ld + i % a.dim] = counted(a.tg[i / a.dim], a.vocab) ? op_store<T>(c * acc[i]) : op_store<T>(0.f);
-}
-
-// dW and db of this piece.
-template <typename T>
-__global__ void __launch_bounds__(256) ce_dw_kernel(const CeArgs a, int v0, const float *G, const float *dloss,
-                                                    const float *count, int mean, T *dw, long ld) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const int m0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const T *x = static_cast<const T *>(a.x);
-  const int V = min(kPiece, a.vocab - v0);
-  float acc[4][4];
-  tile_product([&](int m, int k) { return m0 + m < V ? G[(size_t)k * kPiece + m0 + m] : 0.f; },
-               [&](int n, int k) {
-                 return n0 + n < a.dim && counted(a.tg[k], a.vocab) ? op_load<T>(x[(long)k * a.x_ld + n0 + n]) : 0.f;
-               },
-               a.rows, acc, sa, sb);
-  const float c = ce_scale(dloss, count, mean);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = m0 + 4 * ty + i, col = n0 + 4 * tx + j;
-      if (row < V && col < a.dim) dw[(long)(v0 + row) * ld + col] = op_store<T>(c * acc[i][j]);
-    }
-}
-template <typename T>
-__global__ void ce_db_kernel(const CeArgs a, int v0, const float *G, const float *dloss, const float *count, int mean,
-                             T *db) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= min(kPiece, a.vocab - v0)) return;
-  float s = 0.f;
-  for (int n = 0; n < a.rows; ++n) s += G[(size_t)n * kPiece + c];
-  db[v0 + c] = op_store<T>(ce_scale(dloss, count, mean) * s);
-}
-
+// ---- host --------------------------------------------------------------------
 int check_args(const aideen_linear_ce_args *a) {
   OP_CHECK(a, "linear_ce: null args");
   OP_CHECK(a->dtype <= AIDEEN_F16, "linear_ce: unknown dtype");
@@ -247,57 +836,216 @@ int check_args(const aideen_linear_ce_args *a) {
   return AIDEEN_OK;
 }
 
+// Everything a call lays out.  The row count on the device is only known there,
+// so sizes follow from all rows.
 struct Plan {
-  float2 *part;
-  float *picked, *row_loss, *count, *G, *dx;
+  int planes, pairs, tiles_m, tiles_n, pitch;
+  long mpad;
+  bool w_direct;       // TMA reads the caller's W
+  size_t xplane, wplane;
+  // loss
+  int32_t *slot;
+  int *count;
+  uint16_t *xc, *wc;
+  float2 *stats;
+  float *row_loss;
+  // gradient
+  float *lse2, *slab;
+  int32_t *tgt;
+  uint16_t *G;
+  int piece;           // columns of a piece, a multiple of 256
+  int splits, bn, tiles_d;
+  long dpitch;
   size_t loss_bytes, grad_bytes;
 };
+
+// Columns of G held at a time: about 96 MB of it, which the L2 cache nearly
+// holds, but at least 2048 columns (a product with G needs depth), and whole
+// equal pieces.
+int piece_columns(long mpad, int planes, int tiles_n) {
+  long most = (96L << 20) / (mpad * 2 * planes) / kTileN;
+  if (most < 8) most = 8;
+  if (most >= tiles_n) return tiles_n * kTileN;
+  const long n = (tiles_n + most - 1) / most;
+  return (int)((tiles_n + n - 1) / n) * kTileN;
+}
+
 Plan make_plan(const aideen_linear_ce_args *a, void *ws) {
   Plan p{};
+  p.planes = a->dtype == AIDEEN_F32 ? 3 : 1;
+  p.pairs = op_sm_count() / 2;
+  p.tiles_m = (int)((a->rows + kTileM - 1) / kTileM);
+  p.tiles_n = (int)((a->vocab + kTileN - 1) / kTileN);
+  p.pitch = (int)op_round(a->dim, 8);
+  p.mpad = (long)p.tiles_m * kTileM;
+  p.w_direct = p.planes == 1 && a->w_ld % 8 == 0;
+  p.xplane = (size_t)p.mpad * p.pitch;
+  p.wplane = (size_t)a->vocab * p.pitch;
   OpCarve c(ws);
-  p.part = c.take<float2>((size_t)a->rows * kSlices);
-  p.picked = c.take<float>(a->rows);
+  p.slot = c.take<int32_t>(a->rows);
+  p.count = c.take<int>(1);
+  p.xc = c.take<uint16_t>(p.xplane * p.planes);
+  p.wc = c.take<uint16_t>(p.w_direct ? 0 : p.wplane * p.planes);
+  OpCarve g = c;
+  p.stats = c.take<float2>((size_t)(p.pairs + p.tiles_m) * 2 * kTileM);
   p.row_loss = c.take<float>(a->rows);
   p.loss_bytes = c.used;
-  OpCarve g(ws);
-  p.count = g.take<float>(1);
-  p.G = g.take<float>((size_t)a->rows * kPiece);
-  p.dx = g.take<float>((size_t)a->rows * a->dim);
+  p.piece = p.tiles_m ? piece_columns(p.mpad, p.planes, p.tiles_n) : kTileN;
+  p.bn = (a->dim + 127) / 128 % 2 ? 128 : 256;  // fewer padded columns
+  p.tiles_d = (int)((a->dim + p.bn - 1) / p.bn);
+  // splits of dx over the piece: enough tiles for every pair, none below 16 slices
+  const long tiles = (long)p.tiles_m * p.tiles_d, ktot = p.piece / kBlockK;
+  p.splits = 1;
+  while (tiles * (p.splits + 1) <= p.pairs && ktot / (p.splits + 1) >= 16) ++p.splits;
+  p.dpitch = (long)op_round(a->dim, 4);
+  p.lse2 = g.take<float>(a->rows);
+  p.tgt = g.take<int32_t>(a->rows);
+  p.G = g.take<uint16_t>((size_t)p.mpad * p.piece * p.planes);
+  p.slab = g.take<float>((size_t)p.splits * p.mpad * p.dpitch);
   p.grad_bytes = g.used;
   return p;
 }
 
-CeArgs ce_args(const aideen_linear_ce_args *g, const void *x, const void *w, const void *b, const int32_t *tg) {
-  CeArgs a{};
-  a.x = x; a.w = w; a.b = b; a.tg = tg; a.x_ld = g->x_ld; a.w_ld = g->w_ld;
-  a.rows = (int)g->rows; a.dim = (int)g->dim; a.vocab = (int)g->vocab;
+// Tensor map of a matrix (or its planes); strides in bytes.
+bool make_map(CUtensorMap *m, CUtensorMapDataType type, const void *base, size_t e0, size_t e1, size_t e2, size_t s1,
+              size_t s2, uint32_t b0, uint32_t b1) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {e0, e1, e2};
+  const cuuint64_t strides[2] = {s1, s2};
+  const cuuint32_t box[3] = {b0, b1, 1};
+  const cuuint32_t step[3] = {1, 1, 1};
+  return fn(m, type, 3, const_cast<void *>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+constexpr auto kU16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
+constexpr auto kF32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+
+// x and W as operands, in boxes of 64 columns by `rows` rows.
+bool map_x(CUtensorMap *m, const Plan &p, int dim, uint32_t rows) {
+  return make_map(m, kU16, p.xc, dim, p.mpad, p.planes, (size_t)p.pitch * 2, p.xplane * 2, 64, rows);
+}
+bool map_w(CUtensorMap *m, const Plan &p, const aideen_linear_ce_args *g, const void *w, uint32_t rows) {
+  if (p.w_direct)
+    return make_map(m, kU16, w, g->dim, g->vocab, 1, (size_t)g->w_ld * 2, (size_t)g->w_ld * 2 * g->vocab, 64, rows);
+  return make_map(m, kU16, p.wc, g->dim, g->vocab, p.planes, (size_t)p.pitch * 2, p.wplane * 2, 64, rows);
+}
+
+template <int MODE, typename T>
+cudaError_t launch_mma(const Plan &p, const Maps &maps, const MmaArgs &a, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(ce_mma_kernel<MODE, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+  if (e != cudaSuccess) return e;
+  ce_mma_kernel<MODE, T><<<2 * p.pairs, kThreads, kSmemBytes, st>>>(maps, a);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t stage_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, const T *w, const int32_t *tg,
+                      const float *lse, cudaStream_t st) {
+  ce_index_kernel<<<1, 1024, 0, st>>>(tg, g->rows, (int)g->vocab, p.slot, p.count);
+  ce_stage_rows_kernel<T><<<(unsigned)((g->rows + kTileM + 7) / 8), 256, 0, st>>>(
+      x, g->x_ld, tg, p.slot, p.count, g->rows, (int)g->dim, p.pitch, p.xplane, p.xc, lse, p.lse2, p.tgt);
+  if (!p.w_direct)
+    ce_stage_w_kernel<T><<<(unsigned)((g->vocab + 7) / 8), 256, 0, st>>>(w, g->w_ld, g->vocab, (int)g->dim, p.pitch,
+                                                                        p.wplane, p.wc);
+  return cudaGetLastError();
+}
+
+template <typename T>
+MmaArgs mma_args(const aideen_linear_ce_args *g, const Plan &p, const T *bias) {
+  MmaArgs a{};
+  a.count = p.count;
+  a.vocab = (int)g->vocab; a.dim = (int)g->dim; a.planes = p.planes; a.dtype = g->dtype;
+  const uint32_t type = g->dtype == AIDEEN_F16 ? 0u : 1u;  // f16 or bf16 operands, f32 accumulator
+  a.idesc = (1u << 4) | (type << 7) | (type << 10);
+  a.bias = bias;
+  a.g_scale = g->dtype == AIDEEN_F16 ? kHalfScale : 1.f;
+  a.mean = g->reduction == AIDEEN_CE_MEAN;
   return a;
 }
 
 template <typename T>
-cudaError_t loss_run(const CeArgs &a, const Plan &p, int mean, float *loss, float *row_loss, float *lse, cudaStream_t st) {
+cudaError_t loss_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, const T *w, const T *bias,
+                     const int32_t *tg, float *loss, float *row_loss, float *lse, cudaStream_t st) {
+  cudaError_t e = stage_run<T>(g, p, x, w, tg, nullptr, st);
+  if (e != cudaSuccess) return e;
+  Maps maps{};
+  if (!map_x(&maps.a, p, (int)g->dim, 128) || !map_w(&maps.b, p, g, w, 128)) return cudaErrorInvalidValue;
+  MmaArgs a = mma_args<T>(g, p, bias);
+  a.tiles_n = p.tiles_n;
+  a.stats = p.stats;
+  e = launch_mma<kStats, T>(p, maps, a, st);
+  if (e != cudaSuccess) return e;
   float *rl = row_loss ? row_loss : p.row_loss;
-  const int tiles = (a.vocab + kTile - 1) / kTile, slices = tiles < kSlices ? tiles : kSlices;
-  ce_stats_kernel<T><<<dim3((a.rows + kTile - 1) / kTile, slices), 256, 0, st>>>(a, p.part, p.picked);
-  ce_rows_kernel<<<(a.rows + 255) / 256, 256, 0, st>>>(a, p.part, slices, p.picked, rl, lse);
-  if (loss) ce_loss_kernel<<<1, 1024, 0, st>>>(a, rl, mean, loss, nullptr);
+  ce_rows_kernel<T><<<(unsigned)((g->rows + 7) / 8), 256, 0, st>>>(x, g->x_ld, w, g->w_ld, bias, tg, p.slot, p.count,
+                                                                   g->rows, (int)g->dim, p.tiles_n, p.pairs, p.stats,
+                                                                   rl, lse);
+  if (loss) ce_loss_kernel<<<1, 1024, 0, st>>>(rl, g->rows, p.count, a.mean, loss);
   return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t grad_run(const CeArgs &a, const Plan &p, int mean, const float *dloss, T *dx, long dx_ld, T *dw, long dw_ld,
-                     T *db, cudaStream_t st) {
-  ce_loss_kernel<<<1, 1024, 0, st>>>(a, nullptr, mean, nullptr, p.count);
-  const int mt = (a.rows + kTile - 1) / kTile, dt = (a.dim + kTile - 1) / kTile;
-  for (int v0 = 0; v0 < a.vocab; v0 += kPiece) {
-    const int V = a.vocab - v0 < kPiece ? a.vocab - v0 : kPiece, vt = (V + kTile - 1) / kTile;
-    ce_piece_kernel<T><<<dim3(mt, vt), 256, 0, st>>>(a, v0, p.G);
-    if (dx) ce_dx_kernel<T><<<dim3(mt, dt), 256, 0, st>>>(a, v0, p.G, p.dx, v0 == 0);
-    if (dw) ce_dw_kernel<T><<<dim3(vt, dt), 256, 0, st>>>(a, v0, p.G, dloss, p.count, mean, dw, dw_ld);
-    if (db) ce_db_kernel<T><<<(V + 255) / 256, 256, 0, st>>>(a, v0, p.G, dloss, p.count, mean, db);
+cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, const T *w, const T *bias,
+                     const int32_t *tg, const float *lse, const float *dloss, T *dx, T *dw, T *db, cudaStream_t st) {
+  cudaError_t e = stage_run<T>(g, p, x, w, tg, lse, st);
+  if (e != cudaSuccess) return e;
+  const int dim = (int)g->dim;
+  const size_t gplane = (size_t)p.mpad * p.piece;
+  Maps lm{}, pm{};
+  bool ok = map_x(&lm.a, p, dim, 128) && map_w(&lm.b, p, g, w, 128) &&
+            make_map(&lm.c, kU16, p.G, p.piece, p.mpad, p.planes, (size_t)p.piece * 2, gplane * 2, 64, 32);
+  ok = ok && make_map(&pm.a, kU16, p.G, p.piece, p.mpad, p.planes, (size_t)p.piece * 2, gplane * 2, 64, 128) &&
+       map_w(&pm.b, p, g, w, 64) &&
+       make_map(&pm.a2, kU16, p.G, p.piece, p.mpad, p.planes, (size_t)p.piece * 2, gplane * 2, 64, 64) &&
+       map_x(&pm.b2, p, dim, 64) &&
+       make_map(&pm.c, kF32, p.slab, dim, p.mpad, p.splits, p.dpitch * 4, p.mpad * p.dpitch * 4, 32, 32);
+  const size_t el = sizeof(T);
+  const bool dw_tma = dw && op_vec16(dw, g->dw_ld, el);
+  if (dw_tma)
+    ok = ok && make_map(&pm.c2, el == 4 ? kF32 : kU16, dw, dim, g->vocab, 1, g->dw_ld * el,
+                        (size_t)g->dw_ld * el * g->vocab, 128 / el, 32);
+  if (!ok) return cudaErrorInvalidValue;
+  MmaArgs a = mma_args<T>(g, p, bias);
+  a.lse2 = p.lse2; a.tgt = p.tgt;
+  a.bn = p.bn; a.tiles_d = p.tiles_d; a.splits = dx ? p.splits : 0;
+  a.dw = dw; a.dw_ld = g->dw_ld; a.dw_tma = dw_tma; a.dloss = dloss;
+  for (int v0 = 0; v0 < (int)g->vocab; v0 += p.piece) {
+    const int left = (int)g->vocab - v0, cols = left < p.piece ? (left + kTileN - 1) / kTileN * kTileN : p.piece;
+    a.v0 = v0;
+    a.tiles_n = cols / kTileN;
+    e = launch_mma<kPiece, T>(p, lm, a, st);
+    if (e != cudaSuccess) return e;
+    if (dx || dw) {
+      a.piece_k = cols / kBlockK;
+      a.tiles_v = dw ? cols / kTileM : 0;
+      a.first = v0 == 0;
+      e = launch_mma<kProducts, T>(p, pm, a, st);
+      if (e != cudaSuccess) return e;
+    }
+    if (db)
+      ce_db_kernel<T><<<cols / 64, 1024, 0, st>>>(p.G, p.piece, gplane, p.planes, p.count, v0, (int)g->vocab, dloss,
+                                                  a.mean, 1.f / a.g_scale, db);
   }
-  if (dx) ce_dx_store_kernel<T><<<op_sm_count() * 4, 256, 0, st>>>(a, p.dx, dloss, p.count, mean, dx, dx_ld);
+  if (dx)
+    ce_dx_kernel<T><<<(unsigned)((g->rows + 7) / 8), 256, 0, st>>>(p.slab, (size_t)p.mpad * p.dpitch, p.splits,
+                                                                   (int)p.dpitch, p.slot, g->rows, dim, dloss, p.count,
+                                                                   a.mean, 1.f / a.g_scale, dx, g->dx_ld);
   return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t loss_typed(const aideen_linear_ce_args *g, const Plan &p, const void *x, const void *w, const void *bias,
+                       const int32_t *tg, float *loss, float *row_loss, float *lse, cudaStream_t st) {
+  return loss_run<T>(g, p, static_cast<const T *>(x), static_cast<const T *>(w), static_cast<const T *>(bias), tg, loss,
+                     row_loss, lse, st);
+}
+template <typename T>
+cudaError_t grad_typed(const aideen_linear_ce_args *g, const Plan &p, const void *x, const void *w, const void *bias,
+                       const int32_t *tg, const float *lse, const float *dloss, void *dx, void *dw, void *db,
+                       cudaStream_t st) {
+  return grad_run<T>(g, p, static_cast<const T *>(x), static_cast<const T *>(w), static_cast<const T *>(bias), tg, lse,
+                     dloss, static_cast<T *>(dx), static_cast<T *>(dw), static_cast<T *>(db), st);
 }
 
 }  // namespace
@@ -336,13 +1084,13 @@ extern "C" int aideen_linear_ce(const aideen_linear_ce_args *args, const void *x
   OP_CHECK(loss || row_loss || lse, "linear_ce: no output wanted");
   OP_CHECK(x && w && targets, "linear_ce: null x, w or targets");
   const Plan p = make_plan(args, workspace);
+  OP_CHECK(!p.w_direct || op_aligned(w, 16), "linear_ce: w must be 16-byte aligned at this type and row stride");
   OP_CHECK(workspace && op_aligned(workspace, 256) && workspace_bytes >= p.loss_bytes,
            "linear_ce: workspace missing, misaligned or too small");
-  const CeArgs a = ce_args(args, x, w, bias, targets);
-  const int mean = args->reduction == AIDEEN_CE_MEAN;
-  if (args->dtype == AIDEEN_F32) return op_cuda(loss_run<float>(a, p, mean, loss, row_loss, lse, st));
-  if (args->dtype == AIDEEN_BF16) return op_cuda(loss_run<__nv_bfloat16>(a, p, mean, loss, row_loss, lse, st));
-  return op_cuda(loss_run<__half>(a, p, mean, loss, row_loss, lse, st));
+  if (args->dtype == AIDEEN_F32) return op_cuda(loss_typed<float>(args, p, x, w, bias, targets, loss, row_loss, lse, st));
+  if (args->dtype == AIDEEN_BF16)
+    return op_cuda(loss_typed<__nv_bfloat16>(args, p, x, w, bias, targets, loss, row_loss, lse, st));
+  return op_cuda(loss_typed<__half>(args, p, x, w, bias, targets, loss, row_loss, lse, st));
 }
 
 extern "C" int aideen_linear_ce_grad(const aideen_linear_ce_args *args, const void *x, const void *w, const void *bias,
@@ -367,18 +1115,12 @@ extern "C" int aideen_linear_ce_grad(const aideen_linear_ce_args *args, const vo
   OP_CHECK(dx || dw || dbias, "linear_ce_grad: no output wanted");
   OP_CHECK(x && w && targets && lse, "linear_ce_grad: null x, w, targets or lse");
   const Plan p = make_plan(args, workspace);
+  OP_CHECK(!p.w_direct || op_aligned(w, 16), "linear_ce_grad: w must be 16-byte aligned at this type and row stride");
   OP_CHECK(workspace && op_aligned(workspace, 256) && workspace_bytes >= p.grad_bytes,
            "linear_ce_grad: workspace missing, misaligned or too small");
-  CeArgs a = ce_args(args, x, w, bias, targets);
-  a.lse = lse;
-  const int mean = args->reduction == AIDEEN_CE_MEAN;
   if (args->dtype == AIDEEN_F32)
-    return op_cuda(grad_run<float>(a, p, mean, dloss, static_cast<float *>(dx), args->dx_ld, static_cast<float *>(dw),
-                                   args->dw_ld, static_cast<float *>(dbias), st));
+    return op_cuda(grad_typed<float>(args, p, x, w, bias, targets, lse, dloss, dx, dw, dbias, st));
   if (args->dtype == AIDEEN_BF16)
-    return op_cuda(grad_run<__nv_bfloat16>(a, p, mean, dloss, static_cast<__nv_bfloat16 *>(dx), args->dx_ld,
-                                           static_cast<__nv_bfloat16 *>(dw), args->dw_ld,
-                                           static_cast<__nv_bfloat16 *>(dbias), st));
-  return op_cuda(grad_run<__half>(a, p, mean, dloss, static_cast<__half *>(dx), args->dx_ld, static_cast<__half *>(dw),
-                                  args->dw_ld, static_cast<__half *>(dbias), st));
+    return op_cuda(grad_typed<__nv_bfloat16>(args, p, x, w, bias, targets, lse, dloss, dx, dw, dbias, st));
+  return op_cuda(grad_typed<__half>(args, p, x, w, bias, targets, lse, dloss, dx, dw, dbias, st));
 }

@@ -214,8 +214,11 @@ def _ce_args(what, x, weight, targets, bias, reduction):
     if n == 0:
         xld = dim
     vocab, _, wld = _rows(weight, what, "weight")
+    if x.element_size() == 2 and wld % 8 == 0 and weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)  # the library reads it in place and needs 16 bytes
+        wld = dim
     bp = _vector(bias, what, "bias", vocab, x)
-    return LinearCeArgs(_DTYPES[x.dtype], n, dim, vocab, _REDUCTIONS[reduction], xld, wld, dim, dim), tp, bp
+    return LinearCeArgs(_DTYPES[x.dtype], n, dim, vocab, _REDUCTIONS[reduction], xld, wld, dim, dim), weight, tp, bp
 
 
 def linear_ce(x, weight, targets, bias=None, reduction: str = "mean"):
@@ -223,7 +226,7 @@ def linear_ce(x, weight, targets, bias=None, reduction: str = "mean"):
     against int32 targets; the logits are not kept.  Rows whose target lies
     outside [0, vocab) are not counted (row_loss and lse 0)."""
     what = "linear_ce"
-    a, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)
+    a, weight, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)
     lib, size = load_library(), C.c_size_t()
     with torch.cuda.device(x.device):
         _check(lib.aideen_linear_ce_workspace(C.byref(a), C.byref(size), None), what)
@@ -243,7 +246,7 @@ def linear_ce_grad(x, weight, targets, lse, bias=None, dloss=None, reduction: st
     `want` names the gradients to form; the others, and dbias without a bias,
     are None."""
     what = "linear_ce_grad"
-    a, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)
+    a, weight, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)
     lp = _vector(lse, what, "lse", a.rows, x, torch.float32)
     gp = _vector(dloss, what, "dloss", 1, x, torch.float32)
     lib, size = load_library(), C.c_size_t()

@@ -408,7 +408,9 @@ int aideen_layer_norm_grad(const aideen_layer_norm_args *args, const void *dy, c
 /* Softmax cross entropy of a linear head, without keeping the logits
  * z = x W^T + bias:  lse[n] = log sum_v exp z[n][v],  row_loss[n] = lse[n] -
  * z[n][targets[n]],  loss = sum of row_loss / (counted rows, at least 1), or the
- * plain sum.  A row whose target is outside [0, vocab) is not counted: its
+ * plain sum.  At 16 bits with w_ld a multiple of 8, w must be 16-byte aligned
+ * (TMA reads it in place; at any other stride, and in float32, it is first laid
+ * out in the workspace).  A row whose target is outside [0, vocab) is not counted: its
  * row_loss and lse are 0, and what its x holds reaches no result. */
 enum { AIDEEN_CE_MEAN = 0, AIDEEN_CE_SUM = 1 };
 typedef struct aideen_linear_ce_args {

@@ -391,6 +391,20 @@ def test_linear_ce_peaked_rows(dtype):
     ce_check(x, w, b, tg, dloss=64.0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_ce_at_odd_addresses(dtype):
+    """Views that start between 16-byte boundaries, with row strides that are and
+    are not multiples of 16 bytes."""
+    for pad in (1, 8):
+        x, w, b, tg = ce_inputs(14, 40, 63, 301, dtype, True, 0.1)
+        bx = torch.zeros(40, 63 + pad, dtype=dtype, device="cuda")
+        bw = torch.zeros(301, 63 + pad, dtype=dtype, device="cuda")
+        bx[:, 1:64], bw[:, 1:64] = x, w
+        bb = torch.zeros(302, dtype=dtype, device="cuda")
+        bb[1:] = b
+        ce_check(bx[:, 1:64], bw[:, 1:64], bb[1:], tg, dloss=16.0)
+
+
 def test_linear_ce_parts_alone():
     x, w, b, tg = ce_inputs(2, 70, 48, 333, BF16, True, 0.2)
     _, _, lse = K.linear_ce(x, w, tg, bias=b)

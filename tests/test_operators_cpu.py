@@ -114,6 +114,13 @@ def test_linear_ce_refuses_bad_pointers(lib):
     refused(lib, grad(C.byref(ce_args(dx_ld=7)), P, P, P, P, P, P, P, P, P, P, m.value, None), "stride")
 
 
+def test_linear_ce_refuses_a_16_bit_weight_that_tma_cannot_read(lib):
+    a, n, m = ce_args(dtype=1), C.c_size_t(), C.c_size_t()
+    assert lib.aideen_linear_ce_workspace(C.byref(a), C.byref(n), C.byref(m)) == OK
+    refused(lib, lib.aideen_linear_ce(C.byref(a), P, P + 8, P, P, P, P, P, P, n.value, None), "16-byte")
+    refused(lib, lib.aideen_linear_ce_grad(C.byref(a), P, P + 2, P, P, P, P, P, P, P, P, m.value, None), "16-byte")
+
+
 def test_workspaces_grow_with_the_sizes_and_stay_below_the_logits(lib):
     """The point of the pieces: at the training shard's size the gradient's
     workspace is a fraction of the float32 logits, and it stops growing with the
