@@ -60,15 +60,17 @@ struct MmaArgs {
   const void *bias;
   uint32_t dtype;     // of bias, dW
   float2 *stats;      // kStats: [slot][2][256] (maximum, sum) in base 2
-  const float *lse2;  // kPiece: compacted rows' lse in base 2
+  const float *lse;   // kPiece: compacted rows' lse
   const int32_t *tgt; // and their targets
+  float *db_part;     // [8 tiles_m][tiles_n * 256] column sums of 32 rows each, or null
   float g_scale;
   // kProducts
   int bn;             // columns of an output tile: 128 or 256
   int tiles_d;        // of dim
   int piece_k;        // 64-deep slices of the piece
-  int tiles_v;        // dW tiles of the piece (0: dW not wanted)
-  int splits;         // K splits of dx (0: dx not wanted)
+  int full_k;         // and of the first piece (the last may be shorter)
+  int want_dw;
+  int slabs;          // slabs of dx (0: dx not wanted)
   int first;          // first piece: dx slabs are written, not added to
   int dw_tma;         // dW can be stored by TMA
   void *dw;
@@ -174,70 +176,108 @@ struct Unit {
   int m, n;      // tile coordinates (rows of 256, columns of kTileN or bn)
   int kb0, nkb;  // 64-deep slices
   int dw;        // kProducts: 1 = dW tile, 0 = dx tile
-  int z;         // dx: split
+  int z;         // dx: slab
 };
 
+// How a piece's two products are dealt out over the pairs.  dW tiles go out whole
+// (tiles of the piece x tiles_d, each as deep as the rows): pairs below n_a
+// take w + 1 of them, the others w.  dx fills up what is missing to an equal
+// load: its slices, ordered by (tile, depth), are cut into one run per pair, a
+// slices for a pair below n_a and b for the others.  A tile that several pairs
+// work on takes one float32 slab from each, added in order at the end; a run is
+// never shorter than a tile's depth / (slabs - 1), so `slabs` are enough.
+struct Deal {
+  int w, n_a, depth;
+  long a, b, total, load;
+  __host__ __device__ Deal(long n_dw, long k_rows, long dx_tiles, int depth_, int slabs, int pairs) {
+    depth = depth_;
+    w = (int)(n_dw / pairs);
+    n_a = (int)(n_dw % pairs);
+    total = dx_tiles * depth;
+    const long least = slabs > 1 ? (depth + slabs - 2) / (slabs - 1) : depth;
+    load = (n_dw * k_rows + total + pairs - 1) / pairs;
+    a = n_a ? load - (w + 1) * k_rows : 0;
+    b = load - w * k_rows;
+    if (a < least) {
+      a = 0;
+      b = (total + pairs - n_a - 1) / (pairs - n_a);
+    }
+    if (b < least) b = least;
+    if (b < 1) b = 1;
+    const long la = n_a ? (w + 1) * k_rows + a : 0, lb = w * k_rows + (total ? b : 0);
+    load = la > lb ? la : lb;
+  }
+  __host__ __device__ long begin(int pair) const {
+    const long at = pair < n_a ? pair * a : n_a * a + (pair - n_a) * b;
+    return at < total ? at : total;
+  }
+  __device__ int owner(long slice) const {
+    return slice < n_a * a ? (int)(slice / a) : n_a + (int)((slice - n_a * a) / b);
+  }
+  // slabs that a tile takes
+  __device__ int cover(long tile) const { return owner((tile + 1) * depth - 1) - owner(tile * depth) + 1; }
+};
+
+// Rows that are worked on: whole tiles, and one tile of zeros (it writes dW)
+// where no row is counted.
+__device__ __forceinline__ int row_tiles(int count) { return max(1, (count + kTileM - 1) / kTileM); }
+__device__ __forceinline__ Deal deal_of(int count, int tiles_v, int tiles_d, int depth, int want_dw, int slabs, int pairs) {
+  return Deal(want_dw ? (long)tiles_v * tiles_d : 0, max(1, (count + kBlockK - 1) / kBlockK),
+              slabs ? (long)row_tiles(count) * tiles_d : 0, depth, slabs, pairs);
+}
+
 // Units of one pair.  kStats and kPiece: a contiguous share of the (row tile,
-// vocabulary tile) order, so that a pair stays on one row tile.  kProducts: dW tiles,
-// then dx tiles, dealt out round robin.
+// vocabulary tile) order, so that a pair stays on one row tile.  kProducts: its
+// dW tiles, then its run of dx.
 template <int MODE>
 struct Units {
-  long next, end, step;
-  int tiles_n, k_dim, k_rows;
   const MmaArgs &a;
-  int count;
-  __device__ __forceinline__ Units(const MmaArgs &args, int cnt) : a(args), count(cnt) {
-    const long pairs = gridDim.x >> 1, p = blockIdx.x >> 1;
-    // without a counted row one tile of zeros still writes dW
-    const int tiles_m = max(1, (count + kTileM - 1) / kTileM);
+  Deal deal;
+  int pair, k_dim, k_rows;
+  long next, end;    // tiles (kStats, kPiece) or dW tiles
+  long dx, dx_end;   // slices of dx
+  __device__ __forceinline__ Units(const MmaArgs &args, int count)
+      : a(args),
+        deal(deal_of(count, args.piece_k * kBlockK / kTileM, args.tiles_d, args.piece_k, args.want_dw, args.slabs,
+                     (int)(gridDim.x >> 1))) {
+    const long pairs = gridDim.x >> 1;
+    pair = (int)(blockIdx.x >> 1);
     k_dim = (a.dim + kBlockK - 1) / kBlockK;
     k_rows = max(1, (count + kBlockK - 1) / kBlockK);
-    tiles_n = a.tiles_n;
     if (MODE == kProducts) {
-      next = p;
-      end = (long)a.tiles_v * a.tiles_d + (long)tiles_m * a.tiles_d * a.splits;
-      step = pairs;
+      next = (long)pair * deal.w + min(pair, deal.n_a);
+      end = next + deal.w + (pair < deal.n_a ? 1 : 0);
+      dx = deal.begin(pair);
+      dx_end = deal.begin(pair + 1);
     } else {
-      const long total = (long)tiles_m * tiles_n;
-      next = p * total / pairs;
-      end = (p + 1) * total / pairs;
-      step = 1;
+      const long total = (long)row_tiles(count) * a.tiles_n;
+      next = pair * total / pairs;
+      end = (pair + 1) * total / pairs;
+      dx = dx_end = 0;
     }
   }
   __device__ __forceinline__ bool get(Unit &u) {
-    do {
-      if (next >= end) return false;
-      at(u);
-      next += step;
-    } while (u.nkb == 0);  // a short last piece may leave a split nothing
-    return true;
-  }
-  __device__ __forceinline__ void at(Unit &u) const {
-    if (MODE != kProducts) {
-      u.m = (int)(next / tiles_n);
-      u.n = (int)(next % tiles_n);
+    if (next < end) {
+      const int per = MODE == kProducts ? a.tiles_d : a.tiles_n;
+      u.m = (int)(next / per);
+      u.n = (int)(next % per);
       u.kb0 = 0;
-      u.nkb = k_dim;
-      u.dw = u.z = 0;
-    } else {
-      const long nw = (long)a.tiles_v * a.tiles_d;
-      if (next < nw) {
-        u.dw = 1;
-        u.m = (int)(next / a.tiles_d);
-        u.n = (int)(next % a.tiles_d);
-        u.kb0 = 0;
-        u.nkb = k_rows;
-        u.z = 0;
-      } else {
-        const long i = next - nw;
-        u.dw = 0;
-        u.n = (int)(i % a.tiles_d);
-        u.z = (int)(i / a.tiles_d % a.splits);
-        u.m = (int)(i / a.tiles_d / a.splits);
-        u.kb0 = (int)((long)u.z * a.piece_k / a.splits);
-        u.nkb = (int)((long)(u.z + 1) * a.piece_k / a.splits) - u.kb0;
-      }
+      u.nkb = MODE == kProducts ? k_rows : k_dim;
+      u.dw = MODE == kProducts;
+      u.z = 0;
+      ++next;
+      return true;
     }
+    if (MODE != kProducts || dx >= dx_end) return false;
+    const long tile = dx / deal.depth;
+    u.m = (int)(tile / a.tiles_d);
+    u.n = (int)(tile % a.tiles_d);
+    u.kb0 = (int)(dx % deal.depth);
+    u.nkb = (int)min((long)(deal.depth - u.kb0), dx_end - dx);
+    u.dw = 0;
+    u.z = pair - deal.owner(tile * deal.depth);
+    dx += u.nkb;
+    return true;
   }
 };
 
@@ -257,6 +297,22 @@ __device__ __forceinline__ void box_put32(unsigned char *box, int lane, const fl
   for (int k = 0; k < 8; ++k)
     *reinterpret_cast<float4 *>(box + lane * 128 + ((k ^ (lane & 7)) * 16)) =
         make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+}
+
+// Adds this lane's two columns of a box of 64 (32 rows; every bank once per row).
+template <typename T>
+__device__ __forceinline__ void box_sums(const unsigned char *box, int lane, float2 &sum) {
+  float2 even = make_float2(0.f, 0.f), odd = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int r = 0; r < 32; ++r) {
+    const OpVec<T, 2> g =
+        *reinterpret_cast<const OpVec<T, 2> *>(box + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
+    float2 &s = r & 1 ? odd : even;
+    s.x += op_load<T>(g.v[0]);
+    s.y += op_load<T>(g.v[1]);
+  }
+  sum.x += even.x + odd.x;
+  sum.y += even.y + odd.y;
 }
 
 // One warp's two staging boxes: take() gives the one whose last store has been
@@ -422,9 +478,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int etid = tid - 64;
     int j = 0, last_m = -1;
     float run_m = -INFINITY, run_s = 0.f;  // kStats: this row's statistics over the pair's tiles
-    float lse2 = 0.f;
+    float lse = 0.f;
     int32_t tgt = -1;
     const float scale = MODE == kProducts ? grad_scale(a.dloss, a.count, a.mean) / a.g_scale : 0.f;
+    const Deal full_deal = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs,
+                                   (int)(gridDim.x >> 1));
     auto flush = [&]() {
       if (last_m < 0) return;
       const size_t slot = (size_t)(blockIdx.x >> 1) + last_m;
@@ -435,11 +493,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int acc = j & 1;
       const float *sb = sbias + acc * kTileN;
       if (MODE != kProducts) {
-        // this tile's bias in base 2 (-Inf behind the vocabulary); the buffer's last
-        // reader passed the barrier of the tile before
+        // this tile's bias, in base 2 but for float32's G (-Inf behind the vocabulary);
+        // the buffer's last reader passed the barrier of the tile before
+        constexpr float unit = MODE == kPiece && sizeof(T) == 4 ? 1.f : kLog2e;
         const int v = a.v0 + u.n * kTileN + etid;
         float b = -INFINITY;
-        if (v < a.vocab) b = a.bias ? op_load<T>(static_cast<const T *>(a.bias)[v]) * kLog2e : 0.f;
+        if (v < a.vocab) b = a.bias ? op_load<T>(static_cast<const T *>(a.bias)[v]) * unit : 0.f;
         sbias[acc * kTileN + etid] = b;
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
         if (u.m != last_m) {
@@ -449,7 +508,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             run_s = 0.f;
           } else {
             const int row = u.m * kTileM + (int)rank * 128 + q * 32 + lane;
-            lse2 = row < count ? a.lse2[row] : INFINITY;  // rows behind the last: G = 0
+            lse = row < count ? a.lse[row] : INFINITY;  // rows behind the last: G = 0
+            if (sizeof(T) == 2) lse *= kLog2e;
             tgt = row < count ? a.tgt[row] : -1;
           }
           last_m = u.m;
@@ -512,10 +572,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const float4 b = b4[k];
-              v[h][4 * k] = exp2_fast(fmaf(v[h][4 * k], kLog2e, b.x - lse2));
-              v[h][4 * k + 1] = exp2_fast(fmaf(v[h][4 * k + 1], kLog2e, b.y - lse2));
-              v[h][4 * k + 2] = exp2_fast(fmaf(v[h][4 * k + 2], kLog2e, b.z - lse2));
-              v[h][4 * k + 3] = exp2_fast(fmaf(v[h][4 * k + 3], kLog2e, b.w - lse2));
+              const float bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float &x = v[h][4 * k + i];
+                // float32 subtracts lse before the change of base: the largest probabilities
+                // then have small exponents, rounded finely
+                if constexpr (sizeof(T) == 4) x = exp2_fast((x + bb[i] - lse) * kLog2e);
+                else x = exp2_fast(fmaf(x, kLog2e, bb[i] - lse));
+              }
             }
           }
           if (c + 64 == hcols) release();
@@ -527,6 +592,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               for (int k = 0; k < 32; ++k)
                 if (32 * h + k == at) v[h][k] -= 1.f;
           }
+          float2 col_sum = make_float2(0.f, 0.f);
           if constexpr (sizeof(T) == 2) {
             if (a.g_scale != 1.f) {
 #pragma unroll
@@ -538,21 +604,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             box_put16<T>(bx, lane, 0, v[0]);
             box_put16<T>(bx, lane, 1, v[1]);
             box.send(lane, &maps.c, bx, n0 + c, row0, 0, false);
+            if (a.db_part) box_sums<T>(bx, lane, col_sum);
           } else {
             for (int p = 0; p < 3; ++p) {
               unsigned char *bx = box.take(lane);
               box_put16<__nv_bfloat16>(bx, lane, 0, v[0]);
               box_put16<__nv_bfloat16>(bx, lane, 1, v[1]);
               box.send(lane, &maps.c, bx, n0 + c, row0, p, false);
+              if (a.db_part) box_sums<__nv_bfloat16>(bx, lane, col_sum);
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int k = 0; k < 32; ++k) v[h][k] -= __bfloat162float(__float2bfloat16_rn(v[h][k]));
             }
           }
+          if (a.db_part)
+            *reinterpret_cast<float2 *>(a.db_part + (size_t)(row0 >> 5) * a.tiles_n * kTileN + n0 + c + 2 * lane) = col_sum;
         }
       } else {
         const int n0 = u.n * bn + half * hcols;
+        const bool add = !a.first && u.z < full_deal.cover((long)u.m * a.tiles_d + u.n);  // else this slab is new
 #pragma unroll 1
         for (int c = 0; c < hcols; c += 64) {
           float v[2][32];
@@ -595,7 +666,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               if (col + 32 * h >= a.dim) continue;
               unsigned char *bx = box.take(lane);
               box_put32(bx, lane, h ? v[1] : v[0]);
-              box.send(lane, &maps.c, bx, col + 32 * h, row0, u.z, !a.first);
+              box.send(lane, &maps.c, bx, col + 32 * h, row0, u.z, add);
             }
           }
         }
@@ -673,11 +744,11 @@ __device__ __forceinline__ void put_pieces(uint16_t *dst, size_t plane, float v)
 }
 
 // x rows to their slots, zeros behind the last up to a whole tile (one at least); with lse the
-// compacted targets and base-2 lse.  One warp per row.
+// compacted targets and lse.  One warp per row.
 template <typename T>
 __global__ void ce_stage_rows_kernel(const T *__restrict__ x, long x_ld, const int32_t *__restrict__ tg,
                                      const int32_t *__restrict__ slot, const int *__restrict__ count, long rows, int dim,
-                                     int pitch, size_t plane, uint16_t *xc, const float *__restrict__ lse, float *lse2,
+                                     int pitch, size_t plane, uint16_t *xc, const float *__restrict__ lse, float *lse_c,
                                      int32_t *tgt) {
   const int lane = threadIdx.x & 31;
   const long n = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -687,7 +758,7 @@ __global__ void ce_stage_rows_kernel(const T *__restrict__ x, long x_ld, const i
     uint16_t *o = xc + (size_t)at * pitch;
     for (int c = lane; c < dim; c += 32) put_pieces<T>(o + c, plane, op_load<T>(x[n * x_ld + c]));
     if (lse && lane == 0) {
-      lse2[at] = lse[n] * kLog2e;
+      lse_c[at] = lse[n];
       tgt[at] = tg[n];
     }
   } else {
@@ -771,55 +842,44 @@ __global__ void __launch_bounds__(1024) ce_loss_kernel(const float *__restrict__
   if (threadIdx.x == 0) *loss = mean ? v[0] / fmaxf((float)*count, 1.f) : v[0];
 }
 
-// dx: the splits' slabs added in order, scaled, back to the rows' places.
+// dx: the slabs added in order, scaled, back to the rows' places.
 template <typename T>
-__global__ void ce_dx_kernel(const float *__restrict__ slab, size_t slab_stride, int splits, int pitch,
-                             const int32_t *__restrict__ slot, long rows, int dim, const float *__restrict__ dloss,
-                             const int *__restrict__ count, int mean, float inv_g, T *dx, long dx_ld) {
+__global__ void ce_dx_kernel(const float *__restrict__ slab, size_t slab_stride, int pitch, const MmaArgs a, int last_k,
+                             int pairs, const int32_t *__restrict__ slot, long rows, T *dx, long dx_ld) {
   const int lane = threadIdx.x & 31;
   const long n = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (n >= rows) return;
-  const int at = slot[n];
-  const float c = grad_scale(dloss, count, mean) * inv_g;
-  for (int i = lane; i < dim; i += 32) {
-    float s = 0.f;
-    if (at >= 0)
-      for (int k = 0; k < splits; ++k) s += slab[k * slab_stride + (size_t)at * pitch + i];
-    dx[n * dx_ld + i] = op_store<T>(c * s);
+  const int at = slot[n], count = *a.count;
+  const float c = grad_scale(a.dloss, a.count, a.mean) / a.g_scale;
+  const Deal full = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs, pairs);
+  const Deal last = deal_of(count, last_k * kBlockK / kTileM, a.tiles_d, last_k, a.want_dw, a.slabs, pairs);
+  for (int t = 0; t < a.tiles_d; ++t) {
+    const long tile = (long)(at / kTileM) * a.tiles_d + t;
+    const int slabs = at < 0 ? 0 : max(full.cover(tile), last.cover(tile));
+    const int end = min(a.dim, (t + 1) * a.bn);
+    for (int i = t * a.bn + lane; i < end; i += 32) {
+      float s = 0.f;
+      for (int k = 0; k < slabs; ++k) s += slab[k * slab_stride + (size_t)at * pitch + i];
+      dx[n * dx_ld + i] = op_store<T>(c * s);
+    }
   }
 }
 
-// db of a piece: column sums of G, 64 columns per CTA, the warps' sums added in order.
+// db of a piece: the sums of 32 rows each added in order, 32 columns and 8 strided
+// partial sums per CTA.
 template <typename T>
-__global__ void __launch_bounds__(1024) ce_db_kernel(const uint16_t *__restrict__ G, long pitch, size_t plane, int planes,
-                                                     const int *__restrict__ count, int v0, int vocab,
-                                                     const float *__restrict__ dloss, int mean, float inv_g, T *db) {
-  __shared__ float sh[32][65];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rows = *count;
-  float s0 = 0.f, s1 = 0.f;
-  using G2 = OpVec<uint16_t, 2>;
-  for (int p = planes - 1; p >= 0; --p) {
-#pragma unroll 8
-    for (int n = warp; n < rows; n += 32) {
-      const G2 g = *reinterpret_cast<const G2 *>(G + p * plane + (size_t)n * pitch + blockIdx.x * 64 + 2 * lane);
-      if constexpr (sizeof(T) == 2) {
-        s0 += op_load<T>(reinterpret_cast<const T &>(g.v[0]));
-        s1 += op_load<T>(reinterpret_cast<const T &>(g.v[1]));
-      } else {
-        s0 += __bfloat162float(reinterpret_cast<const __nv_bfloat16 &>(g.v[0]));
-        s1 += __bfloat162float(reinterpret_cast<const __nv_bfloat16 &>(g.v[1]));
-      }
-    }
-  }
-  sh[warp][2 * lane] = s0;
-  sh[warp][2 * lane + 1] = s1;
+__global__ void ce_db_kernel(const float *__restrict__ part, long pitch, const int *__restrict__ count, int v0, int vocab,
+                             const float *__restrict__ dloss, int mean, float inv_g, T *db) {
+  __shared__ float sh[8][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = row_tiles(*count) * 8;
+  float s = 0.f;
+#pragma unroll 4
+  for (int g = warp; g < groups; g += 8) s += part[g * pitch + blockIdx.x * 32 + lane];
+  sh[warp][lane] = s;
   __syncthreads();
-  if (threadIdx.x < 64) {
-    const int v = v0 + blockIdx.x * 64 + threadIdx.x;
-    if (v >= vocab) return;
-    float s = 0.f;
-    for (int w = 0; w < 32; ++w) s += sh[w][threadIdx.x];
+  const int v = v0 + blockIdx.x * 32 + lane;
+  if (warp == 0 && v < vocab) {
+    for (int k = 1; k < 8; ++k) s += sh[k][lane];
     db[v] = op_store<T>(grad_scale(dloss, count, mean) * inv_g * s);
   }
 }
@@ -850,24 +910,41 @@ struct Plan {
   float2 *stats;
   float *row_loss;
   // gradient
-  float *lse2, *slab;
+  float *lse_c, *slab, *db_part;
   int32_t *tgt;
   uint16_t *G;
   int piece;           // columns of a piece, a multiple of 256
-  int splits, bn, tiles_d;
+  int slabs, bn, tiles_d;
   long dpitch;
   size_t loss_bytes, grad_bytes;
 };
 
-// Columns of G held at a time: about 96 MB of it, which the L2 cache nearly
-// holds, but at least 2048 columns (a product with G needs depth), and whole
-// equal pieces.
-int piece_columns(long mpad, int planes, int tiles_n) {
-  long most = (96L << 20) / (mpad * 2 * planes) / kTileN;
-  if (most < 8) most = 8;
-  if (most >= tiles_n) return tiles_n * kTileN;
-  const long n = (tiles_n + most - 1) / most;
-  return (int)((tiles_n + n - 1) / n) * kTileN;
+// Vocabulary tiles of a piece.  G of a piece stays within 160 MB, but for the
+// columns that dW needs to keep half of the pairs busy (a tile goes to one pair
+// whole).  Among those sizes the one is taken whose launches cost least: the
+// busiest pair's slices, and about 16 slices' time for each launch.
+int piece_tiles(const aideen_linear_ce_args *a, const Plan &p) {
+  const long bytes = p.mpad * kTileN * 2 * p.planes;
+  const long half = (p.pairs / 2 + p.tiles_d - 1) / p.tiles_d;
+  long most = (160L << 20) / bytes;
+  if (most < half) most = half;
+  if (most >= p.tiles_n) most = p.tiles_n;
+  const long products = p.planes == 1 ? 1 : 6, k_dim = (a->dim + kBlockK - 1) / kBlockK;
+  const long k_rows = ((long)a->rows + kBlockK - 1) / kBlockK;
+  auto cost = [&](long tiles) {
+    const Deal d(tiles * p.tiles_d, k_rows, (long)p.tiles_m * p.tiles_d, (int)tiles * (kTileN / kBlockK), p.slabs, p.pairs);
+    return ((tiles * p.tiles_m + p.pairs - 1) / p.pairs * k_dim + d.load) * products + 32;
+  };
+  long best = most, best_cost = -1;
+  for (long tiles = most; tiles >= 1 && tiles * 3 >= most; --tiles) {
+    const long n = p.tiles_n / tiles, rest = p.tiles_n % tiles;
+    const long c = n * cost(tiles) + (rest ? cost(rest) : 0);
+    if (best_cost < 0 || c < best_cost) {
+      best = tiles;
+      best_cost = c;
+    }
+  }
+  return (int)best;
 }
 
 Plan make_plan(const aideen_linear_ce_args *a, void *ws) {
@@ -890,18 +967,17 @@ Plan make_plan(const aideen_linear_ce_args *a, void *ws) {
   p.stats = c.take<float2>((size_t)(p.pairs + p.tiles_m) * 2 * kTileM);
   p.row_loss = c.take<float>(a->rows);
   p.loss_bytes = c.used;
-  p.piece = p.tiles_m ? piece_columns(p.mpad, p.planes, p.tiles_n) : kTileN;
   p.bn = (a->dim + 127) / 128 % 2 ? 128 : 256;  // fewer padded columns
   p.tiles_d = (int)((a->dim + p.bn - 1) / p.bn);
-  // splits of dx over the piece: enough tiles for every pair, none below 16 slices
-  const long tiles = (long)p.tiles_m * p.tiles_d, ktot = p.piece / kBlockK;
-  p.splits = 1;
-  while (tiles * (p.splits + 1) <= p.pairs && ktot / (p.splits + 1) >= 16) ++p.splits;
+  const int dx_tiles = p.tiles_m ? p.tiles_m * p.tiles_d : 1;
+  p.slabs = (p.pairs + dx_tiles - 1) / dx_tiles + 2;  // a run is about depth * dx_tiles / pairs long
+  p.piece = (p.tiles_m ? piece_tiles(a, p) : 1) * kTileN;
   p.dpitch = (long)op_round(a->dim, 4);
-  p.lse2 = g.take<float>(a->rows);
+  p.lse_c = g.take<float>(a->rows);
   p.tgt = g.take<int32_t>(a->rows);
   p.G = g.take<uint16_t>((size_t)p.mpad * p.piece * p.planes);
-  p.slab = g.take<float>((size_t)p.splits * p.mpad * p.dpitch);
+  p.slab = g.take<float>((size_t)p.slabs * p.mpad * p.dpitch);
+  p.db_part = g.take<float>((size_t)p.tiles_m * 8 * p.piece);
   p.grad_bytes = g.used;
   return p;
 }
@@ -945,7 +1021,7 @@ cudaError_t stage_run(const aideen_linear_ce_args *g, const Plan &p, const T *x,
                       const float *lse, cudaStream_t st) {
   ce_index_kernel<<<1, 1024, 0, st>>>(tg, g->rows, (int)g->vocab, p.slot, p.count);
   ce_stage_rows_kernel<T><<<(unsigned)((g->rows + kTileM + 7) / 8), 256, 0, st>>>(
-      x, g->x_ld, tg, p.slot, p.count, g->rows, (int)g->dim, p.pitch, p.xplane, p.xc, lse, p.lse2, p.tgt);
+      x, g->x_ld, tg, p.slot, p.count, g->rows, (int)g->dim, p.pitch, p.xplane, p.xc, lse, p.lse_c, p.tgt);
   if (!p.w_direct)
     ce_stage_w_kernel<T><<<(unsigned)((g->vocab + 7) / 8), 256, 0, st>>>(w, g->w_ld, g->vocab, (int)g->dim, p.pitch,
                                                                         p.wplane, p.wc);
@@ -999,7 +1075,7 @@ cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
        map_w(&pm.b, p, g, w, 64) &&
        make_map(&pm.a2, kU16, p.G, p.piece, p.mpad, p.planes, (size_t)p.piece * 2, gplane * 2, 64, 64) &&
        map_x(&pm.b2, p, dim, 64) &&
-       make_map(&pm.c, kF32, p.slab, dim, p.mpad, p.splits, p.dpitch * 4, p.mpad * p.dpitch * 4, 32, 32);
+       make_map(&pm.c, kF32, p.slab, dim, p.mpad, p.slabs, p.dpitch * 4, p.mpad * p.dpitch * 4, 32, 32);
   const size_t el = sizeof(T);
   const bool dw_tma = dw && op_vec16(dw, g->dw_ld, el);
   if (dw_tma)
@@ -1007,8 +1083,9 @@ cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
                         (size_t)g->dw_ld * el * g->vocab, 128 / el, 32);
   if (!ok) return cudaErrorInvalidValue;
   MmaArgs a = mma_args<T>(g, p, bias);
-  a.lse2 = p.lse2; a.tgt = p.tgt;
-  a.bn = p.bn; a.tiles_d = p.tiles_d; a.splits = dx ? p.splits : 0;
+  a.lse = p.lse_c; a.tgt = p.tgt; a.db_part = db ? p.db_part : nullptr;
+  a.bn = p.bn; a.tiles_d = p.tiles_d; a.slabs = dx ? p.slabs : 0; a.want_dw = dw != nullptr;
+  a.full_k = p.piece / kBlockK;
   a.dw = dw; a.dw_ld = g->dw_ld; a.dw_tma = dw_tma; a.dloss = dloss;
   for (int v0 = 0; v0 < (int)g->vocab; v0 += p.piece) {
     const int left = (int)g->vocab - v0, cols = left < p.piece ? (left + kTileN - 1) / kTileN * kTileN : p.piece;
@@ -1016,21 +1093,19 @@ cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
     a.tiles_n = cols / kTileN;
     e = launch_mma<kPiece, T>(p, lm, a, st);
     if (e != cudaSuccess) return e;
+    if (db)
+      ce_db_kernel<T><<<cols / 32, 256, 0, st>>>(p.db_part, cols, p.count, v0, (int)g->vocab, dloss, a.mean,
+                                                 1.f / a.g_scale, db);
     if (dx || dw) {
       a.piece_k = cols / kBlockK;
-      a.tiles_v = dw ? cols / kTileM : 0;
       a.first = v0 == 0;
       e = launch_mma<kProducts, T>(p, pm, a, st);
       if (e != cudaSuccess) return e;
     }
-    if (db)
-      ce_db_kernel<T><<<cols / 64, 1024, 0, st>>>(p.G, p.piece, gplane, p.planes, p.count, v0, (int)g->vocab, dloss,
-                                                  a.mean, 1.f / a.g_scale, db);
   }
   if (dx)
-    ce_dx_kernel<T><<<(unsigned)((g->rows + 7) / 8), 256, 0, st>>>(p.slab, (size_t)p.mpad * p.dpitch, p.splits,
-                                                                   (int)p.dpitch, p.slot, g->rows, dim, dloss, p.count,
-                                                                   a.mean, 1.f / a.g_scale, dx, g->dx_ld);
+    ce_dx_kernel<T><<<(unsigned)((g->rows + 7) / 8), 256, 0, st>>>(p.slab, (size_t)p.mpad * p.dpitch, (int)p.dpitch, a,
+                                                                   a.piece_k, p.pairs, p.slot, g->rows, dx, g->dx_ld);
   return cudaGetLastError();
 }
 
