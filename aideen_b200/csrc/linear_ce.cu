@@ -38,7 +38,8 @@ namespace {
 __device__ unsigned int g_ce_timeout;
 
 constexpr int kTileM = 256, kTileN = 256, kBlockK = 64;
-constexpr int kStages = 5, kHalfBytes = 128 * kBlockK * 2, kStageBytes = 2 * kHalfBytes;
+constexpr int kHalfBytes = 128 * kBlockK * 2;  // one CTA's half of an operand slice: 16 KB
+constexpr int kMaxStages = 8, kMaxHeld = 8;    // ring depth; slices of x that stay in shared memory
 constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
 constexpr int kBoxBytes = 4096;  // 32 rows of 128 bytes
 constexpr uint32_t kWaitLimit = 1u << 24;
@@ -46,7 +47,9 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // float16 keeps softmax - onehot times 2^12: probabilities down to 2^-26 stay
 // normal numbers, and the largest magnitude is 2^12
 constexpr float kHalfScale = 4096.f;
-constexpr size_t kSmemBytes = (size_t)kStages * kStageBytes + kEpiWarps * 2 * kBoxBytes + 2 * kTileN * 4 + 256;
+// Shared memory of a CTA: held slices of x, the ring, the epilogue's boxes, the
+// bias of two tiles, barriers.
+constexpr int kSmemLimit = 232448, kSmemFixed = 2 * kTileN * 4 + 512;
 
 enum { kStats = 0, kPiece = 1, kProducts = 2 };
 
@@ -55,6 +58,7 @@ struct MmaArgs {
   int vocab, dim;
   int planes;         // 16-bit pieces per operand element: 1, or 3 for float32
   uint32_t idesc;     // operand types of the instruction descriptor
+  int stages;         // ring depth
   // kStats, kPiece: vocabulary tiles [0, tiles_n) from column v0 on
   int v0, tiles_n;
   const void *bias;
@@ -98,13 +102,22 @@ __device__ __forceinline__ uint32_t leader_addr(const void *p) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
   return a;
 }
+// True in one lane of a converged warp, the same one at every call.  With it, not
+// with lane == 0, the compiler knows that a single thread follows, and issues MMAs
+// and copies straight from uniform registers (at 8192 x 50257 x 512 the loss kernel
+// without its loads went from 1410 to 1680 TFLOP/s).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 __device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity) {
   const uint32_t addr = smem_u32(bar);
   for (uint32_t i = 0; i < kWaitLimit; ++i) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done)
         : "r"(addr), "r"(parity)
@@ -138,7 +151,7 @@ __device__ __forceinline__ void pair_commit(uint64_t *bar) {
       : "memory");
 }
 __device__ __forceinline__ void remote_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
   uint32_t r[32];
@@ -315,22 +328,23 @@ __device__ __forceinline__ void box_sums(const unsigned char *box, int lane, flo
   sum.y += even.y + odd.y;
 }
 
-// One warp's two staging boxes: take() gives the one whose last store has been
-// read, send() hands it to TMA.
+// One warp's N staging boxes, used in turn: take() gives one whose last store has
+// been read, send() hands it to TMA.
+template <int N>
 struct Boxes {
   unsigned char *base;
   int n = 0;
-  __device__ __forceinline__ unsigned char *take(int lane) {
-    unsigned char *b = base + (n & 1) * kBoxBytes;
-    if (lane == 0) bulk_wait_read<1>();
+  __device__ __forceinline__ unsigned char *take() {
+    unsigned char *b = base + (N == 2 ? (n & 1) * kBoxBytes : 0);
+    if (elect_one()) bulk_wait_read<N == 2 ? 1 : 0>();
     __syncwarp();
     return b;
   }
-  __device__ __forceinline__ void send(int lane, const CUtensorMap *map, const unsigned char *box, int x, int y, int z,
+  __device__ __forceinline__ void send(const CUtensorMap *map, const unsigned char *box, int x, int y, int z,
                                        bool add) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
-    if (lane == 0) {
+    if (elect_one()) {
       if (add) tma_reduce_add_3d(map, box, x, y, z);
       else tma_store_3d(map, box, x, y, z);
       bulk_commit();
@@ -345,7 +359,9 @@ struct Maps {
   CUtensorMap c, c2;   // stores: kPiece: G.  kProducts: dx slabs, dW
 };
 
-template <int MODE, typename T>
+// HELD (kStats, kPiece with one piece per element and dim <= 512): the row tile of x stays in
+// shared memory while the pair walks along the vocabulary, and the ring carries W only.
+template <int MODE, typename T, bool HELD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ce_mma_kernel(const __grid_constant__ Maps maps, const MmaArgs a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -354,11 +370,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) atomicCAS(&g_ce_timeout, 0u, 1u);
     return;
   }
-  unsigned char *boxes = sm + kStages * kStageBytes;
-  float *sbias = reinterpret_cast<float *>(boxes + kEpiWarps * 2 * kBoxBytes);  // [2][kTileN]
+  constexpr int kStageBytes = HELD ? kHalfBytes : 2 * kHalfBytes;
+  constexpr int kBoxesPerWarp = MODE == kStats ? 0 : HELD ? 1 : 2;
+  const int stages = a.stages, held = HELD ? (a.dim + kBlockK - 1) / kBlockK : 0;
+  unsigned char *ring = sm + held * kHalfBytes;
+  unsigned char *boxes = ring + stages * kStageBytes;
+  float *sbias = reinterpret_cast<float *>(boxes + kEpiWarps * kBoxesPerWarp * kBoxBytes);  // [2][kTileN]
   uint64_t *full = reinterpret_cast<uint64_t *>(sbias + 2 * kTileN);
-  uint64_t *empty = full + kStages;
-  uint64_t *tfull = empty + kStages;
+  uint64_t *empty = full + kMaxStages;
+  uint64_t *hfull = empty + kMaxStages;   // held slices loaded
+  uint64_t *hempty = hfull + kMaxHeld;    // and no longer read
+  uint64_t *tfull = hempty + kMaxHeld;
   uint64_t *tempty = tfull + 2;
   uint64_t *done = tempty + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
@@ -368,9 +390,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int count = *a.count;
 
   if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < kMaxHeld; ++s) {
+      mbar_init(&hfull[s], 1);
+      mbar_init(&hempty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
@@ -396,25 +422,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   Unit u;
 
   if (warp == 0) {
-    if (lane == 0) {  // ---------------- loads
-      uint32_t it = 0;
+    if (elect_one()) {  // ---------------- loads
+      uint32_t it = 0, s = 0, turn = 0;  // slices so far, ring place, turn of the ring
+      int gen = -1, last_m = -1;         // row tiles held so far
       bool ok = true;
-      const uint32_t bytes = 2u * (kHalfBytes + bn / 2 * kBlockK * 2);  // of both CTAs
+      const uint32_t bytes = 2u * ((HELD ? 0 : kHalfBytes) + bn / 2 * kBlockK * 2);  // of both CTAs
       while (ok && units.get(u)) {
         const int m0 = u.m * kTileM + (int)rank * 128, n0 = u.n * bn + (int)rank * (bn / 2);
+        const bool fresh = HELD && u.m != last_m;
+        if (fresh) ++gen;
+        last_m = u.m;
         for (int j = 0; j < products && ok; ++j) {
           int pa, pb;
           product_pair(a.planes, j, pa, pb);
           for (int kb = 0; kb < u.nkb; ++kb, ++it) {
-            const int s = it % kStages;
-            if (it >= (uint32_t)kStages && !wait_bounded(&empty[s], ((it / kStages) - 1) & 1)) { ok = false; break; }
-            if (*(volatile uint32_t *)err) { ok = false; break; }
-            unsigned char *sa = sm + s * kStageBytes, *sb = sa + kHalfBytes;
+            const int k0 = (u.kb0 + kb) * kBlockK;
+            if (fresh) {
+              if (gen > 0 && !wait_bounded(&hempty[kb], (gen - 1) & 1)) { ok = false; break; }
+              if (rank == 0) mbar_expect_tx(&hfull[kb], 2 * kHalfBytes);
+              pair_load(sm + kb * kHalfBytes, &maps.a, leader_addr(&hfull[kb]), k0, m0, 0);
+            }
+            if (turn > 0 && !wait_bounded(&empty[s], (turn - 1) & 1)) { ok = false; break; }
+            unsigned char *sa = ring + s * kStageBytes, *sb = HELD ? sa : sa + kHalfBytes;
             const uint32_t bar = leader_addr(&full[s]);
             if (rank == 0) mbar_expect_tx(&full[s], bytes);
-            const int k0 = (u.kb0 + kb) * kBlockK;
             if (MODE != kProducts) {
-              pair_load(sa, &maps.a, bar, k0, m0, pa);
+              if (!HELD) pair_load(sa, &maps.a, bar, k0, m0, pa);
               pair_load(sb, &maps.b, bar, k0, a.v0 + n0, pb);
             } else if (u.dw) {
               for (int c = 0; c < 2; ++c) pair_load(sa + c * 8192, &maps.a2, bar, m0 + 64 * c, k0, pa);
@@ -423,25 +456,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               pair_load(sa, &maps.a, bar, k0, m0, pa);
               for (int c = 0; c < bn / 128; ++c) pair_load(sb + c * 8192, &maps.b, bar, n0 + 64 * c, a.v0 + k0, pb);
             }
+            if (++s == (uint32_t)stages) { s = 0; ++turn; }
           }
         }
       }
       if (!ok) atomicExch(err, 1u);
-      // every stage's last use is over (its arrival has landed here) before this CTA may leave
-      for (uint32_t j = it > (uint32_t)kStages ? it - kStages : 0; j < it && ok; ++j)
-        if (!wait_bounded(&empty[j % kStages], (j / kStages) & 1)) { ok = false; atomicExch(err, 1u); }
-      if (!ok && rank == 0) {  // let the copies in flight land
-        for (uint32_t j = it > (uint32_t)kStages ? it - kStages : 0; j < it; ++j)
-          wait_bounded(&full[j % kStages], (j / kStages) & 1);
+      // every place's last use is over (its arrival has landed here) before this CTA may leave
+      const uint32_t used = it < (uint32_t)stages ? it : (uint32_t)stages;
+      for (uint32_t i = 0; i < used; ++i) {
+        const uint32_t t = i < s ? turn : turn - 1;  // the turn of place i's last load
+        if (ok && !wait_bounded(&empty[i], t & 1)) { ok = false; atomicExch(err, 1u); }
+        if (!ok && rank == 0) wait_bounded(&full[i], t & 1);  // let a copy in flight land
+      }
+      for (int kb = 0; kb < held && gen >= 0; ++kb) {
+        if (ok && !wait_bounded(&hempty[kb], gen & 1)) { ok = false; atomicExch(err, 1u); }
+        if (!ok && rank == 0) wait_bounded(&hfull[kb], gen & 1);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {  // ---------------- MMAs
-      uint32_t it = 0;
-      int j = 0;
+    if (rank == 0 && elect_one()) {  // ---------------- MMAs
+      uint32_t s = 0, turn = 0;
+      int j = 0, gen = -1, last_m = -1;
       bool ok = true;
       for (; ok && units.get(u); ++j) {
         const int acc = j & 1;
+        const bool fresh = HELD && u.m != last_m;
+        const bool leaving = HELD && (u.n == a.tiles_n - 1 || units.next >= units.end);  // last tile of these rows
+        if (fresh) ++gen;
+        last_m = u.m;
         if (j >= 2 && !wait_bounded(&tempty[acc], ((j >> 1) - 1) & 1)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         // rows by 64: 128-byte rows, 8-row groups 1024 apart; columns by 64: blocks of 64
@@ -452,17 +494,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t lbo_a = acol ? 8192u : 16u, lbo_b = bcol ? 8192u : 16u;
         const uint32_t ka = acol ? 2048u : 32u, kb_ = bcol ? 2048u : 32u;  // 16 deep
         const uint32_t d = tmem + (uint32_t)acc * kTileN;
+        const uint64_t desc_a = sdesc(sm, lbo_a, 1024u, 2u);
+        const uint64_t desc_b = sdesc(sm + (HELD ? 0 : kHalfBytes), lbo_b, 1024u, 2u);
+        const int ring_at = held * kHalfBytes;
         const int total = products * u.nkb;
-        for (int k = 0; k < total; ++k, ++it) {
-          const int s = it % kStages;
-          if (!wait_bounded(&full[s], (it / kStages) & 1) || *(volatile uint32_t *)err) { ok = false; break; }
+        for (int k = 0; k < total; ++k) {
+          if (fresh && !wait_bounded(&hfull[k], gen & 1)) { ok = false; break; }
+          if (!wait_bounded(&full[s], turn & 1)) { ok = false; break; }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          unsigned char *sa = sm + s * kStageBytes, *sb = sa + kHalfBytes;
+          const uint64_t da = desc_a + ((HELD ? k * kHalfBytes : ring_at + (int)s * kStageBytes) >> 4);
+          const uint64_t db = desc_b + ((ring_at + (int)s * kStageBytes) >> 4);
 #pragma unroll
-          for (int q = 0; q < kBlockK / 16; ++q)
-            pair_mma(d, sdesc(sa + q * ka, lbo_a, 1024u, 2u), sdesc(sb + q * kb_, lbo_b, 1024u, 2u), idesc,
-                     k > 0 || q > 0 ? 1u : 0u);
+          for (int q = 0; q < kBlockK / 16; ++q) pair_mma(d, da + q * (ka >> 4), db + q * (kb_ >> 4), idesc, k > 0 || q > 0);
           pair_commit(&empty[s]);
+          if (leaving) pair_commit(&hempty[k]);
+          if (++s == (uint32_t)stages) { s = 0; ++turn; }
         }
         if (!ok) break;
         pair_commit(&tfull[acc]);
@@ -474,7 +520,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else {  // ---------------- epilogue: lanes are accumulator rows
     const int q = warp & 3, half = (warp - 2) >> 2;  // tensor-memory lane quarter, half of the columns
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16);
-    Boxes box{boxes + (warp - 2) * 2 * kBoxBytes};
+    Boxes<kBoxesPerWarp> box{boxes + (warp - 2) * kBoxesPerWarp * kBoxBytes};
     const int etid = tid - 64;
     int j = 0, last_m = -1;
     float run_m = -INFINITY, run_s = 0.f;  // kStats: this row's statistics over the pair's tiles
@@ -530,7 +576,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       auto release = [&]() {  // the accumulator has been read: hand it back
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) remote_arrive(leader_addr(&tempty[acc]));
+        if (elect_one()) remote_arrive(leader_addr(&tempty[acc]));
       };
       if (MODE == kStats) {
 #pragma unroll 1
@@ -600,17 +646,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int k = 0; k < 32; ++k) v[h][k] *= a.g_scale;
             }
-            unsigned char *bx = box.take(lane);
+            unsigned char *bx = box.take();
             box_put16<T>(bx, lane, 0, v[0]);
             box_put16<T>(bx, lane, 1, v[1]);
-            box.send(lane, &maps.c, bx, n0 + c, row0, 0, false);
+            box.send(&maps.c, bx, n0 + c, row0, 0, false);
             if (a.db_part) box_sums<T>(bx, lane, col_sum);
           } else {
             for (int p = 0; p < 3; ++p) {
-              unsigned char *bx = box.take(lane);
+              unsigned char *bx = box.take();
               box_put16<__nv_bfloat16>(bx, lane, 0, v[0]);
               box_put16<__nv_bfloat16>(bx, lane, 1, v[1]);
-              box.send(lane, &maps.c, bx, n0 + c, row0, p, false);
+              box.send(&maps.c, bx, n0 + c, row0, p, false);
               if (a.db_part) box_sums<__nv_bfloat16>(bx, lane, col_sum);
 #pragma unroll
               for (int h = 0; h < 2; ++h)
@@ -648,32 +694,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               }
             } else if constexpr (sizeof(T) == 2) {
               if (col < a.dim && vrow < a.vocab) {
-                unsigned char *bx = box.take(lane);
+                unsigned char *bx = box.take();
                 box_put16<T>(bx, lane, 0, v[0]);
                 box_put16<T>(bx, lane, 1, v[1]);
-                box.send(lane, &maps.c2, bx, col, vrow, 0, false);
+                box.send(&maps.c2, bx, col, vrow, 0, false);
               }
             } else {
               for (int h = 0; h < 2; ++h) {
                 if (col + 32 * h >= a.dim || vrow >= a.vocab) continue;
-                unsigned char *bx = box.take(lane);
+                unsigned char *bx = box.take();
                 box_put32(bx, lane, h ? v[1] : v[0]);
-                box.send(lane, &maps.c2, bx, col + 32 * h, vrow, 0, false);
+                box.send(&maps.c2, bx, col + 32 * h, vrow, 0, false);
               }
             }
           } else {
             for (int h = 0; h < 2; ++h) {
               if (col + 32 * h >= a.dim) continue;
-              unsigned char *bx = box.take(lane);
+              unsigned char *bx = box.take();
               box_put32(bx, lane, h ? v[1] : v[0]);
-              box.send(lane, &maps.c, bx, col + 32 * h, row0, u.z, add);
+              box.send(&maps.c, bx, col + 32 * h, row0, u.z, add);
             }
           }
         }
       }
     }
     if (MODE == kStats) flush();
-    if (lane == 0) bulk_wait<0>();  // stores complete before the shared memory goes away
+    if (elect_one()) bulk_wait<0>();  // stores complete before the shared memory goes away
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -1008,12 +1054,26 @@ bool map_w(CUtensorMap *m, const Plan &p, const aideen_linear_ce_args *g, const 
   return make_map(m, kU16, p.wc, g->dim, g->vocab, p.planes, (size_t)p.pitch * 2, p.wplane * 2, 64, rows);
 }
 
+template <int MODE, typename T, bool HELD>
+cudaError_t launch_as(const Plan &p, const Maps &maps, MmaArgs a, cudaStream_t st) {
+  const int held = HELD ? (a.dim + kBlockK - 1) / kBlockK : 0;
+  const int boxes = kEpiWarps * (MODE == kStats ? 0 : HELD ? 1 : 2) * kBoxBytes;
+  const int stage = HELD ? kHalfBytes : 2 * kHalfBytes;
+  a.stages = (kSmemLimit - kSmemFixed - boxes - held * kHalfBytes) / stage;
+  if (a.stages > kMaxStages) a.stages = kMaxStages;
+  const int smem = held * kHalfBytes + a.stages * stage + boxes + kSmemFixed;
+  auto kernel = ce_mma_kernel<MODE, T, HELD>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<2 * p.pairs, kThreads, smem, st>>>(maps, a);
+  return cudaGetLastError();
+}
 template <int MODE, typename T>
 cudaError_t launch_mma(const Plan &p, const Maps &maps, const MmaArgs &a, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(ce_mma_kernel<MODE, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
-  if (e != cudaSuccess) return e;
-  ce_mma_kernel<MODE, T><<<2 * p.pairs, kThreads, kSmemBytes, st>>>(maps, a);
-  return cudaGetLastError();
+  if constexpr (MODE != kProducts && sizeof(T) == 2) {
+    if (a.dim <= kMaxHeld * kBlockK) return launch_as<MODE, T, true>(p, maps, a, st);
+  }
+  return launch_as<MODE, T, false>(p, maps, a, st);
 }
 
 template <typename T>
