@@ -77,7 +77,7 @@ struct MmaArgs {
   int slabs;          // slabs of dx (0: dx not wanted)
   int first;          // first piece: dx slabs are written, not added to
   int dw_tma;         // dW can be stored by TMA
-  void *dw;
+  void *dw, *db;
   long dw_ld;
   const float *dloss;
   int mean;
@@ -359,6 +359,27 @@ struct Maps {
   CUtensorMap c, c2;   // stores: kPiece: G.  kProducts: dx slabs, dW
 };
 
+// db of a piece, by the epilogue warps while they have nothing to drain yet: the
+// sums of 32 rows each are added in order, 64 columns and 4 strided partial sums per
+// CTA and turn.
+template <typename T>
+__device__ __forceinline__ void db_columns(const MmaArgs &a, int count, int etid, float *sh) {
+  const int groups = row_tiles(count) * 8, cols = a.tiles_n * kTileN;
+  const float scale = grad_scale(a.dloss, a.count, a.mean) / a.g_scale;
+  for (int c0 = blockIdx.x * 64; c0 < cols; c0 += gridDim.x * 64) {
+    const float *part = a.db_part + c0 + (etid & 63);
+    float s = 0.f;
+#pragma unroll 8
+    for (int g = etid >> 6; g < groups; g += 4) s += part[(size_t)g * cols];
+    sh[etid] = s;
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+    const int v = a.v0 + c0 + etid;
+    if (etid < 64 && v < a.vocab)
+      static_cast<T *>(a.db)[v] = op_store<T>(scale * (((sh[etid] + sh[etid + 64]) + sh[etid + 128]) + sh[etid + 192]));
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+  }
+}
+
 // HELD (kStats, kPiece with one piece per element and dim <= 512): the row tile of x stays in
 // shared memory while the pair walks along the vocabulary, and the ring carries W only.
 template <int MODE, typename T, bool HELD>
@@ -387,7 +408,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint32_t *err = tmem_slot + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
-  const int count = *a.count;
 
   if (tid == 0) {
     for (int s = 0; s < kMaxStages; ++s) {
@@ -416,6 +436,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_barrier();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
+  op_begin();
+  const int count = *a.count;
   const int products = a.planes == 1 ? 1 : 6;
   const int bn = MODE == kProducts ? a.bn : kTileN;  // columns of a tile; either CTA loads half
   Units<MODE> units(a, count);
@@ -529,6 +551,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const float scale = MODE == kProducts ? grad_scale(a.dloss, a.count, a.mean) / a.g_scale : 0.f;
     const Deal full_deal = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs,
                                    (int)(gridDim.x >> 1));
+    if (MODE == kProducts && a.db_part) db_columns<T>(a, count, etid, sbias);
     auto flush = [&]() {
       if (last_m < 0) return;
       const size_t slot = (size_t)(blockIdx.x >> 1) + last_m;
@@ -734,46 +757,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // ---- staging ----------------------------------------------------------------
 __device__ __forceinline__ bool counted(int32_t t, int vocab) { return t >= 0 && t < vocab; }
 
-// Position of every counted row among them (-1: not counted), and their number.
-// One CTA: 8 targets per thread and turn.
-__global__ void __launch_bounds__(1024) ce_index_kernel(const int32_t *__restrict__ tg, long n, int vocab,
-                                                        int32_t *slot, int *count) {
-  __shared__ int wsum[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int base = 0;
-  for (long i0 = 0; i0 < n; i0 += 8192) {
-    const long i = i0 + threadIdx.x * 8;
-    int flag[8], mine = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      flag[k] = i + k < n && counted(tg[i + k], vocab);
-      mine += flag[k];
-    }
-    int x = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) wsum[warp] = x;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) before += wsum[w];
-      all += wsum[w];
-    }
-    int at = base + before + x - mine;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (i + k < n) slot[i + k] = flag[k] ? at : -1;
-      at += flag[k];
-    }
-    base += all;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) *count = base;
-}
-
 // Splits v into bfloat16 pieces (one piece: itself rounded, exact for 16-bit input).
 template <typename T>
 __device__ __forceinline__ void put_pieces(uint16_t *dst, size_t plane, float v) {
@@ -789,42 +772,115 @@ __device__ __forceinline__ void put_pieces(uint16_t *dst, size_t plane, float v)
   }
 }
 
-// x rows to their slots, zeros behind the last up to a whole tile (one at least); with lse the
-// compacted targets and lse.  One warp per row.
-template <typename T>
-__global__ void ce_stage_rows_kernel(const T *__restrict__ x, long x_ld, const int32_t *__restrict__ tg,
-                                     const int32_t *__restrict__ slot, const int *__restrict__ count, long rows, int dim,
-                                     int pitch, size_t plane, uint16_t *xc, const float *__restrict__ lse, float *lse_c,
-                                     int32_t *tgt) {
-  const int lane = threadIdx.x & 31;
-  const long n = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (n < rows) {
-    const int at = slot[n];
-    if (at < 0) return;
-    uint16_t *o = xc + (size_t)at * pitch;
-    for (int c = lane; c < dim; c += 32) put_pieces<T>(o + c, plane, op_load<T>(x[n * x_ld + c]));
-    if (lse && lane == 0) {
-      lse_c[at] = lse[n];
-      tgt[at] = tg[n];
+// One row of 16-bit operands from `src` (null: zeros), by one warp; VEC elements per
+// access where the addresses allow.
+template <typename T, int VEC>
+__device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *src, int dim, int lane) {
+  for (int c = lane * VEC; c < dim; c += 32 * VEC) {
+    if constexpr (VEC == 1) {
+      put_pieces<T>(dst + c, plane, src ? op_load<T>(src[c]) : 0.f);
+    } else if constexpr (sizeof(T) == 2) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (src) v = *reinterpret_cast<const uint4 *>(src + c);
+      *reinterpret_cast<uint4 *>(dst + c) = v;
+    } else {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (src) v = *reinterpret_cast<const float4 *>(src + c);
+      float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        OpVec<__nv_bfloat16, 4> b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          b.v[i] = __float2bfloat16_rn(x[i]);
+          x[i] -= __bfloat162float(b.v[i]);
+        }
+        *reinterpret_cast<OpVec<__nv_bfloat16, 4> *>(dst + p * plane + c) = b;
+      }
     }
-  } else {
-    const int c0 = *count;
-    const long at = c0 + (n - rows);
-    if (at >= max(1, (c0 + kTileM - 1) / kTileM) * kTileM) return;
-    uint16_t *o = xc + (size_t)at * pitch;
-    for (int c = lane; c < dim; c += 32) put_pieces<T>(o + c, plane, 0.f);
   }
 }
 
-// W (any stride and alignment) as 16-bit operands.
-template <typename T>
-__global__ void ce_stage_w_kernel(const T *__restrict__ w, long w_ld, long vocab, int dim, int pitch, size_t plane,
-                                  uint16_t *wc) {
-  const int lane = threadIdx.x & 31;
-  const long v = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (v >= vocab) return;
-  uint16_t *o = wc + (size_t)v * pitch;
-  for (int c = lane; c < dim; c += 32) put_pieces<T>(o + c, plane, op_load<T>(w[v * w_ld + c]));
+struct StageArgs {
+  const void *x;
+  long x_ld, rows;
+  const int32_t *tg;
+  int vocab, dim, pitch, per_cta;  // rows per CTA, a multiple of 32
+  size_t plane;
+  uint16_t *xc;
+  int32_t *slot;
+  int *count;
+  unsigned int *ticket;
+  const float *lse;  // gradient only
+  float *lse_c;
+  int32_t *tgt;
+};
+
+// Finds the counted rows' places (every CTA counts the targets itself: they are few
+// bytes, and a scan would be one launch more), gathers x there, with lse also lse and
+// targets, and zeros the rows behind the last up to a whole tile.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) ce_stage_rows_kernel(const StageArgs a) {
+  __shared__ int sh[2][8];
+  op_begin();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long r0 = (long)blockIdx.x * a.per_cta;
+  int before = 0, total = 0;
+#pragma unroll 8
+  for (long n = threadIdx.x; n < a.rows; n += 256) {
+    const int c = counted(a.tg[n], a.vocab);
+    total += c;
+    if (n < r0) before += c;
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  total = __reduce_add_sync(0xffffffffu, total);
+  if (lane == 0) {
+    sh[0][warp] = before;
+    sh[1][warp] = total;
+  }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    before += sh[0][w];
+    total += sh[1][w];
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *a.count = total;
+    *a.ticket = 0;
+  }
+  const T *x = static_cast<const T *>(a.x);
+  for (long g0 = r0; g0 < a.rows && g0 < r0 + a.per_cta; g0 += 32) {  // 32 rows at a time, 4 per warp
+    const int32_t t = g0 + lane < a.rows ? a.tg[g0 + lane] : -1;
+    const bool in = counted(t, a.vocab);
+    const uint32_t mask = __ballot_sync(0xffffffffu, in);
+    const int at = before + __popc(mask & ((1u << lane) - 1u));
+    if (warp == 0 && g0 + lane < a.rows) {
+      a.slot[g0 + lane] = in ? at : -1;
+      if (in && a.lse) {
+        a.lse_c[at] = a.lse[g0 + lane];
+        a.tgt[at] = t;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = warp * 4 + i, to = __shfl_sync(0xffffffffu, at, k);
+      if (mask >> k & 1) put_row<T, VEC>(a.xc + (size_t)to * a.pitch, a.plane, x + (g0 + k) * a.x_ld, a.dim, lane);
+    }
+    before += __popc(mask);
+  }
+  const long end = (long)row_tiles(total) * kTileM;
+  for (long j = total + (long)blockIdx.x * 8 + warp; j < end; j += (long)gridDim.x * 8)
+    put_row<T, VEC>(a.xc + (size_t)j * a.pitch, a.plane, static_cast<const T *>(nullptr), a.dim, lane);
+}
+
+// W (any stride and alignment) as 16-bit operands, one warp per row.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) ce_stage_w_kernel(const T *w, long w_ld, long vocab, int dim, int pitch,
+                                                         size_t plane, uint16_t *wc) {
+  op_begin();
+  const long v = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (v < vocab) put_row<T, VEC>(wc + (size_t)v * pitch, plane, w + v * w_ld, dim, threadIdx.x & 31);
 }
 
 // ---- joins -------------------------------------------------------------------
@@ -834,99 +890,133 @@ __device__ __forceinline__ void merge2(float &m, float &s, float m2, float s2) {
   m = top;
 }
 
-// One warp per row: the pairs' partial statistics of its tile, and its target's logit.
-template <typename T>
-__global__ void ce_rows_kernel(const T *__restrict__ x, long x_ld, const T *__restrict__ w, long w_ld,
-                               const T *__restrict__ bias, const int32_t *__restrict__ tg,
-                               const int32_t *__restrict__ slot, const int *__restrict__ count, long rows, int dim,
-                               int tiles_n, int pairs, const float2 *__restrict__ stats, float *row_loss, float *lse) {
-  const int lane = threadIdx.x & 31;
-  const long n = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (n >= rows) return;
-  const int at = slot[n];
-  if (at < 0) {
-    if (lane == 0) {
-      row_loss[n] = 0.f;
-      if (lse) lse[n] = 0.f;
-    }
-    return;
-  }
-  const long t = tg[n];
-  float dot = 0.f;
-  for (int c = lane; c < dim; c += 32) dot = fmaf(op_load<T>(x[n * x_ld + c]), op_load<T>(w[t * w_ld + c]), dot);
-  dot = warp_sum(dot);
-  // pairs that worked on this row tile (see Units): pair of tile i = ((i + 1) pairs - 1) / total
-  const long m = at / kTileM, total = (long)((*count + kTileM - 1) / kTileM) * tiles_n;
-  const long p0 = ((m * tiles_n + 1) * pairs - 1) / total, p1 = ((m + 1) * tiles_n * pairs - 1) / total;
-  float top = -INFINITY, sum = 0.f;
-  for (long i = lane; i < 2 * (p1 - p0 + 1); i += 32) {
-    const long p = p0 + i / 2;
-    if (p * total / pairs == (p + 1) * total / pairs) continue;  // fewer tiles than pairs: this one had none
-    const float2 v = stats[((size_t)(p + m) * 2 + i % 2) * kTileM + at % kTileM];
-    merge2(top, sum, v.x, v.y);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, top, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
-    merge2(top, sum, m2, s2);
-  }
-  if (lane == 0) {
-    const float l = (top + log2f(sum)) * kLn2;
-    if (lse) lse[n] = l;
-    row_loss[n] = l - (dot + (bias ? op_load<T>(bias[t]) : 0.f));
-  }
-}
+struct RowsArgs {
+  const void *x, *w, *bias;
+  long x_ld, w_ld, rows;
+  const int32_t *tg, *slot;
+  const int *count;
+  int dim, tiles_n, pairs, mean;
+  const float2 *stats;
+  float *row_loss, *lse, *loss;
+  unsigned int *ticket;
+};
 
-// loss: the rows' sum in a fixed order.
-__global__ void __launch_bounds__(1024) ce_loss_kernel(const float *__restrict__ row_loss, long rows,
-                                                       const int *__restrict__ count, int mean, float *loss) {
+// One warp per row: joins the pairs' partial statistics of its tile and forms its
+// target's logit.  The CTA that finishes last adds the rows' losses in a fixed order.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) ce_rows_kernel(const RowsArgs a) {
   __shared__ float red[2 * 8 * 32];
+  __shared__ bool last;
+  op_begin();
+  const int lane = threadIdx.x & 31;
+  const long n = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const T *w = static_cast<const T *>(a.w), *bias = static_cast<const T *>(a.bias);
+  const int count = *a.count;
+  const int at = n < a.rows ? a.slot[n] : -1;
+  if (at >= 0) {
+    const long t = a.tg[n];
+    const T *xr = static_cast<const T *>(a.x) + n * a.x_ld, *wr = w + t * a.w_ld;
+    float dot = 0.f;
+    for (int c = lane * VEC; c < a.dim; c += 32 * VEC) {
+      float p[VEC], q[VEC];
+      op_load_vec<T, VEC>(xr + c, p);
+      op_load_vec<T, VEC>(wr + c, q);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dot = fmaf(p[i], q[i], dot);
+    }
+    // pairs that worked on this row tile (see Units): pair of tile i = ((i + 1) pairs - 1) / total
+    const long m = at / kTileM, total = (long)row_tiles(count) * a.tiles_n;
+    const long p0 = ((m * a.tiles_n + 1) * a.pairs - 1) / total, p1 = ((m + 1) * a.tiles_n * a.pairs - 1) / total;
+    float top = -INFINITY, sum = 0.f;
+    for (long i = lane; i < 2 * (p1 - p0 + 1); i += 32) {
+      const long p = p0 + i / 2;
+      // fewer tiles than pairs: some had none
+      if (total < a.pairs && p * total / a.pairs == (p + 1) * total / a.pairs) continue;
+      const float2 v = a.stats[((size_t)(p + m) * 2 + i % 2) * kTileM + at % kTileM];
+      merge2(top, sum, v.x, v.y);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      const float m2 = __shfl_xor_sync(0xffffffffu, top, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
+      merge2(top, sum, m2, s2);
+    }
+    if (lane == 0) {
+      const float l = (top + log2f(sum)) * kLn2;
+      if (a.lse) a.lse[n] = l;
+      a.row_loss[n] = l - (dot + (bias ? op_load<T>(bias[t]) : 0.f));
+    }
+  } else if (n < a.rows && lane == 0) {
+    a.row_loss[n] = 0.f;
+    if (a.lse) a.lse[n] = 0.f;
+  }
+  if (!a.loss) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
   BlockReducer br(red);
   float v[1] = {0.f};
-  for (long n = threadIdx.x; n < rows; n += 1024) v[0] += row_loss[n];
+#pragma unroll 8
+  for (long i = threadIdx.x; i < a.rows; i += 256) v[0] += __ldcg(a.row_loss + i);
   br.sum<1>(v);
-  if (threadIdx.x == 0) *loss = mean ? v[0] / fmaxf((float)*count, 1.f) : v[0];
+  if (threadIdx.x == 0) *a.loss = a.mean ? v[0] / fmaxf((float)count, 1.f) : v[0];
 }
 
-// dx: the slabs added in order, scaled, back to the rows' places.
+// dx: the slabs added in order, scaled, back to the rows' places.  A CTA takes
+// `per_cta` rows, 8 / per_cta warps each.
 template <typename T>
-__global__ void ce_dx_kernel(const float *__restrict__ slab, size_t slab_stride, int pitch, const MmaArgs a, int last_k,
-                             int pairs, const int32_t *__restrict__ slot, long rows, T *dx, long dx_ld) {
-  const int lane = threadIdx.x & 31;
-  const long n = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (n >= rows) return;
-  const int at = slot[n], count = *a.count;
-  const float c = grad_scale(a.dloss, a.count, a.mean) / a.g_scale;
-  const Deal full = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs, pairs);
-  const Deal last = deal_of(count, last_k * kBlockK / kTileM, a.tiles_d, last_k, a.want_dw, a.slabs, pairs);
-  for (int t = 0; t < a.tiles_d; ++t) {
-    const long tile = (long)(at / kTileM) * a.tiles_d + t;
-    const int slabs = at < 0 ? 0 : max(full.cover(tile), last.cover(tile));
-    const int end = min(a.dim, (t + 1) * a.bn);
-    for (int i = t * a.bn + lane; i < end; i += 32) {
-      float s = 0.f;
-      for (int k = 0; k < slabs; ++k) s += slab[k * slab_stride + (size_t)at * pitch + i];
-      dx[n * dx_ld + i] = op_store<T>(c * s);
+__global__ void __launch_bounds__(256) ce_dx_kernel(const float *slab, size_t slab_stride, int pitch, const MmaArgs a,
+                                                    int last_k, int pairs, const int32_t *slot, long rows, int per_cta,
+                                                    int vec, T *dx, long dx_ld) {
+  extern __shared__ uint8_t cover[];  // [2][tiles_d] slabs of the CTA's row tiles
+  op_begin();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, count = *a.count;
+  const long r0 = (long)blockIdx.x * per_cta;
+  const int per_row = 8 / per_cta;
+  const long n = r0 + warp / per_row;
+  // consecutive rows have consecutive places: they lie in two row tiles at most
+  int first = 0x7fffffff;
+  for (int i = 0; i < per_cta; ++i)
+    if (r0 + i < rows && slot[r0 + i] >= 0) first = min(first, slot[r0 + i] / kTileM);
+  if (first < 0x7fffffff) {
+    const Deal full = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs, pairs);
+    const Deal last = deal_of(count, last_k * kBlockK / kTileM, a.tiles_d, last_k, a.want_dw, a.slabs, pairs);
+    for (int t = threadIdx.x; t < 2 * a.tiles_d; t += 256) {
+      const long tile = (long)first * a.tiles_d + t;
+      cover[t] = tile < (long)row_tiles(count) * a.tiles_d ? (uint8_t)max(full.cover(tile), last.cover(tile)) : 0;
     }
   }
-}
-
-// db of a piece: the sums of 32 rows each added in order, 32 columns and 8 strided
-// partial sums per CTA.
-template <typename T>
-__global__ void ce_db_kernel(const float *__restrict__ part, long pitch, const int *__restrict__ count, int v0, int vocab,
-                             const float *__restrict__ dloss, int mean, float inv_g, T *db) {
-  __shared__ float sh[8][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = row_tiles(*count) * 8;
-  float s = 0.f;
-#pragma unroll 4
-  for (int g = warp; g < groups; g += 8) s += part[g * pitch + blockIdx.x * 32 + lane];
-  sh[warp][lane] = s;
   __syncthreads();
-  const int v = v0 + blockIdx.x * 32 + lane;
-  if (warp == 0 && v < vocab) {
-    for (int k = 1; k < 8; ++k) s += sh[k][lane];
-    db[v] = op_store<T>(grad_scale(dloss, count, mean) * inv_g * s);
+  if (n >= rows) return;
+  const int at = slot[n];
+  const float c = grad_scale(a.dloss, a.count, a.mean) / a.g_scale;
+  const uint8_t *mine = cover + (at >= 0 && at / kTileM != first ? a.tiles_d : 0);
+  for (int i = ((warp % per_row) * 32 + lane) * 4; i < a.dim; i += per_row * 128) {
+    float s[4] = {};
+    if (at >= 0) {
+      const int slabs = mine[i / a.bn];
+      const float *p = slab + (size_t)at * pitch + i;  // whole groups of 4: the pitch has room for them
+#pragma unroll 8
+      for (int k = 0; k < slabs; ++k) {
+        float v[4];
+        op_load_vec<float, 4>(p + k * slab_stride, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] *= c;
+    T *o = dx + n * dx_ld + i;
+    if (vec) {
+      op_store_vec<T, 4>(o, s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < a.dim) o[e] = op_store<T>(s[e]);
+    }
   }
 }
 
@@ -952,6 +1042,7 @@ struct Plan {
   // loss
   int32_t *slot;
   int *count;
+  unsigned int *ticket;
   uint16_t *xc, *wc;
   float2 *stats;
   float *row_loss;
@@ -1007,6 +1098,7 @@ Plan make_plan(const aideen_linear_ce_args *a, void *ws) {
   OpCarve c(ws);
   p.slot = c.take<int32_t>(a->rows);
   p.count = c.take<int>(1);
+  p.ticket = c.take<unsigned int>(1);
   p.xc = c.take<uint16_t>(p.xplane * p.planes);
   p.wc = c.take<uint16_t>(p.w_direct ? 0 : p.wplane * p.planes);
   OpCarve g = c;
@@ -1065,8 +1157,7 @@ cudaError_t launch_as(const Plan &p, const Maps &maps, MmaArgs a, cudaStream_t s
   auto kernel = ce_mma_kernel<MODE, T, HELD>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<2 * p.pairs, kThreads, smem, st>>>(maps, a);
-  return cudaGetLastError();
+  return op_launch(kernel, 2 * p.pairs, kThreads, smem, st, maps, a);
 }
 template <int MODE, typename T>
 cudaError_t launch_mma(const Plan &p, const Maps &maps, const MmaArgs &a, cudaStream_t st) {
@@ -1079,13 +1170,20 @@ cudaError_t launch_mma(const Plan &p, const Maps &maps, const MmaArgs &a, cudaSt
 template <typename T>
 cudaError_t stage_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, const T *w, const int32_t *tg,
                       const float *lse, cudaStream_t st) {
-  ce_index_kernel<<<1, 1024, 0, st>>>(tg, g->rows, (int)g->vocab, p.slot, p.count);
-  ce_stage_rows_kernel<T><<<(unsigned)((g->rows + kTileM + 7) / 8), 256, 0, st>>>(
-      x, g->x_ld, tg, p.slot, p.count, g->rows, (int)g->dim, p.pitch, p.xplane, p.xc, lse, p.lse_c, p.tgt);
-  if (!p.w_direct)
-    ce_stage_w_kernel<T><<<(unsigned)((g->vocab + 7) / 8), 256, 0, st>>>(w, g->w_ld, g->vocab, (int)g->dim, p.pitch,
-                                                                        p.wplane, p.wc);
-  return cudaGetLastError();
+  constexpr int V = 16 / sizeof(T);
+  StageArgs s{};
+  s.x = x; s.x_ld = g->x_ld; s.rows = g->rows; s.tg = tg; s.vocab = (int)g->vocab; s.dim = (int)g->dim;
+  s.pitch = p.pitch; s.plane = p.xplane; s.xc = p.xc; s.slot = p.slot; s.count = p.count; s.ticket = p.ticket;
+  s.lse = lse; s.lse_c = p.lse_c; s.tgt = p.tgt;
+  const long most = 4L * 2 * p.pairs;  // CTAs
+  s.per_cta = (int)(32 * ((g->rows + 32 * most - 1) / (32 * most)));
+  const unsigned ctas = (unsigned)((g->rows + s.per_cta - 1) / s.per_cta);
+  const bool xv = g->dim % V == 0 && op_vec16(x, g->x_ld, sizeof(T));
+  cudaError_t e = op_launch(xv ? ce_stage_rows_kernel<T, V> : ce_stage_rows_kernel<T, 1>, ctas, 256, 0, st, s);
+  if (e != cudaSuccess || p.w_direct) return e;
+  const bool wv = g->dim % V == 0 && op_vec16(w, g->w_ld, sizeof(T));
+  return op_launch(wv ? ce_stage_w_kernel<T, V> : ce_stage_w_kernel<T, 1>, (g->vocab + 7) / 8, 256, 0, st, w, g->w_ld,
+                   g->vocab, g->dim, p.pitch, p.wplane, p.wc);
 }
 
 template <typename T>
@@ -1113,12 +1211,13 @@ cudaError_t loss_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
   a.stats = p.stats;
   e = launch_mma<kStats, T>(p, maps, a, st);
   if (e != cudaSuccess) return e;
-  float *rl = row_loss ? row_loss : p.row_loss;
-  ce_rows_kernel<T><<<(unsigned)((g->rows + 7) / 8), 256, 0, st>>>(x, g->x_ld, w, g->w_ld, bias, tg, p.slot, p.count,
-                                                                   g->rows, (int)g->dim, p.tiles_n, p.pairs, p.stats,
-                                                                   rl, lse);
-  if (loss) ce_loss_kernel<<<1, 1024, 0, st>>>(rl, g->rows, p.count, a.mean, loss);
-  return cudaGetLastError();
+  RowsArgs r{};
+  r.x = x; r.w = w; r.bias = bias; r.x_ld = g->x_ld; r.w_ld = g->w_ld; r.rows = g->rows; r.tg = tg; r.slot = p.slot;
+  r.count = p.count; r.dim = (int)g->dim; r.tiles_n = p.tiles_n; r.pairs = p.pairs; r.mean = a.mean; r.stats = p.stats;
+  r.row_loss = row_loss ? row_loss : p.row_loss; r.lse = lse; r.loss = loss; r.ticket = p.ticket;
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = g->dim % V == 0 && op_vec16(x, g->x_ld, sizeof(T)) && op_vec16(w, g->w_ld, sizeof(T));
+  return op_launch(vec ? ce_rows_kernel<T, V> : ce_rows_kernel<T, 1>, (g->rows + 7) / 8, 256, 0, st, r);
 }
 
 template <typename T>
@@ -1146,27 +1245,24 @@ cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
   a.lse = p.lse_c; a.tgt = p.tgt; a.db_part = db ? p.db_part : nullptr;
   a.bn = p.bn; a.tiles_d = p.tiles_d; a.slabs = dx ? p.slabs : 0; a.want_dw = dw != nullptr;
   a.full_k = p.piece / kBlockK;
-  a.dw = dw; a.dw_ld = g->dw_ld; a.dw_tma = dw_tma; a.dloss = dloss;
+  a.dw = dw; a.db = db; a.dw_ld = g->dw_ld; a.dw_tma = dw_tma; a.dloss = dloss;
   for (int v0 = 0; v0 < (int)g->vocab; v0 += p.piece) {
     const int left = (int)g->vocab - v0, cols = left < p.piece ? (left + kTileN - 1) / kTileN * kTileN : p.piece;
     a.v0 = v0;
     a.tiles_n = cols / kTileN;
     e = launch_mma<kPiece, T>(p, lm, a, st);
     if (e != cudaSuccess) return e;
-    if (db)
-      ce_db_kernel<T><<<cols / 32, 256, 0, st>>>(p.db_part, cols, p.count, v0, (int)g->vocab, dloss, a.mean,
-                                                 1.f / a.g_scale, db);
-    if (dx || dw) {
-      a.piece_k = cols / kBlockK;
-      a.first = v0 == 0;
-      e = launch_mma<kProducts, T>(p, pm, a, st);
-      if (e != cudaSuccess) return e;
-    }
+    a.piece_k = cols / kBlockK;
+    a.first = v0 == 0;
+    e = launch_mma<kProducts, T>(p, pm, a, st);
+    if (e != cudaSuccess) return e;
   }
-  if (dx)
-    ce_dx_kernel<T><<<(unsigned)((g->rows + 7) / 8), 256, 0, st>>>(p.slab, (size_t)p.mpad * p.dpitch, (int)p.dpitch, a,
-                                                                   a.piece_k, p.pairs, p.slot, g->rows, dx, g->dx_ld);
-  return cudaGetLastError();
+  if (!dx) return cudaSuccess;
+  const bool vec = dim % 4 == 0 && g->dx_ld % 4 == 0 && op_aligned(dx, 4 * el);
+  const int per_cta = g->rows >= 4096 ? 8 : 2;  // with few rows there are many slabs: more warps on each
+  return op_launch(ce_dx_kernel<T>, (g->rows + per_cta - 1) / per_cta, 256, 2 * p.tiles_d, st, p.slab,
+                   (size_t)p.mpad * p.dpitch, p.dpitch, a, a.piece_k, p.pairs, p.slot, g->rows, per_cta, vec, dx,
+                   g->dx_ld);
 }
 
 template <typename T>

@@ -47,6 +47,29 @@ struct OpCarve {
   }
 };
 
+// Launches of one call follow each other as programmatic dependents: a kernel may
+// be placed, and set up what it needs, while the one before it in the stream drains.
+// So every kernel of an operator calls op_begin() in all threads before it touches
+// global memory, which waits until everything before it is complete and visible.
+template <typename... P, typename... A>
+cudaError_t op_launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+__device__ __forceinline__ void op_begin() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 #define OP_CHECK(cond, why)                        \
   do {                                             \
     if (!(cond)) return aideen::op_invalid(why);   \
