@@ -34,6 +34,7 @@ constexpr int kDigits = 256;
 template <typename T, int VEC>
 __global__ void embed_kernel(const int32_t *__restrict__ ids, const T *__restrict__ table, T *__restrict__ out,
                              long n, int dim, int vocab, float scale, long table_ld, long rows_ld) {
+  op_begin();
   const int lane = threadIdx.x & 31;
   const long row = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (row >= n) return;
@@ -79,6 +80,7 @@ __device__ __forceinline__ uint32_t sort_key(int32_t id, uint32_t vocab) {
 
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads)
     embed_sort_kernel(const SortArgs s) {
+  op_begin();
   if (blockIdx.x >= kSortCtas) {  // the clusters past the first clear the gradient
     const size_t t = (size_t)(blockIdx.x - kSortCtas) * kSortThreads + threadIdx.x;
     const size_t step = (size_t)(gridDim.x - kSortCtas) * kSortThreads;
@@ -209,6 +211,7 @@ __device__ __forceinline__ void embed_finish(const SumArgs &a, uint32_t key, int
 // access (blockIdx.y picks 32 of them).  Keys are uniform over the warp.
 template <typename T, int VEC>
 __global__ void embed_sum_kernel(const SumArgs a) {
+  op_begin();
   const int lane = threadIdx.x & 31;
   const uint32_t tile = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const unsigned long long begin = (unsigned long long)tile * a.tile;
@@ -272,6 +275,7 @@ __global__ void embed_sum_kernel(const SumArgs a) {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) embed_join_kernel(const SumArgs a) {
   __shared__ float sh[8][32 * VEC];
+  op_begin();
   const uint32_t tile = blockIdx.x;
   const uint32_t lo = tile * (uint32_t)a.tile;
   const unsigned long long end = (unsigned long long)lo + a.tile;
@@ -335,20 +339,17 @@ GradPlan grad_plan(const aideen_embed_args *args, void *ws) {
 template <typename T, int VEC>
 cudaError_t embed_run(const aideen_embed_args *a, const int32_t *ids, const void *table, void *out, cudaStream_t st) {
   const int warps = a->n_tokens < 8 ? (int)a->n_tokens : 8;
-  embed_kernel<T, VEC><<<(unsigned)(((long)a->n_tokens + warps - 1) / warps), warps * 32, 0, st>>>(
-      ids, static_cast<const T *>(table), static_cast<T *>(out), a->n_tokens, (int)a->dim, (int)a->vocab, a->scale,
-      a->table_ld, a->rows_ld);
-  return cudaGetLastError();
+  return op_launch(embed_kernel<T, VEC>, (unsigned)(((long)a->n_tokens + warps - 1) / warps), warps * 32, 0, st, ids,
+                   static_cast<const T *>(table), static_cast<T *>(out), a->n_tokens, a->dim, a->vocab, a->scale,
+                   a->table_ld, a->rows_ld);
 }
 
 template <typename T, int VEC>
 cudaError_t sum_run(const SumArgs &s, uint32_t tiles, cudaStream_t st) {
   const unsigned slabs = (unsigned)((s.dim + 32 * VEC - 1) / (32 * VEC));
-  embed_sum_kernel<T, VEC><<<dim3((tiles + 7) / 8, slabs), 256, 0, st>>>(s);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = op_launch(embed_sum_kernel<T, VEC>, dim3((tiles + 7) / 8, slabs), 256, 0, st, s);
   if (e != cudaSuccess || tiles < 2) return e;
-  embed_join_kernel<T, VEC><<<dim3(tiles - 1, slabs), 256, 0, st>>>(s);
-  return cudaGetLastError();
+  return op_launch(embed_join_kernel<T, VEC>, dim3(tiles - 1, slabs), 256, 0, st, s);
 }
 
 int check_args(const aideen_embed_args *a) {
@@ -426,8 +427,7 @@ extern "C" int aideen_embed_grad(const aideen_embed_args *args, const int32_t *i
     const size_t want = op_round(ctas, kSortCtas);
     grid += (unsigned)(want < most || most == 0 ? want : most);
   }
-  embed_sort_kernel<<<grid, kSortThreads, 0, st>>>(s);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = op_launch(embed_sort_kernel, grid, kSortThreads, 0, st, s);
   if (e != cudaSuccess || args->n_tokens == 0) return op_cuda(e);
   SumArgs m{};
   m.sorted = p.a; m.dout = dout; m.grad = table_grad; m.part = p.part;

@@ -5,20 +5,29 @@
 //   dx = r (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
 //
 // Bound: HBM (forward reads x and writes y, the gradient reads x and dy and
-// writes dx).  A row stays in the registers of the warps that own it, at most
-// 16 elements per lane, so it is read once: the variance is the mean of the
-// squared differences from the finished mean, not E[x^2] - m^2.  Rows of up to
-// 8192 elements take 1 to 16 warps; longer ones are walked in memory.
+// writes dx).  A row stays in the registers of the warps that own it, 64 bytes per
+// lane at most, so it is read once: the variance is the mean of the squared
+// differences from the finished mean, not E[x^2] - m^2.  A row takes 1 to 16 warps (8 in the
+// gradient, whose column sums need the registers); longer ones are walked in memory.
+#include <type_traits>
+
 #include "common.cuh"
 #include "operators.cuh"
 
 namespace aideen {
 namespace {
 
-constexpr int kLnThreads = 256;       // threads of a CTA (512 when a row needs 16 warps)
-constexpr int kLnLane = 16;           // most elements of a row per lane
-constexpr int kLnMaxWarps = 16;       // most warps per row
-constexpr int kLnMaxDim = kLnLane * 32 * kLnMaxWarps;
+// Most warps that share a row in registers; longer rows are walked in memory.
+constexpr int kLnMaxWarps = 16, kLnMaxGradWarps = 8;
+
+// The gradient's CTAs by the accesses per lane of a row (the rows at work and the
+// column sums stay in registers).
+template <int NV>
+struct LnShape {
+  static constexpr int threads = NV == 1 ? 512 : 256;
+  static constexpr int per_sm = NV == 4 ? 1 : 2;
+  static constexpr int rows = NV == 4 ? 1 : 2;  // that a group of warps works on at a time
+};
 
 struct LnArgs {
   const void *x, *dy, *w, *b;
@@ -54,66 +63,123 @@ __device__ __forceinline__ void row_sum(float (&v)[K], int wpr, int group, float
   }
 }
 
-// One row per group of wpr warps.  NV accesses of VEC elements per lane.
-template <typename T, int VEC, int NV>
-__global__ void layer_norm_kernel(const LnArgs a) {
+// One access of a lane: VEC elements, worked on as pairs (two float32 lanes per
+// instruction; a scalar access is a pair whose second half is 0).
+template <typename T, int VEC>
+struct LnAccess {
+  static constexpr int P = VEC == 1 ? 1 : VEC / 2;
+  OpVec<T, VEC> v;
+  __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const OpVec<T, VEC> *>(p); }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v.v[i] = op_store<T>(0.f);
+  }
+  __device__ __forceinline__ float2 get(int i) const {
+    if constexpr (VEC == 1) {
+      return make_float2(op_load<T>(v.v[0]), 0.f);
+    } else if constexpr (sizeof(T) == 4) {
+      return make_float2(v.v[2 * i], v.v[2 * i + 1]);
+    } else {
+      const uint32_t u = reinterpret_cast<const uint32_t *>(&v)[i];
+      if constexpr (std::is_same<T, __half>::value) return __half22float2(reinterpret_cast<const __half2 &>(u));
+      else return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    }
+  }
+  __device__ __forceinline__ void set(int i, float2 f) {
+    if constexpr (VEC == 1) {
+      v.v[0] = op_store<T>(f.x);
+    } else if constexpr (sizeof(T) == 4) {
+      v.v[2 * i] = f.x;
+      v.v[2 * i + 1] = f.y;
+    } else if constexpr (std::is_same<T, __half>::value) {
+      reinterpret_cast<__half2 *>(&v)[i] = __float22half2_rn(f);
+    } else {
+      reinterpret_cast<__nv_bfloat162 *>(&v)[i] = __float22bfloat162_rn(f);
+    }
+  }
+  __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<OpVec<T, VEC> *>(p) = v; }
+};
+__device__ __forceinline__ float2 pair(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+
+// The part of a row that a lane holds: N accesses, `step` elements apart (zeros behind the row).
+template <typename T, int VEC, int N>
+struct LnRow {
+  LnAccess<T, VEC> v[N];
+  __device__ __forceinline__ void load(const T *row, int c0, int step, int dim) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      v[j].clear();  // first: a store into the registers of a load in flight would wait for it
+      if (c0 + j * step < dim) v[j].load(row + c0 + j * step);
+    }
+  }
+};
+
+// One row per group of wpr warps.
+template <typename T, int VEC, int NV, bool AFFINE>
+__global__ void __launch_bounds__(512, 2) layer_norm_kernel(const LnArgs a) {
+  constexpr int N = VEC == 1 ? 4 * NV : NV, P = LnAccess<T, VEC>::P;
   __shared__ float red[2 * 16];
+  op_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = warp / a.wpr, groups = (int)(blockDim.x >> 5) / a.wpr;
-  const int at = (warp % a.wpr) * 32 + lane, step = 32 * a.wpr * VEC;
+  const int c0 = ((warp % a.wpr) * 32 + lane) * VEC, step = 32 * a.wpr * VEC;
   const long row = (long)blockIdx.x * groups + group;
-  if (group >= groups || row >= a.rows) return;  // whole groups leave together
-  const T *x = static_cast<const T *>(a.x) + row * a.x_ld;
-  float v[NV][VEC];
-  float s[1] = {0.f};
+  if (row >= a.rows) return;  // whole groups leave together
+  const float inv = 1.f / (float)a.dim;
+  float2 d[N][P], t = pair(0.f);
+  {
+    LnRow<T, VEC, N> v;
+    v.load(static_cast<const T *>(a.x) + row * a.x_ld, c0, step, a.dim);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = at * VEC + j * step;
-    if (c < a.dim) {
-      op_load_vec<T, VEC>(x + c, v[j]);
-    } else {
+    for (int j = 0; j < N; ++j)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) s[0] += v[j][i];
+      for (int i = 0; i < P; ++i) t = add2(t, d[j][i] = v.v[j].get(i));
   }
   int parity = 0;
+  float s[1] = {t.x + t.y};
   row_sum<1>(s, a.wpr, group, red, parity);
-  const float m = s[0] / (float)a.dim;
-  s[0] = 0.f;
+  const float m = s[0] * inv;
+  t = pair(0.f);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (at * VEC + j * step < a.dim) {
+  for (int j = 0; j < N; ++j) {
+    if (c0 + j * step < a.dim) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float c = v[j][i] - m;
-        s[0] += c * c;
+      for (int i = 0; i < P; ++i) {
+        d[j][i] = add2(d[j][i], pair(-m));
+        if (VEC == 1) d[j][i].y = 0.f;
+        t = fma2(d[j][i], d[j][i], t);
       }
     }
   }
+  s[0] = t.x + t.y;
   row_sum<1>(s, a.wpr, group, red, parity);
-  const float r = 1.f / sqrtf(s[0] / (float)a.dim + a.eps);
-  if (at == 0) {
+  const float r = 1.f / sqrtf(s[0] * inv + a.eps);
+  if (c0 == 0) {
     if (a.mean) a.mean[row] = m;
     if (a.rstd) a.rstd[row] = r;
   }
-  T *y = static_cast<T *>(a.y) + row * a.y_ld;
+  const T *w = static_cast<const T *>(a.w) + c0, *b = static_cast<const T *>(a.b) + c0;
+  T *y = static_cast<T *>(a.y) + row * a.y_ld + c0;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = at * VEC + j * step;
-    if (c >= a.dim) continue;
-    float w[VEC], b[VEC];
-    if (a.w) op_load_vec<T, VEC>(static_cast<const T *>(a.w) + c, w);
-    if (a.b) op_load_vec<T, VEC>(static_cast<const T *>(a.b) + c, b);
+  for (int j = 0; j < N; ++j) {
+    if (c0 + j * step >= a.dim) continue;
+    LnAccess<T, VEC> k, q, o;
+    if (AFFINE || a.w) k.load(w + j * step);
+    if (AFFINE || a.b) q.load(b + j * step);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      float o = (v[j][i] - m) * r;
-      if (a.w) o *= w[i];
-      if (a.b) o += b[i];
-      v[j][i] = o;
+    for (int i = 0; i < P; ++i) {
+      float2 f = mul2(d[j][i], pair(r));
+      if constexpr (AFFINE) {
+        f = fma2(f, k.get(i), q.get(i));
+      } else {
+        if (a.w) f = mul2(f, k.get(i));
+        if (a.b) f = add2(f, q.get(i));
+      }
+      o.set(i, f);
     }
-    op_store_vec<T, VEC>(y + c, v[j]);
+    o.store(y + j * step);
   }
 }
 
@@ -121,6 +187,7 @@ __global__ void layer_norm_kernel(const LnArgs a) {
 template <typename T>
 __global__ void layer_norm_long_kernel(const LnArgs a) {
   __shared__ float red[2 * 8 * 32];
+  op_begin();
   BlockReducer br(red);
   const long row = blockIdx.x;
   const T *x = static_cast<const T *>(a.x) + row * a.x_ld;
@@ -149,65 +216,89 @@ __global__ void layer_norm_long_kernel(const LnArgs a) {
   }
 }
 
-// Gradient: each group of warps takes rows group, group + all groups, ... and
+// Gradient: each group of warps takes every so many rows and
 // keeps its columns' sums of dy xh and dy in registers; the CTA's groups are
 // added through shared memory in group order into one row of `part`.
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(512) layer_norm_grad_kernel(const LnArgs a) {
+template <typename T, int VEC, int NV, bool WEIGHT>
+__global__ void __launch_bounds__(LnShape<NV>::threads, LnShape<NV>::per_sm) layer_norm_grad_kernel(const LnArgs a) {
+  constexpr int N = VEC == 1 ? 4 * NV : NV, P = LnAccess<T, VEC>::P, R = LnShape<NV>::rows;
   extern __shared__ float sh[];  // [2][dim] when several groups share a CTA
-  __shared__ float red[2 * 2 * 16];
+  __shared__ float red[2 * 2 * R * 16];
+  op_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = warp / a.wpr, groups = (int)(blockDim.x >> 5) / a.wpr;
-  const int at = (warp % a.wpr) * 32 + lane, step = 32 * a.wpr * VEC;
-  float aw[NV][VEC], ab[NV][VEC];
+  const int c0 = ((warp % a.wpr) * 32 + lane) * VEC, step = 32 * a.wpr * VEC;
+  const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy);
+  const T *w = static_cast<const T *>(a.w) + c0;
+  float2 aw[N][P], ab[N][P];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < N; ++j)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) aw[j][i] = ab[j][i] = 0.f;
+    for (int i = 0; i < P; ++i) aw[j][i] = ab[j][i] = pair(0.f);
   int parity = 0;
   const float inv = 1.f / (float)a.dim;
-  for (long row = (long)blockIdx.x * groups + group; row < a.rows; row += (long)gridDim.x * groups) {
-    const T *x = static_cast<const T *>(a.x) + row * a.x_ld;
-    const T *dy = static_cast<const T *>(a.dy) + row * a.y_ld;
-    const float m = a.mean[row], r = a.rstd[row];
-    float xh[NV][VEC], g[NV][VEC];
-    float s[2] = {0.f, 0.f};
+  // R rows at a time: their loads are in flight together and share one reduction
+  for (long row0 = ((long)blockIdx.x * groups + group) * R; row0 < a.rows; row0 += (long)gridDim.x * groups * R) {
+    LnRow<T, VEC, N> xv[R], gv[R];
+    float m[R], r[R];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = at * VEC + j * step;
-      if (c < a.dim) {
-        op_load_vec<T, VEC>(x + c, xh[j]);
-        op_load_vec<T, VEC>(dy + c, g[j]);
-      }
+    for (int q = 0; q < R; ++q) {
+      const long row = row0 + q;
+      const int dim = row < a.rows ? a.dim : 0;  // rows behind the last are zeros and add nothing
+      xv[q].load(x + row * a.x_ld, c0, step, dim);
+      gv[q].load(dy + row * a.y_ld, c0, step, dim);
+      m[q] = dim ? a.mean[row] : 0.f;
+      r[q] = dim ? a.rstd[row] : 0.f;
     }
+    // dy is 0 behind a row (and in a scalar access's second half), so nothing is added there
+    float2 s0[R], s1[R];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = at * VEC + j * step;
-      if (c < a.dim) {
-        float w[VEC];
-        if (a.w) op_load_vec<T, VEC>(static_cast<const T *>(a.w) + c, w);
+    for (int q = 0; q < R; ++q) s0[q] = s1[q] = pair(0.f);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          xh[j][i] = (xh[j][i] - m) * r;
-          aw[j][i] += g[j][i] * xh[j][i];
-          ab[j][i] += g[j][i];
-          if (a.w) g[j][i] *= w[i];
-          s[0] += g[j][i];
-          s[1] += g[j][i] * xh[j][i];
+    for (int j = 0; j < N; ++j) {
+      if (c0 + j * step >= a.dim) continue;
+      LnAccess<T, VEC> k;
+      if (WEIGHT) k.load(w + j * step);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float2 wk = WEIGHT ? k.get(i) : pair(1.f);
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+          const float2 xh = mul2(add2(xv[q].v[j].get(i), pair(-m[q])), pair(r[q])), d = gv[q].v[j].get(i);
+          aw[j][i] = fma2(d, xh, aw[j][i]);
+          ab[j][i] = add2(ab[j][i], d);
+          const float2 g = WEIGHT ? mul2(d, wk) : d;
+          s0[q] = add2(s0[q], g);
+          s1[q] = fma2(g, xh, s1[q]);
         }
       }
     }
     if (!a.dx) continue;
-    row_sum<2>(s, a.wpr, group, red, parity);
-    const float c1 = s[0] * inv, c2 = s[1] * inv;
-    T *dx = static_cast<T *>(a.dx) + row * a.dx_ld;
+    float s[2 * R];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = at * VEC + j * step;
-      if (c >= a.dim) continue;
+    for (int q = 0; q < R; ++q) {
+      s[2 * q] = s0[q].x + s0[q].y;
+      s[2 * q + 1] = s1[q].x + s1[q].y;
+    }
+    row_sum<2 * R>(s, a.wpr, group, red, parity);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) g[j][i] = r * (g[j][i] - c1 - xh[j][i] * c2);
-      op_store_vec<T, VEC>(dx + c, g[j]);
+    for (int j = 0; j < N; ++j) {
+      if (c0 + j * step >= a.dim) continue;
+      LnAccess<T, VEC> k;
+      if (WEIGHT) k.load(w + j * step);
+#pragma unroll
+      for (int q = 0; q < R; ++q) {
+        if (row0 + q >= a.rows) break;
+        const float2 c1 = pair(-s[2 * q] * inv), c2 = pair(-s[2 * q + 1] * inv);
+        LnAccess<T, VEC> o;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const float2 xh = mul2(add2(xv[q].v[j].get(i), pair(-m[q])), pair(r[q]));
+          const float2 g = add2((WEIGHT ? mul2(gv[q].v[j].get(i), k.get(i)) : gv[q].v[j].get(i)), c1);
+          o.set(i, mul2(fma2(xh, c2, g), pair(r[q])));
+        }
+        o.store(static_cast<T *>(a.dx) + (row0 + q) * a.dx_ld + c0 + j * step);
+      }
     }
   }
   if (!a.part) return;
@@ -215,12 +306,12 @@ __global__ void __launch_bounds__(512) layer_norm_grad_kernel(const LnArgs a) {
   for (int k = 0; k < groups; ++k) {
     if (group == k) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = at * VEC + j * step;
+      for (int j = 0; j < N; ++j) {
+        const int c = c0 + j * step;
         if (c >= a.dim) continue;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          float pw = aw[j][i], pb = ab[j][i];
+          float pw = i & 1 ? aw[j][i / 2].y : aw[j][i / 2].x, pb = i & 1 ? ab[j][i / 2].y : ab[j][i / 2].x;
           if (k > 0) {
             pw += sh[c + i];
             pb += sh[a.dim + c + i];
@@ -243,6 +334,7 @@ __global__ void __launch_bounds__(512) layer_norm_grad_kernel(const LnArgs a) {
 template <typename T>
 __global__ void layer_norm_grad_long_kernel(const LnArgs a) {
   __shared__ float red[2 * 8 * 32];
+  op_begin();
   BlockReducer br(red);
   const long row = blockIdx.x;
   const T *x = static_cast<const T *>(a.x) + row * a.x_ld;
@@ -266,6 +358,7 @@ __global__ void layer_norm_grad_long_kernel(const LnArgs a) {
 }
 template <typename T>
 __global__ void layer_norm_columns_kernel(const LnArgs a) {
+  op_begin();
   const int c = blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= a.dim) return;
   const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy);
@@ -280,96 +373,91 @@ __global__ void layer_norm_columns_kernel(const LnArgs a) {
 }
 
 // dweight and dbias: the rows of `part` added in a fixed order, 32 columns and
-// 8 strided partial sums per CTA (blockIdx.y: 0 = dweight, 1 = dbias).
+// 32 strided partial sums per CTA (blockIdx.y: 0 = dweight, 1 = dbias).
 template <typename T>
-__global__ void layer_norm_finish_kernel(const float *part, int n, int dim, T *dw, T *db) {
-  __shared__ float sh[8][33];
+__global__ void __launch_bounds__(1024) layer_norm_finish_kernel(const float *part, int n, int dim, T *dw, T *db) {
+  __shared__ float sh[32][33];
+  op_begin();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + tx;
   T *out = blockIdx.y ? db : dw;
   if (!out) return;
   float s = 0.f;
   if (c < dim) {
-#pragma unroll 4
-    for (int i = ty; i < n; i += 8) s += part[((size_t)i * 2 + blockIdx.y) * dim + c];
+#pragma unroll 8
+    for (int i = ty; i < n; i += 32) s += part[((size_t)i * 2 + blockIdx.y) * dim + c];
   }
   sh[ty][tx] = s;
   __syncthreads();
-  if (ty == 0 && c < dim) {
-    float t = sh[0][tx];
-#pragma unroll
-    for (int k = 1; k < 8; ++k) t += sh[k][tx];
-    out[c] = op_store<T>(t);
-  }
+  const float t = warp_sum(sh[tx][ty]);  // warp ty: column ty's 32 partial sums
+  if (tx == 0 && blockIdx.x * 32 + ty < dim) out[blockIdx.x * 32 + ty] = op_store<T>(t);
 }
 
-// The fewest warps that hold a row at kLnLane elements per lane.
-int warps_per_row(int dim) {
-  int w = 1;
-  while (w * 32 * kLnLane < dim) w *= 2;
-  return w;
+// How a row is spread.  Forward: as few accesses per lane (1, 2 or 4) as hold it in one
+// warp, then as many warps as it takes.  Gradient: up to 2 warps before a lane takes
+// more, so that the column sums leave room for many rows in flight.
+struct Spread {
+  int nv, wpr, threads, groups, per_sm, rows;
+};
+Spread spread(int dim, int elem, bool vec, bool grad) {
+  Spread s{};
+  const int one = vec ? 16 / elem : 4;  // elements of a lane's nv = 1
+  s.nv = 1;
+  while (s.nv < 4 && 32 * (grad ? 2 : 1) * one * s.nv < dim) s.nv *= 2;
+  s.wpr = 1;
+  while (32 * one * s.nv * s.wpr < dim) s.wpr *= 2;
+  s.threads = grad && s.nv == 1 ? LnShape<1>::threads : 256;
+  if (s.threads < 32 * s.wpr) s.threads = 32 * s.wpr;
+  s.groups = s.threads / 32 / s.wpr;
+  s.rows = s.nv == 4 ? LnShape<4>::rows : s.nv == 2 ? LnShape<2>::rows : LnShape<1>::rows;
+  s.per_sm = s.nv == 4 ? LnShape<4>::per_sm : s.nv == 2 ? LnShape<2>::per_sm : LnShape<1>::per_sm;
+  return s;
 }
 
-int grad_ctas(const aideen_layer_norm_args *a) {
-  if (a->dim > (uint32_t)kLnMaxDim) return a->rows < 64 ? (int)a->rows : 64;
-  const int wpr = warps_per_row((int)a->dim);
-  const int groups = (wpr == 16 ? 16 : kLnThreads / 32) / wpr;
-  const long need = ((long)a->rows + groups - 1) / groups;
-  const long most = 2L * op_sm_count();
+// CTAs of the gradient, each leaving one partial row of sums.
+int grad_ctas(const aideen_layer_norm_args *a, const Spread &s) {
+  if (s.wpr > kLnMaxGradWarps) return a->rows < 64 ? (int)a->rows : 64;
+  const long need = ((long)a->rows + s.groups - 1) / s.groups;  // one row per group while there are few
+  const long most = (long)s.per_sm * op_sm_count();
   return (int)(need < most ? need : most);
 }
 
 template <typename T, int VEC, int NV>
-cudaError_t forward_run(const LnArgs &a, cudaStream_t st) {
-  const int threads = a.wpr == 16 ? 512 : kLnThreads, groups = threads / 32 / a.wpr;
-  layer_norm_kernel<T, VEC, NV><<<(unsigned)((a.rows + groups - 1) / groups), threads, 0, st>>>(a);
-  return cudaGetLastError();
+cudaError_t forward_run(const LnArgs &a, const Spread &s, cudaStream_t st) {
+  return op_launch(a.w && a.b ? layer_norm_kernel<T, VEC, NV, true> : layer_norm_kernel<T, VEC, NV, false>,
+                   (unsigned)((a.rows + s.groups - 1) / s.groups), s.threads, 0, st, a);
 }
 
 template <typename T, int VEC, int NV>
-cudaError_t grad_run(const LnArgs &a, int ctas, cudaStream_t st) {
-  const int threads = a.wpr == 16 ? 512 : kLnThreads, groups = threads / 32 / a.wpr;
-  const size_t smem = groups > 1 && a.part ? (size_t)2 * a.dim * sizeof(float) : 0;
-  layer_norm_grad_kernel<T, VEC, NV><<<ctas, threads, smem, st>>>(a);
-  return cudaGetLastError();
+cudaError_t grad_run(const LnArgs &a, const Spread &s, int ctas, cudaStream_t st) {
+  const size_t smem = s.groups > 1 && a.part ? (size_t)2 * a.dim * sizeof(float) : 0;
+  return op_launch(a.w ? layer_norm_grad_kernel<T, VEC, NV, true> : layer_norm_grad_kernel<T, VEC, NV, false>, ctas, s.threads, smem, st, a);
 }
 
 template <typename T>
-cudaError_t forward_typed(const LnArgs &a, bool vec, cudaStream_t st) {
-  if (a.dim > kLnMaxDim) {
-    layer_norm_long_kernel<T><<<(unsigned)a.rows, 1024, 0, st>>>(a);
-    return cudaGetLastError();
-  }
+cudaError_t forward_typed(const LnArgs &a, const Spread &s, bool vec, cudaStream_t st) {
+  if (s.wpr > kLnMaxWarps) return op_launch(layer_norm_long_kernel<T>, (unsigned)a.rows, 1024, 0, st, a);
   constexpr int V = 16 / sizeof(T);
-  // fewer accesses per lane where the row is short: no idle register tiles
-  const int lane = (a.dim + 32 * a.wpr - 1) / (32 * a.wpr);
-  if (!vec) return lane <= 4 ? forward_run<T, 1, 4>(a, st) : forward_run<T, 1, kLnLane>(a, st);
-  if (lane <= V) return forward_run<T, V, 1>(a, st);
-  return forward_run<T, V, kLnLane / V>(a, st);
+  if (vec) return s.nv == 1 ? forward_run<T, V, 1>(a, s, st) : s.nv == 2 ? forward_run<T, V, 2>(a, s, st) : forward_run<T, V, 4>(a, s, st);
+  return s.nv == 1 ? forward_run<T, 1, 1>(a, s, st) : s.nv == 2 ? forward_run<T, 1, 2>(a, s, st) : forward_run<T, 1, 4>(a, s, st);
 }
 
 template <typename T>
-cudaError_t grad_typed(LnArgs a, bool vec, int ctas, T *dw, T *db, cudaStream_t st) {
+cudaError_t grad_typed(const LnArgs &a, const Spread &s, bool vec, int ctas, T *dw, T *db, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
-  if (a.dim > kLnMaxDim) {
-    if (a.dx) {
-      layer_norm_grad_long_kernel<T><<<(unsigned)a.rows, 1024, 0, st>>>(a);
-      e = cudaGetLastError();
-    }
-    if (e == cudaSuccess && a.part) {
-      layer_norm_columns_kernel<T><<<dim3((a.dim + 255) / 256, ctas), 256, 0, st>>>(a);
-      e = cudaGetLastError();
-    }
+  if (s.wpr > kLnMaxGradWarps) {
+    if (a.dx) e = op_launch(layer_norm_grad_long_kernel<T>, (unsigned)a.rows, 1024, 0, st, a);
+    if (e == cudaSuccess && a.part)
+      e = op_launch(layer_norm_columns_kernel<T>, dim3((a.dim + 255) / 256, ctas), 256, 0, st, a);
   } else {
     constexpr int V = 16 / sizeof(T);
-    const int lane = (a.dim + 32 * a.wpr - 1) / (32 * a.wpr);
-    if (!vec) e = lane <= 4 ? grad_run<T, 1, 4>(a, ctas, st) : grad_run<T, 1, kLnLane>(a, ctas, st);
-    else if (lane <= V) e = grad_run<T, V, 1>(a, ctas, st);
-    else e = grad_run<T, V, kLnLane / V>(a, ctas, st);
+    if (vec)
+      e = s.nv == 1 ? grad_run<T, V, 1>(a, s, ctas, st) : s.nv == 2 ? grad_run<T, V, 2>(a, s, ctas, st) : grad_run<T, V, 4>(a, s, ctas, st);
+    else
+      e = s.nv == 1 ? grad_run<T, 1, 1>(a, s, ctas, st) : s.nv == 2 ? grad_run<T, 1, 2>(a, s, ctas, st) : grad_run<T, 1, 4>(a, s, ctas, st);
   }
   if (e != cudaSuccess || !a.part) return e;
-  layer_norm_finish_kernel<T><<<dim3((a.dim + 31) / 32, 2), 256, 0, st>>>(a.part, ctas, a.dim, dw, db);
-  return cudaGetLastError();
+  return op_launch(layer_norm_finish_kernel<T>, dim3((a.dim + 31) / 32, 2), 1024, 0, st, a.part, ctas, a.dim, dw, db);
 }
 
 int check_args(const aideen_layer_norm_args *a) {
@@ -401,20 +489,24 @@ extern "C" int aideen_layer_norm(const aideen_layer_norm_args *args, const void 
   a.x = x; a.w = weight; a.b = bias; a.y = y; a.mean = mean; a.rstd = rstd;
   a.rows = args->rows; a.dim = (int)args->dim; a.eps = args->eps;
   a.x_ld = args->x_ld; a.y_ld = args->y_ld;
-  a.wpr = warps_per_row(a.dim);
   const bool vec = ((size_t)a.dim * el) % 16 == 0 && op_vec16(x, a.x_ld, el) && op_vec16(y, a.y_ld, el) &&
                    op_aligned(weight, 16) && op_aligned(bias, 16);
+  const Spread s = spread(a.dim, (int)el, vec, false);
+  a.wpr = s.wpr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (args->dtype == AIDEEN_F32) return op_cuda(forward_typed<float>(a, vec, st));
-  if (args->dtype == AIDEEN_BF16) return op_cuda(forward_typed<__nv_bfloat16>(a, vec, st));
-  return op_cuda(forward_typed<__half>(a, vec, st));
+  if (args->dtype == AIDEEN_F32) return op_cuda(forward_typed<float>(a, s, vec, st));
+  if (args->dtype == AIDEEN_BF16) return op_cuda(forward_typed<__nv_bfloat16>(a, s, vec, st));
+  return op_cuda(forward_typed<__half>(a, s, vec, st));
 }
 
 extern "C" int aideen_layer_norm_grad_workspace(const aideen_layer_norm_args *args, size_t *bytes) {
   const int rc = check_args(args);
   if (rc != AIDEEN_OK) return rc;
   OP_CHECK(bytes, "layer_norm: null bytes");
-  *bytes = op_round((size_t)grad_ctas(args) * 2 * args->dim * sizeof(float), 256);
+  // either way the rows may be read, whatever the addresses
+  const int el = (int)op_elem(args->dtype);
+  const int c0 = grad_ctas(args, spread((int)args->dim, el, false, true)), c1 = grad_ctas(args, spread((int)args->dim, el, true, true));
+  *bytes = op_round((size_t)(c0 > c1 ? c0 : c1) * 2 * args->dim * sizeof(float), 256);
   return AIDEEN_OK;
 }
 
@@ -448,14 +540,15 @@ extern "C" int aideen_layer_norm_grad(const aideen_layer_norm_args *args, const 
   a.part = sums ? static_cast<float *>(workspace) : nullptr;
   a.rows = args->rows; a.dim = (int)args->dim; a.eps = args->eps;
   a.x_ld = args->x_ld; a.y_ld = args->y_ld; a.dx_ld = args->dx_ld;
-  a.wpr = warps_per_row(a.dim);
   const bool vec = ((size_t)a.dim * el) % 16 == 0 && op_vec16(x, a.x_ld, el) && op_vec16(dy, a.y_ld, el) &&
                    (!dx || op_vec16(dx, a.dx_ld, el)) && op_aligned(weight, 16);
-  const int ctas = grad_ctas(args);
+  const Spread s = spread(a.dim, (int)el, vec, true);
+  a.wpr = s.wpr;
+  const int ctas = grad_ctas(args, s);
   if (args->dtype == AIDEEN_F32)
-    return op_cuda(grad_typed<float>(a, vec, ctas, static_cast<float *>(dweight), static_cast<float *>(dbias), st));
+    return op_cuda(grad_typed<float>(a, s, vec, ctas, static_cast<float *>(dweight), static_cast<float *>(dbias), st));
   if (args->dtype == AIDEEN_BF16)
-    return op_cuda(grad_typed<__nv_bfloat16>(a, vec, ctas, static_cast<__nv_bfloat16 *>(dweight),
+    return op_cuda(grad_typed<__nv_bfloat16>(a, s, vec, ctas, static_cast<__nv_bfloat16 *>(dweight),
                                              static_cast<__nv_bfloat16 *>(dbias), st));
-  return op_cuda(grad_typed<__half>(a, vec, ctas, static_cast<__half *>(dweight), static_cast<__half *>(dbias), st));
+  return op_cuda(grad_typed<__half>(a, s, vec, ctas, static_cast<__half *>(dweight), static_cast<__half *>(dbias), st));
 }

@@ -706,14 +706,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int k = 0; k < 32; ++k) v[h][k] *= scale;
             const int vrow = a.v0 + row0;
-            if (!a.dw_tma) {
-              if (vrow + lane < a.vocab) {
-                T *o = static_cast<T *>(a.dw) + (long)(vrow + lane) * a.dw_ld;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                  for (int k = 0; k < 32; ++k)
-                    if (col + 32 * h + k < a.dim) o[col + 32 * h + k] = op_store<T>(v[h][k]);
+            if (!a.dw_tma) {  // through a box, so that a warp writes along rows
+              T *o = static_cast<T *>(a.dw) + (long)vrow * a.dw_ld + col;
+              for (int h = 0; h < (sizeof(T) == 2 ? 1 : 2); ++h) {
+                constexpr int kCols = 128 / sizeof(T);
+                unsigned char *bx = box.take();
+                if constexpr (sizeof(T) == 2) {
+                  box_put16<T>(bx, lane, 0, v[0]);
+                  box_put16<T>(bx, lane, 1, v[1]);
+                } else {
+                  box_put32(bx, lane, h ? v[1] : v[0]);
+                }
+                __syncwarp();
+                const int rows = min(32, a.vocab - vrow), cols = min(kCols, a.dim - col - h * 32);
+#pragma unroll 4
+                for (int r = 0; r < rows; ++r)
+                  for (int c = lane; c < cols; c += 32)
+                    o[(long)r * a.dw_ld + h * 32 + c] =
+                        *reinterpret_cast<const T *>(bx + r * 128 + (((c * (int)sizeof(T)) ^ ((r & 7) * 16))));
+                __syncwarp();
               }
             } else if constexpr (sizeof(T) == 2) {
               if (col < a.dim && vrow < a.vocab) {
@@ -776,6 +787,7 @@ __device__ __forceinline__ void put_pieces(uint16_t *dst, size_t plane, float v)
 // access where the addresses allow.
 template <typename T, int VEC>
 __device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *src, int dim, int lane) {
+#pragma unroll 4
   for (int c = lane * VEC; c < dim; c += 32 * VEC) {
     if constexpr (VEC == 1) {
       put_pieces<T>(dst + c, plane, src ? op_load<T>(src[c]) : 0.f);
@@ -805,7 +817,7 @@ struct StageArgs {
   const void *x;
   long x_ld, rows;
   const int32_t *tg;
-  int vocab, dim, pitch, per_cta;  // rows per CTA, a multiple of 32
+  int vocab, dim, pitch, per_cta;  // rows per CTA, a multiple of 8
   size_t plane;
   uint16_t *xc;
   int32_t *slot;
@@ -850,23 +862,20 @@ __global__ void __launch_bounds__(256) ce_stage_rows_kernel(const StageArgs a) {
     *a.ticket = 0;
   }
   const T *x = static_cast<const T *>(a.x);
-  for (long g0 = r0; g0 < a.rows && g0 < r0 + a.per_cta; g0 += 32) {  // 32 rows at a time, 4 per warp
-    const int32_t t = g0 + lane < a.rows ? a.tg[g0 + lane] : -1;
+  for (long g0 = r0; g0 < a.rows && g0 < r0 + a.per_cta; g0 += 8) {  // 8 rows at a time, one per warp
+    const int32_t t = lane < 8 && g0 + lane < a.rows ? a.tg[g0 + lane] : -1;
     const bool in = counted(t, a.vocab);
     const uint32_t mask = __ballot_sync(0xffffffffu, in);
     const int at = before + __popc(mask & ((1u << lane) - 1u));
-    if (warp == 0 && g0 + lane < a.rows) {
+    if (warp == 0 && lane < 8 && g0 + lane < a.rows) {
       a.slot[g0 + lane] = in ? at : -1;
       if (in && a.lse) {
         a.lse_c[at] = a.lse[g0 + lane];
         a.tgt[at] = t;
       }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int k = warp * 4 + i, to = __shfl_sync(0xffffffffu, at, k);
-      if (mask >> k & 1) put_row<T, VEC>(a.xc + (size_t)to * a.pitch, a.plane, x + (g0 + k) * a.x_ld, a.dim, lane);
-    }
+    const int to = __shfl_sync(0xffffffffu, at, warp);
+    if (mask >> warp & 1) put_row<T, VEC>(a.xc + (size_t)to * a.pitch, a.plane, x + (g0 + warp) * a.x_ld, a.dim, lane);
     before += __popc(mask);
   }
   const long end = (long)row_tiles(total) * kTileM;
@@ -1176,7 +1185,7 @@ cudaError_t stage_run(const aideen_linear_ce_args *g, const Plan &p, const T *x,
   s.pitch = p.pitch; s.plane = p.xplane; s.xc = p.xc; s.slot = p.slot; s.count = p.count; s.ticket = p.ticket;
   s.lse = lse; s.lse_c = p.lse_c; s.tgt = p.tgt;
   const long most = 4L * 2 * p.pairs;  // CTAs
-  s.per_cta = (int)(32 * ((g->rows + 32 * most - 1) / (32 * most)));
+  s.per_cta = (int)(8 * ((g->rows + 8 * most - 1) / (8 * most)));
   const unsigned ctas = (unsigned)((g->rows + s.per_cta - 1) / s.per_cta);
   const bool xv = g->dim % V == 0 && op_vec16(x, g->x_ld, sizeof(T));
   cudaError_t e = op_launch(xv ? ce_stage_rows_kernel<T, V> : ce_stage_rows_kernel<T, 1>, ctas, 256, 0, st, s);
