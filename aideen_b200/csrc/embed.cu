@@ -6,17 +6,17 @@
 // the launch for a few tokens).
 //
 // Gradient, bound by HBM (dout read once, the table's gradient written once):
-//   1. one cluster of 8 CTAs sorts (id, position) stably, by least-significant
-//      digits of at most 8 bits; every warp ranks its own run of keys with
-//      match.any, the CTAs exchange their digit counts through distributed
+//   1. one cluster of 8 CTAs (one CTA while it can hold the keys) sorts (id, position) stably, by least-significant
+//      digits of at most 8 bits; every warp ranks its own run of keys by
+//      votes, the CTAs exchange their digit counts through distributed
 //      shared memory, and a hardware cluster barrier separates the steps.  The
 //      sort is latency, not bandwidth, so the other CTAs of the same launch
 //      clear the table's gradient meanwhile.
-//   2. the sorted positions are cut into equal tiles, one warp each (per 32
+//   2. the sorted positions are cut into tiles of 8, one warp each (per 32
 //      accesses of a row), whatever the ids are: a frequent id spreads over
 //      many tiles.  A run of one id inside a tile is summed and stored; a run
 //      that crosses tiles leaves float32 partial rows.
-//   3. the partial rows of each crossing run are added in tile order.
+//   3. the partial rows of each crossing run are added in a fixed order.
 // Nothing is added with atomics: the same call gives the same bits.
 #include <cooperative_groups.h>
 
@@ -66,88 +66,156 @@ struct SortArgs {
   const int32_t *ids;
   unsigned long long *a, *b;  // sorted (key << 32 | position) ends in `a`
   uint32_t n, vocab;
-  int passes, digit_bits;
+  int passes, digit_bits, ctas;  // ctas: that sort, 1 or the whole cluster
   // table gradient to clear, or null: rows of row_bytes at a stride of ld_bytes
   unsigned char *clear;
   size_t row_bytes, ld_bytes;
   int clear16;  // rows can be cleared 16 bytes at a time
 };
 
+// Lanes of `live` whose digit is this lane's: one vote per bit (a quarter of the time
+// of match.any here).
+__device__ __forceinline__ uint32_t same_digit(uint32_t live, uint32_t d, int bits) {
+  uint32_t same = live;
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    if (b >= bits) break;
+    const uint32_t v = __ballot_sync(0xffffffffu, d >> b & 1);
+    same &= d >> b & 1 ? v : ~v;
+  }
+  return same;
+}
+
 // Keys are the ids, every id outside [0, vocab) as vocab (sorted last).
 __device__ __forceinline__ uint32_t sort_key(int32_t id, uint32_t vocab) {
   return id >= 0 && (uint32_t)id < vocab ? (uint32_t)id : vocab;
 }
 
+// Clears the rows: whole 32 KB blocks of zeros go out of shared memory by bulk copy
+// where the rows are contiguous, else plain stores.
+__device__ __forceinline__ void clear_rows(const SortArgs &s, uint32_t *zeros, size_t cta, size_t ctas) {
+  constexpr size_t kBlock = sizeof(uint32_t) * kSortWarps * kDigits;
+  const size_t t = cta * kSortThreads + threadIdx.x, step = ctas * kSortThreads;
+  if (s.clear16 && s.row_bytes == s.ld_bytes) {
+    for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) zeros[i] = 0;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    const size_t total = s.row_bytes * s.vocab;
+    if (threadIdx.x == 0) {
+      for (size_t at = cta * kBlock; at < total; at += ctas * kBlock) {
+        const uint32_t n = (uint32_t)(total - at < kBlock ? total - at : kBlock);
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(s.clear + at),
+                     "r"(static_cast<uint32_t>(__cvta_generic_to_shared(zeros))), "r"(n)
+                     : "memory");
+      }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+  } else if (s.clear16) {
+    const size_t per = s.row_bytes / 16, total = per * s.vocab;
+    for (size_t i = t; i < total; i += step)
+      *reinterpret_cast<uint4 *>(s.clear + i / per * s.ld_bytes + i % per * 16) = make_uint4(0, 0, 0, 0);
+  } else {
+    const size_t per = s.row_bytes / 2, total = per * s.vocab;
+    for (size_t i = t; i < total; i += step)
+      *reinterpret_cast<uint16_t *>(s.clear + i / per * s.ld_bytes + i % per * 2) = 0;
+  }
+}
+
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads)
     embed_sort_kernel(const SortArgs s) {
-  op_begin();
-  if (blockIdx.x >= kSortCtas) {  // the clusters past the first clear the gradient
-    const size_t t = (size_t)(blockIdx.x - kSortCtas) * kSortThreads + threadIdx.x;
-    const size_t step = (size_t)(gridDim.x - kSortCtas) * kSortThreads;
-    if (s.clear16 && s.row_bytes == s.ld_bytes) {
-      const size_t total = s.row_bytes / 16 * s.vocab;
-      for (size_t i = t; i < total; i += step) reinterpret_cast<uint4 *>(s.clear)[i] = make_uint4(0, 0, 0, 0);
-    } else if (s.clear16) {
-      const size_t per = s.row_bytes / 16, total = per * s.vocab;
-      for (size_t i = t; i < total; i += step)
-        *reinterpret_cast<uint4 *>(s.clear + i / per * s.ld_bytes + i % per * 16) = make_uint4(0, 0, 0, 0);
-    } else {
-      const size_t per = s.row_bytes / 2, total = per * s.vocab;
-      for (size_t i = t; i < total; i += step)
-        *reinterpret_cast<uint16_t *>(s.clear + i / per * s.ld_bytes + i % per * 2) = 0;
-    }
-    return;
-  }
-  __shared__ uint32_t hist[kSortWarps][kDigits];
+  __shared__ __align__(16) uint32_t hist[kSortWarps][kDigits];
   __shared__ uint32_t total[kDigits];  // this CTA's keys per digit, read by its peers
   __shared__ uint32_t wsum[8];
+  op_begin();
+  if (blockIdx.x >= kSortCtas) {  // the clusters past the first clear the gradient
+    clear_rows(s, &hist[0][0], blockIdx.x - kSortCtas, gridDim.x - kSortCtas);
+    return;
+  }
   cg::cluster_group cluster = cg::this_cluster();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster.block_rank();
-  // every warp of the cluster owns one contiguous run of positions
-  const uint32_t run = (s.n + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps);
+  if (rank >= s.ctas) return;
+  auto sync_all = [&]() {
+    if (s.ctas == 1) __syncthreads();
+    else cluster.sync();
+  };
+  uint32_t count[kSortWarps];
+  // every warp of the sorting CTAs owns one contiguous run of positions
+  const uint32_t run = (s.n + s.ctas * kSortWarps - 1) / (s.ctas * kSortWarps);
   const uint32_t w = (uint32_t)(rank * kSortWarps + warp);
   const uint32_t lo = (unsigned long long)w * run < s.n ? w * run : s.n;
   const uint32_t hi = s.n - lo < run ? s.n : lo + run;
   const uint32_t mask = (1u << s.digit_bits) - 1u;
   const uint32_t below = (1u << lane) - 1u;
+  constexpr int U = 8;  // keys per lane loaded ahead
   for (int p = 0; p < s.passes; ++p) {
     const int shift = p * s.digit_bits;
     // the last pass writes into `a`
     unsigned long long *dst = ((s.passes - 1 - p) & 1) ? s.b : s.a;
     const unsigned long long *src = ((s.passes - 1 - p) & 1) ? s.a : s.b;
-    auto load = [&](uint32_t i) -> unsigned long long {
-      if (p == 0) return (unsigned long long)sort_key(s.ids[i], s.vocab) << 32 | i;
-      return __ldcg(src + i);  // written by another CTA of the cluster
+    auto load = [&](uint32_t i0, unsigned long long (&kv)[U]) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t i = i0 + u * 32 + lane;
+        kv[u] = 0;
+        if (i < hi) {
+          if (p == 0) kv[u] = (unsigned long long)sort_key(s.ids[i], s.vocab) << 32 | i;
+          else kv[u] = __ldcg(src + i);  // written by another CTA of the cluster
+        }
+      }
     };
     for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
-    for (uint32_t i0 = lo; i0 < hi; i0 += 32) {
-      const bool in = i0 + lane < hi;
-      const uint32_t live = __ballot_sync(0xffffffffu, in);
-      if (in) {
-        const uint32_t d = ((uint32_t)(load(i0 + lane) >> 32) >> shift) & mask;
-        const uint32_t same = __match_any_sync(live, d);
-        if ((same & below) == 0) hist[warp][d] += __popc(same);
+    unsigned long long kv[U];
+    uint32_t same[U];
+    auto peers = [&](uint32_t i0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        same[u] = 0;
+        if (i0 + u * 32 >= hi) continue;
+        const bool in = i0 + u * 32 + lane < hi;
+        const uint32_t live = __ballot_sync(0xffffffffu, in);
+        const uint32_t peer = same_digit(live, ((uint32_t)(kv[u] >> 32) >> shift) & mask, s.digit_bits);
+        if (in) same[u] = peer;
       }
-      __syncwarp();
+    };
+    for (uint32_t i0 = lo; i0 < hi; i0 += 32 * U) {
+      load(i0, kv);
+      peers(i0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {  // the first lane of each digit counts its peers
+        if (i0 + u * 32 >= hi) break;
+        if (same[u] && (same[u] & below) == 0) hist[warp][((uint32_t)(kv[u] >> 32) >> shift) & mask] += __popc(same[u]);
+        __syncwarp();
+      }
     }
     __syncthreads();
     if (threadIdx.x < kDigits) {  // counts of the warps before, per digit
       uint32_t sum = 0;
+#pragma unroll
+      for (int k = 0; k < kSortWarps; ++k) count[k] = hist[k][threadIdx.x];
+#pragma unroll
       for (int k = 0; k < kSortWarps; ++k) {
-        const uint32_t c = hist[k][threadIdx.x];
-        hist[k][threadIdx.x] = sum;
+        const uint32_t c = count[k];
+        count[k] = sum;
         sum += c;
       }
       total[threadIdx.x] = sum;
     }
-    cluster.sync();
+    sync_all();
     uint32_t before = 0, all = 0, x = 0;
     if (threadIdx.x < kDigits) {
-      for (int c = 0; c < kSortCtas; ++c) {
-        const uint32_t v = *cluster.map_shared_rank(&total[threadIdx.x], c);
-        if (c < rank) before += v;
-        all += v;
+      if (s.ctas == 1) {
+        all = total[threadIdx.x];
+      } else {
+        uint32_t v[kSortCtas];
+#pragma unroll
+        for (int c = 0; c < kSortCtas; ++c) v[c] = *cluster.map_shared_rank(&total[threadIdx.x], c);
+#pragma unroll
+        for (int c = 0; c < kSortCtas; ++c) {
+          if (c < rank) before += v[c];
+          all += v[c];
+        }
       }
       x = all;  // inclusive scan over the digits
 #pragma unroll
@@ -161,26 +229,31 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
     if (threadIdx.x < kDigits) {
       uint32_t base = x - all + before;
       for (int k = 0; k < warp; ++k) base += wsum[k];
-      for (int k = 0; k < kSortWarps; ++k) hist[k][threadIdx.x] += base;
+#pragma unroll
+      for (int k = 0; k < kSortWarps; ++k) hist[k][threadIdx.x] = count[k] + base;
     }
     __syncthreads();
-    for (uint32_t i0 = lo; i0 < hi; i0 += 32) {
-      const bool in = i0 + lane < hi;
-      const uint32_t live = __ballot_sync(0xffffffffu, in);
-      uint32_t d = 0, same = 0;
-      if (in) {
-        const unsigned long long kv = load(i0 + lane);
-        d = ((uint32_t)(kv >> 32) >> shift) & mask;
-        same = __match_any_sync(live, d);
-        dst[hist[warp][d] + __popc(same & below)] = kv;
+    for (uint32_t i0 = lo; i0 < hi; i0 += 32 * U) {
+      if (hi - lo > 32 * U) {  // else they are still here
+        load(i0, kv);
+        peers(i0);
       }
-      __syncwarp();
-      if (in && (same & below) == 0) hist[warp][d] += __popc(same);
-      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u * 32 >= hi) break;
+        const uint32_t d = ((uint32_t)(kv[u] >> 32) >> shift) & mask;
+        if (same[u]) dst[hist[warp][d] + __popc(same[u] & below)] = kv[u];
+        __syncwarp();
+        if (same[u] && (same[u] & below) == 0) hist[warp][d] += __popc(same[u]);
+        __syncwarp();
+      }
     }
-    cluster.sync();  // the pass's writes and reads of `total` are done everywhere
+    sync_all();  // the pass's writes and reads of `total` are done everywhere
   }
 }
+
+constexpr int kTile = 8;        // sorted positions per warp: their rows are all in flight together
+constexpr int kJoinWarps = 32;  // tiles that a joining CTA looks at
 
 struct SumArgs {
   const unsigned long long *sorted;
@@ -188,10 +261,20 @@ struct SumArgs {
   void *grad;
   float *part;  // [tiles][2][dim]: the run that enters the tile, the run that leaves it
   uint32_t n, vocab;
-  int dim, tile, accumulate;
+  int dim, accumulate;
   float scale;
   long table_ld, rows_ld;
 };
+
+template <int VEC>
+__device__ __forceinline__ void part_store(float *p, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  }
+}
 
 template <typename T, int VEC>
 __device__ __forceinline__ void embed_finish(const SumArgs &a, uint32_t key, int c, float (&acc)[VEC]) {
@@ -207,116 +290,134 @@ __device__ __forceinline__ void embed_finish(const SumArgs &a, uint32_t key, int
   op_store_vec<T, VEC>(g, acc);
 }
 
-// One warp sums tile blockIdx.x * warps + warp over the columns of one lane's
-// access (blockIdx.y picks 32 of them).  Keys are uniform over the warp.
+// One warp sums tile blockIdx.x * 8 + warp over the columns of one access per lane
+// (blockIdx.y picks 32 of them).  Keys are uniform over the warp.
 template <typename T, int VEC>
-__global__ void embed_sum_kernel(const SumArgs a) {
+__global__ void __launch_bounds__(256) embed_sum_kernel(const SumArgs a) {
   op_begin();
   const int lane = threadIdx.x & 31;
-  const uint32_t tile = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const unsigned long long begin = (unsigned long long)tile * a.tile;
+  const uint32_t tile = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const unsigned long long begin = (unsigned long long)tile * kTile;
   if (begin >= a.n) return;
-  const uint32_t lo = (uint32_t)begin, hi = a.n - lo < (uint32_t)a.tile ? a.n : lo + a.tile;
+  const uint32_t lo = (uint32_t)begin;
+  const int n = a.n - lo < kTile ? (int)(a.n - lo) : kTile;
   const int c = (blockIdx.y * 32 + lane) * VEC;
   const bool live = c < a.dim;
   const T *dout = static_cast<const T *>(a.dout) + c;
-  uint32_t key = (uint32_t)(a.sorted[lo] >> 32);
-  bool entered = lo > 0 && (uint32_t)(a.sorted[lo - 1] >> 32) == key;
-  float acc[VEC] = {};
-  constexpr int U = 8;  // rows in flight
-  for (uint32_t i0 = lo; i0 < hi; i0 += U) {
-    unsigned long long kv[U];
-    float v[U][VEC];
+  // lane 0: the position before the tile, lanes 1..n: the tile, lane n + 1: the one behind
+  const bool there = lane <= n + 1 && lo + lane >= 1 && lo + lane - 1 < a.n;
+  const unsigned long long mine = there ? a.sorted[lo + lane - 1] : ~0ull;
+  const uint32_t key = (uint32_t)(mine >> 32);
+  const uint32_t before = __shfl_up_sync(0xffffffffu, key, 1);
+  // bit i: position i of the tile begins a run; bit n: the run ends with the tile
+  const uint32_t starts = __ballot_sync(0xffffffffu, lane >= 1 && lane <= n + 1 && (!there || key != before)) >> 1;
+  OpVec<T, VEC> v[kTile];
 #pragma unroll
-    for (int u = 0; u < U; ++u) kv[u] = i0 + u < hi ? a.sorted[i0 + u] : ~0ull;
+  for (int u = 0; u < kTile; ++u) {
+    const unsigned long long kv = __shfl_sync(0xffffffffu, mine, u + 1);
+    if (live && u < n && (uint32_t)(kv >> 32) < a.vocab)
+      v[u] = *reinterpret_cast<const OpVec<T, VEC> *>(dout + (long)(uint32_t)kv * a.rows_ld);
+  }
+  for (int u0 = 0; u0 < n;) {
+    const uint32_t k = __shfl_sync(0xffffffffu, key, u0 + 1);
+    if (k >= a.vocab) break;  // outside the table: sorted last
+    const uint32_t later = starts >> (u0 + 1) << (u0 + 1);
+    const int u1 = later & ((1u << n) - 1u) ? __ffs(later) - 1 : n;
+    const bool entered = u0 == 0 && !(starts & 1u), leaves = u1 == n && !(starts >> n & 1u);
+    float acc[VEC] = {};
     if (live) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if ((uint32_t)(kv[u] >> 32) < a.vocab) op_load_vec<T, VEC>(dout + (long)(uint32_t)kv[u] * a.rows_ld, v[u]);
-    }
+      for (int u = 0; u < kTile; ++u) {
+        if (u < u0 || u >= u1) continue;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i0 + u >= hi) break;
-      const uint32_t k = (uint32_t)(kv[u] >> 32);
-      if (k != key) {  // the run before this position is complete
-        if (live && key < a.vocab) {
-          if (entered) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) a.part[(size_t)tile * 2 * a.dim + c + i] = acc[i];
-          } else {
-            embed_finish<T, VEC>(a, key, c, acc);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-        key = k;
-        entered = false;
+        for (int i = 0; i < VEC; ++i) acc[i] += op_load<T>(v[u].v[i]);
       }
-      if (live && k < a.vocab) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] += v[u][i];
-      }
+      if (entered || leaves) part_store<VEC>(a.part + ((size_t)tile * 2 + (entered ? 0 : 1)) * a.dim + c, acc);
+      else embed_finish<T, VEC>(a, k, c, acc);
     }
-  }
-  if (!live || key >= a.vocab) return;
-  const bool leaves = hi < a.n && (uint32_t)(a.sorted[hi] >> 32) == key;
-  if (entered || leaves) {
-    float *p = a.part + ((size_t)tile * 2 + (entered ? 0 : 1)) * a.dim + c;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) p[i] = acc[i];
-  } else {
-    embed_finish<T, VEC>(a, key, c, acc);
+    u0 = u1;
   }
 }
 
-// One CTA per tile whose last run begins in it and leaves it: adds the run's
-// partial rows.  Warp w takes the parts w, w + 8, ...; the warps are then added
-// in order.
+// Adds the partial rows of the runs that cross tiles, in a fixed order.  Each warp looks
+// at one tile: does its last run begin in it and leave it, and how many more tiles does
+// it enter?  Up to kShort of them the warp adds alone; longer runs take the whole CTA
+// (warp w adds the parts w, w + 32, ..., then the warps are added in order).
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) embed_join_kernel(const SumArgs a) {
-  __shared__ float sh[8][32 * VEC];
+__global__ void __launch_bounds__(32 * kJoinWarps) embed_join_kernel(const SumArgs a) {
+  constexpr uint32_t kShort = 16;
+  __shared__ float sh[kJoinWarps][32 * VEC];
+  __shared__ uint32_t more_of[kJoinWarps], key_of[kJoinWarps];
   op_begin();
-  const uint32_t tile = blockIdx.x;
-  const uint32_t lo = tile * (uint32_t)a.tile;
-  const unsigned long long end = (unsigned long long)lo + a.tile;
-  if (end >= a.n) return;
-  const uint32_t hi = (uint32_t)end;
-  const uint32_t key = (uint32_t)(a.sorted[hi - 1] >> 32);
-  if (key >= a.vocab || (uint32_t)(a.sorted[hi] >> 32) != key) return;          // nothing leaves
-  if ((uint32_t)(a.sorted[lo] >> 32) == key && lo > 0 && (uint32_t)(a.sorted[lo - 1] >> 32) == key) return;  // begun earlier
-  // first position behind the run
-  uint32_t l = hi, r = a.n;
-  while (l < r) {
-    const uint32_t m = l + (r - l) / 2;
-    if ((uint32_t)(a.sorted[m] >> 32) > key) r = m;
-    else l = m + 1;
-  }
-  const uint32_t last = (l - 1) / a.tile;  // the tile in which the run ends
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = (blockIdx.y * 32 + lane) * VEC;
-  float acc[VEC] = {};
-  if (c < a.dim) {
-#pragma unroll 4
-    for (uint32_t t = tile + warp; t <= last; t += 8) {
-      const float *p = a.part + ((size_t)t * 2 + (t == tile ? 1 : 0)) * a.dim + c;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] += p[i];
+  const uint32_t tile = blockIdx.x * kJoinWarps + warp;
+  const unsigned long long end = ((unsigned long long)tile + 1) * kTile;
+  uint32_t more = 0, key = ~0u;
+  if (end < a.n) {
+    const uint32_t hi = (uint32_t)end, lo = hi - kTile;
+    key = (uint32_t)(a.sorted[hi - 1] >> 32);
+    const uint32_t next = (uint32_t)(a.sorted[hi] >> 32), first = (uint32_t)(a.sorted[lo] >> 32);
+    const uint32_t prev = lo > 0 ? (uint32_t)(a.sorted[lo - 1] >> 32) : ~0u;
+    if (key < a.vocab && next == key && !(first == key && prev == key)) {
+      for (more = 1;; more += 32) {  // lane i: does the run leave tile + more + i too?
+        const unsigned long long at = ((unsigned long long)tile + more + lane + 1) * kTile;
+        const bool on = at < a.n && (uint32_t)(a.sorted[at] >> 32) == key;
+        const uint32_t off = __ballot_sync(0xffffffffu, !on);
+        if (off) {
+          more += __ffs(off) - 1;
+          break;
+        }
+      }
     }
   }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) sh[warp][lane * VEC + i] = acc[i];
-  __syncthreads();
-  if (warp != 0 || c >= a.dim) return;
-  for (int k = 1; k < 8; ++k) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] += sh[k][lane * VEC + i];
+  if (lane == 0) {
+    more_of[warp] = more;
+    key_of[warp] = key;
   }
-  embed_finish<T, VEC>(a, key, c, acc);
+  const int c = (blockIdx.y * 32 + lane) * VEC;
+  auto add = [&](uint32_t t0, uint32_t from, uint32_t by, uint32_t count, float (&acc)[VEC]) {
+    if (c >= a.dim) return;
+#pragma unroll 4
+    for (uint32_t t = from; t <= count; t += by) {
+      const float *p = a.part + ((size_t)(t0 + t) * 2 + (t == 0 ? 1 : 0)) * a.dim + c;
+      float v[VEC];
+      if constexpr (VEC == 1) {
+        v[0] = *p;
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+          const float4 x = *reinterpret_cast<const float4 *>(p + i);
+          v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] += v[i];
+    }
+  };
+  if (more > 0 && more <= kShort) {
+    float acc[VEC] = {};
+    add(tile, 0, 1, more, acc);
+    if (c < a.dim) embed_finish<T, VEC>(a, key, c, acc);
+  }
+  const uint32_t any = __syncthreads_or(more > kShort);
+  if (!any) return;
+  for (int k = 0; k < kJoinWarps; ++k) {
+    if (more_of[k] <= kShort) continue;
+    float acc[VEC] = {};
+    add(blockIdx.x * kJoinWarps + k, warp, kJoinWarps, more_of[k], acc);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sh[warp][lane * VEC + i] = acc[i];
+    __syncthreads();
+    if (warp == 0 && c < a.dim) {
+      for (int q = 1; q < kJoinWarps; ++q) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] += sh[q][lane * VEC + i];
+      }
+      embed_finish<T, VEC>(a, key_of[k], c, acc);
+    }
+    __syncthreads();
+  }
 }
-
-// Sorted positions per warp: enough warps to fill the GPU while there are few
-// tokens, few partial rows once there are many.
-int tile_of(uint32_t n) { return n <= 16384 ? 8 : 32; }
 
 struct GradPlan {
   unsigned long long *a, *b;
@@ -328,7 +429,7 @@ GradPlan grad_plan(const aideen_embed_args *args, void *ws) {
   GradPlan p{};
   OpCarve c(ws);
   const uint32_t n = args->n_tokens;
-  p.tiles = (uint32_t)(((unsigned long long)n + tile_of(n) - 1) / tile_of(n));
+  p.tiles = (n + kTile - 1) / kTile;
   p.a = c.take<unsigned long long>(n);
   p.b = c.take<unsigned long long>(n);
   p.part = c.take<float>((size_t)p.tiles * 2 * args->dim);
@@ -349,7 +450,7 @@ cudaError_t sum_run(const SumArgs &s, uint32_t tiles, cudaStream_t st) {
   const unsigned slabs = (unsigned)((s.dim + 32 * VEC - 1) / (32 * VEC));
   cudaError_t e = op_launch(embed_sum_kernel<T, VEC>, dim3((tiles + 7) / 8, slabs), 256, 0, st, s);
   if (e != cudaSuccess || tiles < 2) return e;
-  return op_launch(embed_join_kernel<T, VEC>, dim3(tiles - 1, slabs), 256, 0, st, s);
+  return op_launch(embed_join_kernel<T, VEC>, dim3((tiles + kJoinWarps - 1) / kJoinWarps, slabs), 32 * kJoinWarps, 0, st, s);
 }
 
 int check_args(const aideen_embed_args *a) {
@@ -415,23 +516,24 @@ extern "C" int aideen_embed_grad(const aideen_embed_args *args, const int32_t *i
   int bits = 1;
   while (args->vocab >> bits) ++bits;  // keys run up to vocab itself
   s.passes = args->n_tokens ? (bits + 7) / 8 : 0;
+  // one CTA holds 8 keys per lane: below that the cluster's barriers cost more than they save
+  s.ctas = args->n_tokens <= 8 * kSortThreads ? 1 : kSortCtas;
   s.digit_bits = s.passes ? (bits + s.passes - 1) / s.passes : 1;
   unsigned grid = kSortCtas;
   if (!args->accumulate) {
     s.clear = static_cast<unsigned char *>(table_grad);
     s.row_bytes = args->dim * el; s.ld_bytes = (size_t)args->table_ld * el;
     s.clear16 = s.row_bytes % 16 == 0 && op_vec16(table_grad, args->table_ld, el);
-    // one CTA of 1024 threads per remaining SM, in whole clusters, at most one pass over the table
+    // several CTAs per SM, so that uneven placement of the clusters evens out
     const size_t ctas = (s.row_bytes / (s.clear16 ? 16 : 2) * s.vocab + kSortThreads - 1) / kSortThreads;
-    const size_t most = (size_t)(op_sm_count() - kSortCtas) / kSortCtas * kSortCtas;
-    const size_t want = op_round(ctas, kSortCtas);
-    grid += (unsigned)(want < most || most == 0 ? want : most);
+    const size_t most = 4 * op_round(op_sm_count(), kSortCtas), want = op_round(ctas, kSortCtas);
+    grid += (unsigned)(want < most ? want : most);
   }
   const cudaError_t e = op_launch(embed_sort_kernel, grid, kSortThreads, 0, st, s);
   if (e != cudaSuccess || args->n_tokens == 0) return op_cuda(e);
   SumArgs m{};
   m.sorted = p.a; m.dout = dout; m.grad = table_grad; m.part = p.part;
-  m.n = args->n_tokens; m.vocab = args->vocab; m.dim = (int)args->dim; m.tile = tile_of(args->n_tokens);
+  m.n = args->n_tokens; m.vocab = args->vocab; m.dim = (int)args->dim;
   m.accumulate = (int)args->accumulate; m.scale = args->scale;
   m.table_ld = args->table_ld; m.rows_ld = args->rows_ld;
   const bool vec = (args->dim * el) % 16 == 0 && op_vec16(dout, args->rows_ld, el) && op_vec16(table_grad, args->table_ld, el);
