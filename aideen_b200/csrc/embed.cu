@@ -6,7 +6,7 @@
 // the launch for a few tokens).
 //
 // Gradient, bound by HBM (dout read once, the table's gradient written once):
-//   1. one cluster of 8 CTAs (one CTA while it can hold the keys) sorts (id, position) stably, by least-significant
+//   1. one cluster of 1, 8 or 16 CTAs sorts (id, position) stably, by least-significant
 //      digits of at most 8 bits; every warp ranks its own run of keys by
 //      votes, the CTAs exchange their digit counts through distributed
 //      shared memory, and a hardware cluster barrier separates the steps.  The
@@ -28,7 +28,7 @@ namespace cg = cooperative_groups;
 namespace aideen {
 namespace {
 
-constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kMaxSortCtas = 16, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kDigits = 256;
 
 template <typename T, int VEC>
@@ -66,7 +66,8 @@ struct SortArgs {
   const int32_t *ids;
   unsigned long long *a, *b;  // sorted (key << 32 | position) ends in `a`
   uint32_t n, vocab;
-  int passes, digit_bits, ctas;  // ctas: that sort, 1 or the whole cluster
+  int passes, digit_bits;
+  uint32_t ctas;  // that sort: one cluster
   // table gradient to clear, or null: rows of row_bytes at a stride of ld_bytes
   unsigned char *clear;
   size_t row_bytes, ld_bytes;
@@ -122,19 +123,17 @@ __device__ __forceinline__ void clear_rows(const SortArgs &s, uint32_t *zeros, s
   }
 }
 
-__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads)
-    embed_sort_kernel(const SortArgs s) {
+__global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs s) {
   __shared__ __align__(16) uint32_t hist[kSortWarps][kDigits];
   __shared__ uint32_t total[kDigits];  // this CTA's keys per digit, read by its peers
   __shared__ uint32_t wsum[8];
   op_begin();
-  if (blockIdx.x >= kSortCtas) {  // the clusters past the first clear the gradient
-    clear_rows(s, &hist[0][0], blockIdx.x - kSortCtas, gridDim.x - kSortCtas);
+  if (blockIdx.x >= s.ctas) {  // the clusters past the first clear the gradient
+    clear_rows(s, &hist[0][0], blockIdx.x - s.ctas, gridDim.x - s.ctas);
     return;
   }
   cg::cluster_group cluster = cg::this_cluster();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster.block_rank();
-  if (rank >= s.ctas) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)blockIdx.x;
   auto sync_all = [&]() {
     if (s.ctas == 1) __syncthreads();
     else cluster.sync();
@@ -208,11 +207,11 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
       if (s.ctas == 1) {
         all = total[threadIdx.x];
       } else {
-        uint32_t v[kSortCtas];
+        uint32_t v[kMaxSortCtas];
 #pragma unroll
-        for (int c = 0; c < kSortCtas; ++c) v[c] = *cluster.map_shared_rank(&total[threadIdx.x], c);
+        for (int c = 0; c < kMaxSortCtas; ++c) v[c] = c < s.ctas ? *cluster.map_shared_rank(&total[threadIdx.x], c) : 0;
 #pragma unroll
-        for (int c = 0; c < kSortCtas; ++c) {
+        for (int c = 0; c < kMaxSortCtas; ++c) {
           if (c < rank) before += v[c];
           all += v[c];
         }
@@ -516,20 +515,23 @@ extern "C" int aideen_embed_grad(const aideen_embed_args *args, const int32_t *i
   int bits = 1;
   while (args->vocab >> bits) ++bits;  // keys run up to vocab itself
   s.passes = args->n_tokens ? (bits + 7) / 8 : 0;
-  // one CTA holds 8 keys per lane: below that the cluster's barriers cost more than they save
-  s.ctas = args->n_tokens <= 8 * kSortThreads ? 1 : kSortCtas;
+  // up to 4 keys per lane of one CTA the cluster's barriers cost more than they save
+  s.ctas = args->n_tokens <= 4 * kSortThreads ? 1 : args->n_tokens <= 32 * kSortThreads ? 8 : kMaxSortCtas;
   s.digit_bits = s.passes ? (bits + s.passes - 1) / s.passes : 1;
-  unsigned grid = kSortCtas;
+  unsigned grid = s.ctas;
   if (!args->accumulate) {
     s.clear = static_cast<unsigned char *>(table_grad);
     s.row_bytes = args->dim * el; s.ld_bytes = (size_t)args->table_ld * el;
     s.clear16 = s.row_bytes % 16 == 0 && op_vec16(table_grad, args->table_ld, el);
     // several CTAs per SM, so that uneven placement of the clusters evens out
     const size_t ctas = (s.row_bytes / (s.clear16 ? 16 : 2) * s.vocab + kSortThreads - 1) / kSortThreads;
-    const size_t most = 4 * op_round(op_sm_count(), kSortCtas), want = op_round(ctas, kSortCtas);
+    const size_t most = op_round(4 * (size_t)op_sm_count(), s.ctas), want = op_round(ctas, s.ctas);
     grid += (unsigned)(want < most ? want : most);
   }
-  const cudaError_t e = op_launch(embed_sort_kernel, grid, kSortThreads, 0, st, s);
+  cudaError_t e = cudaSuccess;
+  if (s.ctas > 8)  // past the portable size
+    e = cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = op_launch_cluster(embed_sort_kernel, s.ctas, grid, kSortThreads, 0, st, s);
   if (e != cudaSuccess || args->n_tokens == 0) return op_cuda(e);
   SumArgs m{};
   m.sorted = p.a; m.dout = dout; m.grad = table_grad; m.part = p.part;
