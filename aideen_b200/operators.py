@@ -76,35 +76,52 @@ def _vector(t, what: str, name: str, n: int, like, dtype=None):
 def _out(t, what: str, name: str, shape, like):
     """A given output, checked, or a new one."""
     if t is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(shape)
     _tensor(t, what, name, like, like.dtype)
     if tuple(t.shape) != tuple(shape):
         raise AideenError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     return t
 
 
-def _launch(device, what: str, fn, *args):
-    """One call on torch's current stream of `device`, with that device current."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, stream)
-    if rc != 0:
-        _check(rc, what)
+def _like(t, dtype=None):
+    """A new contiguous tensor of t's shape (the cheapest way to allocate one)."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
-def _scratch(nbytes: int, device):
-    # torch's blocks start on 512 bytes; the library asks for 256
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# torch's own short cut to the same handle (2 us less per call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+class _Here:
+    """Stands for `torch.cuda.device` where the device is current already."""
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    """Context with `device` current: the library works on the current one."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _scratch(nbytes: int, like):
+    return like.new_empty(nbytes, dtype=torch.uint8)  # torch's blocks start on 512 bytes; the library asks for 256
 
 
 def check(device=None):
     """Wait for torch's current stream and raise if a bounded wait of an
     operator ran out on the device since the last check."""
     with torch.cuda.device(device):
-        _check(load_library().aideen_operator_check(torch.cuda.current_stream().cuda_stream), "check")
+        _check(load_library().aideen_operator_check(_raw_stream(torch.cuda.current_device())), "check")
 
 
 # ---- embedding -------------------------------------------------------------
@@ -128,7 +145,10 @@ def embed(ids, table, scale: float = 1.0, out=None):
     n = ids.numel()
     old = _rows(out, what, "out")[2] if n else dim
     a = EmbedArgs(_DTYPES[table.dtype], n, dim, vocab, scale, 0, ld, old)
-    _launch(table.device, what, load_library().aideen_embed, C.byref(a), ip, table.data_ptr(), out.data_ptr())
+    with _on(table.device):
+        rc = load_library().aideen_embed(C.byref(a), ip, table.data_ptr(), out.data_ptr(), _raw_stream(table.device.index))
+    if rc:
+        _check(rc, what)
     return out
 
 
@@ -145,11 +165,14 @@ def embed_grad(ids, dout, vocab: int, scale: float = 1.0, into=None):
     grad = _out(into, what, "into", (vocab, dim), dout)
     gld = _rows(grad, what, "into")[2]
     a = EmbedArgs(_DTYPES[dout.dtype], n, dim, vocab, scale, int(into is not None), gld, rld)
-    lib, size = load_library(), C.c_size_t()
-    _check(lib.aideen_embed_grad_workspace(C.byref(a), C.byref(size)), what)
-    ws = _scratch(size.value, dout.device)
-    _launch(dout.device, what, lib.aideen_embed_grad, C.byref(a), ip, dout.data_ptr(), grad.data_ptr(), ws.data_ptr(),
-            size.value)
+    lib, size, r = load_library(), C.c_size_t(), C.byref(a)
+    _check(lib.aideen_embed_grad_workspace(r, C.byref(size)), what)
+    ws = _scratch(size.value, dout)
+    with _on(dout.device):
+        rc = lib.aideen_embed_grad(r, ip, dout.data_ptr(), grad.data_ptr(), ws.data_ptr(), size.value,
+                                   _raw_stream(dout.device.index))
+    if rc:
+        _check(rc, what)
     return grad
 
 
@@ -161,13 +184,19 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     _tensor(x, what, "x")
     n, dim, xld = _rows(x, what, "x")
     wp, bp = _vector(weight, what, "weight", dim, x), _vector(bias, what, "bias", dim, x)
-    y = _out(out, what, "out", x.shape, x)
-    yld = _rows(y, what, "out")[2]
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
+    if out is None:
+        y, yld = _like(x), dim
+    else:
+        y = _out(out, what, "out", x.shape, x)
+        yld = _rows(y, what, "out")[2]
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rstd = _like(mean)
     a = LayerNormArgs(_DTYPES[x.dtype], n, dim, eps, xld, yld, 0)
-    _launch(x.device, what, load_library().aideen_layer_norm, C.byref(a), x.data_ptr(), wp, bp, y.data_ptr(),
-            mean.data_ptr(), rstd.data_ptr())
+    with _on(x.device):
+        rc = load_library().aideen_layer_norm(C.byref(a), x.data_ptr(), wp, bp, y.data_ptr(), mean.data_ptr(),
+                                              rstd.data_ptr(), _raw_stream(x.device.index))
+    if rc:
+        _check(rc, what)
     return y, mean, rstd
 
 
@@ -184,18 +213,21 @@ def layer_norm_grad(dy, x, weight, mean, rstd, want=("x", "weight", "bias")):
     wp = _vector(weight, what, "weight", dim, x)
     mp = _vector(mean, what, "mean", n, x, torch.float32)
     rp = _vector(rstd, what, "rstd", n, x, torch.float32)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if "x" in want else None
-    dw = torch.empty(dim, dtype=x.dtype, device=x.device) if "weight" in want else None
-    db = torch.empty(dim, dtype=x.dtype, device=x.device) if "bias" in want else None
+    dx = _like(x) if "x" in want else None
+    dw = x.new_empty(dim) if "weight" in want else None
+    db = x.new_empty(dim) if "bias" in want else None
     a = LayerNormArgs(_DTYPES[x.dtype], n, dim, 0.0, xld, yld, dim)
-    lib, size, ws = load_library(), C.c_size_t(), None
-    if dw is not None or db is not None:
-        with torch.cuda.device(x.device):  # the size depends on the device's SM count
-            _check(lib.aideen_layer_norm_grad_workspace(C.byref(a), C.byref(size)), what)
-        ws = _scratch(size.value, x.device)
-    _launch(x.device, what, lib.aideen_layer_norm_grad, C.byref(a), dy.data_ptr(), x.data_ptr(), wp, mp, rp,
-            None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
-            None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), size.value)
+    lib, size, ws, r = load_library(), C.c_size_t(), None, C.byref(a)
+    with _on(x.device):
+        if dw is not None or db is not None:
+            _check(lib.aideen_layer_norm_grad_workspace(r, C.byref(size)), what)
+            ws = _scratch(size.value, x)
+        rc = lib.aideen_layer_norm_grad(r, dy.data_ptr(), x.data_ptr(), wp, mp, rp,
+                                        None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+                                        None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
+                                        size.value, _raw_stream(x.device.index))
+    if rc:
+        _check(rc, what)
     return dx, dw, db
 
 
@@ -227,15 +259,17 @@ def linear_ce(x, weight, targets, bias=None, reduction: str = "mean"):
     outside [0, vocab) are not counted (row_loss and lse 0)."""
     what = "linear_ce"
     a, weight, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)
-    lib, size = load_library(), C.c_size_t()
-    with torch.cuda.device(x.device):
-        _check(lib.aideen_linear_ce_workspace(C.byref(a), C.byref(size), None), what)
-    loss = torch.empty(1, dtype=torch.float32, device=x.device)
-    row_loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    lse = torch.empty_like(row_loss)
-    ws = _scratch(size.value, x.device)
-    _launch(x.device, what, lib.aideen_linear_ce, C.byref(a), x.data_ptr(), weight.data_ptr(), bp, tp,
-            loss.data_ptr(), row_loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size.value)
+    lib, size, r = load_library(), C.c_size_t(), C.byref(a)
+    loss = x.new_empty(1, dtype=torch.float32)
+    row_loss = _like(targets, torch.float32)
+    lse = _like(row_loss)
+    with _on(x.device):
+        _check(lib.aideen_linear_ce_workspace(r, C.byref(size), None), what)
+        ws = _scratch(size.value, x)
+        rc = lib.aideen_linear_ce(r, x.data_ptr(), weight.data_ptr(), bp, tp, loss.data_ptr(), row_loss.data_ptr(),
+                                  lse.data_ptr(), ws.data_ptr(), size.value, _raw_stream(x.device.index))
+    if rc:
+        _check(rc, what)
     return loss, row_loss, lse
 
 
@@ -249,14 +283,17 @@ def linear_ce_grad(x, weight, targets, lse, bias=None, dloss=None, reduction: st
     a, weight, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)
     lp = _vector(lse, what, "lse", a.rows, x, torch.float32)
     gp = _vector(dloss, what, "dloss", 1, x, torch.float32)
-    lib, size = load_library(), C.c_size_t()
-    with torch.cuda.device(x.device):
-        _check(lib.aideen_linear_ce_workspace(C.byref(a), None, C.byref(size)), what)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if "x" in want else None
-    dw = torch.empty((a.vocab, a.dim), dtype=x.dtype, device=x.device) if "weight" in want else None
-    db = torch.empty(a.vocab, dtype=x.dtype, device=x.device) if "bias" in want and bias is not None else None
-    ws = _scratch(size.value, x.device)
-    _launch(x.device, what, lib.aideen_linear_ce_grad, C.byref(a), x.data_ptr(), weight.data_ptr(), bp, tp, lp, gp,
-            None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
-            None if db is None else db.data_ptr(), ws.data_ptr(), size.value)
+    lib, size, r = load_library(), C.c_size_t(), C.byref(a)
+    dx = _like(x) if "x" in want else None
+    dw = x.new_empty((a.vocab, a.dim)) if "weight" in want else None
+    db = x.new_empty(a.vocab) if "bias" in want and bias is not None else None
+    with _on(x.device):
+        _check(lib.aideen_linear_ce_workspace(r, None, C.byref(size)), what)
+        ws = _scratch(size.value, x)
+        rc = lib.aideen_linear_ce_grad(r, x.data_ptr(), weight.data_ptr(), bp, tp, lp, gp,
+                                       None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+                                       None if db is None else db.data_ptr(), ws.data_ptr(), size.value,
+                                       _raw_stream(x.device.index))
+    if rc:
+        _check(rc, what)
     return dx, dw, db
