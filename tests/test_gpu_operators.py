@@ -311,6 +311,23 @@ def test_linear_ce(dtype, rows, dim, vocab, bias, ignored, pad):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 7, 8, 9])
+@pytest.mark.parametrize("dim,vocab,pad", [(512, 50257, 0), (1, 3, 0), (77, 1001, 3), (2056, 130, 0), (4104, 33, 0)])
+def test_linear_ce_few_rows(dtype, rows, dim, vocab, pad):
+    x, w, b, tg = ce_inputs(rows * dim, rows, dim, vocab, dtype, True, 0.0, pad)
+    if rows > 2:
+        tg[1], tg[rows - 1] = -1, vocab
+        x[1] = float("nan")
+    loss, row_loss, lse = K.linear_ce(x, w, tg, bias=b)
+    ref = ce_reference(x, w, b, tg, "mean", 1.0, dtype)
+    for got, name in ((loss, "loss"), (row_loss, "rows"), (lse, "lse")):
+        close(got, ref[name][0], ref[name][1] + 1e-30)
+    total, _, _ = K.linear_ce(x, w, tg, bias=b, reduction="sum")
+    kept = int(((tg >= 0) & (tg < vocab)).sum())
+    assert abs(float(total) - float(loss) * kept) <= 4 * U32 * float(total)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_linear_ce_at_the_training_vocabulary(dtype):
     x, w, b, tg = ce_inputs(3, 200, 512, 50257, dtype, True, 0.1)
     ce_check(x, w, b, tg, reduction="sum", dloss=0.25 if dtype != F16 else 8.0)
