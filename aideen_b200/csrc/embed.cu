@@ -7,12 +7,12 @@
 //
 // Gradient, bound by HBM (dout read once, the table's gradient written once):
 //   1. one cluster of 1, 8 or 16 CTAs sorts (id, position) stably, by least-significant
-//      digits of at most 8 bits; every warp ranks its own run of keys by
-//      votes, the CTAs exchange their digit counts through distributed
+//      digits of at most 8 bits; every warp ranks its own run of keys
+//      (lanes of one digit meet in a word of shared memory), the CTAs exchange their digit counts through distributed
 //      shared memory, and a hardware cluster barrier separates the steps.  The
 //      sort is latency, not bandwidth, so the other CTAs of the same launch
 //      clear the table's gradient meanwhile.
-//   2. the sorted positions are cut into tiles of 8, one warp each (per 32
+//   2. the sorted positions are cut into tiles of 8 or 32, one warp each (per 32
 //      accesses of a row), whatever the ids are: a frequent id spreads over
 //      many tiles.  A run of one id inside a tile is summed and stored; a run
 //      that crosses tiles leaves float32 partial rows.
@@ -74,19 +74,6 @@ struct SortArgs {
   int clear16;  // rows can be cleared 16 bytes at a time
 };
 
-// Lanes of `live` whose digit is this lane's: one vote per bit (a quarter of the time
-// of match.any here).
-__device__ __forceinline__ uint32_t same_digit(uint32_t live, uint32_t d, int bits) {
-  uint32_t same = live;
-#pragma unroll
-  for (int b = 0; b < 8; ++b) {
-    if (b >= bits) break;
-    const uint32_t v = __ballot_sync(0xffffffffu, d >> b & 1);
-    same &= d >> b & 1 ? v : ~v;
-  }
-  return same;
-}
-
 // Keys are the ids, every id outside [0, vocab) as vocab (sorted last).
 __device__ __forceinline__ uint32_t sort_key(int32_t id, uint32_t vocab) {
   return id >= 0 && (uint32_t)id < vocab ? (uint32_t)id : vocab;
@@ -95,7 +82,7 @@ __device__ __forceinline__ uint32_t sort_key(int32_t id, uint32_t vocab) {
 // Clears the rows: whole 32 KB blocks of zeros go out of shared memory by bulk copy
 // where the rows are contiguous, else plain stores.
 __device__ __forceinline__ void clear_rows(const SortArgs &s, uint32_t *zeros, size_t cta, size_t ctas) {
-  constexpr size_t kBlock = sizeof(uint32_t) * kSortWarps * kDigits;
+  constexpr size_t kBlock = sizeof(uint32_t) * kSortWarps * kDigits;  // 32 KB
   const size_t t = cta * kSortThreads + threadIdx.x, step = ctas * kSortThreads;
   if (s.clear16 && s.row_bytes == s.ld_bytes) {
     for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) zeros[i] = 0;
@@ -124,12 +111,14 @@ __device__ __forceinline__ void clear_rows(const SortArgs &s, uint32_t *zeros, s
 }
 
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs s) {
-  __shared__ __align__(16) uint32_t hist[kSortWarps][kDigits];
+  extern __shared__ __align__(16) uint32_t sort_smem[];
+  uint32_t(*hist)[kDigits] = reinterpret_cast<uint32_t(*)[kDigits]>(sort_smem);               // keys per warp and digit
+  uint32_t(*lanes)[kDigits] = reinterpret_cast<uint32_t(*)[kDigits]>(sort_smem + kSortWarps * kDigits);  // lanes per digit
   __shared__ uint32_t total[kDigits];  // this CTA's keys per digit, read by its peers
   __shared__ uint32_t wsum[8];
   op_begin();
   if (blockIdx.x >= s.ctas) {  // the clusters past the first clear the gradient
-    clear_rows(s, &hist[0][0], blockIdx.x - s.ctas, gridDim.x - s.ctas);
+    clear_rows(s, sort_smem, blockIdx.x - s.ctas, gridDim.x - s.ctas);
     return;
   }
   cg::cluster_group cluster = cg::this_cluster();
@@ -138,7 +127,6 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
     if (s.ctas == 1) __syncthreads();
     else cluster.sync();
   };
-  uint32_t count[kSortWarps];
   // every warp of the sorting CTAs owns one contiguous run of positions
   const uint32_t run = (s.n + s.ctas * kSortWarps - 1) / (s.ctas * kSortWarps);
   const uint32_t w = (uint32_t)(rank * kSortWarps + warp);
@@ -146,13 +134,18 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
   const uint32_t hi = s.n - lo < run ? s.n : lo + run;
   const uint32_t mask = (1u << s.digit_bits) - 1u;
   const uint32_t below = (1u << lane) - 1u;
-  constexpr int U = 8;  // keys per lane loaded ahead
+  constexpr int U = 4;  // keys per lane at a time
+  for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) (&lanes[0][0])[i] = 0;
   for (int p = 0; p < s.passes; ++p) {
     const int shift = p * s.digit_bits;
     // the last pass writes into `a`
     unsigned long long *dst = ((s.passes - 1 - p) & 1) ? s.b : s.a;
     const unsigned long long *src = ((s.passes - 1 - p) & 1) ? s.a : s.b;
-    auto load = [&](uint32_t i0, unsigned long long (&kv)[U]) {
+    unsigned long long kv[U];
+    uint32_t at[U];  // place among the warp's keys of the same digit
+    // Loads up to 32 U keys and counts them: lanes of a digit meet in its word of
+    // `lanes`, the first of them adds their number to the digit's count.
+    auto walk = [&](uint32_t i0) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const uint32_t i = i0 + u * 32 + lane;
@@ -162,42 +155,36 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
           else kv[u] = __ldcg(src + i);  // written by another CTA of the cluster
         }
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u * 32 >= hi) break;
+        const bool in = i0 + u * 32 + lane < hi;
+        const uint32_t d = ((uint32_t)(kv[u] >> 32) >> shift) & mask;
+        if (in) atomicOr(&lanes[warp][d], 1u << lane);
+        __syncwarp();
+        const uint32_t same = in ? lanes[warp][d] : 0;
+        const uint32_t old = in ? hist[warp][d] : 0;
+        at[u] = old + __popc(same & below);
+        __syncwarp();
+        if (in && (same & below) == 0) {
+          hist[warp][d] = old + __popc(same);
+          lanes[warp][d] = 0;
+        }
+        __syncwarp();
+      }
     };
     for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
-    unsigned long long kv[U];
-    uint32_t same[U];
-    auto peers = [&](uint32_t i0) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        same[u] = 0;
-        if (i0 + u * 32 >= hi) continue;
-        const bool in = i0 + u * 32 + lane < hi;
-        const uint32_t live = __ballot_sync(0xffffffffu, in);
-        const uint32_t peer = same_digit(live, ((uint32_t)(kv[u] >> 32) >> shift) & mask, s.digit_bits);
-        if (in) same[u] = peer;
-      }
-    };
-    for (uint32_t i0 = lo; i0 < hi; i0 += 32 * U) {
-      load(i0, kv);
-      peers(i0);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {  // the first lane of each digit counts its peers
-        if (i0 + u * 32 >= hi) break;
-        if (same[u] && (same[u] & below) == 0) hist[warp][((uint32_t)(kv[u] >> 32) >> shift) & mask] += __popc(same[u]);
-        __syncwarp();
-      }
-    }
+    for (uint32_t i0 = lo; i0 < hi; i0 += 32 * U) walk(i0);
     __syncthreads();
     if (threadIdx.x < kDigits) {  // counts of the warps before, per digit
-      uint32_t sum = 0;
+      uint32_t sum = 0, count[kSortWarps];
 #pragma unroll
       for (int k = 0; k < kSortWarps; ++k) count[k] = hist[k][threadIdx.x];
 #pragma unroll
       for (int k = 0; k < kSortWarps; ++k) {
-        const uint32_t c = count[k];
-        count[k] = sum;
-        sum += c;
+        hist[k][threadIdx.x] = sum;
+        sum += count[k];
       }
       total[threadIdx.x] = sum;
     }
@@ -209,7 +196,7 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
       } else {
         uint32_t v[kMaxSortCtas];
 #pragma unroll
-        for (int c = 0; c < kMaxSortCtas; ++c) v[c] = c < s.ctas ? *cluster.map_shared_rank(&total[threadIdx.x], c) : 0;
+        for (int c = 0; c < kMaxSortCtas; ++c) v[c] = c < (int)s.ctas ? *cluster.map_shared_rank(&total[threadIdx.x], c) : 0;
 #pragma unroll
         for (int c = 0; c < kMaxSortCtas; ++c) {
           if (c < rank) before += v[c];
@@ -226,33 +213,38 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs
     }
     __syncthreads();
     if (threadIdx.x < kDigits) {
-      uint32_t base = x - all + before;
+      uint32_t base = x - all + before, count[kSortWarps];
       for (int k = 0; k < warp; ++k) base += wsum[k];
+#pragma unroll
+      for (int k = 0; k < kSortWarps; ++k) count[k] = hist[k][threadIdx.x];
 #pragma unroll
       for (int k = 0; k < kSortWarps; ++k) hist[k][threadIdx.x] = count[k] + base;
     }
     __syncthreads();
-    for (uint32_t i0 = lo; i0 < hi; i0 += 32 * U) {
-      if (hi - lo > 32 * U) {  // else they are still here
-        load(i0, kv);
-        peers(i0);
-      }
+    if (hi - lo <= 32 * U) {  // the keys and their places are still here
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i0 + u * 32 >= hi) break;
-        const uint32_t d = ((uint32_t)(kv[u] >> 32) >> shift) & mask;
-        if (same[u]) dst[hist[warp][d] + __popc(same[u] & below)] = kv[u];
-        __syncwarp();
-        if (same[u] && (same[u] & below) == 0) hist[warp][d] += __popc(same[u]);
-        __syncwarp();
+      for (int u = 0; u < U; ++u)
+        if (lo + u * 32 + lane < hi) dst[hist[warp][((uint32_t)(kv[u] >> 32) >> shift) & mask] + at[u]] = kv[u];
+    } else {  // count again, from the bases on
+      for (uint32_t i0 = lo; i0 < hi; i0 += 32 * U) {
+        walk(i0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (i0 + u * 32 + lane < hi) dst[at[u]] = kv[u];
       }
     }
     sync_all();  // the pass's writes and reads of `total` are done everywhere
   }
 }
 
-constexpr int kTile = 8;        // sorted positions per warp: their rows are all in flight together
-constexpr int kJoinWarps = 32;  // tiles that a joining CTA looks at
+constexpr int kBatch = 8;       // rows of a warp in flight
+constexpr int kJoinWarps = 16;  // tiles that a joining CTA looks at
+
+// Sorted positions per warp: one batch while that gives the GPU too few warps, else
+// four, for a quarter of the partial rows (the gradient of 65521 x 512 bf16 takes 52 us
+// with two batches, 48 us with four; with 3 CTAs on an SM instead of 4, which leaves a
+// second wave of a few CTAs, 74 us).
+int tile_of(uint32_t n) { return n <= 16384 ? kBatch : 4 * kBatch; }
 
 struct SumArgs {
   const unsigned long long *sorted;
@@ -260,7 +252,7 @@ struct SumArgs {
   void *grad;
   float *part;  // [tiles][2][dim]: the run that enters the tile, the run that leaves it
   uint32_t n, vocab;
-  int dim, accumulate;
+  int dim, tile, slabs, accumulate;  // slabs: of 32 accesses per row
   float scale;
   long table_ld, rows_ld;
 };
@@ -289,77 +281,89 @@ __device__ __forceinline__ void embed_finish(const SumArgs &a, uint32_t key, int
   op_store_vec<T, VEC>(g, acc);
 }
 
-// One warp sums tile blockIdx.x * 8 + warp over the columns of one access per lane
-// (blockIdx.y picks 32 of them).  Keys are uniform over the warp.
+// One warp sums a tile over the columns of one access per lane.  The warps of a row's
+// slabs are neighbours, so that its bytes are asked for together.  Keys are uniform over
+// the warp.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) embed_sum_kernel(const SumArgs a) {
+__global__ void __launch_bounds__(256, 4) embed_sum_kernel(const SumArgs a) {
   op_begin();
   const int lane = threadIdx.x & 31;
-  const uint32_t tile = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const unsigned long long begin = (unsigned long long)tile * kTile;
+  const unsigned long long gw = (unsigned long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t tile = (uint32_t)(gw / a.slabs);
+  const unsigned long long begin = (unsigned long long)tile * a.tile;
   if (begin >= a.n) return;
   const uint32_t lo = (uint32_t)begin;
-  const int n = a.n - lo < kTile ? (int)(a.n - lo) : kTile;
-  const int c = (blockIdx.y * 32 + lane) * VEC;
+  const int n = a.n - lo < (uint32_t)a.tile ? (int)(a.n - lo) : a.tile;
+  const int c = ((int)(gw % a.slabs) * 32 + lane) * VEC;
   const bool live = c < a.dim;
-  const T *dout = static_cast<const T *>(a.dout) + c;
-  // lane 0: the position before the tile, lanes 1..n: the tile, lane n + 1: the one behind
-  const bool there = lane <= n + 1 && lo + lane >= 1 && lo + lane - 1 < a.n;
-  const unsigned long long mine = there ? a.sorted[lo + lane - 1] : ~0ull;
+  // loads without branches (behind the row and outside the table some valid row's start is
+  // read and not used), or each would wait for the one before
+  const T *dout = static_cast<const T *>(a.dout) + (live ? c : 0);
+  const unsigned long long mine = lane < n ? a.sorted[lo + lane] : ~0ull;
+  const unsigned long long outer = lane == 0 ? (lo > 0 ? a.sorted[lo - 1] : ~0ull) : lane == 1 && lo + n < a.n ? a.sorted[lo + n] : ~0ull;
   const uint32_t key = (uint32_t)(mine >> 32);
-  const uint32_t before = __shfl_up_sync(0xffffffffu, key, 1);
-  // bit i: position i of the tile begins a run; bit n: the run ends with the tile
-  const uint32_t starts = __ballot_sync(0xffffffffu, lane >= 1 && lane <= n + 1 && (!there || key != before)) >> 1;
-  OpVec<T, VEC> v[kTile];
+  uint32_t before = __shfl_up_sync(0xffffffffu, key, 1);
+  const uint32_t prev = (uint32_t)(__shfl_sync(0xffffffffu, outer, 0) >> 32), next = (uint32_t)(__shfl_sync(0xffffffffu, outer, 1) >> 32);
+  if (lane == 0) before = prev;
+  const uint32_t starts = __ballot_sync(0xffffffffu, lane < n && key != before);  // positions that begin a run
+  float acc[VEC] = {};
+  bool entered = !(starts & 1u);  // the run at work began in an earlier tile
+  uint32_t at = __shfl_sync(0xffffffffu, key, 0);
+  // Stores the finished run: `leaves` where it goes on in the next tile.
+  auto finish = [&](bool leaves) {
+    if (live && at < a.vocab) {
+      if (entered || leaves) part_store<VEC>(a.part + ((size_t)tile * 2 + (entered ? 0 : 1)) * a.dim + c, acc);
+      else embed_finish<T, VEC>(a, at, c, acc);
+    }
+  };
+  for (int b0 = 0; b0 < n; b0 += kBatch) {
+    OpVec<T, VEC> v[kBatch];
 #pragma unroll
-  for (int u = 0; u < kTile; ++u) {
-    const unsigned long long kv = __shfl_sync(0xffffffffu, mine, u + 1);
-    if (live && u < n && (uint32_t)(kv >> 32) < a.vocab)
-      v[u] = *reinterpret_cast<const OpVec<T, VEC> *>(dout + (long)(uint32_t)kv * a.rows_ld);
-  }
-  for (int u0 = 0; u0 < n;) {
-    const uint32_t k = __shfl_sync(0xffffffffu, key, u0 + 1);
-    if (k >= a.vocab) break;  // outside the table: sorted last
-    const uint32_t later = starts >> (u0 + 1) << (u0 + 1);
-    const int u1 = later & ((1u << n) - 1u) ? __ffs(later) - 1 : n;
-    const bool entered = u0 == 0 && !(starts & 1u), leaves = u1 == n && !(starts >> n & 1u);
-    float acc[VEC] = {};
-    if (live) {
+    for (int u = 0; u < kBatch; ++u) {
+      const uint32_t pos = (uint32_t)__shfl_sync(0xffffffffu, mine, min(b0 + u, n - 1));
+      op_load_ahead<T, VEC>(dout + (long)pos * a.rows_ld, v[u]);
+    }
 #pragma unroll
-      for (int u = 0; u < kTile; ++u) {
-        if (u < u0 || u >= u1) continue;
+    for (int u = 0; u < kBatch; ++u) {
+      if (b0 + u >= n) break;
+      if (b0 + u > 0 && (starts >> (b0 + u) & 1u)) {
+        finish(false);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+        entered = false;
+        at = __shfl_sync(0xffffffffu, key, b0 + u);
+      }
+      if (at < a.vocab) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] += op_load<T>(v[u].v[i]);
       }
-      if (entered || leaves) part_store<VEC>(a.part + ((size_t)tile * 2 + (entered ? 0 : 1)) * a.dim + c, acc);
-      else embed_finish<T, VEC>(a, k, c, acc);
     }
-    u0 = u1;
   }
+  finish(next == at);
 }
 
 // Adds the partial rows of the runs that cross tiles, in a fixed order.  Each warp looks
 // at one tile: does its last run begin in it and leave it, and how many more tiles does
 // it enter?  Up to kShort of them the warp adds alone; longer runs take the whole CTA
-// (warp w adds the parts w, w + 32, ..., then the warps are added in order).
+// (warp w adds the parts w, w + 16, ..., then the warps are added in order).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(32 * kJoinWarps) embed_join_kernel(const SumArgs a) {
-  constexpr uint32_t kShort = 16;
+  constexpr uint32_t kShort = 7;
   __shared__ float sh[kJoinWarps][32 * VEC];
   __shared__ uint32_t more_of[kJoinWarps], key_of[kJoinWarps];
   op_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tile = blockIdx.x * kJoinWarps + warp;
-  const unsigned long long end = ((unsigned long long)tile + 1) * kTile;
+  const unsigned long long end = ((unsigned long long)tile + 1) * a.tile;
   uint32_t more = 0, key = ~0u;
   if (end < a.n) {
-    const uint32_t hi = (uint32_t)end, lo = hi - kTile;
+    const uint32_t hi = (uint32_t)end, lo = hi - a.tile;
     key = (uint32_t)(a.sorted[hi - 1] >> 32);
     const uint32_t next = (uint32_t)(a.sorted[hi] >> 32), first = (uint32_t)(a.sorted[lo] >> 32);
     const uint32_t prev = lo > 0 ? (uint32_t)(a.sorted[lo - 1] >> 32) : ~0u;
     if (key < a.vocab && next == key && !(first == key && prev == key)) {
       for (more = 1;; more += 32) {  // lane i: does the run leave tile + more + i too?
-        const unsigned long long at = ((unsigned long long)tile + more + lane + 1) * kTile;
+        const unsigned long long at = ((unsigned long long)tile + more + lane + 1) * a.tile;
         const bool on = at < a.n && (uint32_t)(a.sorted[at] >> 32) == key;
         const uint32_t off = __ballot_sync(0xffffffffu, !on);
         if (off) {
@@ -376,7 +380,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) embed_join_kernel(const SumAr
   const int c = (blockIdx.y * 32 + lane) * VEC;
   auto add = [&](uint32_t t0, uint32_t from, uint32_t by, uint32_t count, float (&acc)[VEC]) {
     if (c >= a.dim) return;
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t t = from; t <= count; t += by) {
       const float *p = a.part + ((size_t)(t0 + t) * 2 + (t == 0 ? 1 : 0)) * a.dim + c;
       float v[VEC];
@@ -428,7 +432,7 @@ GradPlan grad_plan(const aideen_embed_args *args, void *ws) {
   GradPlan p{};
   OpCarve c(ws);
   const uint32_t n = args->n_tokens;
-  p.tiles = (n + kTile - 1) / kTile;
+  p.tiles = (n + tile_of(n) - 1) / tile_of(n);
   p.a = c.take<unsigned long long>(n);
   p.b = c.take<unsigned long long>(n);
   p.part = c.take<float>((size_t)p.tiles * 2 * args->dim);
@@ -445,11 +449,12 @@ cudaError_t embed_run(const aideen_embed_args *a, const int32_t *ids, const void
 }
 
 template <typename T, int VEC>
-cudaError_t sum_run(const SumArgs &s, uint32_t tiles, cudaStream_t st) {
-  const unsigned slabs = (unsigned)((s.dim + 32 * VEC - 1) / (32 * VEC));
-  cudaError_t e = op_launch(embed_sum_kernel<T, VEC>, dim3((tiles + 7) / 8, slabs), 256, 0, st, s);
+cudaError_t sum_run(SumArgs s, uint32_t tiles, cudaStream_t st) {
+  s.slabs = (s.dim + 32 * VEC - 1) / (32 * VEC);
+  const unsigned long long warps = (unsigned long long)tiles * s.slabs;
+  cudaError_t e = op_launch(embed_sum_kernel<T, VEC>, (unsigned)((warps + 7) / 8), 256, 0, st, s);
   if (e != cudaSuccess || tiles < 2) return e;
-  return op_launch(embed_join_kernel<T, VEC>, dim3((tiles + kJoinWarps - 1) / kJoinWarps, slabs), 32 * kJoinWarps, 0, st, s);
+  return op_launch(embed_join_kernel<T, VEC>, dim3((tiles + kJoinWarps - 1) / kJoinWarps, s.slabs), 32 * kJoinWarps, 0, st, s);
 }
 
 int check_args(const aideen_embed_args *a) {
@@ -528,14 +533,15 @@ extern "C" int aideen_embed_grad(const aideen_embed_args *args, const int32_t *i
     const size_t most = op_round(4 * (size_t)op_sm_count(), s.ctas), want = op_round(ctas, s.ctas);
     grid += (unsigned)(want < most ? want : most);
   }
-  cudaError_t e = cudaSuccess;
-  if (s.ctas > 8)  // past the portable size
+  const int smem = 2 * kSortWarps * kDigits * (int)sizeof(uint32_t);
+  cudaError_t e = cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && s.ctas > 8)  // past the portable size
     e = cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) e = op_launch_cluster(embed_sort_kernel, s.ctas, grid, kSortThreads, 0, st, s);
+  if (e == cudaSuccess) e = op_launch_cluster(embed_sort_kernel, s.ctas, grid, kSortThreads, smem, st, s);
   if (e != cudaSuccess || args->n_tokens == 0) return op_cuda(e);
   SumArgs m{};
   m.sorted = p.a; m.dout = dout; m.grad = table_grad; m.part = p.part;
-  m.n = args->n_tokens; m.vocab = args->vocab; m.dim = (int)args->dim;
+  m.n = args->n_tokens; m.vocab = args->vocab; m.dim = (int)args->dim; m.tile = tile_of(args->n_tokens);
   m.accumulate = (int)args->accumulate; m.scale = args->scale;
   m.table_ld = args->table_ld; m.rows_ld = args->rows_ld;
   const bool vec = (args->dim * el) % 16 == 0 && op_vec16(dout, args->rows_ld, el) && op_vec16(table_grad, args->table_ld, el);

@@ -70,6 +70,7 @@ struct LnAccess {
   static constexpr int P = VEC == 1 ? 1 : VEC / 2;
   OpVec<T, VEC> v;
   __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const OpVec<T, VEC> *>(p); }
+  __device__ __forceinline__ void load_ahead(const T *p) { op_load_ahead<T, VEC>(p, v); }
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v.v[i] = op_store<T>(0.f);
@@ -107,12 +108,14 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a
 template <typename T, int VEC, int N>
 struct LnRow {
   LnAccess<T, VEC> v[N];
-  __device__ __forceinline__ void load(const T *row, int c0, int step, int dim) {
+  // No branches, or each load would wait for the one before: behind the row its start
+  // is read, and cleared.
+  __device__ __forceinline__ void load(const T *row, int c0, int step, int dim, bool there = true) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      v[j].clear();  // first: a store into the registers of a load in flight would wait for it
-      if (c0 + j * step < dim) v[j].load(row + c0 + j * step);
-    }
+    for (int j = 0; j < N; ++j) v[j].load_ahead(row + (c0 + j * step < dim ? c0 + j * step : 0));
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (c0 + j * step >= dim || !there) v[j].clear();
   }
 };
 
@@ -243,12 +246,12 @@ __global__ void __launch_bounds__(LnShape<NV>::threads, LnShape<NV>::per_sm) lay
     float m[R], r[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      const long row = row0 + q;
-      const int dim = row < a.rows ? a.dim : 0;  // rows behind the last are zeros and add nothing
-      xv[q].load(x + row * a.x_ld, c0, step, dim);
-      gv[q].load(dy + row * a.y_ld, c0, step, dim);
-      m[q] = dim ? a.mean[row] : 0.f;
-      r[q] = dim ? a.rstd[row] : 0.f;
+      const bool there = row0 + q < a.rows;  // rows behind the last are zeros and add nothing
+      const long row = there ? row0 + q : a.rows - 1;
+      xv[q].load(x + row * a.x_ld, c0, step, a.dim, there);
+      gv[q].load(dy + row * a.y_ld, c0, step, a.dim, there);
+      m[q] = a.mean[row];
+      r[q] = a.rstd[row];
     }
     // dy is 0 behind a row (and in a scalar access's second half), so nothing is added there
     float2 s0[R], s1[R];

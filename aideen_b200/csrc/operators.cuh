@@ -123,6 +123,26 @@ __device__ __forceinline__ void op_store_vec(T *p, const float (&in)[VEC]) {
   *reinterpret_cast<OpVec<T, VEC> *>(p) = x;
 }
 
+// The same, as a load that stays where it is written: a run of them is in flight
+// together, instead of each being moved down to its use.
+template <typename T, int VEC>
+__device__ __forceinline__ void op_load_ahead(const T *p, OpVec<T, VEC> &out) {
+  if constexpr (sizeof(T) * VEC == 16) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    out = reinterpret_cast<const OpVec<T, VEC> &>(v);
+  } else if constexpr (sizeof(T) * VEC == 4) {
+    uint32_t v;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    out = reinterpret_cast<const OpVec<T, VEC> &>(v);
+  } else {
+    static_assert(sizeof(T) * VEC == 2, "2, 4 or 16 bytes");
+    uint16_t v;
+    asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
+    out = reinterpret_cast<const OpVec<T, VEC> &>(v);
+  }
+}
+
 // Whether rows of this base and stride can be moved 16 bytes at a time.
 inline bool op_vec16(const void *p, int64_t ld, size_t elem) {
   return op_aligned(p, 16) && ((size_t)ld * elem) % 16 == 0;
