@@ -176,6 +176,56 @@ def test_layer_norm(dtype, rows, dim, pad, affine):
     close(y, want, dy + U[dtype] * (want.abs() + dy) + TINY[dtype])
 
 
+# many rows: several for every resident group of warps, at 16-byte and other strides,
+# against the same rows alone
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,pad", [(8001, 512, 0), (7999, 40, 8), (9000, 1000, 0), (3001, 2056, 0),
+                                           (8000, 24, 1), (2500, 4096, 0), (1001, 8192, 8)])
+def test_layer_norm_many_rows(dtype, rows, dim, pad):
+    g = gen(rows + dim + 2)
+    x = strided(rand(g, rows, dim, dtype=dtype, std=1.7, mean=0.3), pad)
+    dy = strided(rand(g, rows, dim, dtype=dtype), pad)
+    w, b = rand(g, dim, dtype=dtype, std=0.1, mean=1.0), rand(g, dim, dtype=dtype, std=0.1)
+    whole = K.layer_norm(x, w, b)
+    grads = K.layer_norm_grad(dy, x, w, whole[1], whole[2])
+    K.check(x.device)
+    # every row alone is what it is among the others, up to the order of its sums
+    some = torch.randint(0, rows, (64,), generator=g, device="cuda").sort().values
+    some[0], some[-1] = 0, rows - 1
+    few = K.layer_norm(x[some], w, b)
+    fewg = K.layer_norm_grad(dy[some], x[some], w, whole[1][some], whole[2][some])
+    c = chain(dim)
+    xd, m, xc, var, r, want = norm_reference(x[some], w, b, 1e-5)
+    for y, mean, rstd in ((whole[0][some], whole[1][some], whole[2][some]), few):
+        dm = c * U32 * xd.abs().mean(1, keepdim=True) + U32 * m.abs()
+        close(mean[:, None], m, dm)
+        dvar = (c + 4) * U32 * var + dm * dm + 2 * U32 * xc.abs().mean(1, keepdim=True) * xd.abs().amax(1, keepdim=True)
+        rel_r = 0.5 * dvar / (var + 1e-5) + 4 * U32
+        close(rstd[:, None], r, r * rel_r * (1 + rel_r))
+        e = w.double().abs() * (r * (dm + 2 * U32 * xc.abs()) + (xc * r).abs() * (rel_r + 2 * U32)) * 1.01 + 2 * U32 * want.abs()
+        close(y, want, e + U[dtype] * (want.abs() + e) + TINY[dtype])
+    md, rd = whole[1].double()[:, None], whole[2].double()[:, None]
+    xh = (x.double() - md) * rd
+    gd = dy.double() * w.double()
+    c1, c2 = gd.mean(1, keepdim=True), (gd * xh).mean(1, keepdim=True)
+    want = rd * (gd - c1 - xh * c2)
+    e1, e2 = (c + 4) * U32 * gd.abs().mean(1, keepdim=True), (c + 8) * U32 * (gd * xh).abs().mean(1, keepdim=True)
+    e = rd * (e1 + xh.abs() * e2 + 6 * U32 * (gd.abs() + c1.abs() + (xh * c2).abs())) * 1.01
+    bound = e + U[dtype] * (want.abs() + e) + TINY[dtype]
+    close(grads[0], want, bound)
+    close(fewg[0], want[some], bound[some])
+    for got, terms in ((grads[1], dy.double() * xh), (grads[2], dy.double())):
+        t = terms.sum(0)
+        e = (rows + 16) * U32 * terms.abs().sum(0)
+        close(got, t, e + U[dtype] * (t.abs() + e) + TINY[dtype])
+    assert all(torch.equal(p, q) for p, q in zip(grads, K.layer_norm_grad(dy, x, w, whole[1], whole[2])))
+    only = K.layer_norm_grad(dy, x, None, whole[1], whole[2], want=("weight", "bias"))
+    assert only[0] is None and torch.equal(only[1], grads[1]) and torch.equal(only[2], grads[2])
+    plain = K.layer_norm(x, None, None)[0]
+    ones = K.layer_norm(x, torch.ones_like(w), torch.zeros_like(b))[0]
+    assert torch.equal(plain, ones)
+
+
 def test_layer_norm_constant_and_extreme_rows():
     # a constant row: variance 0, y is the bias; rows with Inf or NaN spoil only themselves
     x = torch.full((4, 96), 3.0, device="cuda")
