@@ -8,7 +8,7 @@
 // Steps:
 //   stage   counted rows of x are gathered to the front (a padded row costs no
 //           product and its contents reach nothing) as 16-bit operands; float32
-//           is split into three bfloat16 pieces that add up to it exactly.
+//           becomes two float16 pieces (see below).
 //   stats   z tile by tile on the tensor cores; the epilogue keeps a running
 //           maximum and sum per row and stores nothing else.
 //   rows    joins the partial statistics, forms z[n][t[n]] as a plain dot product.
@@ -20,8 +20,13 @@
 // accumulator and loads half of either operand).  Per CTA: warp 0 streams 64-deep
 // slices by TMA into a ring of five 32 KB stages, warp 1 of the leading CTA
 // issues the MMAs into one of two 256-column accumulators in tensor memory, and
-// warps 2..9 drain the other one.  float32 operands take six products of their
-// pieces (all but those below 2^-24), the small ones first.
+// warps 2..9 drain the other one.
+//
+// float32: each of x, W and G = softmax - onehot is scaled by a power of two that brings
+// its largest magnitude (G: 1) to 2^14..2^15 and written as high + low float16 pieces;
+// high x high + high x low + low x high leave out 2^-22 of a product, three passes where
+// bfloat16 pieces would take six (training shard 50257 x 512, 2048 rows: %%A%%).  What
+// lies below 2^-40 of the largest magnitude (G: 2^-39) is rounded off.
 // Bound: the tensor cores (2 N V d for the loss, 6 N V d for the gradient).
 //
 // Every wait is bounded; a wait that runs out sets an error word, issues nothing
@@ -47,6 +52,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // float16 keeps softmax - onehot times 2^12: probabilities down to 2^-26 stay
 // normal numbers, and the largest magnitude is 2^12
 constexpr float kHalfScale = 4096.f;
+// and float32's two pieces of it times 2^14
+constexpr float kPieceScale = 16384.f;
 // Shared memory of a CTA: held slices of x, the ring, the epilogue's boxes, the
 // bias of two tiles, barriers.
 constexpr int kSmemLimit = 232448, kSmemFixed = 2 * kTileN * 4 + 512;
@@ -56,7 +63,8 @@ enum { kStats = 0, kPiece = 1, kProducts = 2 };
 struct MmaArgs {
   const int *count;   // counted rows
   int vocab, dim;
-  int planes;         // 16-bit pieces per operand element: 1, or 3 for float32
+  int planes;         // 16-bit pieces per operand element: 1, or 2 for float32
+  const float *unscale;  // float32: what x and W were divided by, [2]
   uint32_t idesc;     // operand types of the instruction descriptor
   int stages;         // ring depth
   // kStats, kPiece: vocabulary tiles [0, tiles_n) from column v0 on
@@ -174,14 +182,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Products of pieces in the order they are added: (A piece, B piece).
+// Products of pieces in the order they are added: low x high, high x low, high x high.
 __device__ __forceinline__ void product_pair(int planes, int j, int &pa, int &pb) {
-  if (planes == 1) { pa = pb = 0; return; }
-  // lo*hi, hi*lo, mid*mid, mid*hi, hi*mid, hi*hi
-  constexpr uint32_t A = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
-  constexpr uint32_t B = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
-  pa = (A >> (2 * j)) & 3;
-  pb = (B >> (2 * j)) & 3;
+  pa = planes == 2 && j == 0;
+  pb = planes == 2 && j == 1;
 }
 
 // One output tile of a launch.
@@ -438,7 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   op_begin();
   const int count = *a.count;
-  const int products = a.planes == 1 ? 1 : 6;
+  const int products = a.planes == 1 ? 1 : 3;
   const int bn = MODE == kProducts ? a.bn : kTileN;  // columns of a tile; either CTA loads half
   Units<MODE> units(a, count);
   Unit u;
@@ -549,6 +553,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     float lse = 0.f;
     int32_t tgt = -1;
     const float scale = MODE == kProducts ? grad_scale(a.dloss, a.count, a.mean) / a.g_scale : 0.f;
+    const float fx = sizeof(T) == 4 ? a.unscale[0] : 1.f, fw = sizeof(T) == 4 ? a.unscale[1] : 1.f;
     const Deal full_deal = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs,
                                    (int)(gridDim.x >> 1));
     if (MODE == kProducts && a.db_part) db_columns<T>(a, count, etid, sbias);
@@ -612,6 +617,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const float4 b = b4[k];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[4 * k + i] = v[4 * k + i] * fx * fw;
+            }
             v[4 * k] = fmaf(v[4 * k], kLog2e, b.x);
             v[4 * k + 1] = fmaf(v[4 * k + 1], kLog2e, b.y);
             v[4 * k + 2] = fmaf(v[4 * k + 2], kLog2e, b.z);
@@ -647,7 +656,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 float &x = v[h][4 * k + i];
                 // float32 subtracts lse before the change of base: the largest probabilities
                 // then have small exponents, rounded finely
-                if constexpr (sizeof(T) == 4) x = exp2_fast((x + bb[i] - lse) * kLog2e);
+                if constexpr (sizeof(T) == 4) x = exp2_fast((x * fx * fw + bb[i] - lse) * kLog2e);
                 else x = exp2_fast(fmaf(x, kLog2e, bb[i] - lse));
               }
             }
@@ -662,29 +671,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (32 * h + k == at) v[h][k] -= 1.f;
           }
           float2 col_sum = make_float2(0.f, 0.f);
+          if (a.g_scale != 1.f) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[h][k] *= a.g_scale;
+          }
           if constexpr (sizeof(T) == 2) {
-            if (a.g_scale != 1.f) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int k = 0; k < 32; ++k) v[h][k] *= a.g_scale;
-            }
             unsigned char *bx = box.take();
             box_put16<T>(bx, lane, 0, v[0]);
             box_put16<T>(bx, lane, 1, v[1]);
             box.send(&maps.c, bx, n0 + c, row0, 0, false);
             if (a.db_part) box_sums<T>(bx, lane, col_sum);
           } else {
-            for (int p = 0; p < 3; ++p) {
+            for (int p = 0; p < 2; ++p) {
               unsigned char *bx = box.take();
-              box_put16<__nv_bfloat16>(bx, lane, 0, v[0]);
-              box_put16<__nv_bfloat16>(bx, lane, 1, v[1]);
+              box_put16<__half>(bx, lane, 0, v[0]);
+              box_put16<__half>(bx, lane, 1, v[1]);
               box.send(&maps.c, bx, n0 + c, row0, p, false);
-              if (a.db_part) box_sums<__nv_bfloat16>(bx, lane, col_sum);
+              if (a.db_part) box_sums<__half>(bx, lane, col_sum);
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int k = 0; k < 32; ++k) v[h][k] -= __bfloat162float(__float2bfloat16_rn(v[h][k]));
+                for (int k = 0; k < 32; ++k) v[h][k] -= __half2float(__float2half_rn(v[h][k]));
             }
           }
           if (a.db_part)
@@ -704,7 +713,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[h][k] *= scale;
+              for (int k = 0; k < 32; ++k) v[h][k] *= scale * fx;
             const int vrow = a.v0 + row0;
             if (!a.dw_tma) {  // through a box, so that a warp writes along rows
               T *o = static_cast<T *>(a.dw) + (long)vrow * a.dw_ld + col;
@@ -768,29 +777,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // ---- staging ----------------------------------------------------------------
 __device__ __forceinline__ bool counted(int32_t t, int vocab) { return t >= 0 && t < vocab; }
 
-// Splits v into bfloat16 pieces (one piece: itself rounded, exact for 16-bit input).
+// Writes v as a 16-bit operand: itself, or the high and low float16 pieces of v * scale.
 template <typename T>
-__device__ __forceinline__ void put_pieces(uint16_t *dst, size_t plane, float v) {
+__device__ __forceinline__ void put_pieces(uint16_t *dst, size_t plane, float v, float scale) {
   if constexpr (sizeof(T) == 2) {
     reinterpret_cast<T *>(dst)[0] = op_store<T>(v);
   } else {
-#pragma unroll
-    for (int p = 0; p < 3; ++p) {
-      const __nv_bfloat16 b = __float2bfloat16_rn(v);
-      reinterpret_cast<__nv_bfloat16 *>(dst)[p * plane] = b;
-      v -= __bfloat162float(b);
-    }
+    v *= scale;
+    const __half h = __float2half_rn(v);
+    reinterpret_cast<__half *>(dst)[0] = h;
+    reinterpret_cast<__half *>(dst)[plane] = __float2half_rn(v - __half2float(h));
   }
 }
-
 // One row of 16-bit operands from `src` (null: zeros), by one warp; VEC elements per
 // access where the addresses allow.
 template <typename T, int VEC>
-__device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *src, int dim, int lane) {
+__device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *src, int dim, int lane, float scale) {
 #pragma unroll 4
   for (int c = lane * VEC; c < dim; c += 32 * VEC) {
     if constexpr (VEC == 1) {
-      put_pieces<T>(dst + c, plane, src ? op_load<T>(src[c]) : 0.f);
+      put_pieces<T>(dst + c, plane, src ? op_load<T>(src[c]) : 0.f, scale);
     } else if constexpr (sizeof(T) == 2) {
       uint4 v = make_uint4(0, 0, 0, 0);
       if (src) v = *reinterpret_cast<const uint4 *>(src + c);
@@ -798,28 +804,35 @@ __device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *sr
     } else {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (src) v = *reinterpret_cast<const float4 *>(src + c);
-      float x[4] = {v.x, v.y, v.z, v.w};
+      const float x[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+      OpVec<__half, 4> h, l;
 #pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        OpVec<__nv_bfloat16, 4> b;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          b.v[i] = __float2bfloat16_rn(x[i]);
-          x[i] -= __bfloat162float(b.v[i]);
-        }
-        *reinterpret_cast<OpVec<__nv_bfloat16, 4> *>(dst + p * plane + c) = b;
+      for (int i = 0; i < 4; ++i) {
+        h.v[i] = __float2half_rn(x[i]);
+        l.v[i] = __float2half_rn(x[i] - __half2float(h.v[i]));
       }
+      *reinterpret_cast<OpVec<__half, 4> *>(dst + c) = h;
+      *reinterpret_cast<OpVec<__half, 4> *>(dst + plane + c) = l;
     }
   }
 }
+template <typename T>
+__device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *src, int dim, int lane, float scale, bool vec) {
+  if (vec) put_row<T, 16 / sizeof(T)>(dst, plane, src, dim, lane, scale);
+  else put_row<T, 1>(dst, plane, src, dim, lane, scale);
+}
 
 struct StageArgs {
-  const void *x;
-  long x_ld, rows;
+  const void *x, *w;
+  long x_ld, w_ld, rows;
   const int32_t *tg;
-  int vocab, dim, pitch, per_cta;  // rows per CTA, a multiple of 8
-  size_t plane;
-  uint16_t *xc;
+  int vocab, dim, pitch, per_cta, x_ctas;  // per_cta: rows per CTA, a multiple of 8
+  int x_vec, w_vec;                        // 16-byte rows
+  size_t xplane, wplane;
+  uint16_t *xc, *wc;                       // wc null: W is read where it is
+  const uint32_t *range;                   // float32: [range_ctas][2] largest magnitudes
+  int range_ctas;
+  float *unscale;
   int32_t *slot;
   int *count;
   unsigned int *ticket;
@@ -828,14 +841,97 @@ struct StageArgs {
   int32_t *tgt;
 };
 
-// Finds the counted rows' places (every CTA counts the targets itself: they are few
-// bytes, and a scan would be one launch more), gathers x there, with lse also lse and
-// targets, and zeros the rows behind the last up to a whole tile.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) ce_stage_rows_kernel(const StageArgs a) {
-  __shared__ int sh[2][8];
+// float32: each CTA's largest finite magnitude of the counted rows of x and of W, as bits
+// (which order like the magnitudes).
+__global__ void __launch_bounds__(256) ce_range_kernel(const StageArgs a, uint32_t *range) {
+  __shared__ uint32_t sh[2][8];
   op_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long first = (long)blockIdx.x * 8 + warp, step = (long)gridDim.x * 8;
+  uint32_t top[2] = {0, 0};
+  auto take = [&](float f, uint32_t &t) {
+    const uint32_t u = __float_as_uint(f) & 0x7fffffffu;
+    if (u < 0x7f800000u && u > t) t = u;
+  };
+  auto row = [&](const float *p, bool vec, uint32_t &t) {
+    if (vec) {
+#pragma unroll 4
+      for (int c = lane * 4; c < a.dim; c += 128) {
+        const float4 f = *reinterpret_cast<const float4 *>(p + c);
+        take(f.x, t); take(f.y, t); take(f.z, t); take(f.w, t);
+      }
+    } else {
+#pragma unroll 4
+      for (int c = lane; c < a.dim; c += 32) take(p[c], t);
+    }
+  };
+  for (long n = first; n < a.rows; n += step)
+    if (counted(a.tg[n], a.vocab)) row(static_cast<const float *>(a.x) + n * a.x_ld, a.x_vec, top[0]);
+  for (long v = first; v < a.vocab; v += step) row(static_cast<const float *>(a.w) + v * a.w_ld, a.w_vec, top[1]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    top[i] = __reduce_max_sync(0xffffffffu, top[i]);
+    if (lane == 0) sh[i][warp] = top[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    uint32_t t = 0;
+    for (int w = 0; w < 8; ++w) t = max(t, sh[threadIdx.x][w]);
+    range[blockIdx.x * 2 + threadIdx.x] = t;
+  }
+}
+
+// The power of two that brings a largest magnitude to 2^14..2^15 (as far as float32
+// goes), and its inverse.
+__device__ __forceinline__ void range_scale(uint32_t top, float &scale, float &inverse) {
+  int k = 14 - ((int)(top >> 23) - 127);
+  k = top == 0 ? 0 : min(k, 126);
+  scale = __uint_as_float((uint32_t)(k + 127) << 23);
+  inverse = __uint_as_float((uint32_t)(127 - k) << 23);
+}
+
+// The first CTAs find the counted rows' places (each counts the targets itself: they are
+// few bytes, and a scan would be one launch more), gather x there, with lse also lse and
+// targets, and zero the rows behind the last up to a whole tile (one at least).  The
+// others lay W out, one warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) ce_stage_kernel(const StageArgs a) {
+  __shared__ int sh[2][8];
+  __shared__ uint32_t tops[2][8];
+  op_begin();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float xscale = 1.f, wscale = 1.f;
+  if constexpr (sizeof(T) == 4) {
+    uint32_t top[2] = {0, 0};
+    for (int i = threadIdx.x; i < a.range_ctas; i += 256) {
+      top[0] = max(top[0], a.range[2 * i]);
+      top[1] = max(top[1], a.range[2 * i + 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = __reduce_max_sync(0xffffffffu, top[i]);
+      if (lane == 0) tops[i][warp] = top[i];
+    }
+    __syncthreads();
+    top[0] = top[1] = 0;
+    for (int k = 0; k < 8; ++k) {
+      top[0] = max(top[0], tops[0][k]);
+      top[1] = max(top[1], tops[1][k]);
+    }
+    float ix, iw;
+    range_scale(top[0], xscale, ix);
+    range_scale(top[1], wscale, iw);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      a.unscale[0] = ix;
+      a.unscale[1] = iw;
+    }
+  }
+  if (blockIdx.x >= a.x_ctas) {
+    const long v = (long)(blockIdx.x - a.x_ctas) * 8 + warp;
+    if (v < a.vocab)
+      put_row<T>(a.wc + (size_t)v * a.pitch, a.wplane, static_cast<const T *>(a.w) + v * a.w_ld, a.dim, lane, wscale, a.w_vec);
+    return;
+  }
   const long r0 = (long)blockIdx.x * a.per_cta;
   int before = 0, total = 0;
 #pragma unroll 8
@@ -875,21 +971,13 @@ __global__ void __launch_bounds__(256) ce_stage_rows_kernel(const StageArgs a) {
       }
     }
     const int to = __shfl_sync(0xffffffffu, at, warp);
-    if (mask >> warp & 1) put_row<T, VEC>(a.xc + (size_t)to * a.pitch, a.plane, x + (g0 + warp) * a.x_ld, a.dim, lane);
+    if (mask >> warp & 1)
+      put_row<T>(a.xc + (size_t)to * a.pitch, a.xplane, x + (g0 + warp) * a.x_ld, a.dim, lane, xscale, a.x_vec);
     before += __popc(mask);
   }
   const long end = (long)row_tiles(total) * kTileM;
-  for (long j = total + (long)blockIdx.x * 8 + warp; j < end; j += (long)gridDim.x * 8)
-    put_row<T, VEC>(a.xc + (size_t)j * a.pitch, a.plane, static_cast<const T *>(nullptr), a.dim, lane);
-}
-
-// W (any stride and alignment) as 16-bit operands, one warp per row.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) ce_stage_w_kernel(const T *w, long w_ld, long vocab, int dim, int pitch,
-                                                         size_t plane, uint16_t *wc) {
-  op_begin();
-  const long v = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (v < vocab) put_row<T, VEC>(wc + (size_t)v * pitch, plane, w + v * w_ld, dim, threadIdx.x & 31);
+  for (long j = total + (long)blockIdx.x * 8 + warp; j < end; j += (long)a.x_ctas * 8)
+    put_row<T, 1>(a.xc + (size_t)j * a.pitch, a.xplane, static_cast<const T *>(nullptr), a.dim, lane, 1.f);
 }
 
 // ---- joins -------------------------------------------------------------------
@@ -1151,7 +1239,7 @@ __global__ void __launch_bounds__(256) ce_dx_kernel(const float *slab, size_t sl
   __syncthreads();
   if (n >= rows) return;
   const int at = slot[n];
-  const float c = grad_scale(a.dloss, a.count, a.mean) / a.g_scale;
+  const float c = grad_scale(a.dloss, a.count, a.mean) / a.g_scale * (sizeof(T) == 4 ? a.unscale[1] : 1.f);
   const uint8_t *mine = cover + (at >= 0 && at / kTileM != first ? a.tiles_d : 0);
   for (int i = ((warp % per_row) * 32 + lane) * 4; i < a.dim; i += per_row * 128) {
     float s[4] = {};
@@ -1202,6 +1290,9 @@ struct Plan {
   int32_t *slot;
   int *count;
   unsigned int *ticket;
+  float *unscale;
+  uint32_t *range;
+  int range_ctas;
   uint16_t *xc, *wc;
   float2 *stats;
   float *row_loss;
@@ -1225,7 +1316,7 @@ int piece_tiles(const aideen_linear_ce_args *a, const Plan &p) {
   long most = (160L << 20) / bytes;
   if (most < half) most = half;
   if (most >= p.tiles_n) most = p.tiles_n;
-  const long products = p.planes == 1 ? 1 : 6, k_dim = (a->dim + kBlockK - 1) / kBlockK;
+  const long products = p.planes == 1 ? 1 : 3, k_dim = (a->dim + kBlockK - 1) / kBlockK;
   const long k_rows = ((long)a->rows + kBlockK - 1) / kBlockK;
   auto cost = [&](long tiles) {
     const Deal d(tiles * p.tiles_d, k_rows, (long)p.tiles_m * p.tiles_d, (int)tiles * (kTileN / kBlockK), p.slabs, p.pairs);
@@ -1245,7 +1336,7 @@ int piece_tiles(const aideen_linear_ce_args *a, const Plan &p) {
 
 Plan make_plan(const aideen_linear_ce_args *a, void *ws) {
   Plan p{};
-  p.planes = a->dtype == AIDEEN_F32 ? 3 : 1;
+  p.planes = a->dtype == AIDEEN_F32 ? 2 : 1;
   p.pairs = op_sm_count() / 2;
   p.tiles_m = (int)((a->rows + kTileM - 1) / kTileM);
   p.tiles_n = (int)((a->vocab + kTileN - 1) / kTileN);
@@ -1258,6 +1349,9 @@ Plan make_plan(const aideen_linear_ce_args *a, void *ws) {
   p.slot = c.take<int32_t>(a->rows);
   p.count = c.take<int>(1);
   p.ticket = c.take<unsigned int>(1);
+  p.unscale = c.take<float>(2);
+  p.range_ctas = p.planes == 2 ? 4 * op_sm_count() : 0;
+  p.range = c.take<uint32_t>((size_t)2 * p.range_ctas);
   p.xc = c.take<uint16_t>(p.xplane * p.planes);
   p.wc = c.take<uint16_t>(p.w_direct ? 0 : p.wplane * p.planes);
   OpCarve g = c;
@@ -1331,18 +1425,20 @@ cudaError_t stage_run(const aideen_linear_ce_args *g, const Plan &p, const T *x,
                       const float *lse, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   StageArgs s{};
-  s.x = x; s.x_ld = g->x_ld; s.rows = g->rows; s.tg = tg; s.vocab = (int)g->vocab; s.dim = (int)g->dim;
-  s.pitch = p.pitch; s.plane = p.xplane; s.xc = p.xc; s.slot = p.slot; s.count = p.count; s.ticket = p.ticket;
-  s.lse = lse; s.lse_c = p.lse_c; s.tgt = p.tgt;
+  s.x = x; s.w = w; s.x_ld = g->x_ld; s.w_ld = g->w_ld; s.rows = g->rows; s.tg = tg; s.vocab = (int)g->vocab;
+  s.dim = (int)g->dim; s.pitch = p.pitch; s.xplane = p.xplane; s.wplane = p.wplane; s.xc = p.xc; s.wc = p.wc;
+  s.slot = p.slot; s.count = p.count; s.ticket = p.ticket; s.lse = lse; s.lse_c = p.lse_c; s.tgt = p.tgt;
+  s.range = p.range; s.range_ctas = p.range_ctas; s.unscale = p.unscale;
+  s.x_vec = g->dim % V == 0 && op_vec16(x, g->x_ld, sizeof(T));
+  s.w_vec = g->dim % V == 0 && op_vec16(w, g->w_ld, sizeof(T));
   const long most = 4L * 2 * p.pairs;  // CTAs
   s.per_cta = (int)(8 * ((g->rows + 8 * most - 1) / (8 * most)));
-  const unsigned ctas = (unsigned)((g->rows + s.per_cta - 1) / s.per_cta);
-  const bool xv = g->dim % V == 0 && op_vec16(x, g->x_ld, sizeof(T));
-  cudaError_t e = op_launch(xv ? ce_stage_rows_kernel<T, V> : ce_stage_rows_kernel<T, 1>, ctas, 256, 0, st, s);
-  if (e != cudaSuccess || p.w_direct) return e;
-  const bool wv = g->dim % V == 0 && op_vec16(w, g->w_ld, sizeof(T));
-  return op_launch(wv ? ce_stage_w_kernel<T, V> : ce_stage_w_kernel<T, 1>, (g->vocab + 7) / 8, 256, 0, st, w, g->w_ld,
-                   g->vocab, g->dim, p.pitch, p.wplane, p.wc);
+  s.x_ctas = (int)((g->rows + s.per_cta - 1) / s.per_cta);
+  const unsigned w_ctas = p.w_direct ? 0 : (g->vocab + 7) / 8;
+  cudaError_t e = cudaSuccess;
+  if constexpr (sizeof(T) == 4) e = op_launch(ce_range_kernel, p.range_ctas, 256, 0, st, s, p.range);
+  if (e == cudaSuccess) e = op_launch(ce_stage_kernel<T>, s.x_ctas + w_ctas, 256, 0, st, s);
+  return e;
 }
 
 template <typename T>
@@ -1350,10 +1446,11 @@ MmaArgs mma_args(const aideen_linear_ce_args *g, const Plan &p, const T *bias) {
   MmaArgs a{};
   a.count = p.count;
   a.vocab = (int)g->vocab; a.dim = (int)g->dim; a.planes = p.planes; a.dtype = g->dtype;
-  const uint32_t type = g->dtype == AIDEEN_F16 ? 0u : 1u;  // f16 or bf16 operands, f32 accumulator
+  const uint32_t type = g->dtype == AIDEEN_BF16 ? 1u : 0u;  // bf16 or f16 operands, f32 accumulator
   a.idesc = (1u << 4) | (type << 7) | (type << 10);
   a.bias = bias;
-  a.g_scale = g->dtype == AIDEEN_F16 ? kHalfScale : 1.f;
+  a.g_scale = g->dtype == AIDEEN_F16 ? kHalfScale : g->dtype == AIDEEN_F32 ? kPieceScale : 1.f;
+  a.unscale = p.unscale;
   a.mean = g->reduction == AIDEEN_CE_MEAN;
   return a;
 }
