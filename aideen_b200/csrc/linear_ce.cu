@@ -194,6 +194,7 @@ struct Unit {
   int kb0, nkb;  // 64-deep slices
   int dw;        // kProducts: 1 = dW tile, 0 = dx tile
   int z;         // dx: slab
+  bool first;    // chunk of the tile's depth
 };
 
 // How a piece's two products are dealt out over the pairs.  dW tiles go out whole
@@ -243,13 +244,22 @@ __device__ __forceinline__ Deal deal_of(int count, int tiles_v, int tiles_d, int
               slabs ? (long)row_tiles(count) * tiles_d : 0, depth, slabs, pairs);
 }
 
+// float32's products with G take a tile's depth in chunks of this many slices, each
+// added to what the ones before stored: the tensor cores cut where they add, by up to a
+// unit of the sum at each 16 deep, always towards zero.  Over the 16384 rows of a dW that
+// grew to 1.9e-5 of it; in chunks it stays at 1e-6 for any number of rows, at 8% of the
+// gradient's time.  (z is cut the same way over its depth: 4e-7 of it at 512.)
+constexpr int kChunk = 8;
+
 // Units of one pair.  kStats and kPiece: a contiguous share of the (row tile,
 // vocabulary tile) order, so that a pair stays on one row tile.  kProducts: its
 // dW tiles, then its run of dx.
-template <int MODE>
+template <int MODE, bool CHUNKS>
 struct Units {
   const MmaArgs &a;
   Deal deal;
+  Unit tile;
+  int depth = 0;     // slices of `tile` given out
   int pair, k_dim, k_rows;
   long next, end;    // tiles (kStats, kPiece) or dW tiles
   long dx, dx_end;   // slices of dx
@@ -272,8 +282,25 @@ struct Units {
       end = (pair + 1) * total / pairs;
       dx = dx_end = 0;
     }
+    tile.nkb = 0;
   }
   __device__ __forceinline__ bool get(Unit &u) {
+    if (!CHUNKS) {
+      u.first = true;
+      return get_tile(u);
+    }
+    if (depth >= tile.nkb) {
+      if (!get_tile(tile)) return false;
+      depth = 0;
+    }
+    u = tile;
+    u.kb0 += depth;
+    u.nkb = min(kChunk, tile.nkb - depth);
+    u.first = depth == 0;
+    depth += u.nkb;
+    return true;
+  }
+  __device__ __forceinline__ bool get_tile(Unit &u) {
     if (next < end) {
       const int per = MODE == kProducts ? a.tiles_d : a.tiles_n;
       u.m = (int)(next / per);
@@ -444,7 +471,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int count = *a.count;
   const int products = a.planes == 1 ? 1 : 3;
   const int bn = MODE == kProducts ? a.bn : kTileN;  // columns of a tile; either CTA loads half
-  Units<MODE> units(a, count);
+  constexpr bool kChunks = MODE == kProducts && sizeof(T) == 4;
+  Units<MODE, kChunks> units(a, count);
   Unit u;
 
   if (warp == 0) {
@@ -606,12 +634,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (elect_one()) remote_arrive(leader_addr(&tempty[acc]));
       };
+      // 32 of this warp's columns; `last`: the accumulator is not read again
+      auto fetch = [&](int c, float (&v)[32], bool last) {
+        tmem_load32(t0 + c, v);
+        if (last) release();
+      };
       if (MODE == kStats) {
 #pragma unroll 1
-        for (int c = 0; c < hcols; c += 32) {
+        for (int c = 0; c < kTileN / 2; c += 32) {
           float v[32];
-          tmem_load32(t0 + c, v);
-          if (c + 32 == hcols) release();
+          fetch(c, v, c + 32 == kTileN / 2);
           const float4 *b4 = reinterpret_cast<const float4 *>(sb + half * hcols + c);
           float top = run_m;
 #pragma unroll
@@ -641,11 +673,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       } else if (MODE == kPiece) {
         const int n0 = u.n * kTileN + half * hcols;
 #pragma unroll 1
-        for (int c = 0; c < hcols; c += 64) {
+        for (int c = 0; c < kTileN / 2; c += 64) {
           float v[2][32];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            tmem_load32(t0 + c + 32 * h, v[h]);
+            fetch(c + 32 * h, v[h], c + 64 == kTileN / 2 && h == 1);
             const float4 *b4 = reinterpret_cast<const float4 *>(sb + half * hcols + c + 32 * h);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -661,7 +693,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               }
             }
           }
-          if (c + 64 == hcols) release();
           const int at = tgt - (a.v0 + n0 + c);  // the target's column among these 64
           if (__any_sync(0xffffffffu, at >= 0 && at < 64)) {
 #pragma unroll
@@ -701,53 +732,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       } else {
         const int n0 = u.n * bn + half * hcols;
-        const bool add = !a.first && u.z < full_deal.cover((long)u.m * a.tiles_d + u.n);  // else this slab is new
+        // dx: into a slab that an earlier piece wrote already?
+        const bool add = !u.first || (!u.dw && !a.first && u.z < full_deal.cover((long)u.m * a.tiles_d + u.n));
+        if (kChunks && !u.first) {  // the chunks before have to be there
+          if (elect_one()) bulk_wait<0>();
+          __syncwarp();
+        }
+        const int vrow = a.v0 + row0;
+        // through a box, so that a warp writes along rows where TMA cannot
+        auto write_rows = [&](const unsigned char *bx, int col, int width) {
+          __syncwarp();
+          T *o = static_cast<T *>(a.dw) + (long)vrow * a.dw_ld + col;
+          const int rows = min(32, a.vocab - vrow), cols = min(width, a.dim - col);
+#pragma unroll 4
+          for (int r = 0; r < rows; ++r)
+            for (int c = lane; c < cols; c += 32) {
+              T v = *reinterpret_cast<const T *>(bx + r * 128 + ((c * (int)sizeof(T)) ^ ((r & 7) * 16)));
+              if constexpr (kChunks) v += u.first ? 0.f : o[(long)r * a.dw_ld + c];
+              o[(long)r * a.dw_ld + c] = v;
+            }
+          __syncwarp();
+        };
 #pragma unroll 1
         for (int c = 0; c < hcols; c += 64) {
           float v[2][32];
-          tmem_load32(t0 + c, v[0]);
-          tmem_load32(t0 + c + 32, v[1]);
-          if (c + 64 == hcols) release();
+          fetch(c, v[0], false);
+          fetch(c + 32, v[1], c + 64 == hcols);
           const int col = n0 + c;
           if (u.dw) {
+            if (col >= a.dim || vrow >= a.vocab) continue;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int k = 0; k < 32; ++k) v[h][k] *= scale * fx;
-            const int vrow = a.v0 + row0;
-            if (!a.dw_tma) {  // through a box, so that a warp writes along rows
-              T *o = static_cast<T *>(a.dw) + (long)vrow * a.dw_ld + col;
-              for (int h = 0; h < (sizeof(T) == 2 ? 1 : 2); ++h) {
-                constexpr int kCols = 128 / sizeof(T);
-                unsigned char *bx = box.take();
-                if constexpr (sizeof(T) == 2) {
-                  box_put16<T>(bx, lane, 0, v[0]);
-                  box_put16<T>(bx, lane, 1, v[1]);
-                } else {
-                  box_put32(bx, lane, h ? v[1] : v[0]);
-                }
-                __syncwarp();
-                const int rows = min(32, a.vocab - vrow), cols = min(kCols, a.dim - col - h * 32);
-#pragma unroll 4
-                for (int r = 0; r < rows; ++r)
-                  for (int c = lane; c < cols; c += 32)
-                    o[(long)r * a.dw_ld + h * 32 + c] =
-                        *reinterpret_cast<const T *>(bx + r * 128 + (((c * (int)sizeof(T)) ^ ((r & 7) * 16))));
-                __syncwarp();
-              }
-            } else if constexpr (sizeof(T) == 2) {
-              if (col < a.dim && vrow < a.vocab) {
-                unsigned char *bx = box.take();
-                box_put16<T>(bx, lane, 0, v[0]);
-                box_put16<T>(bx, lane, 1, v[1]);
-                box.send(&maps.c2, bx, col, vrow, 0, false);
-              }
+            if constexpr (sizeof(T) == 2) {
+              unsigned char *bx = box.take();
+              box_put16<T>(bx, lane, 0, v[0]);
+              box_put16<T>(bx, lane, 1, v[1]);
+              if (a.dw_tma) box.send(&maps.c2, bx, col, vrow, 0, false);
+              else write_rows(bx, col, 64);
             } else {
               for (int h = 0; h < 2; ++h) {
-                if (col + 32 * h >= a.dim || vrow >= a.vocab) continue;
+                if (col + 32 * h >= a.dim) continue;
                 unsigned char *bx = box.take();
                 box_put32(bx, lane, h ? v[1] : v[0]);
-                box.send(&maps.c2, bx, col + 32 * h, vrow, 0, false);
+                if (a.dw_tma) box.send(&maps.c2, bx, col + 32 * h, vrow, 0, add);
+                else write_rows(bx, col + 32 * h, 32);
               }
             }
           } else {
