@@ -18,16 +18,22 @@
 // Tensor-core kernel (ce_mma_kernel): a persistent grid of CTA pairs, each on
 // 256 x 256 tiles (tcgen05.mma cta_group::2: every CTA holds 128 rows of the
 // accumulator and loads half of either operand).  Per CTA: warp 0 streams 64-deep
-// slices by TMA into a ring of five 32 KB stages, warp 1 of the leading CTA
-// issues the MMAs into one of two 256-column accumulators in tensor memory, and
-// warps 2..9 drain the other one.
+// slices by TMA into a ring that takes what the shared memory has left (up to eight
+// stages of 32 KB, or of 16 KB where the row tile of x stays in shared memory and
+// only W streams), warp 1 of the leading CTA issues the MMAs into one of two
+// 256-column accumulators in tensor memory, and warps 2..9 drain the other one.
+// A pair tile is the largest that leaves two accumulators: an operand byte from L2
+// carries 256 products, so that L2 does not bound it.
 //
 // float32: each of x, W and G = softmax - onehot is scaled by a power of two that brings
 // its largest magnitude (G: 1) to 2^14..2^15 and written as high + low float16 pieces;
 // high x high + high x low + low x high leave out 2^-22 of a product, three passes where
-// bfloat16 pieces would take six (training shard 50257 x 512, 2048 rows: %%A%%).  What
+// bfloat16 pieces would take six (training shard 50257 x 512, 2048 rows, loss and gradient:
+// 2.23 ms with those, 1.43 ms this way).  What
 // lies below 2^-40 of the largest magnitude (G: 2^-39) is rounded off.
-// Bound: the tensor cores (2 N V d for the loss, 6 N V d for the gradient).
+// Bound: the tensor cores (2 N V d for the loss, 6 N V d for the gradient, z being
+// formed twice), and behind them the power limit: 8192 rows, 50257 x 512 bf16, loss and
+// gradient take 1.35 ms, 1.25 PFLOP/s, at clocks that the limit holds at 1.3-1.5 GHz.
 //
 // Every wait is bounded; a wait that runs out sets an error word, issues nothing
 // further, lets its copies land, frees the tensor memory and returns.
@@ -70,7 +76,6 @@ struct MmaArgs {
   // kStats, kPiece: vocabulary tiles [0, tiles_n) from column v0 on
   int v0, tiles_n;
   const void *bias;
-  uint32_t dtype;     // of bias, dW
   float2 *stats;      // kStats: [slot][2][256] (maximum, sum) in base 2
   const float *lse;   // kPiece: compacted rows' lse
   const int32_t *tgt; // and their targets
@@ -582,6 +587,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int32_t tgt = -1;
     const float scale = MODE == kProducts ? grad_scale(a.dloss, a.count, a.mean) / a.g_scale : 0.f;
     const float fx = sizeof(T) == 4 ? a.unscale[0] : 1.f, fw = sizeof(T) == 4 ? a.unscale[1] : 1.f;
+    const float f_lo = fminf(fx, fw), f_hi = fmaxf(fx, fw);  // in this order z overflows only where it has to
     const Deal full_deal = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs,
                                    (int)(gridDim.x >> 1));
     if (MODE == kProducts && a.db_part) db_columns<T>(a, count, etid, sbias);
@@ -610,7 +616,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             run_s = 0.f;
           } else {
             const int row = u.m * kTileM + (int)rank * 128 + q * 32 + lane;
-            lse = row < count ? a.lse[row] : INFINITY;  // rows behind the last: G = 0
+            lse = row < count ? a.lse[row] : 0.f;
             if (sizeof(T) == 2) lse *= kLog2e;
             tgt = row < count ? a.tgt[row] : -1;
           }
@@ -651,7 +657,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const float4 b = b4[k];
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) v[4 * k + i] = v[4 * k + i] * fx * fw;
+              for (int i = 0; i < 4; ++i) v[4 * k + i] = v[4 * k + i] * f_lo * f_hi;
             }
             v[4 * k] = fmaf(v[4 * k], kLog2e, b.x);
             v[4 * k + 1] = fmaf(v[4 * k + 1], kLog2e, b.y);
@@ -688,10 +694,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 float &x = v[h][4 * k + i];
                 // float32 subtracts lse before the change of base: the largest probabilities
                 // then have small exponents, rounded finely
-                if constexpr (sizeof(T) == 4) x = exp2_fast((x * fx * fw + bb[i] - lse) * kLog2e);
+                if constexpr (sizeof(T) == 4) x = exp2_fast((x * f_lo * f_hi + bb[i] - lse) * kLog2e);
                 else x = exp2_fast(fmaf(x, kLog2e, bb[i] - lse));
               }
             }
+          }
+          if (row0 + 32 > count) {  // rows behind the last, whatever an infinite W made of them
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (row0 + lane >= count) v[h][k] = 0.f;
           }
           const int at = tgt - (a.v0 + n0 + c);  // the target's column among these 64
           if (__any_sync(0xffffffffu, at >= 0 && at < 64)) {
@@ -1285,7 +1298,7 @@ __global__ void __launch_bounds__(256) ce_dx_kernel(const float *slab, size_t sl
       }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] *= c;
+    for (int e = 0; e < 4; ++e) s[e] = at >= 0 ? s[e] * c : 0.f;  // 0 whatever dloss is
     T *o = dx + n * dx_ld + i;
     if (vec) {
       op_store_vec<T, 4>(o, s);
@@ -1425,7 +1438,7 @@ bool map_x(CUtensorMap *m, const Plan &p, int dim, uint32_t rows) {
 }
 bool map_w(CUtensorMap *m, const Plan &p, const aideen_linear_ce_args *g, const void *w, uint32_t rows) {
   if (p.w_direct)
-    return make_map(m, kU16, w, g->dim, g->vocab, 1, (size_t)g->w_ld * 2, (size_t)g->w_ld * 2 * g->vocab, 64, rows);
+    return make_map(m, kU16, w, g->dim, g->vocab, 1, (size_t)g->w_ld * 2, (size_t)g->w_ld * 2, 64, rows);
   return make_map(m, kU16, p.wc, g->dim, g->vocab, p.planes, (size_t)p.pitch * 2, p.wplane * 2, 64, rows);
 }
 
@@ -1475,7 +1488,7 @@ template <typename T>
 MmaArgs mma_args(const aideen_linear_ce_args *g, const Plan &p, const T *bias) {
   MmaArgs a{};
   a.count = p.count;
-  a.vocab = (int)g->vocab; a.dim = (int)g->dim; a.planes = p.planes; a.dtype = g->dtype;
+  a.vocab = (int)g->vocab; a.dim = (int)g->dim; a.planes = p.planes;
   const uint32_t type = g->dtype == AIDEEN_BF16 ? 1u : 0u;  // bf16 or f16 operands, f32 accumulator
   a.idesc = (1u << 4) | (type << 7) | (type << 10);
   a.bias = bias;
@@ -1544,8 +1557,8 @@ cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
   const size_t el = sizeof(T);
   const bool dw_tma = dw && op_vec16(dw, g->dw_ld, el);
   if (dw_tma)
-    ok = ok && make_map(&pm.c2, el == 4 ? kF32 : kU16, dw, dim, g->vocab, 1, g->dw_ld * el,
-                        (size_t)g->dw_ld * el * g->vocab, 128 / el, 32);
+    ok = ok && make_map(&pm.c2, el == 4 ? kF32 : kU16, dw, dim, g->vocab, 1, g->dw_ld * el, g->dw_ld * el,
+                        128 / el, 32);
   if (!ok) return cudaErrorInvalidValue;
   MmaArgs a = mma_args<T>(g, p, bias);
   a.lse = p.lse_c; a.tgt = p.tgt; a.db_part = db ? p.db_part : nullptr;

@@ -20,6 +20,7 @@ inline int op_invalid(const char *why) {
 }
 inline int op_cuda(cudaError_t e) {
   if (e == cudaSuccess) return AIDEEN_OK;
+  (void)cudaGetLastError();  // reported here: no later check of the caller's trips over it
   op_set_error(cudaGetErrorString(e));
   return AIDEEN_E_CUDA;
 }

@@ -23,6 +23,7 @@ from .backend import AideenError, EmbedArgs, LayerNormArgs, LinearCeArgs, load_l
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _REDUCTIONS = {"mean": 0, "sum": 1}
+_COUNTS = 1 << 31  # the library's own limits lie below; from here on a count would not fit its field
 
 
 def _check(rc: int, what: str):
@@ -48,9 +49,11 @@ def _rows(t, what: str, name: str):
     if t.dim() < 1 or t.shape[-1] < 1:
         raise AideenError(f"{what}: {name} needs a last dimension of at least 1")
     dim = t.shape[-1]
+    if t.numel() // dim >= _COUNTS or dim >= _COUNTS:
+        raise AideenError(f"{what}: {name} has more rows or columns than the library counts")
     if t.dim() == 1:
-        return 1, dim, dim
-    if t.dim() > 2:
+        t = t.unsqueeze(0)
+    elif t.dim() > 2:
         try:
             t = t.view(-1, dim)
         except RuntimeError:
@@ -127,6 +130,8 @@ def check(device=None):
 # ---- embedding -------------------------------------------------------------
 def _ids(ids, what: str, like, name: str = "ids"):
     _tensor(ids, what, name, like, torch.int32)
+    if ids.numel() >= _COUNTS:
+        raise AideenError(f"{what}: more {name} than the library counts")
     if not ids.is_contiguous():
         raise AideenError(f"{what}: {name} must be contiguous")
     return ids.data_ptr()

@@ -335,9 +335,10 @@ int aideen_adjoint_noalloc(const float *hstar, const float *branch, const float 
  *     in elements, at least the row's length; rows must not overlap).  Outputs
  *     must not overlap inputs or each other.
  *   - scratch memory is the caller's: a *_workspace function gives its size for
- *     the same arguments, the pointer is 256-byte aligned, and its contents
- *     need no initialisation and mean nothing between calls.  Calls that overlap
- *     on the GPU (other streams, graphs replayed side by side) need one each.
+ *     the same arguments on the same current device, the pointer is 256-byte
+ *     aligned, and its contents need no initialisation and mean nothing between
+ *     calls.  Calls that overlap on the GPU (other streams, graphs replayed side
+ *     by side) need one each.
  *   - work is queued on `stream` (a cudaStream_t) and not waited for; every call
  *     may be captured into a CUDA graph.
  *   - arguments are checked before anything is launched: AIDEEN_E_INVALID, and
@@ -434,7 +435,12 @@ int aideen_linear_ce(const aideen_linear_ce_args *args, const void *x, const voi
  * vocabulary.  dx, dw and dbias may be NULL where they are not wanted (not all
  * three).  dx rows that are not counted are zero.  In 16 bits, softmax - onehot
  * is rounded to dtype before its two products (its relative error there is that
- * of one rounding); dx, dW and dbias are rounded once more when stored. */
+ * of one rounding; in float16 it is scaled by 2^12 first, so probabilities below
+ * 2^-26 lose digits); dx, dW and dbias are rounded once more when stored.  In
+ * float32 (in the loss too, but for a few rows) x, W and softmax - onehot enter their
+ * products as two scaled float16 pieces each: 22 bits of a value, and what lies
+ * below 2^-39 of a tensor's largest magnitude is rounded off.  An infinite x or W
+ * makes its logits NaN there. */
 int aideen_linear_ce_grad(const aideen_linear_ce_args *args, const void *x, const void *w, const void *bias,
                           const int32_t *targets, const float *lse, const float *dloss, void *dx, void *dw,
                           void *dbias, void *workspace, size_t workspace_bytes, void *stream);

@@ -450,6 +450,52 @@ def test_linear_ce_nonfinite_rows_spoil_only_themselves():
     assert not bool(torch.isfinite(rows).any())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows", [30, 257])
+def test_linear_ce_infinite_row_of_w(dtype, rows):
+    """A vocabulary entry that W puts at minus infinity has probability 0, and the rows
+    that fill up the last tile do not reach its gradients."""
+    x, w, b, tg = ce_inputs(5, rows, 72, 300, dtype, True)
+    x = x.abs() + 0.25
+    w[41] = float("-inf")
+    tg[tg == 41] = 0
+    _, _, lse = K.linear_ce(x, w, tg, b)
+    _, dw, db = K.linear_ce_grad(x, w, tg, lse, b, want=("weight", "bias"))
+    assert bool((dw[41] == 0).all()) and float(db[41]) == 0
+    keep = [v for v in range(300) if v != 41]
+    tg2 = torch.where(tg > 41, tg - 1, tg)
+    _, _, lse2 = K.linear_ce(x, w[keep], tg2, b[keep])
+    assert bool(torch.isfinite(lse).all())
+    # either lse is off by its 300 terms' roundings and those of its logits, of 72 products each
+    zabs = (x.double().abs() @ w[keep].double().abs().T + b[keep].double().abs()).amax(1)
+    close(lse, lse2.double(), 2 * U32 * (2 * 72 * zabs + 2 * 300 + 4 * lse2.double().abs() + 16))
+
+
+def test_linear_ce_of_a_call_that_is_scaled_to_nan():
+    """dx of rows that are not counted is 0 whatever dloss is."""
+    for dtype in TYPES:
+        x, w, b, tg = ce_inputs(6, 40, 24, 100, dtype, False)
+        tg[::3] = -1
+        _, _, lse = K.linear_ce(x, w, tg)
+        dx, _, _ = K.linear_ce_grad(x, w, tg, lse, dloss=torch.tensor([float("nan")], device="cuda"))
+        assert bool((dx[::3] == 0).all()) and bool(torch.isnan(dx[1::3]).all())
+
+
+def test_linear_ce_in_float32_at_the_ends_of_the_range():
+    """x times a power of two and W divided by it change no logit, so not a bit of the
+    loss, and dW by that power alone (W stays normal: its smallest value is 1/2)."""
+    g = gen(7)
+    x, w = rand(g, 60, 64, std=0.3), torch.rand(200, 64, generator=g, device="cuda") / 2 + 0.5
+    tg = torch.randint(0, 200, (60,), generator=g, device="cuda", dtype=torch.int32)
+    far = 2.0 ** 120
+    loss, row, lse = K.linear_ce(x, w, tg)
+    loss2, row2, lse2 = K.linear_ce(x * far, w / far, tg)
+    assert torch.equal(loss, loss2) and torch.equal(row, row2) and torch.equal(lse, lse2)
+    _, dw, _ = K.linear_ce_grad(x, w, tg, lse, want=("weight",))
+    _, dw2, _ = K.linear_ce_grad(x * far, w / far, tg, lse, want=("weight",))
+    assert torch.equal(dw * far, dw2)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_ce_peaked_rows(dtype):
     """Large logits: the softmax is all but one-hot, the loss near zero or large."""

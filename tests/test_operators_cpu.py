@@ -134,6 +134,19 @@ def test_workspaces_grow_with_the_sizes_and_stay_below_the_logits(lib):
     assert grad_bytes(200000) < 1.5 * grad_bytes(50257)
 
 
+def test_rows_of_a_matrix():
+    x = torch.zeros(4, 6, 10)
+    assert operators._rows(x, "f", "x") == (24, 10, 10)
+    assert operators._rows(x[..., :8], "f", "x") == (24, 8, 10)
+    assert operators._rows(x[0, 0], "f", "x") == (1, 10, 10)
+    assert operators._rows(x[:0], "f", "x") == (0, 10, 10)
+    for bad, word in [(x[..., ::2], "contiguous"), (x[0, 0, ::2], "contiguous"), (x[:, :5, :], "row stride"),
+                      (x[0, :1].expand(3, 10), "overlap"), (torch.tensor(1.0), "dimension"), (x[..., :0], "dimension"),
+                      (torch.zeros(1).expand(1 << 32, 1), "counts"), (torch.zeros(1).expand(2, 1 << 31), "counts")]:
+        with pytest.raises(AideenError, match=word):
+            operators._rows(bad, "f", "x")
+
+
 @pytest.mark.parametrize("call", [
     lambda t, i: operators.embed(i, t),
     lambda t, i: operators.embed_grad(i, t, 4),
