@@ -1352,7 +1352,8 @@ struct Plan {
 // Vocabulary tiles of a piece.  G of a piece stays within 160 MB, but for the
 // columns that dW needs to keep half of the pairs busy (a tile goes to one pair
 // whole).  Among those sizes the one is taken whose launches cost least: the
-// busiest pair's slices, and about 16 slices' time for each launch.
+// busiest pair's slices, and about 16 slices' time for each launch.  About 40 sizes are
+// looked at, so that the search stays near 1 us of the caller's time.
 int piece_tiles(const aideen_linear_ce_args *a, const Plan &p) {
   const long bytes = p.mpad * kTileN * 2 * p.planes;
   const long half = (p.pairs / 2 + p.tiles_d - 1) / p.tiles_d;
@@ -1366,7 +1367,7 @@ int piece_tiles(const aideen_linear_ce_args *a, const Plan &p) {
     return ((tiles * p.tiles_m + p.pairs - 1) / p.pairs * k_dim + d.load) * products + 32;
   };
   long best = most, best_cost = -1;
-  for (long tiles = most; tiles >= 1 && tiles * 3 >= most; --tiles) {
+  for (long tiles = most; tiles >= 1 && tiles * 3 >= most; tiles -= 1 + most / 64) {
     const long n = p.tiles_n / tiles, rest = p.tiles_n % tiles;
     const long c = n * cost(tiles) + (rest ? cost(rest) : 0);
     if (best_cost < 0 || c < best_cost) {
@@ -1377,7 +1378,7 @@ int piece_tiles(const aideen_linear_ce_args *a, const Plan &p) {
   return (int)best;
 }
 
-Plan make_plan(const aideen_linear_ce_args *a, void *ws) {
+Plan make_plan(const aideen_linear_ce_args *a, void *ws, bool grad) {
   Plan p{};
   p.planes = a->dtype == AIDEEN_F32 ? 2 : 1;
   p.pairs = op_sm_count() / 2;
@@ -1401,6 +1402,7 @@ Plan make_plan(const aideen_linear_ce_args *a, void *ws) {
   p.stats = c.take<float2>((size_t)(p.pairs + p.tiles_m) * 2 * kTileM);
   p.row_loss = c.take<float>(a->rows);
   p.loss_bytes = c.used;
+  if (!grad) return p;
   p.bn = (a->dim + 127) / 128 % 2 ? 128 : 256;  // fewer padded columns
   p.tiles_d = (int)((a->dim + p.bn - 1) / p.bn);
   const int dx_tiles = p.tiles_m ? p.tiles_m * p.tiles_d : 1;
@@ -1614,7 +1616,7 @@ using namespace aideen;
 extern "C" int aideen_linear_ce_workspace(const aideen_linear_ce_args *args, size_t *loss_bytes, size_t *grad_bytes) {
   const int rc = check_args(args);
   if (rc != AIDEEN_OK) return rc;
-  const Plan p = make_plan(args, nullptr);
+  const Plan p = make_plan(args, nullptr, grad_bytes != nullptr);
   if (loss_bytes) *loss_bytes = p.loss_bytes;
   if (grad_bytes) *grad_bytes = p.grad_bytes;
   return AIDEEN_OK;
@@ -1633,7 +1635,7 @@ extern "C" int aideen_linear_ce(const aideen_linear_ce_args *args, const void *x
   if (args->rows == 0) return loss ? op_cuda(cudaMemsetAsync(loss, 0, sizeof(float), st)) : AIDEEN_OK;
   OP_CHECK(loss || row_loss || lse, "linear_ce: no output wanted");
   OP_CHECK(x && w && targets, "linear_ce: null x, w or targets");
-  const Plan p = make_plan(args, workspace);
+  const Plan p = make_plan(args, workspace, false);
   OP_CHECK(!p.w_direct || op_aligned(w, 16), "linear_ce: w must be 16-byte aligned at this type and row stride");
   OP_CHECK(workspace && op_aligned(workspace, 256) && workspace_bytes >= p.loss_bytes,
            "linear_ce: workspace missing, misaligned or too small");
@@ -1664,7 +1666,7 @@ extern "C" int aideen_linear_ce_grad(const aideen_linear_ce_args *args, const vo
   }
   OP_CHECK(dx || dw || dbias, "linear_ce_grad: no output wanted");
   OP_CHECK(x && w && targets && lse, "linear_ce_grad: null x, w, targets or lse");
-  const Plan p = make_plan(args, workspace);
+  const Plan p = make_plan(args, workspace, true);
   OP_CHECK(!p.w_direct || op_aligned(w, 16), "linear_ce_grad: w must be 16-byte aligned at this type and row stride");
   OP_CHECK(workspace && op_aligned(workspace, 256) && workspace_bytes >= p.grad_bytes,
            "linear_ce_grad: workspace missing, misaligned or too small");
