@@ -89,7 +89,7 @@ struct MmaArgs {
   int want_dw;
   int slabs;          // slabs of dx (0: dx not wanted)
   int first;          // first piece: dx slabs are written, not added to
-  int dw_tma;         // dW can be stored by TMA
+  int dw_vec;         // dW: elements per access (see row_width); 16 bytes: stored by TMA
   void *dw, *db;
   long dw_ld;
   const float *dloss;
@@ -757,6 +757,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           __syncwarp();
           T *o = static_cast<T *>(a.dw) + (long)vrow * a.dw_ld + col;
           const int rows = min(32, a.vocab - vrow), cols = min(width, a.dim - col);
+          if constexpr (sizeof(T) == 2) {
+            if (a.dw_vec == 2) {
+              if (2 * lane < cols) {
+#pragma unroll 8
+                for (int r = 0; r < rows; ++r)
+                  *reinterpret_cast<uint32_t *>(o + (long)r * a.dw_ld + 2 * lane) =
+                      *reinterpret_cast<const uint32_t *>(bx + r * 128 + ((4 * lane) ^ ((r & 7) * 16)));
+              }
+              __syncwarp();
+              return;
+            }
+          }
 #pragma unroll 4
           for (int r = 0; r < rows; ++r)
             for (int c = lane; c < cols; c += 32) {
@@ -782,14 +794,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               unsigned char *bx = box.take();
               box_put16<T>(bx, lane, 0, v[0]);
               box_put16<T>(bx, lane, 1, v[1]);
-              if (a.dw_tma) box.send(&maps.c2, bx, col, vrow, 0, false);
+              if (a.dw_vec == 8) box.send(&maps.c2, bx, col, vrow, 0, false);
               else write_rows(bx, col, 64);
             } else {
               for (int h = 0; h < 2; ++h) {
                 if (col + 32 * h >= a.dim) continue;
                 unsigned char *bx = box.take();
                 box_put32(bx, lane, h ? v[1] : v[0]);
-                if (a.dw_tma) box.send(&maps.c2, bx, col + 32 * h, vrow, 0, add);
+                if (a.dw_vec == 4) box.send(&maps.c2, bx, col + 32 * h, vrow, 0, add);
                 else write_rows(bx, col + 32 * h, 32);
               }
             }
@@ -832,8 +844,8 @@ __device__ __forceinline__ void put_pieces(uint16_t *dst, size_t plane, float v,
     reinterpret_cast<__half *>(dst)[plane] = __float2half_rn(v - __half2float(h));
   }
 }
-// One row of 16-bit operands from `src` (null: zeros), by one warp; VEC elements per
-// access where the addresses allow.
+// One row of 16-bit operands from `src` (null: zeros, one at a time), by one warp; VEC
+// elements per access where the addresses allow.
 template <typename T, int VEC>
 __device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *src, int dim, int lane, float scale) {
 #pragma unroll 4
@@ -841,12 +853,9 @@ __device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *sr
     if constexpr (VEC == 1) {
       put_pieces<T>(dst + c, plane, src ? op_load<T>(src[c]) : 0.f, scale);
     } else if constexpr (sizeof(T) == 2) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (src) v = *reinterpret_cast<const uint4 *>(src + c);
-      *reinterpret_cast<uint4 *>(dst + c) = v;
+      *reinterpret_cast<OpVec<T, VEC> *>(dst + c) = *reinterpret_cast<const OpVec<T, VEC> *>(src + c);
     } else {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (src) v = *reinterpret_cast<const float4 *>(src + c);
+      const float4 v = *reinterpret_cast<const float4 *>(src + c);
       const float x[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
       OpVec<__half, 4> h, l;
 #pragma unroll
@@ -860,9 +869,18 @@ __device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *sr
   }
 }
 template <typename T>
-__device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *src, int dim, int lane, float scale, bool vec) {
-  if (vec) put_row<T, 16 / sizeof(T)>(dst, plane, src, dim, lane, scale);
-  else put_row<T, 1>(dst, plane, src, dim, lane, scale);
+__device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *src, int dim, int lane, float scale, int vec) {
+  if (vec == 1) {
+    put_row<T, 1>(dst, plane, src, dim, lane, scale);
+    return;
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (vec == 2) {
+      put_row<T, 2>(dst, plane, src, dim, lane, scale);
+      return;
+    }
+  }
+  put_row<T, 16 / sizeof(T)>(dst, plane, src, dim, lane, scale);
 }
 
 struct StageArgs {
@@ -870,7 +888,7 @@ struct StageArgs {
   long x_ld, w_ld, rows;
   const int32_t *tg;
   int vocab, dim, pitch, per_cta, x_ctas;  // per_cta: rows per CTA, a multiple of 8
-  int x_vec, w_vec;                        // 16-byte rows
+  int x_vec, w_vec;                        // elements per access (see row_width)
   size_t xplane, wplane;
   uint16_t *xc, *wc;                       // wc null: W is read where it is
   const uint32_t *range;                   // float32: [range_ctas][2] largest magnitudes
@@ -909,8 +927,8 @@ __global__ void __launch_bounds__(256) ce_range_kernel(const StageArgs a, uint32
     }
   };
   for (long n = first; n < a.rows; n += step)
-    if (counted(a.tg[n], a.vocab)) row(static_cast<const float *>(a.x) + n * a.x_ld, a.x_vec, top[0]);
-  for (long v = first; v < a.vocab; v += step) row(static_cast<const float *>(a.w) + v * a.w_ld, a.w_vec, top[1]);
+    if (counted(a.tg[n], a.vocab)) row(static_cast<const float *>(a.x) + n * a.x_ld, a.x_vec == 4, top[0]);
+  for (long v = first; v < a.vocab; v += step) row(static_cast<const float *>(a.w) + v * a.w_ld, a.w_vec == 4, top[1]);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     top[i] = __reduce_max_sync(0xffffffffu, top[i]);
@@ -1300,8 +1318,12 @@ __global__ void __launch_bounds__(256) ce_dx_kernel(const float *slab, size_t sl
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = at >= 0 ? s[e] * c : 0.f;  // 0 whatever dloss is
     T *o = dx + n * dx_ld + i;
-    if (vec) {
+    if (vec == 4) {
       op_store_vec<T, 4>(o, s);
+    } else if (vec == 2) {
+      const float lo[2] = {s[0], s[1]}, hi[2] = {s[2], s[3]};
+      op_store_vec<T, 2>(o, lo);
+      if (i + 2 < a.dim) op_store_vec<T, 2>(o + 2, hi);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -1345,6 +1367,7 @@ struct Plan {
   uint16_t *G;
   int piece;           // columns of a piece, a multiple of 256
   int slabs, bn, tiles_d;
+  long cost;
   long dpitch;
   size_t loss_bytes, grad_bytes;
 };
@@ -1354,7 +1377,18 @@ struct Plan {
 // whole).  Among those sizes the one is taken whose launches cost least: the
 // busiest pair's slices, and about 16 slices' time for each launch.  About 40 sizes are
 // looked at, so that the search stays near 1 us of the caller's time.
-int piece_tiles(const aideen_linear_ce_args *a, const Plan &p) {
+// The products' tiles are bn columns wide: 256, or 128 where twice the tiles even out
+// the load by more than they cost (a slice of 128 columns takes 0.8 of the time of one
+// of 256, being nearer to what L2 can feed: 2048 x 50257 x 512 float32 1.07 ms at 256
+// and 1.34 ms at 128, but 1021 x 4999 x 250 float16 45 us and 39 us).
+void choose_piece(const aideen_linear_ce_args *a, Plan &p, int bn) {
+  p.bn = bn;
+  p.tiles_d = (int)((a->dim + bn - 1) / bn);
+  const int dx_tiles = p.tiles_m ? p.tiles_m * p.tiles_d : 1;
+  p.slabs = (p.pairs + dx_tiles - 1) / dx_tiles + 2;  // a run is about depth * dx_tiles / pairs long
+  p.piece = kTileN;
+  p.cost = 0;
+  if (!p.tiles_m) return;  // no rows
   const long bytes = p.mpad * kTileN * 2 * p.planes;
   const long half = (p.pairs / 2 + p.tiles_d - 1) / p.tiles_d;
   long most = (160L << 20) / bytes;
@@ -1364,7 +1398,7 @@ int piece_tiles(const aideen_linear_ce_args *a, const Plan &p) {
   const long k_rows = ((long)a->rows + kBlockK - 1) / kBlockK;
   auto cost = [&](long tiles) {
     const Deal d(tiles * p.tiles_d, k_rows, (long)p.tiles_m * p.tiles_d, (int)tiles * (kTileN / kBlockK), p.slabs, p.pairs);
-    return ((tiles * p.tiles_m + p.pairs - 1) / p.pairs * k_dim + d.load) * products + 32;
+    return (5 * ((tiles * p.tiles_m + p.pairs - 1) / p.pairs * k_dim) + (bn == 256 ? 5 : 4) * d.load) * products + 160;
   };
   long best = most, best_cost = -1;
   for (long tiles = most; tiles >= 1 && tiles * 3 >= most; tiles -= 1 + most / 64) {
@@ -1375,7 +1409,8 @@ int piece_tiles(const aideen_linear_ce_args *a, const Plan &p) {
       best_cost = c;
     }
   }
-  return (int)best;
+  p.piece = (int)best * kTileN;
+  p.cost = best_cost;
 }
 
 Plan make_plan(const aideen_linear_ce_args *a, void *ws, bool grad) {
@@ -1403,11 +1438,12 @@ Plan make_plan(const aideen_linear_ce_args *a, void *ws, bool grad) {
   p.row_loss = c.take<float>(a->rows);
   p.loss_bytes = c.used;
   if (!grad) return p;
-  p.bn = (a->dim + 127) / 128 % 2 ? 128 : 256;  // fewer padded columns
-  p.tiles_d = (int)((a->dim + p.bn - 1) / p.bn);
-  const int dx_tiles = p.tiles_m ? p.tiles_m * p.tiles_d : 1;
-  p.slabs = (p.pairs + dx_tiles - 1) / dx_tiles + 2;  // a run is about depth * dx_tiles / pairs long
-  p.piece = (p.tiles_m ? piece_tiles(a, p) : 1) * kTileN;
+  Plan q = p;
+  choose_piece(a, p, 256);
+  choose_piece(a, q, 128);
+  if (q.cost < p.cost) {
+    p.bn = q.bn; p.tiles_d = q.tiles_d; p.slabs = q.slabs; p.piece = q.piece;
+  }
   p.dpitch = (long)op_round(a->dim, 4);
   p.lse_c = g.take<float>(a->rows);
   p.tgt = g.take<int32_t>(a->rows);
@@ -1444,6 +1480,13 @@ bool map_w(CUtensorMap *m, const Plan &p, const aideen_linear_ce_args *g, const 
   return make_map(m, kU16, p.wc, g->dim, g->vocab, p.planes, (size_t)p.pitch * 2, p.wplane * 2, 64, rows);
 }
 
+// Elements that rows of this base and stride can be moved by: 16 bytes, a pair of 16-bit
+// elements, or one.
+int row_width(uint32_t dim, const void *p, int64_t ld, size_t el) {
+  if (dim % (16 / el) == 0 && op_vec16(p, ld, el)) return (int)(16 / el);
+  return el == 2 && dim % 2 == 0 && ld % 2 == 0 && op_aligned(p, 4) ? 2 : 1;
+}
+
 template <int MODE, typename T, bool HELD>
 cudaError_t launch_as(const Plan &p, const Maps &maps, MmaArgs a, cudaStream_t st) {
   const int held = HELD ? (a.dim + kBlockK - 1) / kBlockK : 0;
@@ -1468,14 +1511,13 @@ cudaError_t launch_mma(const Plan &p, const Maps &maps, const MmaArgs &a, cudaSt
 template <typename T>
 cudaError_t stage_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, const T *w, const int32_t *tg,
                       const float *lse, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
   StageArgs s{};
   s.x = x; s.w = w; s.x_ld = g->x_ld; s.w_ld = g->w_ld; s.rows = g->rows; s.tg = tg; s.vocab = (int)g->vocab;
   s.dim = (int)g->dim; s.pitch = p.pitch; s.xplane = p.xplane; s.wplane = p.wplane; s.xc = p.xc; s.wc = p.wc;
   s.slot = p.slot; s.count = p.count; s.ticket = p.ticket; s.lse = lse; s.lse_c = p.lse_c; s.tgt = p.tgt;
   s.range = p.range; s.range_ctas = p.range_ctas; s.unscale = p.unscale;
-  s.x_vec = g->dim % V == 0 && op_vec16(x, g->x_ld, sizeof(T));
-  s.w_vec = g->dim % V == 0 && op_vec16(w, g->w_ld, sizeof(T));
+  s.x_vec = row_width(g->dim, x, g->x_ld, sizeof(T));
+  s.w_vec = row_width(g->dim, w, g->w_ld, sizeof(T));
   const long most = 4L * 2 * p.pairs;  // CTAs
   s.per_cta = (int)(8 * ((g->rows + 8 * most - 1) / (8 * most)));
   s.x_ctas = (int)((g->rows + s.per_cta - 1) / s.per_cta);
@@ -1538,7 +1580,13 @@ cudaError_t loss_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
   r.x = x; r.w = w; r.bias = bias; r.x_ld = g->x_ld; r.w_ld = g->w_ld; r.rows = g->rows; r.tg = tg; r.slot = p.slot;
   r.count = p.count; r.dim = (int)g->dim; r.tiles_n = p.tiles_n; r.pairs = p.pairs; r.mean = a.mean; r.stats = p.stats;
   r.row_loss = row_loss ? row_loss : p.row_loss; r.lse = lse; r.loss = loss; r.ticket = p.ticket;
-  return op_launch(vec ? ce_rows_kernel<T, V> : ce_rows_kernel<T, 1>, (g->rows + 7) / 8, 256, 0, st, r);
+  const int wx = row_width(g->dim, x, g->x_ld, sizeof(T)), ww = row_width(g->dim, w, g->w_ld, sizeof(T));
+  const int width = wx < ww ? wx : ww;
+  auto rows = width == 1 ? ce_rows_kernel<T, 1> : ce_rows_kernel<T, V>;
+  if constexpr (sizeof(T) == 2) {
+    if (width == 2) rows = ce_rows_kernel<T, 2>;
+  }
+  return op_launch(rows, (g->rows + 7) / 8, 256, 0, st, r);
 }
 
 template <typename T>
@@ -1557,8 +1605,8 @@ cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
        map_x(&pm.b2, p, dim, 64) &&
        make_map(&pm.c, kF32, p.slab, dim, p.mpad, p.slabs, p.dpitch * 4, p.mpad * p.dpitch * 4, 32, 32);
   const size_t el = sizeof(T);
-  const bool dw_tma = dw && op_vec16(dw, g->dw_ld, el);
-  if (dw_tma)
+  const int dw_vec = !dw ? 1 : op_vec16(dw, g->dw_ld, el) ? (int)(16 / el) : row_width(g->dim, dw, g->dw_ld, el);
+  if (dw_vec > 2)
     ok = ok && make_map(&pm.c2, el == 4 ? kF32 : kU16, dw, dim, g->vocab, 1, g->dw_ld * el, g->dw_ld * el,
                         128 / el, 32);
   if (!ok) return cudaErrorInvalidValue;
@@ -1566,7 +1614,7 @@ cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
   a.lse = p.lse_c; a.tgt = p.tgt; a.db_part = db ? p.db_part : nullptr;
   a.bn = p.bn; a.tiles_d = p.tiles_d; a.slabs = dx ? p.slabs : 0; a.want_dw = dw != nullptr;
   a.full_k = p.piece / kBlockK;
-  a.dw = dw; a.db = db; a.dw_ld = g->dw_ld; a.dw_tma = dw_tma; a.dloss = dloss;
+  a.dw = dw; a.db = db; a.dw_ld = g->dw_ld; a.dw_vec = dw_vec; a.dloss = dloss;
   for (int v0 = 0; v0 < (int)g->vocab; v0 += p.piece) {
     const int left = (int)g->vocab - v0, cols = left < p.piece ? (left + kTileN - 1) / kTileN * kTileN : p.piece;
     a.v0 = v0;
@@ -1579,7 +1627,8 @@ cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
     if (e != cudaSuccess) return e;
   }
   if (!dx) return cudaSuccess;
-  const bool vec = dim % 4 == 0 && g->dx_ld % 4 == 0 && op_aligned(dx, 4 * el);
+  auto fits = [&](int n) { return dim % n == 0 && g->dx_ld % n == 0 && op_aligned(dx, n * el); };
+  const int vec = fits(4) ? 4 : fits(2) ? 2 : 1;
   const int per_cta = g->rows >= 4096 ? 8 : 2;  // with few rows there are many slabs: more warps on each
   return op_launch(ce_dx_kernel<T>, (g->rows + per_cta - 1) / per_cta, 256, 2 * p.tiles_d, st, p.slab,
                    (size_t)p.mpad * p.dpitch, p.dpitch, a, a.piece_k, p.pairs, p.slot, g->rows, per_cta, vec, dx,

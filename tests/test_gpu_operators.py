@@ -518,6 +518,15 @@ def test_linear_ce_at_odd_addresses(dtype):
         ce_check(bx[:, 1:64], bw[:, 1:64], bb[1:], tg, dloss=16.0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,pad_x,pad_w", [(250, 0, 0), (64, 2, 0), (64, 0, 2), (66, 1, 0), (66, 0, 2), (64, 4, 8)])
+def test_linear_ce_row_widths(dtype, dim, pad_x, pad_w):
+    """Rows that move by 16 bytes, by pairs of 16-bit elements or one by one, x and W
+    alike or not."""
+    x, w, b, tg = ce_inputs(15, 300, dim, 1030, dtype, True, 0.1)
+    ce_check(strided(x, pad_x), strided(w, pad_w), b, tg, dloss=16.0)
+
+
 def test_linear_ce_parts_alone():
     x, w, b, tg = ce_inputs(2, 70, 48, 333, BF16, True, 0.2)
     _, _, lse = K.linear_ce(x, w, tg, bias=b)
