@@ -88,6 +88,7 @@ struct MmaArgs {
   int full_k;         // and of the first piece (the last may be shorter)
   int want_dw;
   int slabs;          // slabs of dx (0: dx not wanted)
+  uint8_t *cover;     // [row tiles][tiles_d] slabs that hold something
   int first;          // first piece: dx slabs are written, not added to
   int dw_vec;         // dW: elements per access (see row_width); 16 bytes: stored by TMA
   void *dw, *db;
@@ -590,6 +591,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const float f_lo = fminf(fx, fw), f_hi = fmaxf(fx, fw);  // in this order z overflows only where it has to
     const Deal full_deal = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs,
                                    (int)(gridDim.x >> 1));
+    if (MODE == kProducts && a.slabs) {  // the last piece may be shorter than the others, and deal dx differently
+      const long tiles = (long)row_tiles(count) * a.tiles_d;
+      for (long t = (long)blockIdx.x * 32 * kEpiWarps + etid; t < tiles; t += (long)gridDim.x * 32 * kEpiWarps)
+        a.cover[t] = (uint8_t)max(full_deal.cover(t), units.deal.cover(t));
+    }
     if (MODE == kProducts && a.db_part) db_columns<T>(a, count, etid, sbias);
     auto flush = [&]() {
       if (last_m < 0) return;
@@ -1274,45 +1280,33 @@ __global__ void __launch_bounds__(32 * kFewRows) ce_few_join_kernel(const FewArg
 }
 
 // dx: the slabs added in order, scaled, back to the rows' places.  A CTA takes
-// `per_cta` rows, 8 / per_cta warps each.
-template <typename T>
+// `per_cta` rows, 8 / per_cta warps each; BATCH slabs are in flight at a time (behind the
+// last, the last again, not added).
+template <typename T, int BATCH>
 __global__ void __launch_bounds__(256) ce_dx_kernel(const float *slab, size_t slab_stride, int pitch, const MmaArgs a,
-                                                    int last_k, int pairs, const int32_t *slot, long rows, int per_cta,
-                                                    int vec, T *dx, long dx_ld) {
-  extern __shared__ uint8_t cover[];  // [2][tiles_d] slabs of the CTA's row tiles
+                                                    const int32_t *slot, long rows, int per_cta, int vec, T *dx,
+                                                    long dx_ld) {
   op_begin();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, count = *a.count;
-  const long r0 = (long)blockIdx.x * per_cta;
-  const int per_row = 8 / per_cta;
-  const long n = r0 + warp / per_row;
-  // consecutive rows have consecutive places: they lie in two row tiles at most
-  int first = 0x7fffffff;
-  for (int i = 0; i < per_cta; ++i)
-    if (r0 + i < rows && slot[r0 + i] >= 0) first = min(first, slot[r0 + i] / kTileM);
-  if (first < 0x7fffffff) {
-    const Deal full = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs, pairs);
-    const Deal last = deal_of(count, last_k * kBlockK / kTileM, a.tiles_d, last_k, a.want_dw, a.slabs, pairs);
-    for (int t = threadIdx.x; t < 2 * a.tiles_d; t += 256) {
-      const long tile = (long)first * a.tiles_d + t;
-      cover[t] = tile < (long)row_tiles(count) * a.tiles_d ? (uint8_t)max(full.cover(tile), last.cover(tile)) : 0;
-    }
-  }
-  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_row = 8 / per_cta;
+  const long n = (long)blockIdx.x * per_cta + warp / per_row;
   if (n >= rows) return;
   const int at = slot[n];
   const float c = grad_scale(a.dloss, a.count, a.mean) / a.g_scale * (sizeof(T) == 4 ? a.unscale[1] : 1.f);
-  const uint8_t *mine = cover + (at >= 0 && at / kTileM != first ? a.tiles_d : 0);
   for (int i = ((warp % per_row) * 32 + lane) * 4; i < a.dim; i += per_row * 128) {
     float s[4] = {};
     if (at >= 0) {
-      const int slabs = mine[i / a.bn];
+      const int slabs = a.cover[(size_t)(at / kTileM) * a.tiles_d + i / a.bn];
       const float *p = slab + (size_t)at * pitch + i;  // whole groups of 4: the pitch has room for them
-#pragma unroll 8
-      for (int k = 0; k < slabs; ++k) {
-        float v[4];
-        op_load_vec<float, 4>(p + k * slab_stride, v);
+      for (int k0 = 0; k0 < slabs; k0 += BATCH) {
+        float v[BATCH][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v[e];
+        for (int k = 0; k < BATCH; ++k) op_load_vec<float, 4>(p + min(k0 + k, slabs - 1) * slab_stride, v[k]);
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          if (k0 + k >= slabs) break;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[e] += v[k][e];
+        }
       }
     }
 #pragma unroll
@@ -1363,6 +1357,7 @@ struct Plan {
   float *row_loss;
   // gradient
   float *lse_c, *slab, *db_part;
+  uint8_t *cover;
   int32_t *tgt;
   uint16_t *G;
   int piece;           // columns of a piece, a multiple of 256
@@ -1450,6 +1445,7 @@ Plan make_plan(const aideen_linear_ce_args *a, void *ws, bool grad) {
   p.G = g.take<uint16_t>((size_t)p.mpad * p.piece * p.planes);
   p.slab = g.take<float>((size_t)p.slabs * p.mpad * p.dpitch);
   p.db_part = g.take<float>((size_t)p.tiles_m * 8 * p.piece);
+  p.cover = g.take<uint8_t>((size_t)(p.tiles_m ? p.tiles_m : 1) * p.tiles_d);
   p.grad_bytes = g.used;
   return p;
 }
@@ -1612,7 +1608,7 @@ cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
   if (!ok) return cudaErrorInvalidValue;
   MmaArgs a = mma_args<T>(g, p, bias);
   a.lse = p.lse_c; a.tgt = p.tgt; a.db_part = db ? p.db_part : nullptr;
-  a.bn = p.bn; a.tiles_d = p.tiles_d; a.slabs = dx ? p.slabs : 0; a.want_dw = dw != nullptr;
+  a.bn = p.bn; a.tiles_d = p.tiles_d; a.slabs = dx ? p.slabs : 0; a.cover = p.cover; a.want_dw = dw != nullptr;
   a.full_k = p.piece / kBlockK;
   a.dw = dw; a.db = db; a.dw_ld = g->dw_ld; a.dw_vec = dw_vec; a.dloss = dloss;
   for (int v0 = 0; v0 < (int)g->vocab; v0 += p.piece) {
@@ -1630,9 +1626,8 @@ cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
   auto fits = [&](int n) { return dim % n == 0 && g->dx_ld % n == 0 && op_aligned(dx, n * el); };
   const int vec = fits(4) ? 4 : fits(2) ? 2 : 1;
   const int per_cta = g->rows >= 4096 ? 8 : 2;  // with few rows there are many slabs: more warps on each
-  return op_launch(ce_dx_kernel<T>, (g->rows + per_cta - 1) / per_cta, 256, 2 * p.tiles_d, st, p.slab,
-                   (size_t)p.mpad * p.dpitch, p.dpitch, a, a.piece_k, p.pairs, p.slot, g->rows, per_cta, vec, dx,
-                   g->dx_ld);
+  return op_launch(p.slabs <= 4 ? ce_dx_kernel<T, 4> : ce_dx_kernel<T, 8>, (g->rows + per_cta - 1) / per_cta, 256, 0, st,
+                   p.slab, (size_t)p.mpad * p.dpitch, p.dpitch, a, p.slot, g->rows, per_cta, vec, dx, g->dx_ld);
 }
 
 template <typename T>
