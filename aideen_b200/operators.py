@@ -49,8 +49,11 @@ def _rows(t, what: str, name: str):
     if t.dim() < 1 or t.shape[-1] < 1:
         raise AideenError(f"{what}: {name} needs a last dimension of at least 1")
     dim = t.shape[-1]
-    if t.numel() // dim >= _COUNTS or dim >= _COUNTS:
+    n = t.numel() // dim
+    if n >= _COUNTS or dim >= _COUNTS:
         raise AideenError(f"{what}: {name} has more rows or columns than the library counts")
+    if t.is_contiguous():
+        return n, dim, dim
     if t.dim() == 1:
         t = t.unsqueeze(0)
     elif t.dim() > 2:
@@ -58,7 +61,6 @@ def _rows(t, what: str, name: str):
             t = t.view(-1, dim)
         except RuntimeError:
             raise AideenError(f"{what}: {name}'s leading dimensions have no common row stride") from None
-    n = t.shape[0]
     if dim > 1 and t.stride(1) != 1:
         raise AideenError(f"{what}: {name}'s last dimension is not contiguous")
     ld = t.stride(0) if n > 1 else dim
@@ -77,9 +79,7 @@ def _vector(t, what: str, name: str, n: int, like, dtype=None):
 
 
 def _out(t, what: str, name: str, shape, like):
-    """A given output, checked, or a new one."""
-    if t is None:
-        return like.new_empty(shape)
+    """A given output, checked."""
     _tensor(t, what, name, like, like.dtype)
     if tuple(t.shape) != tuple(shape):
         raise AideenError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
@@ -146,9 +146,13 @@ def embed(ids, table, scale: float = 1.0, out=None):
         raise AideenError(f"{what}: table must be [vocab, dim]")
     vocab, dim, ld = _rows(table, what, "table")
     ip = _ids(ids, what, table)
-    out = _out(out, what, "out", (*ids.shape, dim), table)
-    n = ids.numel()
-    old = _rows(out, what, "out")[2] if n else dim
+    n, old = ids.numel(), dim
+    if out is None:
+        out = table.new_empty((*ids.shape, dim))
+    else:
+        _out(out, what, "out", (*ids.shape, dim), table)
+        if n:
+            old = _rows(out, what, "out")[2]
     a = EmbedArgs(_DTYPES[table.dtype], n, dim, vocab, scale, 0, ld, old)
     with _on(table.device):
         rc = load_library().aideen_embed(C.byref(a), ip, table.data_ptr(), out.data_ptr(), _raw_stream(table.device.index))
@@ -167,8 +171,13 @@ def embed_grad(ids, dout, vocab: int, scale: float = 1.0, into=None):
         raise AideenError(f"{what}: dout must have ids' shape and one more dimension")
     dim, n = dout.shape[-1], ids.numel()
     rld = _rows(dout, what, "dout")[2] if n else dim
-    grad = _out(into, what, "into", (vocab, dim), dout)
-    gld = _rows(grad, what, "into")[2]
+    if not 0 < vocab < _COUNTS:
+        raise AideenError(f"{what}: vocab must be in [1, 2^31)")
+    if into is None:
+        grad, gld = dout.new_empty((vocab, dim)), dim
+    else:
+        grad = _out(into, what, "into", (vocab, dim), dout)
+        gld = _rows(grad, what, "into")[2]
     a = EmbedArgs(_DTYPES[dout.dtype], n, dim, vocab, scale, int(into is not None), gld, rld)
     lib, size, r = load_library(), C.c_size_t(), C.byref(a)
     _check(lib.aideen_embed_grad_workspace(r, C.byref(size)), what)

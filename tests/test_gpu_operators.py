@@ -658,6 +658,17 @@ def test_python_refusals():
             call()
 
 
+def test_python_refusals_of_strided_vectors_and_counts():
+    t = torch.zeros(4, 8, device="cuda")
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for call in (lambda: K.layer_norm(t[0, ::2]), lambda: K.linear_ce(t[0, ::2], t[:, :4], i[0]),
+                 lambda: K.embed_grad(i, t, -1), lambda: K.embed_grad(i, t, 1 << 32)):
+        with pytest.raises(AideenError):
+            call()
+    y, mean, rstd = K.layer_norm(t[0] + torch.arange(8, device="cuda"))
+    assert y.shape == (8,) and mean.shape == rstd.shape == () and float(mean) == 3.5
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_tensors_on_another_device_than_the_current_one():
     a = model_inputs(21, BF16)
