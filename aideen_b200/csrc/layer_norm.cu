@@ -66,22 +66,29 @@ __device__ __forceinline__ void row_sum(float (&v)[K], int wpr, int group, float
   }
 }
 
-// One access of a lane: VEC elements, worked on as pairs (two float32 lanes per
-// instruction; a scalar access is a pair whose second half is 0).
-template <typename T, int VEC>
+// One access of a lane: 16 bytes, worked on as pairs (two float32 lanes per instruction).
+template <typename T>
 struct LnAccess {
-  static constexpr int P = VEC == 1 ? 1 : VEC / 2;
-  OpVec<T, VEC> v;
-  __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const OpVec<T, VEC> *>(p); }
-  __device__ __forceinline__ void load_ahead(const T *p) { op_load_ahead<T, VEC>(p, v); }
+  static constexpr int V = 16 / sizeof(T), P = V / 2;
+  OpVec<T, V> v;
+  __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const OpVec<T, V> *>(p); }
+  __device__ __forceinline__ void load_ahead(const T *p) { op_load_ahead<T, V>(p, v); }
+  // From a vector of `dim` elements; ANY: wherever it starts, and 0 behind its end.
+  template <bool ANY>
+  __device__ __forceinline__ void load_of(const T *base, int c, int dim) {
+    if (!ANY || (c + V <= dim && (reinterpret_cast<uintptr_t>(base) & 15) == 0)) {
+      load(base + c);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v.v[i] = c + i < dim ? base[c + i] : op_store<T>(0.f);
+    }
+  }
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v.v[i] = op_store<T>(0.f);
+    for (int i = 0; i < V; ++i) v.v[i] = op_store<T>(0.f);
   }
   __device__ __forceinline__ float2 get(int i) const {
-    if constexpr (VEC == 1) {
-      return make_float2(op_load<T>(v.v[0]), 0.f);
-    } else if constexpr (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4) {
       return make_float2(v.v[2 * i], v.v[2 * i + 1]);
     } else {
       const uint32_t u = reinterpret_cast<const uint32_t *>(&v)[i];
@@ -90,9 +97,7 @@ struct LnAccess {
     }
   }
   __device__ __forceinline__ void set(int i, float2 f) {
-    if constexpr (VEC == 1) {
-      v.v[0] = op_store<T>(f.x);
-    } else if constexpr (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4) {
       v.v[2 * i] = f.x;
       v.v[2 * i + 1] = f.y;
     } else if constexpr (std::is_same<T, __half>::value) {
@@ -101,91 +106,132 @@ struct LnAccess {
       reinterpret_cast<__nv_bfloat162 *>(&v)[i] = __float22bfloat162_rn(f);
     }
   }
-  __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<OpVec<T, VEC> *>(p) = v; }
+  __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<OpVec<T, V> *>(p) = v; }
 };
 __device__ __forceinline__ float2 pair(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 
-// The part of a row that a lane holds: N accesses, `step` elements apart (zeros behind the row).
-template <typename T, int VEC, int N>
+// The part of a row that a lane holds: N accesses, `step` elements apart (zeros behind
+// the row).  ANY: rows that start anywhere.
+template <typename T, int N, bool ANY>
 struct LnRow {
-  LnAccess<T, VEC> v[N];
+  LnAccess<T> v[N];
   // No branches, or each load would wait for the one before: behind the row its start
   // is read, and cleared.
-  __device__ __forceinline__ void load(const T *row, int c0, int step, int dim, bool there = true) {
+  __device__ __forceinline__ void load(const T *row, int c0, int step, int dim, const OpExtent &e, bool there = true) {
+    if constexpr (ANY) {
+      OpAny<T> x[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j].load_ahead(row + (c0 + j * step < dim ? c0 + j * step : 0));
+      for (int j = 0; j < N; ++j) x[j].load(row + c0 + j * step, dim - (c0 + j * step), e);
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (c0 + j * step >= dim || !there) v[j].clear();
+      for (int j = 0; j < N; ++j) v[j].v = x[j].take(row + c0 + j * step, there ? dim - (c0 + j * step) : 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j].load_ahead(row + (c0 + j * step < dim ? c0 + j * step : 0));
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (c0 + j * step >= dim || !there) v[j].clear();
+    }
   }
 };
 
-// One row per group of wpr warps.
-template <typename T, int VEC, int NV, bool AFFINE>
-__global__ void __launch_bounds__(512, 2) layer_norm_kernel(const LnArgs a) {
-  constexpr int N = VEC == 1 ? 4 * NV : NV, P = LnAccess<T, VEC>::P;
-  __shared__ float red[2 * 16];
+// R rows per group of wpr warps: short rows come several at a time, so that a warp has
+// as many loads in flight as with a long one.
+template <typename T, int N, int R, bool AFFINE, bool ANY>
+__global__ void __launch_bounds__(512, ANY ? 1 : 2) layer_norm_kernel(const LnArgs a) {
+  constexpr int V = LnAccess<T>::V, P = LnAccess<T>::P;
+  __shared__ float red[2 * R * 16];
   op_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = warp / a.wpr, groups = (int)(blockDim.x >> 5) / a.wpr;
-  const int c0 = ((warp % a.wpr) * 32 + lane) * VEC, step = 32 * a.wpr * VEC;
-  const long row = (long)blockIdx.x * groups + group;
-  if (row >= a.rows) return;  // whole groups leave together
+  // rows that start anywhere: a warp's columns lie next to each other, for its stores
+  const int c0 = ((warp % a.wpr) * (ANY ? N : 1) * 32 + lane) * V, step = 32 * (ANY ? 1 : a.wpr) * V;
+  const long row0 = ((long)blockIdx.x * groups + group) * R;
+  if (row0 >= a.rows) return;  // whole groups leave together
   const float inv = 1.f / (float)a.dim;
-  float2 d[N][P], t = pair(0.f);
+  float2 d[R][N][P];
+  float s[R], m[R], r[R];
   {
-    LnRow<T, VEC, N> v;
-    v.load(static_cast<const T *>(a.x) + row * a.x_ld, c0, step, a.dim);
+    LnRow<T, N, ANY> v[R];
+    const OpExtent ex(a.x, a.rows, a.x_ld, a.dim, sizeof(T));
 #pragma unroll
-    for (int j = 0; j < N; ++j)
+    for (int q = 0; q < R; ++q)  // behind the last row, the last again, not stored
+      v[q].load(static_cast<const T *>(a.x) + min(row0 + q, a.rows - 1) * a.x_ld, c0, step, a.dim, ex);
 #pragma unroll
-      for (int i = 0; i < P; ++i) t = add2(t, d[j][i] = v.v[j].get(i));
+    for (int q = 0; q < R; ++q) {
+      float2 t = pair(0.f);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int i = 0; i < P; ++i) t = add2(t, d[q][j][i] = v[q].v[j].get(i));
+      s[q] = t.x + t.y;
+    }
   }
   int parity = 0;
-  float s[1] = {t.x + t.y};
-  row_sum<1>(s, a.wpr, group, red, parity);
-  const float m = s[0] * inv;
-  t = pair(0.f);
+  row_sum<R>(s, a.wpr, group, red, parity);
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    m[q] = s[q] * inv;
+    float2 t = pair(0.f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int valid = a.dim - (c0 + j * step);
+      if (valid > 0) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          d[q][j][i] = add2(d[q][j][i], pair(-m[q]));
+          if (ANY && valid < V) {  // behind the row
+            if (2 * i + 1 >= valid) d[q][j][i].y = 0.f;
+            if (2 * i >= valid) d[q][j][i].x = 0.f;
+          }
+          t = fma2(d[q][j][i], d[q][j][i], t);
+        }
+      }
+    }
+    s[q] = t.x + t.y;
+  }
+  row_sum<R>(s, a.wpr, group, red, parity);
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    r[q] = 1.f / sqrtf(s[q] * inv + a.eps);
+    if (c0 == 0 && row0 + q < a.rows) {
+      if (a.mean) a.mean[row0 + q] = m[q];
+      if (a.rstd) a.rstd[row0 + q] = r[q];
+    }
+  }
+  const T *w = static_cast<const T *>(a.w), *b = static_cast<const T *>(a.b);
+  T *y = static_cast<T *>(a.y) + row0 * a.y_ld;
+  OpVec<T, V> out[R][N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    if (c0 + j * step < a.dim) {
+    const int c = c0 + j * step;
+    if (c >= a.dim) continue;
+    LnAccess<T> k, z, o;
+    if (AFFINE || a.w) k.template load_of<ANY>(w, c, a.dim);
+    if (AFFINE || a.b) z.template load_of<ANY>(b, c, a.dim);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if (row0 + q >= a.rows) break;
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        d[j][i] = add2(d[j][i], pair(-m));
-        if (VEC == 1) d[j][i].y = 0.f;
-        t = fma2(d[j][i], d[j][i], t);
+        float2 f = mul2(d[q][j][i], pair(r[q]));
+        if constexpr (AFFINE) {
+          f = fma2(f, k.get(i), z.get(i));
+        } else {
+          if (a.w) f = mul2(f, k.get(i));
+          if (a.b) f = add2(f, z.get(i));
+        }
+        o.set(i, f);
       }
+      if constexpr (ANY) out[q][j] = o.v;
+      else o.store(y + q * a.y_ld + c);
     }
   }
-  s[0] = t.x + t.y;
-  row_sum<1>(s, a.wpr, group, red, parity);
-  const float r = 1.f / sqrtf(s[0] * inv + a.eps);
-  if (c0 == 0) {
-    if (a.mean) a.mean[row] = m;
-    if (a.rstd) a.rstd[row] = r;
-  }
-  const T *w = static_cast<const T *>(a.w) + c0, *b = static_cast<const T *>(a.b) + c0;
-  T *y = static_cast<T *>(a.y) + row * a.y_ld + c0;
+  if constexpr (ANY) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    if (c0 + j * step >= a.dim) continue;
-    LnAccess<T, VEC> k, q, o;
-    if (AFFINE || a.w) k.load(w + j * step);
-    if (AFFINE || a.b) q.load(b + j * step);
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      float2 f = mul2(d[j][i], pair(r));
-      if constexpr (AFFINE) {
-        f = fma2(f, k.get(i), q.get(i));
-      } else {
-        if (a.w) f = mul2(f, k.get(i));
-        if (a.b) f = add2(f, q.get(i));
-      }
-      o.set(i, f);
-    }
-    o.store(y + j * step);
+    for (int q = 0; q < R; ++q)
+      if (row0 + q < a.rows) op_store_any<T, N>(y + q * a.y_ld + c0, out[q], a.dim - c0);
   }
 }
 
@@ -225,17 +271,17 @@ __global__ void layer_norm_long_kernel(const LnArgs a) {
 // Gradient: each group of warps takes every so many rows and
 // keeps its columns' sums of dy xh and dy in registers; the CTA's groups are
 // added through shared memory in group order into one row of `part`.
-template <typename T, int VEC, int NV, bool WEIGHT>
-__global__ void __launch_bounds__(LnShape<NV>::threads, LnShape<NV>::per_sm) layer_norm_grad_kernel(const LnArgs a) {
-  constexpr int N = VEC == 1 ? 4 * NV : NV, P = LnAccess<T, VEC>::P, R = LnShape<NV>::rows;
-  extern __shared__ float sh[];  // [2][dim] when several groups share a CTA
+template <typename T, int N, bool WEIGHT, bool ANY>
+__global__ void __launch_bounds__(LnShape<N>::threads, LnShape<N>::per_sm) layer_norm_grad_kernel(const LnArgs a) {
+  constexpr int V = LnAccess<T>::V, P = LnAccess<T>::P, R = ANY ? 1 : LnShape<N>::rows;
+  extern __shared__ __align__(16) float sh[];  // [groups][2][dim] when several share a CTA: 32 KB at most
   __shared__ float red[2 * 2 * R * 16];
   op_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = warp / a.wpr, groups = (int)(blockDim.x >> 5) / a.wpr;
-  const int c0 = ((warp % a.wpr) * 32 + lane) * VEC, step = 32 * a.wpr * VEC;
-  const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy);
-  const T *w = static_cast<const T *>(a.w) + c0;
+  const int c0 = ((warp % a.wpr) * (ANY ? N : 1) * 32 + lane) * V, step = 32 * (ANY ? 1 : a.wpr) * V;
+  const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy), *w = static_cast<const T *>(a.w);
+  const OpExtent ex(x, a.rows, a.x_ld, a.dim, sizeof(T)), edy(dy, a.rows, a.y_ld, a.dim, sizeof(T));
   float2 aw[N][P], ab[N][P];
 #pragma unroll
   for (int j = 0; j < N; ++j)
@@ -245,26 +291,26 @@ __global__ void __launch_bounds__(LnShape<NV>::threads, LnShape<NV>::per_sm) lay
   const float inv = 1.f / (float)a.dim;
   // R rows at a time: their loads are in flight together and share one reduction
   for (long row0 = ((long)blockIdx.x * groups + group) * R; row0 < a.rows; row0 += (long)gridDim.x * groups * R) {
-    LnRow<T, VEC, N> xv[R], gv[R];
+    LnRow<T, N, ANY> xv[R], gv[R];
     float m[R], r[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       const bool there = row0 + q < a.rows;  // rows behind the last are zeros and add nothing
       const long row = there ? row0 + q : a.rows - 1;
-      xv[q].load(x + row * a.x_ld, c0, step, a.dim, there);
-      gv[q].load(dy + row * a.y_ld, c0, step, a.dim, there);
+      xv[q].load(x + row * a.x_ld, c0, step, a.dim, ex, there);
+      gv[q].load(dy + row * a.y_ld, c0, step, a.dim, edy, there);
       m[q] = a.mean[row];
       r[q] = a.rstd[row];
     }
-    // dy is 0 behind a row (and in a scalar access's second half), so nothing is added there
+    // dy is 0 behind a row, so nothing is added there
     float2 s0[R], s1[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) s0[q] = s1[q] = pair(0.f);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if (c0 + j * step >= a.dim) continue;
-      LnAccess<T, VEC> k;
-      if (WEIGHT) k.load(w + j * step);
+      LnAccess<T> k;
+      if (WEIGHT) k.template load_of<ANY>(w, c0 + j * step, a.dim);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         const float2 wk = WEIGHT ? k.get(i) : pair(1.f);
@@ -287,52 +333,58 @@ __global__ void __launch_bounds__(LnShape<NV>::threads, LnShape<NV>::per_sm) lay
       s[2 * q + 1] = s1[q].x + s1[q].y;
     }
     row_sum<2 * R>(s, a.wpr, group, red, parity);
+    OpVec<T, V> out[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      if (c0 + j * step >= a.dim) continue;
-      LnAccess<T, VEC> k;
-      if (WEIGHT) k.load(w + j * step);
+      const int c = c0 + j * step;
+      if (c >= a.dim) continue;
+      LnAccess<T> k;
+      if (WEIGHT) k.template load_of<ANY>(w, c, a.dim);
 #pragma unroll
       for (int q = 0; q < R; ++q) {
         if (row0 + q >= a.rows) break;
         const float2 c1 = pair(-s[2 * q] * inv), c2 = pair(-s[2 * q + 1] * inv);
-        LnAccess<T, VEC> o;
+        LnAccess<T> o;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           const float2 xh = mul2(add2(xv[q].v[j].get(i), pair(-m[q])), pair(r[q]));
           const float2 g = add2((WEIGHT ? mul2(gv[q].v[j].get(i), k.get(i)) : gv[q].v[j].get(i)), c1);
           o.set(i, mul2(fma2(xh, c2, g), pair(r[q])));
         }
-        o.store(static_cast<T *>(a.dx) + (row0 + q) * a.dx_ld + c0 + j * step);
+        if constexpr (ANY) out[j] = o.v;
+        else o.store(static_cast<T *>(a.dx) + (row0 + q) * a.dx_ld + c);
+      }
+    }
+    if constexpr (ANY) op_store_any<T, N>(static_cast<T *>(a.dx) + row0 * a.dx_ld + c0, out, a.dim - c0);
+  }
+  if (!a.part) return;
+  // every group's sums side by side in shared memory, then added in group order
+  float *out = a.part + (size_t)blockIdx.x * 2 * a.dim, *mine = groups > 1 ? sh + (size_t)group * 2 * a.dim : out;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = c0 + j * step;
+    if (c >= a.dim) continue;
+    if constexpr (ANY) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (c + i >= a.dim) break;
+        mine[c + i] = i & 1 ? aw[j][i / 2].y : aw[j][i / 2].x;
+        mine[a.dim + c + i] = i & 1 ? ab[j][i / 2].y : ab[j][i / 2].x;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < P; i += 2) {
+        *reinterpret_cast<float4 *>(mine + c + 2 * i) = make_float4(aw[j][i].x, aw[j][i].y, aw[j][i + 1].x, aw[j][i + 1].y);
+        *reinterpret_cast<float4 *>(mine + a.dim + c + 2 * i) = make_float4(ab[j][i].x, ab[j][i].y, ab[j][i + 1].x, ab[j][i + 1].y);
       }
     }
   }
-  if (!a.part) return;
-  float *out = a.part + (size_t)blockIdx.x * 2 * a.dim;
-  for (int k = 0; k < groups; ++k) {
-    if (group == k) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int c = c0 + j * step;
-        if (c >= a.dim) continue;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          float pw = i & 1 ? aw[j][i / 2].y : aw[j][i / 2].x, pb = i & 1 ? ab[j][i / 2].y : ab[j][i / 2].x;
-          if (k > 0) {
-            pw += sh[c + i];
-            pb += sh[a.dim + c + i];
-          }
-          if (k + 1 < groups) {
-            sh[c + i] = pw;
-            sh[a.dim + c + i] = pb;
-          } else {
-            out[c + i] = pw;
-            out[a.dim + c + i] = pb;
-          }
-        }
-      }
-    }
-    if (k + 1 < groups) __syncthreads();
+  if (groups == 1) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * a.dim; c += blockDim.x) {
+    float t = sh[c];
+    for (int k = 1; k < groups; ++k) t += sh[(size_t)k * 2 * a.dim + c];
+    out[c] = t;
   }
 }
 
@@ -400,16 +452,22 @@ __global__ void __launch_bounds__(1024) layer_norm_finish_kernel(const float *pa
 }
 
 // How a row is spread.  Forward: as few accesses per lane (1, 2 or 4) as hold it in one
-// warp, then as many warps as it takes.  Gradient: up to 2 warps before a lane takes
-// more, so that the column sums leave room for many rows in flight.
+// warp, then as many warps as it takes (a barrier costs more than it gives: 32768 x 1024
+// bf16 26 us with one warp, 38 us with two).  Gradient: up to 2 warps before a lane takes
+// two, 8 before it takes four, so that the column sums leave room for many rows in
+// flight (16384 x 1024 f32 41 us with two accesses and four warps, 53 us the other way).
 struct Spread {
   int nv, wpr, threads, groups, per_sm, rows;
 };
-Spread spread(int dim, int elem, bool vec, bool grad) {
+Spread spread(int dim, int elem, bool grad) {
   Spread s{};
-  const int one = vec ? 16 / elem : 4;  // elements of a lane's nv = 1
+  const int one = 16 / elem;  // elements of an access
   s.nv = 1;
-  while (s.nv < 4 && 32 * (grad ? 2 : 1) * one * s.nv < dim) s.nv *= 2;
+  if (grad) {
+    if (32 * 2 * one < dim) s.nv = 32 * 2 * one * kLnMaxGradWarps < dim ? 4 : 2;
+  } else {
+    while (s.nv < 4 && 32 * one * s.nv < dim) s.nv *= 2;
+  }
   s.wpr = 1;
   while (32 * one * s.nv * s.wpr < dim) s.wpr *= 2;
   s.threads = grad && s.nv == 1 ? LnShape<1>::threads : 256;
@@ -428,26 +486,37 @@ int grad_ctas(const aideen_layer_norm_args *a, const Spread &s) {
   return (int)(need < most ? need : most);
 }
 
-template <typename T, int VEC, int NV>
+template <typename T, int N, bool ANY>
 cudaError_t forward_run(const LnArgs &a, const Spread &s, cudaStream_t st) {
-  return op_launch(a.w && a.b ? layer_norm_kernel<T, VEC, NV, true> : layer_norm_kernel<T, VEC, NV, false>,
-                   (unsigned)((a.rows + s.groups - 1) / s.groups), s.threads, 0, st, a);
+  auto run = [&](auto one, auto affine, int rows) {
+    const long per = (long)s.groups * rows;
+    return op_launch(a.w && a.b ? affine : one, (unsigned)((a.rows + per - 1) / per), s.threads, 0, st, a);
+  };
+  // several rows per warp once that leaves every SM some warps of them
+  constexpr int R = 4 / N;
+  if (R > 1 && s.wpr == 1 && a.rows >= (long)op_sm_count() * 16 * R)
+    return run(layer_norm_kernel<T, N, R, false, ANY>, layer_norm_kernel<T, N, R, true, ANY>, R);
+  return run(layer_norm_kernel<T, N, 1, false, ANY>, layer_norm_kernel<T, N, 1, true, ANY>, 1);
 }
-
-template <typename T, int VEC, int NV>
-cudaError_t grad_run(const LnArgs &a, const Spread &s, int ctas, cudaStream_t st) {
-  const size_t smem = s.groups > 1 && a.part ? (size_t)2 * a.dim * sizeof(float) : 0;
-  return op_launch(a.w ? layer_norm_grad_kernel<T, VEC, NV, true> : layer_norm_grad_kernel<T, VEC, NV, false>, ctas, s.threads, smem, st, a);
+template <typename T, bool ANY>
+cudaError_t forward_any(const LnArgs &a, const Spread &s, cudaStream_t st) {
+  return s.nv == 1 ? forward_run<T, 1, ANY>(a, s, st) : s.nv == 2 ? forward_run<T, 2, ANY>(a, s, st) : forward_run<T, 4, ANY>(a, s, st);
 }
-
 template <typename T>
 cudaError_t forward_typed(const LnArgs &a, const Spread &s, bool vec, cudaStream_t st) {
   if (s.wpr > kLnMaxWarps) return op_launch(layer_norm_long_kernel<T>, (unsigned)a.rows, 1024, 0, st, a);
-  constexpr int V = 16 / sizeof(T);
-  if (vec) return s.nv == 1 ? forward_run<T, V, 1>(a, s, st) : s.nv == 2 ? forward_run<T, V, 2>(a, s, st) : forward_run<T, V, 4>(a, s, st);
-  return s.nv == 1 ? forward_run<T, 1, 1>(a, s, st) : s.nv == 2 ? forward_run<T, 1, 2>(a, s, st) : forward_run<T, 1, 4>(a, s, st);
+  return vec ? forward_any<T, false>(a, s, st) : forward_any<T, true>(a, s, st);
 }
 
+template <typename T, int N, bool ANY>
+cudaError_t grad_run(const LnArgs &a, const Spread &s, int ctas, cudaStream_t st) {
+  const size_t smem = s.groups > 1 && a.part ? (size_t)s.groups * 2 * a.dim * sizeof(float) : 0;
+  return op_launch(a.w ? layer_norm_grad_kernel<T, N, true, ANY> : layer_norm_grad_kernel<T, N, false, ANY>, ctas, s.threads, smem, st, a);
+}
+template <typename T, bool ANY>
+cudaError_t grad_any(const LnArgs &a, const Spread &s, int ctas, cudaStream_t st) {
+  return s.nv == 1 ? grad_run<T, 1, ANY>(a, s, ctas, st) : s.nv == 2 ? grad_run<T, 2, ANY>(a, s, ctas, st) : grad_run<T, 4, ANY>(a, s, ctas, st);
+}
 template <typename T>
 cudaError_t grad_typed(const LnArgs &a, const Spread &s, bool vec, int ctas, T *dw, T *db, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
@@ -456,11 +525,7 @@ cudaError_t grad_typed(const LnArgs &a, const Spread &s, bool vec, int ctas, T *
     if (e == cudaSuccess && a.part)
       e = op_launch(layer_norm_columns_kernel<T>, dim3((a.dim + 255) / 256, ctas), 256, 0, st, a);
   } else {
-    constexpr int V = 16 / sizeof(T);
-    if (vec)
-      e = s.nv == 1 ? grad_run<T, V, 1>(a, s, ctas, st) : s.nv == 2 ? grad_run<T, V, 2>(a, s, ctas, st) : grad_run<T, V, 4>(a, s, ctas, st);
-    else
-      e = s.nv == 1 ? grad_run<T, 1, 1>(a, s, ctas, st) : s.nv == 2 ? grad_run<T, 1, 2>(a, s, ctas, st) : grad_run<T, 1, 4>(a, s, ctas, st);
+    e = vec ? grad_any<T, false>(a, s, ctas, st) : grad_any<T, true>(a, s, ctas, st);
   }
   if (e != cudaSuccess || !a.part) return e;
   return op_launch(layer_norm_finish_kernel<T>, dim3((a.dim + 31) / 32, 2), 1024, 0, st, a.part, ctas, a.dim, dw, db);
@@ -497,7 +562,7 @@ extern "C" int aideen_layer_norm(const aideen_layer_norm_args *args, const void 
   a.x_ld = args->x_ld; a.y_ld = args->y_ld;
   const bool vec = ((size_t)a.dim * el) % 16 == 0 && op_vec16(x, a.x_ld, el) && op_vec16(y, a.y_ld, el) &&
                    op_aligned(weight, 16) && op_aligned(bias, 16);
-  const Spread s = spread(a.dim, (int)el, vec, false);
+  const Spread s = spread(a.dim, (int)el, false);
   a.wpr = s.wpr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (args->dtype == AIDEEN_F32) return op_cuda(forward_typed<float>(a, s, vec, st));
@@ -509,10 +574,8 @@ extern "C" int aideen_layer_norm_grad_workspace(const aideen_layer_norm_args *ar
   const int rc = check_args(args);
   if (rc != AIDEEN_OK) return rc;
   OP_CHECK(bytes, "layer_norm: null bytes");
-  // either way the rows may be read, whatever the addresses
-  const int el = (int)op_elem(args->dtype);
-  const int c0 = grad_ctas(args, spread((int)args->dim, el, false, true)), c1 = grad_ctas(args, spread((int)args->dim, el, true, true));
-  *bytes = op_round((size_t)(c0 > c1 ? c0 : c1) * 2 * args->dim * sizeof(float), 256);
+  const Spread s = spread((int)args->dim, (int)op_elem(args->dtype), true);
+  *bytes = op_round((size_t)grad_ctas(args, s) * 2 * args->dim * sizeof(float), 256);
   return AIDEEN_OK;
 }
 
@@ -548,7 +611,7 @@ extern "C" int aideen_layer_norm_grad(const aideen_layer_norm_args *args, const 
   a.x_ld = args->x_ld; a.y_ld = args->y_ld; a.dx_ld = args->dx_ld;
   const bool vec = ((size_t)a.dim * el) % 16 == 0 && op_vec16(x, a.x_ld, el) && op_vec16(dy, a.y_ld, el) &&
                    (!dx || op_vec16(dx, a.dx_ld, el)) && op_aligned(weight, 16);
-  const Spread s = spread(a.dim, (int)el, vec, true);
+  const Spread s = spread(a.dim, (int)el, true);
   a.wpr = s.wpr;
   const int ctas = grad_ctas(args, s);
   if (args->dtype == AIDEEN_F32)

@@ -144,6 +144,100 @@ __device__ __forceinline__ void op_load_ahead(const T *p, OpVec<T, VEC> &out) {
   }
 }
 
+// ---- rows that do not start on 16 bytes ------------------------------------------
+// Such a row is still moved 16 bytes at a time: lane by lane the same columns as in an
+// aligned row, each lane's 16 bytes cut out of the two aligned blocks that they lie in.
+
+// Bytes [shift, shift + 16) of the 32 in a, b; shift is even and below 16.
+__device__ __forceinline__ uint4 op_cut(const uint4 &a, const uint4 &b, uint32_t shift) {
+  uint32_t w0 = a.x, w1 = a.y, w2 = a.z, w3 = a.w, w4 = b.x, w5 = b.y;
+  if (shift & 8) {
+    w0 = a.z; w1 = a.w; w2 = b.x; w3 = b.y; w4 = b.z; w5 = b.w;
+  }
+  if (shift & 4) {
+    w0 = w1; w1 = w2; w2 = w3; w3 = w4; w4 = w5;
+  }
+  const uint32_t bits = (shift & 3) * 8;
+  return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                    __funnelshift_r(w3, w4, bits));
+}
+// Where a tensor lies: blocks that reach out of it are not read whole.
+struct OpExtent {
+  const unsigned char *lo, *hi;
+  __device__ __forceinline__ OpExtent(const void *p, long rows, long ld, long dim, int elem)
+      : lo(static_cast<const unsigned char *>(p)), hi(lo + ((rows - 1) * ld + dim) * elem) {}
+};
+// 16 bytes from p on in two steps, so that the loads of several can be in flight
+// together; elements from `valid` on become 0 (the tensor has them only below that).
+template <typename T>
+struct OpAny {
+  static constexpr int V = 16 / sizeof(T);
+  uint4 a, b;
+  __device__ __forceinline__ void load(const T *p, int valid, const OpExtent &e) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), blk = at & ~(uintptr_t)15;
+    const uint32_t shift = (uint32_t)(at & 15);
+    a = b = make_uint4(0, 0, 0, 0);
+    if (blk >= reinterpret_cast<uintptr_t>(e.lo) && blk + (shift ? 32 : 16) <= reinterpret_cast<uintptr_t>(e.hi)) {
+      asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w) : "l"(blk) : "memory");
+      if (shift)
+        asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(blk + 16) : "memory");
+    } else {  // at the tensor's ends: one by one, put where take() finds them
+      OpVec<T, V> one[2] = {};
+      const int first = (int)(shift / sizeof(T));
+#pragma unroll
+      for (int i = 0; i < 2 * V; ++i)
+        if (i >= first && i - first < valid && i - first < V) one[i / V].v[i % V] = p[i - first];
+      a = reinterpret_cast<const uint4 &>(one[0]);
+      b = reinterpret_cast<const uint4 &>(one[1]);
+    }
+  }
+  __device__ __forceinline__ OpVec<T, V> take(const T *p, int valid) const {
+    const uint4 w = op_cut(a, b, (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15));
+    OpVec<T, V> v = reinterpret_cast<const OpVec<T, V> &>(w);
+    if (valid < V) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i >= valid) v.v[i] = op_store<T>(0.f);
+    }
+    return v;
+  }
+};
+// Stores N accesses of a warp that lie next to each other: p is the place of the lane's
+// first column, lane 0 of access j follows lane 31 of access j - 1, and the first
+// `valid` elements from p on belong to the row.  A lane stores the aligned block that its
+// first element lies in, with the last elements of the one before; where a neighbour
+// is missing (the warp's ends, the row's end), one by one.  All lanes call it.
+template <typename T, int N>
+__device__ __forceinline__ void op_store_any(T *p, const OpVec<T, 16 / sizeof(T)> (&v)[N], int valid) {
+  constexpr int V = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31;
+  const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15);
+  const int head = V - (int)(shift / sizeof(T));  // elements in the first block
+  uint4 last = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int j = 0; j < N; ++j, p += 32 * V, valid -= 32 * V) {
+    const uint4 w = reinterpret_cast<const uint4 &>(v[j]);
+    const uint4 give = lane == 31 ? last : w;
+    const int from = (lane + 31) & 31;
+    const uint4 before = make_uint4(__shfl_sync(0xffffffffu, give.x, from), __shfl_sync(0xffffffffu, give.y, from),
+                                    __shfl_sync(0xffffffffu, give.z, from), __shfl_sync(0xffffffffu, give.w, from));
+    last = w;
+    const bool whole = valid >= head && (lane > 0 || j > 0 || shift == 0);
+    const bool next = valid - V >= head && (lane < 31 || j + 1 < N);
+    if (whole) *reinterpret_cast<uint4 *>(reinterpret_cast<uintptr_t>(p) - shift) = shift ? op_cut(before, w, 16 - shift) : w;
+    if (!whole && valid > 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < min(valid, head)) p[i] = v[j].v[i];
+    }
+    if (!next && valid > head) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i >= head && i < valid) p[i] = v[j].v[i];
+    }
+  }
+}
+
 // Whether rows of this base and stride can be moved 16 bytes at a time.
 inline bool op_vec16(const void *p, int64_t ld, size_t elem) {
   return op_aligned(p, 16) && ((size_t)ld * elem) % 16 == 0;
