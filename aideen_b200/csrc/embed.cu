@@ -74,7 +74,7 @@ struct SortArgs {
   // table gradient to clear, or null: rows of row_bytes at a stride of ld_bytes
   unsigned char *clear;
   size_t row_bytes, ld_bytes;
-  int clear16;  // rows can be cleared 16 bytes at a time
+  int flat, clear16;  // contiguous rows from 16 bytes on; rows can be cleared 16 bytes at a time
 };
 
 // Keys are the ids, every id outside [0, vocab) as vocab (sorted last).
@@ -87,11 +87,12 @@ __device__ __forceinline__ uint32_t sort_key(int32_t id, uint32_t vocab) {
 __device__ __forceinline__ void clear_rows(const SortArgs &s, uint32_t *zeros, size_t cta, size_t ctas) {
   constexpr size_t kBlock = sizeof(uint32_t) * kSortWarps * kDigits;  // 32 KB
   const size_t t = cta * kSortThreads + threadIdx.x, step = ctas * kSortThreads;
-  if (s.clear16 && s.row_bytes == s.ld_bytes) {
+  if (s.flat) {
     for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) zeros[i] = 0;
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
-    const size_t total = s.row_bytes * s.vocab;
+    const size_t all = s.row_bytes * s.vocab, total = all & ~(size_t)15;
+    if (cta == 0 && threadIdx.x < (all - total) / 2) reinterpret_cast<uint16_t *>(s.clear + total)[threadIdx.x] = 0;
     if (threadIdx.x == 0) {
       for (size_t at = cta * kBlock; at < total; at += ctas * kBlock) {
         const uint32_t n = (uint32_t)(total - at < kBlock ? total - at : kBlock);
@@ -530,7 +531,8 @@ extern "C" int aideen_embed_grad(const aideen_embed_args *args, const int32_t *i
   if (!args->accumulate) {
     s.clear = static_cast<unsigned char *>(table_grad);
     s.row_bytes = args->dim * el; s.ld_bytes = (size_t)args->table_ld * el;
-    s.clear16 = s.row_bytes % 16 == 0 && op_vec16(table_grad, args->table_ld, el);
+    s.flat = s.row_bytes == s.ld_bytes && op_aligned(table_grad, 16);
+    s.clear16 = s.flat || (s.row_bytes % 16 == 0 && op_vec16(table_grad, args->table_ld, el));
     // several CTAs per SM, so that uneven placement of the clusters evens out
     const size_t ctas = (s.row_bytes / (s.clear16 ? 16 : 2) * s.vocab + kSortThreads - 1) / kSortThreads;
     const size_t most = op_round(4 * (size_t)op_sm_count(), s.ctas), want = op_round(ctas, s.ctas);
