@@ -9,9 +9,14 @@
 // lane at most, so it is read once: the variance is the mean of the squared
 // differences from the finished mean, not E[x^2] - m^2.  A row takes 1 to 16 warps (8 in the
 // gradient, whose column sums need the registers); longer ones are walked in memory.
-// 32768 x 1024 bf16 forward: 27 us, 5.0 TB/s (a device copy of the same bytes: 24 us).
-// 32749 x 1000 f16 gradient with dw and db: 51 us, 3.9 TB/s (a copy: 69 us).  2048 x 512
-// f32 gradient: 6.8 us.
+// 32768 x 1024 bf16 forward: 26 us, 5.1 TB/s (a device copy of the same bytes: 22-24 us).
+// 32749 x 1000 f16 gradient with dw and db: 48 us, 4.1 TB/s, where an elementwise sum of
+// the same bytes takes 30 us: the 20 operations per element and the row's reduction
+// stand between the loads, and the column sums take the registers that more rows in
+// flight would need (one row at a time with three CTAs per SM: 55 us).  2048 x 512 f32
+// gradient: 7 us.
+// Rows that do not start on 16 bytes cost 1.5 to 2.2 times as much (32768 x 1001 bf16:
+// 58 us and 104 us; element by element 78 and 190).
 #include <type_traits>
 
 #include "common.cuh"
@@ -348,7 +353,7 @@ __global__ void __launch_bounds__(LnShape<N>::threads, LnShape<N>::per_sm) layer
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           const float2 xh = mul2(add2(xv[q].v[j].get(i), pair(-m[q])), pair(r[q]));
-          const float2 g = add2((WEIGHT ? mul2(gv[q].v[j].get(i), k.get(i)) : gv[q].v[j].get(i)), c1);
+          const float2 g = WEIGHT ? fma2(gv[q].v[j].get(i), k.get(i), c1) : add2(gv[q].v[j].get(i), c1);
           o.set(i, mul2(fma2(xh, c2, g), pair(r[q])));
         }
         if constexpr (ANY) out[j] = o.v;
