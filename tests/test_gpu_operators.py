@@ -276,6 +276,41 @@ def test_layer_norm_grad(dtype, rows, dim, pad, affine):
     assert only[0] is None and only[1] is None and torch.equal(only[2], db)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,pad", [(37, 9, 0), (37, 121, 0), (2400, 121, 0), (37, 257, 3), (37, 777, 0), (37, 1001, 1),
+                                           (600, 513, 0), (9, 2047, 0), (5, 5003, 0), (1, 3, 0), (2, 1, 0)])
+def test_layer_norm_rows_at_any_address(dtype, rows, dim, pad):
+    """Rows that start between 16-byte boundaries: the same bits wherever they start, and
+    nothing outside them is written."""
+    g = gen(rows * dim)
+    v = 128 // torch.finfo(dtype).bits
+    x, dy = rand(g, rows, dim, dtype=dtype, std=1.7), rand(g, rows, dim, dtype=dtype)
+    w, b = rand(g, dim, dtype=dtype), rand(g, dim, dtype=dtype)
+    ld = dim + pad
+
+    def place(t, offset):
+        big = torch.full((rows * ld + 2 * v,), 7.0, dtype=dtype, device="cuda")
+        view = big[offset:offset + rows * ld].view(rows, ld)[:, :dim]
+        if t is not None:
+            view.copy_(t)
+        return big, view
+
+    first = None
+    for offset in range(1, v):
+        xv, dv = place(x, offset)[1], place(dy, (offset * 3) % v)[1]
+        big, y = place(None, (offset * 5) % v)
+        wv = torch.cat([w[:1]] * (offset % 3) + [w])[offset % 3:]
+        _, mean, rstd = K.layer_norm(xv, wv, b, out=y)
+        got = (y.clone(), mean, rstd, *K.layer_norm_grad(dv, xv, wv, mean, rstd))
+        if first is None:
+            first = got
+        assert all(torch.equal(p, q) for p, q in zip(first, got))
+        y.fill_(7.0)
+        assert bool((big == 7.0).all())
+    test_layer_norm(dtype, rows, dim, pad, True)
+    test_layer_norm_grad(dtype, rows, dim, pad, True)
+
+
 # ---- cross entropy of a linear head -----------------------------------------
 def ce_reference(x, w, b, tg, reduction, dloss, dtype):
     """Results in float64 and their bounds."""
