@@ -673,6 +673,56 @@ def test_streams_and_captured_graphs():
         assert all(torch.equal(p, q) for p, q in zip(outs[k], want[k + 1]))
 
 
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: their last rows are what those rows alone give."""
+    n, dim, k = 2_150_000, 1001, 70
+    g = gen(31)
+    big = torch.zeros(n, dim, dtype=F16, device="cuda")
+    big[-k:] = rand(g, k, dim, dtype=F16)
+    last = big[-k:].clone()
+    ids = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    ids[-k:] = torch.randint(0, 5, (k,), generator=g, device="cuda", dtype=torch.int32)
+    assert torch.equal(K.embed(n - k + torch.arange(k, device="cuda", dtype=torch.int32), big, 2.0), last * 2)
+    out = K.embed(ids, last, 1.5)
+    assert torch.equal(out[-k:], K.embed(ids[-k:], last, 1.5)) and not bool(out[:-k:9999].any())
+    got = K.embed_grad(ids, big, 5)
+    for v in range(5):
+        terms = last[ids[-k:] == v].double()
+        e = (k + 2) * U32 * terms.abs().sum(0)
+        close(got[v], terms.sum(0), e + U[F16] * (terms.sum(0).abs() + e) + TINY[F16])
+    y, mean, rstd = K.layer_norm(big, out=out)
+    y1, mean1, rstd1 = K.layer_norm(last)
+    assert torch.equal(y[-k:], y1) and torch.equal(mean[-k:], mean1) and torch.equal(rstd[-k:], rstd1)
+    dx = K.layer_norm_grad(big, big, None, mean, rstd, want=("x",))[0]
+    assert torch.equal(dx[-k:], K.layer_norm_grad(last, last, None, mean1, rstd1, want=("x",))[0])
+
+
+def test_linear_ce_over_a_vocabulary_past_32_bits():
+    """All entries but the last 1000 masked: the statistics and gradients are theirs alone."""
+    vocab, dim, rows, k = (1 << 22) + 1000, 512, 130, 1000
+    g = gen(32)
+    x, w1 = rand(g, rows, dim, dtype=BF16), rand(g, k, dim, dtype=BF16, std=0.1)
+    w = torch.zeros(vocab, dim, dtype=BF16, device="cuda")
+    w[-k:] = w1
+    b = torch.full((vocab,), float("-inf"), dtype=BF16, device="cuda")
+    b[-k:] = rand(g, k, dtype=BF16)
+    tg1 = torch.randint(0, k, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    tg = tg1 + (vocab - k)
+    _, _, lse = K.linear_ce(x, w, tg, b)
+    _, _, lse1 = K.linear_ce(x, w1, tg1, b[-k:].clone())
+    # either is a sum of 1000 terms, whose exponents are off by a rounding each
+    close(lse, lse1.double(), 2 * (k + 64) * U32 * (1 + lse1.double().abs()))
+    dx, dw, db = K.linear_ce_grad(x, w, tg, lse1, b)
+    dx1, dw1, db1 = K.linear_ce_grad(x, w1, tg1, lse1, b[-k:].clone())
+    # the same lse, so the same softmax - onehot bit by bit; dx adds it up in other parts
+    assert torch.equal(dw[-k:], dw1) and torch.equal(db[-k:], db1)
+    assert not bool(dw[:-k].any()) and not bool(db[:-k].any())
+    p = torch.softmax(x.double() @ w1.double().T + b[-k:].double(), 1)
+    p[torch.arange(rows, device="cuda"), tg1.long()] -= 1
+    terms = (p.abs() / rows) @ w1.double().abs()
+    close(dx, dx1.double(), 2 * U[BF16] * dx1.double().abs() + 4 * (k + 64) * U32 * terms + 2 * TINY[BF16])
+
+
 def test_python_refusals():
     t = torch.zeros(4, 8, device="cuda")
     i = torch.zeros(4, dtype=torch.int32, device="cuda")
