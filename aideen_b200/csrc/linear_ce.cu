@@ -1499,7 +1499,9 @@ cudaError_t launch_as(const Plan &p, const Maps &maps, MmaArgs a, cudaStream_t s
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   const int smem = held * kHalfBytes + a.stages * stage + boxes + kSmemFixed;
   auto kernel = ce_mma_kernel<MODE, T, HELD>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // the attribute belongs to the kernel, not to the call: always the same value, or a call
+  // of another thread could lower it between here and the launch
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
   if (e != cudaSuccess) return e;
   return op_launch(kernel, 2 * p.pairs, kThreads, smem, st, maps, a);
 }
@@ -1551,7 +1553,7 @@ cudaError_t few_run(FewArgs a, size_t smem, int sms, cudaStream_t st) {
   auto kernel = R == 1 ? ce_few_kernel<T, VEC, 1> : R == 2 ? ce_few_kernel<T, VEC, 2> : R == 4 ? ce_few_kernel<T, VEC, 4> : ce_few_kernel<T, VEC, 8>;
   a.ctas = (R <= 2 ? 2 : 1) * sms;
   a.picked = reinterpret_cast<float *>(a.part + (size_t)a.ctas * R);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(smem * R));
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewSmem);  // as in launch_as
   if (e == cudaSuccess) e = op_launch(kernel, a.ctas, kFewThreads, smem * R, st, a);
   if (e == cudaSuccess) e = op_launch(ce_few_join_kernel, 1, 32 * kFewRows, 0, st, a, R);
   return e;

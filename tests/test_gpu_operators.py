@@ -6,6 +6,8 @@ operation counts: U32 = 2^-24 is half a step of float32, U[t] of the stored
 type, TINY[t] half of the smallest number it can hold, and a float32 sum of k
 terms is off by at most k U32 sum |terms| (2 k U32 where the tensor cores add,
 which may cut instead of round)."""
+import threading
+
 import pytest
 import torch
 
@@ -671,6 +673,40 @@ def test_streams_and_captured_graphs():
     K.check()
     for k in range(2):
         assert all(torch.equal(p, q) for p, q in zip(outs[k], want[k + 1]))
+
+
+def test_calls_of_several_host_threads():
+    """Threads that call at once, each on its own stream and at its own sizes (so with other
+    amounts of shared memory), get what they get alone."""
+    jobs = [ce_inputs(40 + i, rows, dim, 600, BF16, True) for i, (rows, dim) in
+            enumerate([(200, 64), (200, 512), (1, 512), (1, 2048), (7, 64), (8, 2048)])]
+
+    def work(x, w, b, tg):
+        loss, row_loss, lse = K.linear_ce(x, w, tg, bias=b)
+        return (loss, row_loss, lse) + K.linear_ce_grad(x, w, tg, lse, bias=b)
+    want = [work(*job) for job in jobs]
+    torch.cuda.synchronize()
+    start, wrong = threading.Barrier(len(jobs)), []
+
+    def caller(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait()
+            for _ in range(400):
+                try:
+                    got = work(*jobs[k])
+                except AideenError as e:
+                    wrong.append((k, str(e)))
+                    return
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(p, q) for p, q in zip(got, want[k])):
+                wrong.append((k, "other bits"))
+    threads = [threading.Thread(target=caller, args=(k,)) for k in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    K.check()
 
 
 def test_offsets_past_32_bits():
