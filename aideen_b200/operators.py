@@ -251,6 +251,8 @@ def _ce_args(what, x, weight, targets, bias, reduction):
     _tensor(weight, what, "weight", x, x.dtype)
     if reduction not in _REDUCTIONS:
         raise AideenError(f"{what}: reduction must be 'mean' or 'sum'")
+    if x.dim() < 1:
+        raise AideenError(f"{what}: x needs a last dimension of at least 1")
     if weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
         raise AideenError(f"{what}: weight must be [vocab, {x.shape[-1]}]")
     tp = _ids(targets, what, x, "targets")

@@ -790,6 +790,13 @@ def test_python_refusals_of_strided_vectors_and_counts():
     assert y.shape == (8,) and mean.shape == rstd.shape == () and float(mean) == 3.5
 
 
+def test_linear_ce_refuses_a_number_for_x():
+    x, w, i = torch.tensor(1.0, device="cuda"), torch.zeros(4, 1, device="cuda"), torch.tensor(0, device="cuda").int()
+    for call in (lambda: K.linear_ce(x, w, i), lambda: K.linear_ce_grad(x, w, i, x)):
+        with pytest.raises(AideenError, match="dimension"):
+            call()
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_tensors_on_another_device_than_the_current_one():
     a = model_inputs(21, BF16)
