@@ -86,6 +86,18 @@ def _out(t, what: str, name: str, shape, like):
     return t
 
 
+_GRADS = ("x", "weight", "bias")
+
+
+def _wanted(want, what: str):
+    """The names of gradients to form, checked (one name may come alone)."""
+    want = (want,) if isinstance(want, str) else tuple(want)
+    for name in want:
+        if name not in _GRADS:
+            raise AideenError(f"{what}: want names 'x', 'weight' and 'bias', not {name!r}")
+    return want
+
+
 def _like(t, dtype=None):
     """A new contiguous tensor of t's shape (the cheapest way to allocate one)."""
     return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
@@ -218,6 +230,7 @@ def layer_norm_grad(dy, x, weight, mean, rstd, want=("x", "weight", "bias")):
     """(dx, dweight, dbias) from the forward's x, mean and rstd; weight may be
     None (1).  `want` names the gradients to form; the others are None."""
     what = "layer_norm_grad"
+    want = _wanted(want, what)
     _tensor(x, what, "x")
     _tensor(dy, what, "dy", x, x.dtype)
     if dy.shape != x.shape:
@@ -296,6 +309,7 @@ def linear_ce_grad(x, weight, targets, lse, bias=None, dloss=None, reduction: st
     `want` names the gradients to form; the others, and dbias without a bias,
     are None."""
     what = "linear_ce_grad"
+    want = _wanted(want, what)
     a, weight, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)
     lp = _vector(lse, what, "lse", a.rows, x, torch.float32)
     gp = _vector(dloss, what, "dloss", 1, x, torch.float32)

@@ -157,3 +157,14 @@ def test_rows_of_a_matrix():
 def test_host_tensors_are_refused(call):
     with pytest.raises(AideenError, match="CUDA tensor"):
         call(torch.zeros(4, 8), torch.zeros(4, dtype=torch.int32))
+
+
+def test_wanted_gradients_are_named_rightly():
+    t, i = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int32)
+    for bad in (("weigth",), ("x", "w"), "dx", ["weight", None]):
+        with pytest.raises(AideenError, match="want"):
+            operators.layer_norm_grad(t, t, None, t, t, want=bad)
+        with pytest.raises(AideenError, match="want"):
+            operators.linear_ce_grad(t, t, i, t, want=bad)
+    assert tuple(operators._wanted("weight", "f")) == ("weight",)
+    assert tuple(operators._wanted(["bias", "x"], "f")) == ("bias", "x")
