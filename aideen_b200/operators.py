@@ -86,6 +86,28 @@ def _out(t, what: str, name: str, shape, like):
     return t
 
 
+def _apart(what: str, name: str, out, **inputs):
+    """Refuses an output that shares bytes with an input.  Column blocks of one buffer
+    (rows of the same stride, side by side) share none."""
+    def place(t):
+        n, dim, ld = _rows(t, what, name) if t.dim() > 0 else (1, 1, 1)
+        el = t.element_size()
+        return t.data_ptr(), n, dim * el, ld * el
+    if out.numel() == 0:
+        return
+    p, n, width, ld = place(out)
+    for other, t in inputs.items():
+        if t is None or t.numel() == 0:
+            continue
+        q, m, w, step = place(t)
+        if p + (n - 1) * ld + width <= q or q + (m - 1) * step + w <= p:
+            continue
+        pitch = ld if n > 1 else step  # of whichever has several rows
+        if (n == 1 or m == 1 or ld == step) and (q - p) % pitch >= width and (q - p) % pitch + w <= pitch:
+            continue
+        raise AideenError(f"{what}: {name} overlaps {other}")
+
+
 _GRADS = ("x", "weight", "bias")
 
 
@@ -151,7 +173,7 @@ def _ids(ids, what: str, like, name: str = "ids"):
 
 def embed(ids, table, scale: float = 1.0, out=None):
     """`scale * table[ids]` (ids int32, any shape; table [vocab, dim]); an id
-    outside [0, vocab) gives a row of zeros."""
+    outside [0, vocab) gives a row of zeros.  `out` must not overlap the inputs."""
     what = "embed"
     _tensor(table, what, "table")
     if table.dim() != 2:
@@ -165,6 +187,7 @@ def embed(ids, table, scale: float = 1.0, out=None):
         _out(out, what, "out", (*ids.shape, dim), table)
         if n:
             old = _rows(out, what, "out")[2]
+            _apart(what, "out", out, table=table, ids=ids)
     a = EmbedArgs(_DTYPES[table.dtype], n, dim, vocab, scale, 0, ld, old)
     with _on(table.device):
         rc = load_library().aideen_embed(C.byref(a), ip, table.data_ptr(), out.data_ptr(), _raw_stream(table.device.index))
@@ -175,7 +198,8 @@ def embed(ids, table, scale: float = 1.0, out=None):
 
 def embed_grad(ids, dout, vocab: int, scale: float = 1.0, into=None):
     """Gradient of `embed` by its table: [vocab, dim], or added to `into` (only
-    rows that occur in `ids` are touched then) and `into` returned."""
+    rows that occur in `ids` are touched then) and `into` returned; `into` must
+    not overlap the inputs."""
     what = "embed_grad"
     _tensor(dout, what, "dout")
     ip = _ids(ids, what, dout)
@@ -190,6 +214,7 @@ def embed_grad(ids, dout, vocab: int, scale: float = 1.0, into=None):
     else:
         grad = _out(into, what, "into", (vocab, dim), dout)
         gld = _rows(grad, what, "into")[2]
+        _apart(what, "into", grad, dout=dout, ids=ids)
     a = EmbedArgs(_DTYPES[dout.dtype], n, dim, vocab, scale, int(into is not None), gld, rld)
     lib, size, r = load_library(), C.c_size_t(), C.byref(a)
     _check(lib.aideen_embed_grad_workspace(r, C.byref(size)), what)
@@ -205,7 +230,8 @@ def embed_grad(ids, dout, vocab: int, scale: float = 1.0, into=None):
 # ---- layer normalisation ----------------------------------------------------
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     """(y, mean, rstd): each row of x (its last dimension) normalised; mean and
-    rstd are float32 with x's leading shape, for `layer_norm_grad`."""
+    rstd are float32 with x's leading shape, for `layer_norm_grad`.  `out` may be
+    x itself and must not overlap the inputs otherwise."""
     what = "layer_norm"
     _tensor(x, what, "x")
     n, dim, xld = _rows(x, what, "x")
@@ -215,6 +241,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     else:
         y = _out(out, what, "out", x.shape, x)
         yld = _rows(y, what, "out")[2]
+        _apart(what, "out", y, x=None if y.data_ptr() == x.data_ptr() and yld == xld else x, weight=weight, bias=bias)
     mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = _like(mean)
     a = LayerNormArgs(_DTYPES[x.dtype], n, dim, eps, xld, yld, 0)

@@ -386,7 +386,8 @@ int aideen_embed_grad(const aideen_embed_args *args, const int32_t *ids, const v
 
 /* Layer normalisation of each row: y = (x - mean) * rstd * weight + bias with
  * rstd = 1 / sqrt(var + eps).  weight, bias [dim] may be NULL (1 and 0); mean
- * and rstd [rows] may be NULL when the gradient is not needed. */
+ * and rstd [rows] may be NULL when the gradient is not needed.  y may be x itself
+ * (y_ld == x_ld): a row is read whole before it is written. */
 typedef struct aideen_layer_norm_args {
   uint32_t dtype;
   uint32_t rows;         /* 0 is allowed */

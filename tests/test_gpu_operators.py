@@ -790,6 +790,26 @@ def test_python_refusals_of_strided_vectors_and_counts():
     assert y.shape == (8,) and mean.shape == rstd.shape == () and float(mean) == 3.5
 
 
+def test_python_refuses_outputs_over_inputs():
+    t, i = torch.zeros(6, 8, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    for call in (lambda: K.embed(i, t[:5], out=t[2:]), lambda: K.embed(t[3].view(torch.int32)[2:4], t[:2], out=t[3:5]),
+                 lambda: K.embed_grad(i, t[:4], 3, into=t[3:]), lambda: K.layer_norm(t[1:], out=t[:5]),
+                 lambda: K.layer_norm(t[:2], t[3], out=t[2:4])):
+        with pytest.raises(AideenError, match="overlap"):
+            call()
+    assert not bool(t.any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim", [(1, 512), (700, 1024), (301, 777), (33, 24), (5, 20011), (3000, 96)])
+def test_layer_norm_in_place(dtype, rows, dim):
+    g = gen(rows + dim)
+    x, w, b = rand(g, rows, dim, dtype=dtype, mean=2.0), rand(g, dim, dtype=dtype), rand(g, dim, dtype=dtype)
+    want = K.layer_norm(x, w, b)
+    got = K.layer_norm(x, w, b, out=x)
+    assert got[0] is x and all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_linear_ce_refuses_a_number_for_x():
     x, w, i = torch.tensor(1.0, device="cuda"), torch.zeros(4, 1, device="cuda"), torch.tensor(0, device="cuda").int()
     for call in (lambda: K.linear_ce(x, w, i), lambda: K.linear_ce_grad(x, w, i, x)):

@@ -168,3 +168,19 @@ def test_wanted_gradients_are_named_rightly():
             operators.linear_ce_grad(t, t, i, t, want=bad)
     assert tuple(operators._wanted("weight", "f")) == ("weight",)
     assert tuple(operators._wanted(["bias", "x"], "f")) == ("bias", "x")
+
+
+def test_outputs_must_not_overlap_inputs():
+    buf = torch.zeros(40, 24)
+    for out, t in [(buf[:, :8], buf[:, 8:]), (buf[:, 16:], buf[:, :16]), (buf[:20], buf[20:]), (buf[:, :8], buf[3, 8:20]),
+                   (buf[5, 20:], buf[:, 4:20]), (buf[1, :4], buf[1, 4:]), (buf[:, :8], None), (buf[:0], buf),
+                   (buf, buf[:0]), (buf[:8, :6], buf[10:, :6]), (buf[:, 0:1], buf[:, 1:2])]:
+        operators._apart("f", "out", out, x=t)
+        if t is not None:
+            operators._apart("f", "out", t, x=out)
+    for out, t in [(buf, buf), (buf[:, :8], buf[:, 7:]), (buf[:21], buf[20:]), (buf[:, :8], buf[3, 7:20]),
+                   (buf[:, 16:], buf.view(-1)[24 * 4 + 10:24 * 4 + 17]), (buf[1, :5], buf[1, 4:]),
+                   (buf, buf.view(-1)[960 - 1:]), (buf.view(20, 48)[:, :8], buf[:, :8]), (buf[:, :8], buf[0, 0])]:
+        for a, b in ((out, t), (t, out)):
+            with pytest.raises(AideenError, match="overlaps x"):
+                operators._apart("f", "out", a, x=b)
