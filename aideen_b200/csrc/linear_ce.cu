@@ -1345,6 +1345,14 @@ int check_args(const aideen_linear_ce_args *a) {
   return AIDEEN_OK;
 }
 
+// The loss of up to kFewRows rows whose x fits ce_few_kernel's shared memory.
+bool few_rows(const aideen_linear_ce_args *a) {
+  return a->rows <= kFewRows && (size_t)a->dim * kFewRows * sizeof(float) <= kFewSmem;
+}
+// Its grid: CTAs, and the power of two of rows that each takes.
+int few_width(uint32_t rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8; }
+int few_ctas(uint32_t rows, int sms) { return (few_width(rows) <= 2 ? 2 : 1) * sms; }
+
 // Everything a call lays out.  The row count on the device is only known there,
 // so sizes follow from all rows.
 struct Plan {
@@ -1427,6 +1435,13 @@ Plan make_plan(const aideen_linear_ce_args *a, void *ws, bool grad) {
   p.xplane = (size_t)p.mpad * p.pitch;
   p.wplane = (size_t)a->vocab * p.pitch;
   OpCarve c(ws);
+  if (!grad && few_rows(a)) {  // W is read where it is: the CTAs' statistics and the targets' logits
+    const size_t n = few_width(a->rows);
+    p.stats = c.take<float2>(few_ctas(a->rows, 2 * p.pairs) * n);
+    p.row_loss = c.take<float>(n);
+    p.loss_bytes = c.used;
+    return p;
+  }
   p.slot = c.take<int32_t>(a->rows);
   p.count = c.take<int>(1);
   p.ticket = c.take<unsigned int>(1);
@@ -1549,10 +1564,9 @@ MmaArgs mma_args(const aideen_linear_ce_args *g, const Plan &p, const T *bias) {
 
 template <typename T, int VEC>
 cudaError_t few_run(FewArgs a, size_t smem, int sms, cudaStream_t st) {
-  const int R = a.rows <= 1 ? 1 : a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : 8;
+  const int R = few_width(a.rows);
   auto kernel = R == 1 ? ce_few_kernel<T, VEC, 1> : R == 2 ? ce_few_kernel<T, VEC, 2> : R == 4 ? ce_few_kernel<T, VEC, 4> : ce_few_kernel<T, VEC, 8>;
-  a.ctas = (R <= 2 ? 2 : 1) * sms;
-  a.picked = reinterpret_cast<float *>(a.part + (size_t)a.ctas * R);
+  a.ctas = few_ctas(a.rows, sms);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewSmem);  // as in launch_as
   if (e == cudaSuccess) e = op_launch(kernel, a.ctas, kFewThreads, smem * R, st, a);
   if (e == cudaSuccess) e = op_launch(ce_few_join_kernel, 1, 32 * kFewRows, 0, st, a, R);
@@ -1564,11 +1578,11 @@ cudaError_t loss_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
                      const int32_t *tg, float *loss, float *row_loss, float *lse, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = g->dim % V == 0 && op_vec16(x, g->x_ld, sizeof(T)) && op_vec16(w, g->w_ld, sizeof(T));
-  if (g->rows <= kFewRows && (size_t)g->dim * kFewRows * sizeof(float) <= kFewSmem) {
+  if (few_rows(g)) {
     FewArgs f{};
     f.x = x; f.w = w; f.bias = bias; f.x_ld = g->x_ld; f.w_ld = g->w_ld; f.tg = tg; f.rows = (int)g->rows;
     f.dim = (int)g->dim; f.vocab = (int)g->vocab; f.mean = g->reduction == AIDEEN_CE_MEAN;
-    f.part = p.stats; f.row_loss = row_loss; f.lse = lse; f.loss = loss;
+    f.part = p.stats; f.picked = p.row_loss; f.row_loss = row_loss; f.lse = lse; f.loss = loss;
     const size_t smem = op_round(g->dim, V) * sizeof(float);
     return vec ? few_run<T, V>(f, smem, 2 * p.pairs, st) : few_run<T, 1>(f, smem, 2 * p.pairs, st);
   }
@@ -1669,9 +1683,8 @@ using namespace aideen;
 extern "C" int aideen_linear_ce_workspace(const aideen_linear_ce_args *args, size_t *loss_bytes, size_t *grad_bytes) {
   const int rc = check_args(args);
   if (rc != AIDEEN_OK) return rc;
-  const Plan p = make_plan(args, nullptr, grad_bytes != nullptr);
-  if (loss_bytes) *loss_bytes = p.loss_bytes;
-  if (grad_bytes) *grad_bytes = p.grad_bytes;
+  if (loss_bytes) *loss_bytes = make_plan(args, nullptr, false).loss_bytes;
+  if (grad_bytes) *grad_bytes = make_plan(args, nullptr, true).grad_bytes;
   return AIDEEN_OK;
 }
 

@@ -134,6 +134,17 @@ def test_workspaces_grow_with_the_sizes_and_stay_below_the_logits(lib):
     assert grad_bytes(200000) < 1.5 * grad_bytes(50257)
 
 
+@pytest.mark.parametrize("rows,dim,most", [(1, 512, 1 << 14), (8, 2048, 1 << 16), (8, 2049, None), (9, 512, None)])
+def test_workspace_of_a_few_scored_rows(lib, rows, dim, most):
+    """The loss of up to 8 rows reads W where it is; more rows of float32 have it laid out."""
+    n, both, m = C.c_size_t(), C.c_size_t(), C.c_size_t()
+    a = ce_args(rows=rows, dim=dim, vocab=50257, x_ld=dim, w_ld=dim)
+    assert lib.aideen_linear_ce_workspace(C.byref(a), C.byref(n), None) == OK
+    assert lib.aideen_linear_ce_workspace(C.byref(a), C.byref(both), C.byref(m)) == OK
+    assert both.value == n.value and m.value >= 4 * dim * 50257
+    assert n.value <= most if most else n.value >= 4 * dim * 50257
+
+
 def test_rows_of_a_matrix():
     x = torch.zeros(4, 6, 10)
     assert operators._rows(x, "f", "x") == (24, 10, 10)
