@@ -54,7 +54,7 @@ constexpr int kMaxStages = 8, kMaxHeld = 8;    // ring depth; slices of x that s
 constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
 constexpr int kBoxBytes = 4096;  // 32 rows of 128 bytes
 constexpr uint32_t kWaitLimit = 1u << 24;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 // float16 keeps softmax - onehot times 2^12: probabilities down to 2^-26 stay
 // normal numbers, and the largest magnitude is 2^12
 constexpr float kHalfScale = 4096.f;
@@ -76,7 +76,7 @@ struct MmaArgs {
   // kStats, kPiece: vocabulary tiles [0, tiles_n) from column v0 on
   int v0, tiles_n;
   const void *bias;
-  float2 *stats;      // kStats: [slot][2][256] (maximum, sum) in base 2
+  float2 *stats;      // kStats: [slot][2][256] (maximum, sum of e^(z - maximum))
   const float *lse;   // kPiece: compacted rows' lse
   const int32_t *tgt; // and their targets
   float *db_part;     // [8 tiles_m][tiles_n * 256] column sums of 32 rows each, or null
@@ -187,6 +187,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// e^(a - b).  The difference comes before the change of base: a logit that float32 holds need
+// not fit it in base 2, and the largest terms get small exponents, rounded finely.
+__device__ __forceinline__ float exp_diff(float a, float b) { return exp2_fast((a - b) * kLog2e); }
 
 // Products of pieces in the order they are added: low x high, high x low, high x high.
 __device__ __forceinline__ void product_pair(int planes, int j, int &pa, int &pb) {
@@ -612,12 +616,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int acc = j & 1;
       const float *sb = sbias + acc * kTileN;
       if (MODE != kProducts) {
-        // this tile's bias, in base 2 but for float32's G (-Inf behind the vocabulary);
-        // the buffer's last reader passed the barrier of the tile before
-        constexpr float unit = MODE == kPiece && sizeof(T) == 4 ? 1.f : kLog2e;
+        // this tile's bias (-Inf behind the vocabulary); the buffer's last reader passed
+        // the barrier of the tile before
         const int v = a.v0 + u.n * kTileN + etid;
         float b = -INFINITY;
-        if (v < a.vocab) b = a.bias ? op_load<T>(static_cast<const T *>(a.bias)[v]) * unit : 0.f;
+        if (v < a.vocab) b = a.bias ? op_load<T>(static_cast<const T *>(a.bias)[v]) : 0.f;
         sbias[acc * kTileN + etid] = b;
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
         if (u.m != last_m) {
@@ -628,7 +631,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           } else {
             const int row = u.m * kTileM + (int)rank * 128 + q * 32 + lane;
             lse = row < count ? a.lse[row] : 0.f;
-            if (sizeof(T) == 2) lse *= kLog2e;
             tgt = row < count ? a.tgt[row] : -1;
           }
           last_m = u.m;
@@ -670,10 +672,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int i = 0; i < 4; ++i) v[4 * k + i] = v[4 * k + i] * f_lo * f_hi;
             }
-            v[4 * k] = fmaf(v[4 * k], kLog2e, b.x);
-            v[4 * k + 1] = fmaf(v[4 * k + 1], kLog2e, b.y);
-            v[4 * k + 2] = fmaf(v[4 * k + 2], kLog2e, b.z);
-            v[4 * k + 3] = fmaf(v[4 * k + 3], kLog2e, b.w);
+            v[4 * k] += b.x;
+            v[4 * k + 1] += b.y;
+            v[4 * k + 2] += b.z;
+            v[4 * k + 3] += b.w;
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, v[4 * k + i]);
           }
@@ -681,10 +683,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           float s0 = 0.f, s1 = 0.f;
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            s0 += exp2_fast(v[k] - ref);
-            s1 += exp2_fast(v[k + 1] - ref);
+            s0 += exp_diff(v[k], ref);
+            s1 += exp_diff(v[k + 1], ref);
           }
-          run_s = run_s * exp2_fast(run_m - ref) + (s0 + s1);
+          run_s = run_s * exp_diff(run_m, ref) + (s0 + s1);
           run_m = top;
         }
       } else if (MODE == kPiece) {
@@ -703,10 +705,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 float &x = v[h][4 * k + i];
-                // float32 subtracts lse before the change of base: the largest probabilities
-                // then have small exponents, rounded finely
-                if constexpr (sizeof(T) == 4) x = exp2_fast((x * f_lo * f_hi + bb[i] - lse) * kLog2e);
-                else x = exp2_fast(fmaf(x, kLog2e, bb[i] - lse));
+                if constexpr (sizeof(T) == 4) x = x * f_lo * f_hi;
+                x = exp_diff(x + bb[i], lse);
               }
             }
           }
@@ -1057,7 +1057,7 @@ __global__ void __launch_bounds__(256) ce_stage_kernel(const StageArgs a) {
 // ---- joins -------------------------------------------------------------------
 __device__ __forceinline__ void merge2(float &m, float &s, float m2, float s2) {
   const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
-  s = s * exp2f(m - ref) + s2 * exp2f(m2 - ref);
+  s = s * exp2f((m - ref) * kLog2e) + s2 * exp2f((m2 - ref) * kLog2e);
   m = top;
 }
 
@@ -1113,9 +1113,9 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const RowsArgs a) {
       merge2(top, sum, m2, s2);
     }
     if (lane == 0) {
-      const float l = (top + log2f(sum)) * kLn2;
-      if (a.lse) a.lse[n] = l;
-      a.row_loss[n] = l - (dot + (bias ? op_load<T>(bias[t]) : 0.f));
+      const float l = logf(sum);
+      if (a.lse) a.lse[n] = top + l;
+      a.row_loss[n] = top - (dot + (bias ? op_load<T>(bias[t]) : 0.f)) + l;
     }
   } else if (n < a.rows && lane == 0) {
     a.row_loss[n] = 0.f;
@@ -1149,7 +1149,7 @@ struct FewArgs {
   long x_ld, w_ld;
   const int32_t *tg;
   int rows, dim, vocab, mean, ctas;
-  float2 *part;   // [CTAs][R] (maximum, sum) in base 2
+  float2 *part;   // [CTAs][R] (maximum, sum of e^(z - maximum))
   float *picked;  // [R] target logits
   float *row_loss, *lse, *loss;
 };
@@ -1220,10 +1220,10 @@ __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 2 : 1) ce_few_kernel(con
     }
     const long v = v0 + q;
     if (v < a.vocab) {
-      const float z = acc[0] + (bias ? op_load<T>(bias[v]) : 0.f), z2 = z * kLog2e;
+      const float z = acc[0] + (bias ? op_load<T>(bias[v]) : 0.f);
       if (v == tgt) a.picked[r] = z;
-      const float now = fmaxf(top, z2), ref = now == -INFINITY ? 0.f : now;
-      sum = sum * exp2_fast(top - ref) + exp2_fast(z2 - ref);
+      const float now = fmaxf(top, z), ref = now == -INFINITY ? 0.f : now;
+      sum = sum * exp_diff(top, ref) + exp_diff(z, ref);
       top = now;
     }
   }
@@ -1265,8 +1265,9 @@ __global__ void __launch_bounds__(32 * kFewRows) ce_few_join_kernel(const FewArg
       const float m2 = __shfl_xor_sync(0xffffffffu, top, off), s2 = __shfl_xor_sync(0xffffffffu, sum, off);
       merge2(top, sum, m2, s2);
     }
-    l = (top + log2f(sum)) * kLn2;
-    loss = l - a.picked[r];
+    l = logf(sum);
+    loss = top - a.picked[r] + l;
+    l += top;
   }
   if (lane == 0) {
     rl[r] = loss;

@@ -473,6 +473,44 @@ def test_linear_ce_masked_vocabulary(dtype):
     assert bool((dw[dead] == 0).all()) and bool((db[dead] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [3, 140])
+def test_linear_ce_logits_near_the_ends_of_float32(dtype, rows):
+    """Finite logits have a finite loss, also above 2^128 ln 2 = 2.36e38, where float32 does
+    not hold them in base 2, and also where every entry is at the type's lowest value: such
+    logits round to that value in float32, all alike, so the row's loss is log(vocabulary)."""
+    x, w, b, tg = ce_inputs(61, rows, 64, 600, dtype, True)
+    b.fill_(torch.finfo(dtype).min)
+    loss, row_loss, lse = K.linear_ce(x, w, tg, bias=b)
+    assert bool((lse == torch.finfo(dtype).min).all())
+    want = torch.full((rows,), 600.0, device="cuda", dtype=torch.float64).log()
+    close(row_loss, want, 700 * U32 * want)  # 600 terms of e^0, added up and joined, and a logarithm
+    close(loss, want[:1], 900 * U32 * want[:1])
+    b.normal_()
+    b[77], b[300] = 3e38, -3e38
+    tg[0], tg[1], tg[2] = 77, 300, 5
+    loss, row_loss, lse = K.linear_ce(x, w, tg, bias=b)
+    top = float(b[77].double())
+    gone = top - torch.where(tg == 300, float(b[300].double()), 0.0)
+    gone[tg == 77] = 0.0
+    gone[tg == 300] = float("inf")  # 6e38: the one loss that float32 does not hold
+    assert bool((lse.double() - top).abs().max() <= 2 * U32 * top)
+    near = tg != 300
+    close(row_loss[near], gone[near].double(), 4 * U32 * gone[near].double() + 1e-30)
+    assert bool((row_loss[~near] == float("inf")).all())
+    tg[tg == 300] = 5
+    _, _, lse = K.linear_ce(x, w, tg, bias=b)
+    dx, dw, db = K.linear_ce_grad(x, w, tg, lse, bias=b)
+    p = torch.zeros(rows, 600, device="cuda", dtype=torch.float64)
+    p[:, 77] = 1.0
+    p[torch.arange(rows, device="cuda"), tg.long()] -= 1.0
+    p /= rows
+    for got, want, mag in ((dx, p @ w.double(), p.abs() @ w.double().abs()), (dw, p.t() @ x.double(), p.abs().t() @ x.double().abs()),
+                           (db, p.sum(0), p.abs().sum(0))):
+        e = 2 * (rows + 600 + 32) * U32 * mag
+        close(got, want, e + U[dtype] * (want.abs() + e) + TINY[dtype])
+
+
 def test_linear_ce_nonfinite_rows_spoil_only_themselves():
     x, w, b, tg = ce_inputs(8, 64, 32, 100, F32, True)
     x[5, 3], x[9, 1] = float("nan"), float("inf")
