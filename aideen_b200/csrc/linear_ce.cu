@@ -353,20 +353,24 @@ __device__ __forceinline__ void box_put32(unsigned char *box, int lane, const fl
         make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
 }
 
-// Adds this lane's two columns of a box of 64 (32 rows; every bank once per row).
-template <typename T>
-__device__ __forceinline__ void box_sums(const unsigned char *box, int lane, float2 &sum) {
-  float2 even = make_float2(0.f, 0.f), odd = make_float2(0.f, 0.f);
+// Sums of 32 columns over the warp's 32 rows; lane l gets column l.  Halves of the columns
+// change hands while a lane has several.
+__device__ __forceinline__ float column_sums(const float (&v)[32], int lane) {
+  float t[16];
 #pragma unroll
-  for (int r = 0; r < 32; ++r) {
-    const OpVec<T, 2> g =
-        *reinterpret_cast<const OpVec<T, 2> *>(box + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
-    float2 &s = r & 1 ? odd : even;
-    s.x += op_load<T>(g.v[0]);
-    s.y += op_load<T>(g.v[1]);
+  for (int i = 0; i < 16; ++i) {
+    const float send = lane & 16 ? v[i] : v[i + 16], keep = lane & 16 ? v[i + 16] : v[i];
+    t[i] = keep + __shfl_xor_sync(0xffffffffu, send, 16);
   }
-  sum.x += even.x + odd.x;
-  sum.y += even.y + odd.y;
+#pragma unroll
+  for (int n = 8; n > 0; n >>= 1) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float send = lane & n ? t[i] : t[i + n], keep = lane & n ? t[i + n] : t[i];
+      t[i] = keep + __shfl_xor_sync(0xffffffffu, send, n);
+    }
+  }
+  return t[0];
 }
 
 // One warp's N staging boxes, used in turn: take() gives one whose last store has
@@ -725,34 +729,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               for (int k = 0; k < 32; ++k)
                 if (32 * h + k == at) v[h][k] -= 1.f;
           }
-          float2 col_sum = make_float2(0.f, 0.f);
           if (a.g_scale != 1.f) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int k = 0; k < 32; ++k) v[h][k] *= a.g_scale;
           }
+          if (a.db_part) {  // before any rounding
+            float *sums = a.db_part + (size_t)(row0 >> 5) * a.tiles_n * kTileN + n0 + c + lane;
+            sums[0] = column_sums(v[0], lane);
+            sums[32] = column_sums(v[1], lane);
+          }
           if constexpr (sizeof(T) == 2) {
             unsigned char *bx = box.take();
             box_put16<T>(bx, lane, 0, v[0]);
             box_put16<T>(bx, lane, 1, v[1]);
             box.send(&maps.c, bx, n0 + c, row0, 0, false);
-            if (a.db_part) box_sums<T>(bx, lane, col_sum);
           } else {
             for (int p = 0; p < 2; ++p) {
               unsigned char *bx = box.take();
               box_put16<__half>(bx, lane, 0, v[0]);
               box_put16<__half>(bx, lane, 1, v[1]);
               box.send(&maps.c, bx, n0 + c, row0, p, false);
-              if (a.db_part) box_sums<__half>(bx, lane, col_sum);
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int k = 0; k < 32; ++k) v[h][k] -= __half2float(__float2half_rn(v[h][k]));
             }
           }
-          if (a.db_part)
-            *reinterpret_cast<float2 *>(a.db_part + (size_t)(row0 >> 5) * a.tiles_n * kTileN + n0 + c + 2 * lane) = col_sum;
         }
       } else {
         const int n0 = u.n * bn + half * hcols;

@@ -437,7 +437,8 @@ int aideen_linear_ce(const aideen_linear_ce_args *args, const void *x, const voi
  * three).  dx rows that are not counted are zero.  In 16 bits, softmax - onehot
  * is rounded to dtype before its two products (its relative error there is that
  * of one rounding; in float16 it is scaled by 2^12 first, so probabilities below
- * 2^-26 lose digits); dx, dW and dbias are rounded once more when stored.  In
+ * 2^-26 lose digits); dbias sums it unrounded; dx, dW and dbias are rounded once
+ * when stored.  In
  * float32 (in the loss too, but for a few rows) x, W and softmax - onehot enter their
  * products as two scaled float16 pieces each: 22 bits of a value, and what lies
  * below 2^-39 of a tensor's largest magnitude is rounded off.  An infinite x or W

@@ -602,6 +602,21 @@ def test_linear_ce_row_widths(dtype, dim, pad_x, pad_w):
     ce_check(strided(x, pad_x), strided(w, pad_w), b, tg, dloss=16.0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,vocab", [(300, 64, 700), (33, 520, 300), (1, 24, 40), (1100, 32, 257)])
+def test_linear_ce_bias_gradient_is_summed_in_float32(dtype, rows, dim, vocab):
+    """softmax - onehot enters dbias unrounded: the bound has float32's steps, and the type's
+    one for the result alone."""
+    x, w, b, tg = ce_inputs(rows + vocab, rows, dim, vocab, dtype, True, 0.1)
+    if rows > 1:
+        tg[:rows // 2] = 3  # a target that comes often: its sum is all but cancelled rounding
+    tg[0] = 1
+    _, _, lse = K.linear_ce(x, w, tg, bias=b)
+    db = K.linear_ce_grad(x, w, tg, lse, bias=b, want=("bias",))[2]
+    want, e = ce_reference(x, w, b, tg, "mean", 1.0, F32)["db"]
+    close(db, want, e + U[dtype] * (want.abs() + e) + TINY[dtype])
+
+
 def test_linear_ce_parts_alone():
     x, w, b, tg = ce_inputs(2, 70, 48, 333, BF16, True, 0.2)
     _, _, lse = K.linear_ce(x, w, tg, bias=b)
