@@ -192,6 +192,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // not fit it in base 2, and the largest terms get small exponents, rounded finely.
 __device__ __forceinline__ float exp_diff(float a, float b) { return exp2_fast((a - b) * kLog2e); }
 
+// About the square root of a power of two.  f = half_power(f) * rest, either applied before
+// and after another factor, leaves float32's range only where the result does: what one
+// multiplication by both would round to a subnormal number, or overflow, may be in range.
+__device__ __forceinline__ float half_power(float f) {
+  const int e = ((int)(__float_as_uint(f) >> 23) & 255) - 127;
+  return __uint_as_float((uint32_t)((e >> 1) + 127) << 23);
+}
+
 // Products of pieces in the order they are added: low x high, high x low, high x high.
 __device__ __forceinline__ void product_pair(int planes, int j, int &pa, int &pb) {
   pa = planes == 2 && j == 0;
@@ -602,6 +610,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const float scale = MODE == kProducts ? grad_scale(a.dloss, a.count, a.mean) / a.g_scale : 0.f;
     const float fx = sizeof(T) == 4 ? a.unscale[0] : 1.f, fw = sizeof(T) == 4 ? a.unscale[1] : 1.f;
     const float f_lo = fminf(fx, fw), f_hi = fmaxf(fx, fw);  // in this order z overflows only where it has to
+    const float fx1 = half_power(fx), fx2 = fx / fx1;
     const Deal full_deal = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs,
                                    (int)(gridDim.x >> 1));
     if (MODE == kProducts && a.slabs) {  // the last piece may be shorter than the others, and deal dx differently
@@ -804,7 +813,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[h][k] *= scale * fx;
+              for (int k = 0; k < 32; ++k) {
+                if constexpr (sizeof(T) == 4) v[h][k] = v[h][k] * fx1 * scale * fx2;
+                else v[h][k] *= scale;
+              }
             if constexpr (sizeof(T) == 2) {
               unsigned char *bx = box.take();
               box_put16<T>(bx, lane, 0, v[0]);
@@ -1303,7 +1315,8 @@ __global__ void __launch_bounds__(256) ce_dx_kernel(const float *slab, size_t sl
   const long n = (long)blockIdx.x * per_cta + warp / per_row;
   if (n >= rows) return;
   const int at = slot[n];
-  const float c = grad_scale(a.dloss, a.count, a.mean) / a.g_scale * (sizeof(T) == 4 ? a.unscale[1] : 1.f);
+  const float c = grad_scale(a.dloss, a.count, a.mean) / a.g_scale;
+  const float fw1 = sizeof(T) == 4 ? half_power(a.unscale[1]) : 1.f, fw2 = sizeof(T) == 4 ? a.unscale[1] / fw1 : 1.f;
   for (int i = ((warp % per_row) * 32 + lane) * 4; i < a.dim; i += per_row * 128) {
     float s[4] = {};
     if (at >= 0) {
@@ -1322,7 +1335,7 @@ __global__ void __launch_bounds__(256) ce_dx_kernel(const float *slab, size_t sl
       }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = at >= 0 ? s[e] * c : 0.f;  // 0 whatever dloss is
+    for (int e = 0; e < 4; ++e) s[e] = at >= 0 ? s[e] * fw1 * c * fw2 : 0.f;  // 0 whatever dloss is
     T *o = dx + n * dx_ld + i;
     if (vec == 4) {
       op_store_vec<T, 4>(o, s);

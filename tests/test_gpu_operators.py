@@ -571,6 +571,21 @@ def test_linear_ce_in_float32_at_the_ends_of_the_range():
     assert torch.equal(dw * far, dw2)
 
 
+@pytest.mark.parametrize("power", [-108, 108])
+@pytest.mark.parametrize("dloss", [1.0, 2.0 ** 20, 2.0 ** -20])
+def test_linear_ce_gradients_in_float32_at_the_ends_of_the_range(power, dloss):
+    """As above, for both gradients: they scale by that power, bit by bit (what becomes
+    subnormal is rounded once more, in the kernel as here)."""
+    g = gen(8)
+    x, w = rand(g, 60, 64, std=0.3), torch.rand(200, 64, generator=g, device="cuda") / 2 + 0.5
+    tg = torch.randint(0, 200, (60,), generator=g, device="cuda", dtype=torch.int32)
+    far, c = 2.0 ** power, torch.tensor([dloss], device="cuda")
+    _, _, lse = K.linear_ce(x, w, tg)
+    dx, dw, _ = K.linear_ce_grad(x, w, tg, lse, dloss=c)
+    dx2, dw2, _ = K.linear_ce_grad(x * far, w / far, tg, lse, dloss=c)
+    assert torch.equal(dw * far, dw2) and torch.equal(dx / far, dx2)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_ce_peaked_rows(dtype):
     """Large logits: the softmax is all but one-hot, the loss near zero or large."""
