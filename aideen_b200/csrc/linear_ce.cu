@@ -39,6 +39,8 @@
 // further, lets its copies land, frees the tensor memory and returns.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "operators.cuh"
 #include "tc_common.cuh"
@@ -191,6 +193,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // e^(a - b).  The difference comes before the change of base: a logit that float32 holds need
 // not fit it in base 2, and the largest terms get small exponents, rounded finely.
 __device__ __forceinline__ float exp_diff(float a, float b) { return exp2_fast((a - b) * kLog2e); }
+// The same for two at a time (two float32 lanes per instruction), b given as (-b, -b).
+__device__ __forceinline__ float2 exp_diff(float2 a, float2 minus_b) {
+  const float2 e = __fmul2_rn(__fadd2_rn(a, minus_b), make_float2(kLog2e, kLog2e));
+  return make_float2(exp2_fast(e.x), exp2_fast(e.y));
+}
 
 // About the square root of a power of two.  f = half_power(f) * rest, either applied before
 // and after another factor, leaves float32's range only where the result does: what one
@@ -628,6 +635,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (; units.get(u); ++j) {
       const int acc = j & 1;
       const float *sb = sbias + acc * kTileN;
+      uint32_t some_out = 0;
       if (MODE != kProducts) {
         // this tile's bias (-Inf behind the vocabulary); the buffer's last reader passed
         // the barrier of the tile before
@@ -635,7 +643,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float b = -INFINITY;
         if (v < a.vocab) b = a.bias ? op_load<T>(static_cast<const T *>(a.bias)[v]) : 0.f;
         sbias[acc * kTileN + etid] = b;
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+        // (and whether a bias of -Inf or the vocabulary's end takes some columns out)
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "setp.ne.u32 q, %1, 0;\n\t"
+            "bar.red.or.pred p, 1, %2, q;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(some_out)
+            : "r"((uint32_t)(b == -INFINITY)), "n"(32 * kEpiWarps)
+            : "memory");
         if (u.m != last_m) {
           if (MODE == kStats) {
             flush();
@@ -671,39 +687,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tmem_load32(t0 + c, v);
         if (last) release();
       };
+      // Which of 32 columns are taken out, whatever their logits are: an overflow to +Inf would
+      // make them NaN.
+      auto masked = [&](int c) { return __ballot_sync(0xffffffffu, sb[half * hcols + c + lane] == -INFINITY); };
       if (MODE == kStats) {
+        auto walk = [&](auto some) {  // some: columns may be taken out
 #pragma unroll 1
-        for (int c = 0; c < kTileN / 2; c += 32) {
-          float v[32];
-          fetch(c, v, c + 32 == kTileN / 2);
-          const float4 *b4 = reinterpret_cast<const float4 *>(sb + half * hcols + c);
-          float top = run_m;
+          for (int c = 0; c < kTileN / 2; c += 32) {
+            float v[32];
+            fetch(c, v, c + 32 == kTileN / 2);
+            float2 z[16];
+            const float4 *b4 = reinterpret_cast<const float4 *>(sb + half * hcols + c);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float4 b = b4[k];
-            if constexpr (sizeof(T) == 4) {
+            for (int k = 0; k < 8; ++k) {
+              const float4 b = b4[k];
+              if constexpr (sizeof(T) == 4) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) v[4 * k + i] = v[4 * k + i] * f_lo * f_hi;
+                for (int i = 0; i < 4; ++i) v[4 * k + i] = v[4 * k + i] * f_lo * f_hi;
+              }
+              z[2 * k] = __fadd2_rn(make_float2(v[4 * k], v[4 * k + 1]), make_float2(b.x, b.y));
+              z[2 * k + 1] = __fadd2_rn(make_float2(v[4 * k + 2], v[4 * k + 3]), make_float2(b.z, b.w));
             }
-            v[4 * k] += b.x;
-            v[4 * k + 1] += b.y;
-            v[4 * k + 2] += b.z;
-            v[4 * k + 3] += b.w;
+            if constexpr (decltype(some)::value) {
+              const uint32_t out = masked(c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, v[4 * k + i]);
-          }
-          const float ref = top == -INFINITY ? 0.f : top;  // nothing but -Inf so far
-          float s0 = 0.f, s1 = 0.f;
+              for (int k = 0; k < 16; ++k) {
+                if (out >> (2 * k) & 1) z[k].x = -INFINITY;
+                if (out >> (2 * k + 1) & 1) z[k].y = -INFINITY;
+              }
+            }
+            float top = run_m;
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            s0 += exp_diff(v[k], ref);
-            s1 += exp_diff(v[k + 1], ref);
+            for (int k = 0; k < 16; ++k) top = fmaxf(fmaxf(top, z[k].x), z[k].y);
+            const float ref = top == -INFINITY ? 0.f : top;  // nothing but -Inf so far
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) sum = __fadd2_rn(sum, exp_diff(z[k], make_float2(-ref, -ref)));
+            run_s = run_s * exp_diff(run_m, ref) + (sum.x + sum.y);
+            run_m = top;
           }
-          run_s = run_s * exp_diff(run_m, ref) + (s0 + s1);
-          run_m = top;
-        }
+        };
+        // (a test for them in every step costs 3% at 8192 x 50257 x 128 bf16)
+        if (some_out) walk(std::true_type{});
+        else walk(std::false_type{});
       } else if (MODE == kPiece) {
         const int n0 = u.n * kTileN + half * hcols;
+        const float2 nlse = make_float2(-lse, -lse);
 #pragma unroll 1
         for (int c = 0; c < kTileN / 2; c += 64) {
           float v[2][32];
@@ -714,21 +743,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const float4 b = b4[k];
-              const float bb[4] = {b.x, b.y, b.z, b.w};
+              if constexpr (sizeof(T) == 4) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float &x = v[h][4 * k + i];
-                if constexpr (sizeof(T) == 4) x = x * f_lo * f_hi;
-                x = exp_diff(x + bb[i], lse);
+                for (int i = 0; i < 4; ++i) v[h][4 * k + i] = v[h][4 * k + i] * f_lo * f_hi;
               }
+              const float2 p = exp_diff(__fadd2_rn(make_float2(v[h][4 * k], v[h][4 * k + 1]), make_float2(b.x, b.y)), nlse);
+              const float2 q = exp_diff(__fadd2_rn(make_float2(v[h][4 * k + 2], v[h][4 * k + 3]), make_float2(b.z, b.w)), nlse);
+              v[h][4 * k] = p.x; v[h][4 * k + 1] = p.y;
+              v[h][4 * k + 2] = q.x; v[h][4 * k + 3] = q.y;
             }
           }
-          if (row0 + 32 > count) {  // rows behind the last, whatever an infinite W made of them
+          if (some_out || row0 + 32 > count) {  // and rows behind the last, whatever an infinite W made of them
+            const float p = exp_diff(-INFINITY, lse);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t out = masked(c + 32 * h);
 #pragma unroll
-              for (int k = 0; k < 32; ++k)
+              for (int k = 0; k < 32; ++k) {
+                if (out >> k & 1) v[h][k] = p;
                 if (row0 + lane >= count) v[h][k] = 0.f;
+              }
+            }
           }
           const int at = tgt - (a.v0 + n0 + c);  // the target's column among these 64
           if (__any_sync(0xffffffffu, at >= 0 && at < 64)) {
@@ -742,7 +777,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[h][k] *= a.g_scale;
+              for (int k = 0; k < 32; k += 2) {
+                const float2 g = __fmul2_rn(make_float2(v[h][k], v[h][k + 1]), make_float2(a.g_scale, a.g_scale));
+                v[h][k] = g.x; v[h][k + 1] = g.y;
+              }
           }
           if (a.db_part) {  // before any rounding
             float *sums = a.db_part + (size_t)(row0 >> 5) * a.tiles_n * kTileN + n0 + c + lane;
@@ -1070,6 +1108,9 @@ __global__ void __launch_bounds__(256) ce_stage_kernel(const StageArgs a) {
     put_row<T, 1>(a.xc + (size_t)j * a.pitch, a.xplane, static_cast<const T *>(nullptr), a.dim, lane, 1.f);
 }
 
+// A bias of -Inf takes an entry out whatever its product is.
+__device__ __forceinline__ float add_bias(float z, float b) { return b == -INFINITY ? b : z + b; }
+
 // ---- joins -------------------------------------------------------------------
 __device__ __forceinline__ void merge2(float &m, float &s, float m2, float s2) {
   const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
@@ -1131,7 +1172,7 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const RowsArgs a) {
     if (lane == 0) {
       const float l = logf(sum);
       if (a.lse) a.lse[n] = top + l;
-      a.row_loss[n] = top - (dot + (bias ? op_load<T>(bias[t]) : 0.f)) + l;
+      a.row_loss[n] = top - add_bias(dot, bias ? op_load<T>(bias[t]) : 0.f) + l;
     }
   } else if (n < a.rows && lane == 0) {
     a.row_loss[n] = 0.f;
@@ -1236,7 +1277,7 @@ __global__ void __launch_bounds__(kFewThreads, R <= 2 ? 2 : 1) ce_few_kernel(con
     }
     const long v = v0 + q;
     if (v < a.vocab) {
-      const float z = acc[0] + (bias ? op_load<T>(bias[v]) : 0.f);
+      const float z = add_bias(acc[0], bias ? op_load<T>(bias[v]) : 0.f);
       if (v == tgt) a.picked[r] = z;
       const float now = fmaxf(top, z), ref = now == -INFINITY ? 0.f : now;
       sum = sum * exp_diff(top, ref) + exp_diff(z, ref);

@@ -511,6 +511,36 @@ def test_linear_ce_logits_near_the_ends_of_float32(dtype, rows):
         close(got, want, e + U[dtype] * (want.abs() + e) + TINY[dtype])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [4, 40, 300])
+def test_linear_ce_masked_logits_that_overflow(dtype, rows):
+    """An entry that a bias of -Inf masks has probability 0, also where its product with x is
+    too large for float32 (in float16: where W holds an infinity), at either sign."""
+    x, w, b, tg = ce_inputs(rows, rows, 48, 600, dtype, True)
+    w[100:300:2] = torch.where(torch.rand(100, 1, device="cuda", generator=gen(1)) < 0.5, -1.0, 1.0).to(dtype)
+    w[100:300:2] *= 3e38 if dtype != F16 else float("inf")
+    out = torch.zeros(600, dtype=torch.bool, device="cuda")
+    out[100:300:2] = True
+    b[out] = -float("inf")
+    tg[out[tg.long()]] = 1
+    keep = (~out).nonzero()[:, 0]
+    back = torch.zeros(600, dtype=torch.int32, device="cuda")
+    back[keep] = torch.arange(keep.numel(), device="cuda", dtype=torch.int32)
+    x = x.abs() + 0.25
+    x[:, 0] *= 8
+    ref = ce_reference(x, w[keep], b[keep], back[tg.long()], "mean", 1.0, dtype)
+    loss, row_loss, lse = K.linear_ce(x, w, tg, b)
+    _, dw, db = K.linear_ce_grad(x, w, tg, lse, b, want=("weight", "bias"))
+    if dtype != F32 or rows < 9:  # W's largest magnitude is float32's scale
+        for got, name in ((loss, "loss"), (row_loss, "rows"), (lse, "lse")):
+            close(got, ref[name][0], ref[name][1])
+        for got, name in ((dw[keep], "dw"), (db[keep], "db")) if dtype != F32 else ():
+            want, e = ref[name]
+            close(got, want, e + U[dtype] * (want.abs() + e) + TINY[dtype])
+    assert not bool(dw[out].any()) and not bool(db[out].any())
+    assert bool(torch.isfinite(lse).all())
+
+
 def test_linear_ce_nonfinite_rows_spoil_only_themselves():
     x, w, b, tg = ce_inputs(8, 64, 32, 100, F32, True)
     x[5, 3], x[9, 1] = float("nan"), float("inf")
