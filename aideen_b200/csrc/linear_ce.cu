@@ -25,12 +25,15 @@
 // A pair tile is the largest that leaves two accumulators: an operand byte from L2
 // carries 256 products, so that L2 does not bound it.
 //
-// float32: each of x, W and G = softmax - onehot is scaled by a power of two that brings
+// float32: each of x, W and G = softmax - onehot is scaled by powers of two that bring
 // its largest magnitude (G: 1) to 2^14..2^15 and written as high + low float16 pieces;
 // high x high + high x low + low x high leave out 2^-22 of a product, three passes where
 // bfloat16 pieces would take six (training shard 50257 x 512, 2048 rows, loss and gradient:
-// 2.23 ms with those, 1.43 ms this way).  What
-// lies below 2^-40 of the largest magnitude (G: 2^-39) is rounded off.
+// 2.23 ms with those, 1.43 ms this way).  For the logits every row of x and of W has its own
+// scale, so that a row of W that dwarfs the others costs them nothing: with one scale, a
+// masked row 10^8 times the others put lse off by 1e-3.  The products with G add up over
+// rows, so there x and W have one scale each, in a second layout of the gradient, where what
+// lies below 2^-40 of the largest magnitude is rounded off.
 // Bound: the tensor cores (2 N V d for the loss, 6 N V d for the gradient, z being
 // formed twice), and behind them the power limit: 8192 rows, nine in ten counted, 50257 x 512
 // bf16, loss and gradient take 1.35 ms, 1.12 PFLOP/s, at clocks that the limit holds at 1.3-1.5 GHz.
@@ -63,8 +66,11 @@ constexpr float kHalfScale = 4096.f;
 // and float32's two pieces of it times 2^14
 constexpr float kPieceScale = 16384.f;
 // Shared memory of a CTA: held slices of x, the ring, the epilogue's boxes, the
-// bias of two tiles, barriers.
-constexpr int kSmemLimit = 232448, kSmemFixed = 2 * kTileN * 4 + 512;
+// bias of two tiles, barriers, and in float32 the exponents of W's factors.
+constexpr int kSmemLimit = 232448, kSmemBarriers = 512;
+constexpr int smem_fixed(int mode, size_t elem) {
+  return 2 * kTileN * 4 + kSmemBarriers + (elem == 4 && mode != 2 ? 2 * kTileN : 0);
+}
 
 enum { kStats = 0, kPiece = 1, kProducts = 2 };
 
@@ -72,7 +78,9 @@ struct MmaArgs {
   const int *count;   // counted rows
   int vocab, dim;
   int planes;         // 16-bit pieces per operand element: 1, or 2 for float32
-  const float *unscale;  // float32: what x and W were divided by, [2]
+  // float32: what x and W were divided by: counted rows' and vocabulary rows' own factors
+  // (kStats, kPiece), [2] for the products
+  const float *xinv, *winv, *unscale;
   uint32_t idesc;     // operand types of the instruction descriptor
   int stages;         // ring depth
   // kStats, kPiece: vocabulary tiles [0, tiles_n) from column v0 on
@@ -199,12 +207,13 @@ __device__ __forceinline__ float2 exp_diff(float2 a, float2 minus_b) {
   return make_float2(exp2_fast(e.x), exp2_fast(e.y));
 }
 
-// About the square root of a power of two.  f = half_power(f) * rest, either applied before
-// and after another factor, leaves float32's range only where the result does: what one
-// multiplication by both would round to a subnormal number, or overflow, may be in range.
-__device__ __forceinline__ float half_power(float f) {
-  const int e = ((int)(__float_as_uint(f) >> 23) & 255) - 127;
-  return __uint_as_float((uint32_t)((e >> 1) + 127) << 23);
+// A power of two f in two halves, f.x about its square root and f.x f.y = f (also where f is
+// Inf).  Applied before and after another factor they leave float32's range only where the
+// result does: what one multiplication by both would round to a subnormal number, or
+// overflow, may be in range.
+__device__ __forceinline__ float2 halves(float f) {
+  const int e = (((int)(__float_as_uint(f) >> 23) & 255) - 127) >> 1;
+  return make_float2(__uint_as_float((uint32_t)(127 + e) << 23), f * __uint_as_float((uint32_t)(127 - e) << 23));
 }
 
 // Products of pieces in the order they are added: low x high, high x low, high x high.
@@ -471,6 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint64_t *done = tempty + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
   uint32_t *err = tmem_slot + 1;
+  uint8_t *sfac = reinterpret_cast<uint8_t *>(full) + kSmemBarriers;  // float32: [2][kTileN]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
 
@@ -615,9 +625,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     float lse = 0.f;
     int32_t tgt = -1;
     const float scale = MODE == kProducts ? grad_scale(a.dloss, a.count, a.mean) / a.g_scale : 0.f;
-    const float fx = sizeof(T) == 4 ? a.unscale[0] : 1.f, fw = sizeof(T) == 4 ? a.unscale[1] : 1.f;
-    const float f_lo = fminf(fx, fw), f_hi = fmaxf(fx, fw);  // in this order z overflows only where it has to
-    const float fx1 = half_power(fx), fx2 = fx / fx1;
+    // float32: x's factor, of the products or of this lane's row
+    float2 fx = MODE == kProducts && sizeof(T) == 4 ? halves(a.unscale[0]) : make_float2(1.f, 1.f);
     const Deal full_deal = deal_of(count, a.full_k * kBlockK / kTileM, a.tiles_d, a.full_k, a.want_dw, a.slabs,
                                    (int)(gridDim.x >> 1));
     if (MODE == kProducts && a.slabs) {  // the last piece may be shorter than the others, and deal dx differently
@@ -643,6 +652,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float b = -INFINITY;
         if (v < a.vocab) b = a.bias ? op_load<T>(static_cast<const T *>(a.bias)[v]) : 0.f;
         sbias[acc * kTileN + etid] = b;
+        if (sizeof(T) == 4) sfac[acc * kTileN + etid] = v < a.vocab ? (uint8_t)(__float_as_uint(a.winv[v]) >> 23) : 127;
         // (and whether a bias of -Inf or the vocabulary's end takes some columns out)
         asm volatile(
             "{\n\t.reg .pred p, q;\n\t"
@@ -653,12 +663,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             : "r"((uint32_t)(b == -INFINITY)), "n"(32 * kEpiWarps)
             : "memory");
         if (u.m != last_m) {
+          const int row = u.m * kTileM + (int)rank * 128 + q * 32 + lane;
+          if (sizeof(T) == 4) fx = halves(row < count ? a.xinv[row] : 1.f);
           if (MODE == kStats) {
             flush();
             run_m = -INFINITY;
             run_s = 0.f;
           } else {
-            const int row = u.m * kTileM + (int)rank * 128 + q * 32 + lane;
             lse = row < count ? a.lse[row] : 0.f;
             tgt = row < count ? a.tgt[row] : -1;
           }
@@ -690,6 +701,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // Which of 32 columns are taken out, whatever their logits are: an overflow to +Inf would
       // make them NaN.
       auto masked = [&](int c) { return __ballot_sync(0xffffffffu, sb[half * hcols + c + lane] == -INFINITY); };
+      // float32: z of columns c.. c + 3 (of this warp's, c a multiple of 4) from their accumulators
+      auto unscale4 = [&](float *v, int c) {
+        const uint32_t e = reinterpret_cast<const uint32_t *>(sfac + acc * kTileN + half * hcols)[c >> 2];
+        const float2 f[2] = {make_float2(__uint_as_float(e << 23 & 0x7f800000u), __uint_as_float(e << 15 & 0x7f800000u)),
+                             make_float2(__uint_as_float(e << 7 & 0x7f800000u), __uint_as_float(e >> 1 & 0x7f800000u))};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float2 z = __fmul2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(fx.x, fx.x));
+          z = __fmul2_rn(__fmul2_rn(z, f[i]), make_float2(fx.y, fx.y));
+          v[2 * i] = z.x;
+          v[2 * i + 1] = z.y;
+        }
+      };
       if (MODE == kStats) {
         auto walk = [&](auto some) {  // some: columns may be taken out
 #pragma unroll 1
@@ -701,10 +725,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const float4 b = b4[k];
-              if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[4 * k + i] = v[4 * k + i] * f_lo * f_hi;
-              }
+              if constexpr (sizeof(T) == 4) unscale4(v + 4 * k, c + 4 * k);
               z[2 * k] = __fadd2_rn(make_float2(v[4 * k], v[4 * k + 1]), make_float2(b.x, b.y));
               z[2 * k + 1] = __fadd2_rn(make_float2(v[4 * k + 2], v[4 * k + 3]), make_float2(b.z, b.w));
             }
@@ -743,10 +764,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const float4 b = b4[k];
-              if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[h][4 * k + i] = v[h][4 * k + i] * f_lo * f_hi;
-              }
+              if constexpr (sizeof(T) == 4) unscale4(v[h] + 4 * k, c + 32 * h + 4 * k);
               const float2 p = exp_diff(__fadd2_rn(make_float2(v[h][4 * k], v[h][4 * k + 1]), make_float2(b.x, b.y)), nlse);
               const float2 q = exp_diff(__fadd2_rn(make_float2(v[h][4 * k + 2], v[h][4 * k + 3]), make_float2(b.z, b.w)), nlse);
               v[h][4 * k] = p.x; v[h][4 * k + 1] = p.y;
@@ -852,7 +870,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int k = 0; k < 32; ++k) {
-                if constexpr (sizeof(T) == 4) v[h][k] = v[h][k] * fx1 * scale * fx2;
+                if constexpr (sizeof(T) == 4) v[h][k] = v[h][k] * fx.x * scale * fx.y;
                 else v[h][k] *= scale;
               }
             if constexpr (sizeof(T) == 2) {
@@ -948,66 +966,6 @@ __device__ __forceinline__ void put_row(uint16_t *dst, size_t plane, const T *sr
   put_row<T, 16 / sizeof(T)>(dst, plane, src, dim, lane, scale);
 }
 
-struct StageArgs {
-  const void *x, *w;
-  long x_ld, w_ld, rows;
-  const int32_t *tg;
-  int vocab, dim, pitch, per_cta, x_ctas;  // per_cta: rows per CTA, a multiple of 8
-  int x_vec, w_vec;                        // elements per access (see row_width)
-  size_t xplane, wplane;
-  uint16_t *xc, *wc;                       // wc null: W is read where it is
-  const uint32_t *range;                   // float32: [range_ctas][2] largest magnitudes
-  int range_ctas;
-  float *unscale;
-  int32_t *slot;
-  int *count;
-  unsigned int *ticket;
-  const float *lse;  // gradient only
-  float *lse_c;
-  int32_t *tgt;
-};
-
-// float32: each CTA's largest finite magnitude of the counted rows of x and of W, as bits
-// (which order like the magnitudes).  Bound by HBM: 107 MB at 2048 x 50257 x 512 take
-// 22 us, 4.8 TB/s.
-__global__ void __launch_bounds__(256) ce_range_kernel(const StageArgs a, uint32_t *range) {
-  __shared__ uint32_t sh[2][8];
-  op_begin();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long first = (long)blockIdx.x * 8 + warp, step = (long)gridDim.x * 8;
-  uint32_t top[2] = {0, 0};
-  auto take = [&](float f, uint32_t &t) {
-    const uint32_t u = __float_as_uint(f) & 0x7fffffffu;
-    if (u < 0x7f800000u && u > t) t = u;
-  };
-  auto row = [&](const float *p, bool vec, uint32_t &t) {
-    if (vec) {
-#pragma unroll 4
-      for (int c = lane * 4; c < a.dim; c += 128) {
-        const float4 f = *reinterpret_cast<const float4 *>(p + c);
-        take(f.x, t); take(f.y, t); take(f.z, t); take(f.w, t);
-      }
-    } else {
-#pragma unroll 4
-      for (int c = lane; c < a.dim; c += 32) take(p[c], t);
-    }
-  };
-  for (long n = first; n < a.rows; n += step)
-    if (counted(a.tg[n], a.vocab)) row(static_cast<const float *>(a.x) + n * a.x_ld, a.x_vec == 4, top[0]);
-  for (long v = first; v < a.vocab; v += step) row(static_cast<const float *>(a.w) + v * a.w_ld, a.w_vec == 4, top[1]);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    top[i] = __reduce_max_sync(0xffffffffu, top[i]);
-    if (lane == 0) sh[i][warp] = top[i];
-  }
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    uint32_t t = 0;
-    for (int w = 0; w < 8; ++w) t = max(t, sh[threadIdx.x][w]);
-    range[blockIdx.x * 2 + threadIdx.x] = t;
-  }
-}
-
 // The power of two that brings a largest magnitude to 2^14..2^15 (as far as float32
 // goes), and its inverse.
 __device__ __forceinline__ void range_scale(uint32_t top, float &scale, float &inverse) {
@@ -1017,47 +975,108 @@ __device__ __forceinline__ void range_scale(uint32_t top, float &scale, float &i
   inverse = __uint_as_float((uint32_t)(127 - k) << 23);
 }
 
+// A float32 row with infinities, for the logits: they become +-2^14 and everything finite 0,
+// and the row's factor is infinite, so that z is infinite (or NaN, where the other side is 0).
+__device__ __forceinline__ void put_infinite_row(uint16_t *dst, size_t plane, const float *src, int dim, int lane) {
+  for (int c = lane; c < dim; c += 32) {
+    const float v = src[c];
+    put_pieces<float>(dst + c, plane, fabsf(v) == INFINITY ? copysignf(16384.f, v) : 0.f, 1.f);
+  }
+}
+
+struct StageArgs {
+  const void *x, *w, *bias;
+  long x_ld, w_ld, rows;
+  const int32_t *tg;
+  int vocab, dim, pitch, per_cta, x_ctas;  // per_cta: rows per CTA, a multiple of 8
+  int x_vec, w_vec;                        // elements per access (see row_width)
+  size_t xplane, wplane;
+  uint16_t *xc, *wc;                       // wc null: W is read where it is
+  float *xinv, *winv;                      // float32: what the rows were divided by
+  uint32_t *range;                         // float32, gradient: [range_ctas][2] largest magnitudes
+  int range_ctas;
+  uint16_t *xt, *wt;                       // and the layouts for the products with G, or null
+  float *unscale;                          // and what those were divided by
+  int32_t *slot;
+  int *count;
+  unsigned int *ticket;
+  const float *lse;  // gradient only
+  float *lse_c;
+  int32_t *tgt;
+};
+
+// Largest finite magnitude of a float32 row, as bits (which order like the magnitudes), by one
+// warp; `infinite`: it holds an infinity.
+__device__ __forceinline__ uint32_t row_top(const float *p, int dim, int lane, bool vec, bool &infinite) {
+  uint32_t top = 0, any = 0;
+  auto take = [&](float f) {
+    const uint32_t u = __float_as_uint(f) & 0x7fffffffu;
+    any = max(any, u);
+    if (u < 0x7f800000u) top = max(top, u);
+  };
+  if (vec) {
+#pragma unroll 4
+    for (int c = lane * 4; c < dim; c += 128) {
+      const float4 f = *reinterpret_cast<const float4 *>(p + c);
+      take(f.x); take(f.y); take(f.z); take(f.w);
+    }
+  } else {
+#pragma unroll 4
+    for (int c = lane; c < dim; c += 32) take(p[c]);
+  }
+  infinite = __reduce_max_sync(0xffffffffu, any) == 0x7f800000u;
+  return __reduce_max_sync(0xffffffffu, top);
+}
+// Lays a float32 row out for the logits, scaled by its own largest magnitude (its second
+// pass finds the row in L1), and returns that magnitude.
+__device__ __forceinline__ uint32_t stage_row(uint16_t *dst, size_t plane, const float *src, int dim, int lane, int vec, float *inverse) {
+  bool infinite;
+  const uint32_t top = row_top(src, dim, lane, vec == 4, infinite);
+  float scale, inv;
+  range_scale(top, scale, inv);
+  if (infinite) put_infinite_row(dst, plane, src, dim, lane);
+  else put_row<float>(dst, plane, src, dim, lane, scale, vec);
+  if (lane == 0) *inverse = infinite ? INFINITY : inv;
+  return top;
+}
+
 // The first CTAs find the counted rows' places (each counts the targets itself: they are
 // few bytes, and a scan would be one launch more), gather x there, with lse also lse and
 // targets, and zero the rows behind the last up to a whole tile (one at least).  The
-// others lay W out, one warp per row (float32, 50257 x 512: 39 us, 206 MB in and out at
-// 5.4 TB/s; 16-bit rows that TMA reads in place need no copy of W, and 8192 rows of x take 9 us).
+// others lay W out, one warp per row (16-bit rows that TMA reads in place need no copy of W,
+// and 8192 rows of x take 9 us).  Each CTA leaves the largest magnitudes that it met for
+// ce_second_kernel: of x, and of W but for rows that a bias of -Inf masks and that are nobody's
+// target, since G is 0 there.
 template <typename T>
 __global__ void __launch_bounds__(256) ce_stage_kernel(const StageArgs a) {
   __shared__ int sh[2][8];
   __shared__ uint32_t tops[2][8];
   op_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float xscale = 1.f, wscale = 1.f;
-  if constexpr (sizeof(T) == 4) {
-    uint32_t top[2] = {0, 0};
-    for (int i = threadIdx.x; i < a.range_ctas; i += 256) {
-      top[0] = max(top[0], a.range[2 * i]);
-      top[1] = max(top[1], a.range[2 * i + 1]);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[i] = __reduce_max_sync(0xffffffffu, top[i]);
-      if (lane == 0) tops[i][warp] = top[i];
-    }
+  uint32_t top[2] = {0, 0};
+  auto leave_tops = [&]() {
+    if (sizeof(T) == 2 || !a.range) return;
+    if (lane < 2) tops[lane][warp] = lane ? top[1] : top[0];
     __syncthreads();
-    top[0] = top[1] = 0;
-    for (int k = 0; k < 8; ++k) {
-      top[0] = max(top[0], tops[0][k]);
-      top[1] = max(top[1], tops[1][k]);
+    if (threadIdx.x < 2) {
+      uint32_t t = 0;
+      for (int k = 0; k < 8; ++k) t = max(t, tops[threadIdx.x][k]);
+      a.range[blockIdx.x * 2 + threadIdx.x] = t;
     }
-    float ix, iw;
-    range_scale(top[0], xscale, ix);
-    range_scale(top[1], wscale, iw);
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-      a.unscale[0] = ix;
-      a.unscale[1] = iw;
-    }
-  }
+  };
   if (blockIdx.x >= a.x_ctas) {
     const long v = (long)(blockIdx.x - a.x_ctas) * 8 + warp;
-    if (v < a.vocab)
-      put_row<T>(a.wc + (size_t)v * a.pitch, a.wplane, static_cast<const T *>(a.w) + v * a.w_ld, a.dim, lane, wscale, a.w_vec);
+    if (v < a.vocab) {
+      const T *w = static_cast<const T *>(a.w) + v * a.w_ld;
+      uint16_t *wc = a.wc + (size_t)v * a.pitch;
+      if constexpr (sizeof(T) == 4) {
+        const uint32_t t = stage_row(wc, a.wplane, w, a.dim, lane, a.w_vec, a.winv + v);
+        if (!a.bias || static_cast<const float *>(a.bias)[v] != -INFINITY) top[1] = t;
+      } else {
+        put_row<T>(wc, a.wplane, w, a.dim, lane, 1.f, a.w_vec);
+      }
+    }
+    leave_tops();
     return;
   }
   const long r0 = (long)blockIdx.x * a.per_cta;
@@ -1099,13 +1118,77 @@ __global__ void __launch_bounds__(256) ce_stage_kernel(const StageArgs a) {
       }
     }
     const int to = __shfl_sync(0xffffffffu, at, warp);
-    if (mask >> warp & 1)
-      put_row<T>(a.xc + (size_t)to * a.pitch, a.xplane, x + (g0 + warp) * a.x_ld, a.dim, lane, xscale, a.x_vec);
+    if (mask >> warp & 1) {
+      const T *src = x + (g0 + warp) * a.x_ld;
+      uint16_t *xc = a.xc + (size_t)to * a.pitch;
+      if constexpr (sizeof(T) == 4) {
+        top[0] = max(top[0], stage_row(xc, a.xplane, src, a.dim, lane, a.x_vec, a.xinv + to));
+        const int32_t target = a.tg[g0 + warp];
+        if (a.bias && static_cast<const float *>(a.bias)[target] == -INFINITY) {
+          bool infinite;
+          top[1] = max(top[1], row_top(static_cast<const float *>(a.w) + target * a.w_ld, a.dim, lane, a.w_vec == 4, infinite));
+        }
+      } else {
+        put_row<T>(xc, a.xplane, src, a.dim, lane, 1.f, a.x_vec);
+      }
+    }
     before += __popc(mask);
   }
   const long end = (long)row_tiles(total) * kTileM;
   for (long j = total + (long)blockIdx.x * 8 + warp; j < end; j += (long)a.x_ctas * 8)
     put_row<T, 1>(a.xc + (size_t)j * a.pitch, a.xplane, static_cast<const T *>(nullptr), a.dim, lane, 1.f);
+  leave_tops();
+}
+
+// float32, gradient: x and W once more, each divided by one number, for the products with G.
+__global__ void __launch_bounds__(256) ce_second_kernel(const StageArgs a) {
+  __shared__ uint32_t tops[2][8];
+  op_begin();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t top[2] = {0, 0};
+#pragma unroll 8
+  for (int i = threadIdx.x; i < a.range_ctas; i += 256) {
+    const uint2 t = reinterpret_cast<const uint2 *>(a.range)[i];
+    top[0] = max(top[0], t.x);
+    top[1] = max(top[1], t.y);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    top[i] = __reduce_max_sync(0xffffffffu, top[i]);
+    if (lane == 0) tops[i][warp] = top[i];
+  }
+  __syncthreads();
+  for (int k = 0; k < 8; ++k) {
+    top[0] = max(top[0], tops[0][k]);
+    top[1] = max(top[1], tops[1][k]);
+  }
+  float xscale, wscale, ix, iw;
+  range_scale(top[0], xscale, ix);
+  range_scale(top[1], wscale, iw);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.unscale[0] = ix;
+    a.unscale[1] = iw;
+  }
+  const long first = (long)blockIdx.x * 8 + warp, step = (long)gridDim.x * 8;
+  if (a.xt) {
+    for (long n = first; n < a.rows; n += step) {
+      const int at = a.slot[n];
+      if (at >= 0)
+        put_row<float>(a.xt + (size_t)at * a.pitch, a.xplane, static_cast<const float *>(a.x) + n * a.x_ld, a.dim, lane, xscale, a.x_vec);
+    }
+    const int total = *a.count;
+    const long end = (long)row_tiles(total) * kTileM;
+    for (long j = total + first; j < end; j += step)
+      put_row<float, 1>(a.xt + (size_t)j * a.pitch, a.xplane, nullptr, a.dim, lane, 1.f);
+  }
+  if (a.wt) {
+    for (long v = first; v < a.vocab; v += step) {
+      const float inv = a.winv[v];
+      // a row above the range is masked and nobody's target
+      put_row<float>(a.wt + (size_t)v * a.pitch, a.wplane, static_cast<const float *>(a.w) + v * a.w_ld, a.dim, lane,
+                     inv > iw && inv != INFINITY ? 0.f : wscale, a.w_vec);
+    }
+  }
 }
 
 // A bias of -Inf takes an entry out whatever its product is.
@@ -1357,7 +1440,7 @@ __global__ void __launch_bounds__(256) ce_dx_kernel(const float *slab, size_t sl
   if (n >= rows) return;
   const int at = slot[n];
   const float c = grad_scale(a.dloss, a.count, a.mean) / a.g_scale;
-  const float fw1 = sizeof(T) == 4 ? half_power(a.unscale[1]) : 1.f, fw2 = sizeof(T) == 4 ? a.unscale[1] / fw1 : 1.f;
+  const float2 fw = sizeof(T) == 4 ? halves(a.unscale[1]) : make_float2(1.f, 1.f);
   for (int i = ((warp % per_row) * 32 + lane) * 4; i < a.dim; i += per_row * 128) {
     float s[4] = {};
     if (at >= 0) {
@@ -1376,7 +1459,7 @@ __global__ void __launch_bounds__(256) ce_dx_kernel(const float *slab, size_t sl
       }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = at >= 0 ? s[e] * fw1 * c * fw2 : 0.f;  // 0 whatever dloss is
+    for (int e = 0; e < 4; ++e) s[e] = at >= 0 ? s[e] * fw.x * c * fw.y : 0.f;  // 0 whatever dloss is
     T *o = dx + n * dx_ld + i;
     if (vec == 4) {
       op_store_vec<T, 4>(o, s);
@@ -1412,6 +1495,8 @@ bool few_rows(const aideen_linear_ce_args *a) {
 int few_width(uint32_t rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8; }
 int few_ctas(uint32_t rows, int sms) { return (few_width(rows) <= 2 ? 2 : 1) * sms; }
 
+constexpr int kStageCtas = 8;  // CTAs per pair of SMs that gather x, at most
+
 // Everything a call lays out.  The row count on the device is only known there,
 // so sizes follow from all rows.
 struct Plan {
@@ -1423,10 +1508,9 @@ struct Plan {
   int32_t *slot;
   int *count;
   unsigned int *ticket;
-  float *unscale;
+  float *unscale, *xinv, *winv;
   uint32_t *range;
-  int range_ctas;
-  uint16_t *xc, *wc;
+  uint16_t *xc, *wc, *xt, *wt;
   float2 *stats;
   float *row_loss;
   // gradient
@@ -1504,9 +1588,10 @@ Plan make_plan(const aideen_linear_ce_args *a, void *ws, bool grad) {
   p.slot = c.take<int32_t>(a->rows);
   p.count = c.take<int>(1);
   p.ticket = c.take<unsigned int>(1);
-  p.unscale = c.take<float>(2);
-  p.range_ctas = p.planes == 2 ? 4 * op_sm_count() : 0;
-  p.range = c.take<uint32_t>((size_t)2 * p.range_ctas);
+  if (p.planes == 2) {
+    p.xinv = c.take<float>(a->rows);
+    p.winv = c.take<float>(a->vocab);
+  }
   p.xc = c.take<uint16_t>(p.xplane * p.planes);
   p.wc = c.take<uint16_t>(p.w_direct ? 0 : p.wplane * p.planes);
   OpCarve g = c;
@@ -1521,6 +1606,14 @@ Plan make_plan(const aideen_linear_ce_args *a, void *ws, bool grad) {
     p.bn = q.bn; p.tiles_d = q.tiles_d; p.slabs = q.slabs; p.piece = q.piece;
   }
   p.dpitch = (long)op_round(a->dim, 4);
+  p.xt = p.xc;
+  p.wt = p.wc;
+  if (p.planes == 2) {
+    p.unscale = g.take<float>(2);
+    p.range = g.take<uint32_t>(2 * ((size_t)kStageCtas * p.pairs + (a->vocab + 7) / 8));
+    p.xt = g.take<uint16_t>(p.xplane * p.planes);
+    p.wt = g.take<uint16_t>(p.wplane * p.planes);
+  }
   p.lse_c = g.take<float>(a->rows);
   p.tgt = g.take<int32_t>(a->rows);
   p.G = g.take<uint16_t>((size_t)p.mpad * p.piece * p.planes);
@@ -1547,14 +1640,14 @@ bool make_map(CUtensorMap *m, CUtensorMapDataType type, const void *base, size_t
 constexpr auto kU16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
 constexpr auto kF32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
 
-// x and W as operands, in boxes of 64 columns by `rows` rows.
-bool map_x(CUtensorMap *m, const Plan &p, int dim, uint32_t rows) {
-  return make_map(m, kU16, p.xc, dim, p.mpad, p.planes, (size_t)p.pitch * 2, p.xplane * 2, 64, rows);
+// x and W as operands (one of their layouts), in boxes of 64 columns by `rows` rows.
+bool map_x(CUtensorMap *m, const Plan &p, const uint16_t *x, int dim, uint32_t rows) {
+  return make_map(m, kU16, x, dim, p.mpad, p.planes, (size_t)p.pitch * 2, p.xplane * 2, 64, rows);
 }
-bool map_w(CUtensorMap *m, const Plan &p, const aideen_linear_ce_args *g, const void *w, uint32_t rows) {
+bool map_w(CUtensorMap *m, const Plan &p, const uint16_t *laid_out, const aideen_linear_ce_args *g, const void *w, uint32_t rows) {
   if (p.w_direct)
     return make_map(m, kU16, w, g->dim, g->vocab, 1, (size_t)g->w_ld * 2, (size_t)g->w_ld * 2, 64, rows);
-  return make_map(m, kU16, p.wc, g->dim, g->vocab, p.planes, (size_t)p.pitch * 2, p.wplane * 2, 64, rows);
+  return make_map(m, kU16, laid_out, g->dim, g->vocab, p.planes, (size_t)p.pitch * 2, p.wplane * 2, 64, rows);
 }
 
 // Elements that rows of this base and stride can be moved by: 16 bytes, a pair of 16-bit
@@ -1569,9 +1662,10 @@ cudaError_t launch_as(const Plan &p, const Maps &maps, MmaArgs a, cudaStream_t s
   const int held = HELD ? (a.dim + kBlockK - 1) / kBlockK : 0;
   const int boxes = kEpiWarps * (MODE == kStats ? 0 : HELD ? 1 : 2) * kBoxBytes;
   const int stage = HELD ? kHalfBytes : 2 * kHalfBytes;
-  a.stages = (kSmemLimit - kSmemFixed - boxes - held * kHalfBytes) / stage;
+  constexpr int fixed = smem_fixed(MODE, sizeof(T));
+  a.stages = (kSmemLimit - fixed - boxes - held * kHalfBytes) / stage;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
-  const int smem = held * kHalfBytes + a.stages * stage + boxes + kSmemFixed;
+  const int smem = held * kHalfBytes + a.stages * stage + boxes + fixed;
   auto kernel = ce_mma_kernel<MODE, T, HELD>;
   // the attribute belongs to the kernel, not to the call: always the same value, or a call
   // of another thread could lower it between here and the launch
@@ -1588,22 +1682,28 @@ cudaError_t launch_mma(const Plan &p, const Maps &maps, const MmaArgs &a, cudaSt
 }
 
 template <typename T>
-cudaError_t stage_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, const T *w, const int32_t *tg,
-                      const float *lse, cudaStream_t st) {
+cudaError_t stage_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, const T *w, const T *bias,
+                      const int32_t *tg, const float *lse, bool want_dx, bool want_dw, cudaStream_t st) {
   StageArgs s{};
   s.x = x; s.w = w; s.x_ld = g->x_ld; s.w_ld = g->w_ld; s.rows = g->rows; s.tg = tg; s.vocab = (int)g->vocab;
   s.dim = (int)g->dim; s.pitch = p.pitch; s.xplane = p.xplane; s.wplane = p.wplane; s.xc = p.xc; s.wc = p.wc;
   s.slot = p.slot; s.count = p.count; s.ticket = p.ticket; s.lse = lse; s.lse_c = p.lse_c; s.tgt = p.tgt;
-  s.range = p.range; s.range_ctas = p.range_ctas; s.unscale = p.unscale;
+  s.bias = bias; s.xinv = p.xinv; s.winv = p.winv;
   s.x_vec = row_width(g->dim, x, g->x_ld, sizeof(T));
   s.w_vec = row_width(g->dim, w, g->w_ld, sizeof(T));
-  const long most = 4L * 2 * p.pairs;  // CTAs
+  const long most = (long)kStageCtas * p.pairs;
   s.per_cta = (int)(8 * ((g->rows + 8 * most - 1) / (8 * most)));
   s.x_ctas = (int)((g->rows + s.per_cta - 1) / s.per_cta);
   const unsigned w_ctas = p.w_direct ? 0 : (g->vocab + 7) / 8;
-  cudaError_t e = cudaSuccess;
-  if constexpr (sizeof(T) == 4) e = op_launch(ce_range_kernel, p.range_ctas, 256, 0, st, s, p.range);
-  if (e == cudaSuccess) e = op_launch(ce_stage_kernel<T>, s.x_ctas + w_ctas, 256, 0, st, s);
+  if constexpr (sizeof(T) == 4) {
+    if (want_dx || want_dw) {
+      s.range = p.range; s.range_ctas = (int)(s.x_ctas + w_ctas); s.unscale = p.unscale;
+      s.xt = want_dw ? p.xt : nullptr;
+      s.wt = want_dx ? p.wt : nullptr;
+    }
+  }
+  cudaError_t e = op_launch(ce_stage_kernel<T>, s.x_ctas + w_ctas, 256, 0, st, s);
+  if (e == cudaSuccess && s.range) e = op_launch(ce_second_kernel, 12 * p.pairs, 256, 0, st, s);
   return e;
 }
 
@@ -1616,7 +1716,7 @@ MmaArgs mma_args(const aideen_linear_ce_args *g, const Plan &p, const T *bias) {
   a.idesc = (1u << 4) | (type << 7) | (type << 10);
   a.bias = bias;
   a.g_scale = g->dtype == AIDEEN_F16 ? kHalfScale : g->dtype == AIDEEN_F32 ? kPieceScale : 1.f;
-  a.unscale = p.unscale;
+  a.xinv = p.xinv; a.winv = p.winv; a.unscale = p.unscale;
   a.mean = g->reduction == AIDEEN_CE_MEAN;
   return a;
 }
@@ -1645,10 +1745,10 @@ cudaError_t loss_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
     const size_t smem = op_round(g->dim, V) * sizeof(float);
     return vec ? few_run<T, V>(f, smem, 2 * p.pairs, st) : few_run<T, 1>(f, smem, 2 * p.pairs, st);
   }
-  cudaError_t e = stage_run<T>(g, p, x, w, tg, nullptr, st);
+  cudaError_t e = stage_run<T>(g, p, x, w, bias, tg, nullptr, false, false, st);
   if (e != cudaSuccess) return e;
   Maps maps{};
-  if (!map_x(&maps.a, p, (int)g->dim, 128) || !map_w(&maps.b, p, g, w, 128)) return cudaErrorInvalidValue;
+  if (!map_x(&maps.a, p, p.xc, (int)g->dim, 128) || !map_w(&maps.b, p, p.wc, g, w, 128)) return cudaErrorInvalidValue;
   MmaArgs a = mma_args<T>(g, p, bias);
   a.tiles_n = p.tiles_n;
   a.stats = p.stats;
@@ -1670,17 +1770,17 @@ cudaError_t loss_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, 
 template <typename T>
 cudaError_t grad_run(const aideen_linear_ce_args *g, const Plan &p, const T *x, const T *w, const T *bias,
                      const int32_t *tg, const float *lse, const float *dloss, T *dx, T *dw, T *db, cudaStream_t st) {
-  cudaError_t e = stage_run<T>(g, p, x, w, tg, lse, st);
+  cudaError_t e = stage_run<T>(g, p, x, w, bias, tg, lse, dx, dw, st);
   if (e != cudaSuccess) return e;
   const int dim = (int)g->dim;
   const size_t gplane = (size_t)p.mpad * p.piece;
   Maps lm{}, pm{};
-  bool ok = map_x(&lm.a, p, dim, 128) && map_w(&lm.b, p, g, w, 128) &&
+  bool ok = map_x(&lm.a, p, p.xc, dim, 128) && map_w(&lm.b, p, p.wc, g, w, 128) &&
             make_map(&lm.c, kU16, p.G, p.piece, p.mpad, p.planes, (size_t)p.piece * 2, gplane * 2, 64, 32);
   ok = ok && make_map(&pm.a, kU16, p.G, p.piece, p.mpad, p.planes, (size_t)p.piece * 2, gplane * 2, 64, 128) &&
-       map_w(&pm.b, p, g, w, 64) &&
+       map_w(&pm.b, p, p.wt, g, w, 64) &&
        make_map(&pm.a2, kU16, p.G, p.piece, p.mpad, p.planes, (size_t)p.piece * 2, gplane * 2, 64, 64) &&
-       map_x(&pm.b2, p, dim, 64) &&
+       map_x(&pm.b2, p, p.xt, dim, 64) &&
        make_map(&pm.c, kF32, p.slab, dim, p.mpad, p.slabs, p.dpitch * 4, p.mpad * p.dpitch * 4, 32, 32);
   const size_t el = sizeof(T);
   const int dw_vec = !dw ? 1 : op_vec16(dw, g->dw_ld, el) ? (int)(16 / el) : row_width(g->dim, dw, g->dw_ld, el);

@@ -438,11 +438,15 @@ int aideen_linear_ce(const aideen_linear_ce_args *args, const void *x, const voi
  * is rounded to dtype before its two products (its relative error there is that
  * of one rounding; in float16 it is scaled by 2^12 first, so probabilities below
  * 2^-26 lose digits); dbias sums it unrounded; dx, dW and dbias are rounded once
- * when stored.  In
- * float32 (in the loss too, but for a few rows) x, W and softmax - onehot enter their
- * products as two scaled float16 pieces each: 22 bits of a value, and what lies
- * below 2^-39 of a tensor's largest magnitude is rounded off.  An infinite x or W
- * makes its logits NaN there. */
+ * when stored.  In float32 (in the loss too, but for a few rows) x, W and
+ * softmax - onehot enter their products as two scaled float16 pieces each: 22 bits
+ * of a value.  In the logits every row of x and of W has its own scale, and what
+ * lies below 2^-39 of its row's largest magnitude is rounded off; in the two
+ * products with softmax - onehot, what lies below 2^-39 of the tensor's (of W
+ * without the rows that a bias of -Inf masks, unless they are targets).  An
+ * infinite x or W makes its logits infinite in the loss and NaN in dx or dW.
+ * An entry whose bias is -Inf has probability 0, also where its logit without the
+ * bias would overflow. */
 int aideen_linear_ce_grad(const aideen_linear_ce_args *args, const void *x, const void *w, const void *bias,
                           const int32_t *targets, const float *lse, const float *dloss, void *dx, void *dw,
                           void *dbias, void *workspace, size_t workspace_bytes, void *stream);

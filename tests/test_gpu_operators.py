@@ -576,6 +576,84 @@ def test_linear_ce_infinite_row_of_w(dtype, rows):
     close(lse, lse2.double(), 2 * U32 * (2 * 72 * zabs + 2 * 300 + 4 * lse2.double().abs() + 16))
 
 
+@pytest.mark.parametrize("rows", [30, 257])
+def test_linear_ce_infinities_in_float32(rows):
+    """As above in float32: an entry at minus infinity has probability 0, one at plus infinity
+    all of it, and an infinite x has infinite logits."""
+    x, w, b, tg = ce_inputs(5, rows, 72, 300, F32, True)
+    x = x.abs() + 0.25
+    tg[tg == 41] = 0
+    keep = [v for v in range(300) if v != 41]
+    ref = ce_reference(x, w[keep], b[keep], torch.where(tg > 41, tg - 1, tg), "mean", 1.0, F32)
+    for where in (7, slice(None)):
+        low = w.clone()
+        low[41, where] = float("-inf")
+        loss, row_loss, lse = K.linear_ce(x, low, tg, b)
+        for got, name in ((loss, "loss"), (row_loss, "rows"), (lse, "lse")):
+            close(got, ref[name][0], ref[name][1])
+        _, dw, db = K.linear_ce_grad(x, low, tg, lse, b, want=("weight", "bias"))
+        assert bool((dw[41] == 0).all()) and float(db[41]) == 0
+        close(dw[keep], ref["dw"][0], ref["dw"][1] + U32 * ref["dw"][0].abs())
+        close(db[keep], ref["db"][0], ref["db"][1] + U32 * ref["db"][0].abs())
+    high = w.clone()
+    high[41] = float("inf")
+    assert not bool(torch.isfinite(K.linear_ce(x, high, tg, b)[1]).any())
+    x[3, 5] = float("inf")
+    w[:, 5] = w[:, 5].abs() + 0.25
+    row_loss = K.linear_ce(x, w, tg, b)[1]
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    bad[3] = True
+    assert torch.equal(~torch.isfinite(row_loss), bad)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [5, 40])
+@pytest.mark.parametrize("power", [20, 33, 100, 126])
+def test_linear_ce_masked_entry_that_dwarfs_the_others(dtype, rows, power):
+    """An entry that a bias of -Inf masks takes no digits from the others, whatever its row of
+    W holds: an unused entry's memory, say."""
+    x, w, b, tg = ce_inputs(rows + power, rows, 512, 600, dtype, True)
+    if dtype == F16:
+        power = 14  # as large as it holds
+    big = (w[100].float() * 2.0 ** power).to(dtype)
+    assert bool(torch.isfinite(big).all())
+    w[100], b[100] = big, -float("inf")
+    tg[tg == 100] = 1
+    keep = [v for v in range(600) if v != 100]
+    ref = ce_reference(x, w[keep], b[keep], torch.where(tg > 100, tg - 1, tg), "mean", 1.0, dtype)
+    loss, row_loss, lse = K.linear_ce(x, w, tg, b)
+    dx, dw, db = K.linear_ce_grad(x, w, tg, lse, b)
+    for got, name in ((loss, "loss"), (row_loss, "rows"), (lse, "lse")):
+        close(got, ref[name][0], ref[name][1])
+    for got, name in ((dx, "dx"), (dw[keep], "dw"), (db[keep], "db")):
+        want, e = ref[name]
+        close(got, want, e + U[dtype] * (want.abs() + e) + TINY[dtype])
+    assert not bool(dw[100].any()) and float(db[100]) == 0
+
+
+@pytest.mark.parametrize("rows", [7, 60, 300])
+def test_linear_ce_in_float32_with_rows_of_any_magnitude(rows):
+    """Rows of x and of W at powers of two apart keep all their digits in the logits: each
+    logit's bound is made of its own row's and entry's products."""
+    x, w, b, tg = ce_inputs(rows, rows, 96, 500, F32, True)
+    g = gen(77)
+    w *= 2.0 ** torch.randint(-40, 3, (500, 1), generator=g, device="cuda").float()
+    w[3] *= 2.0 ** 60
+    x *= 2.0 ** torch.randint(-30, 2, (rows, 1), generator=g, device="cuda").float()
+    x[0], w[4] = 0.0, 0.0
+    x[1] *= 2.0 ** 40
+    loss, row_loss, lse = K.linear_ce(x, w, tg, b)
+    ref = ce_reference(x, w, b, tg, "mean", 1.0, F32)
+    for got, name in ((loss, "loss"), (row_loss, "rows")):
+        close(got, ref[name][0], ref[name][1])
+    # lse: off by the logits' bounds weighted with their probabilities, and by its sum's
+    z = x.double() @ w.double().t() + b.double()
+    ez = 2 * (96 + 16) * U32 * (x.double().abs() @ w.double().abs().t() + b.double().abs()) + 4 * U32 * z.abs()
+    want = torch.logsumexp(z, 1)
+    p = (z - want[:, None]).exp()
+    close(lse, want, 2 * (p * ez.clamp(max=1e30)).sum(1) + 600 * U32 + 4 * U32 * want.abs())
+
+
 def test_linear_ce_of_a_call_that_is_scaled_to_nan():
     """dx of rows that are not counted is 0 whatever dloss is."""
     for dtype in TYPES:
