@@ -192,6 +192,21 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const float (&v)[32]) {
+  uint32_t r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+      "%28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -228,7 +243,7 @@ struct Unit {
   int kb0, nkb;  // 64-deep slices
   int dw;        // kProducts: 1 = dW tile, 0 = dx tile
   int z;         // dx: slab
-  bool first;    // chunk of the tile's depth
+  bool first, last;  // chunks of the tile's depth
 };
 
 // How a piece's two products are dealt out over the pairs.  dW tiles go out whole
@@ -282,7 +297,8 @@ __device__ __forceinline__ Deal deal_of(int count, int tiles_v, int tiles_d, int
 // added to what the ones before stored: the tensor cores cut where they add, by up to a
 // unit of the sum at each 16 deep, always towards zero.  Over the 16384 rows of a dW that
 // grew to 1.9e-5 of it; in chunks it stays at 1e-6 for any number of rows, at 8% of the
-// gradient's time.  (z is cut the same way over its depth: 4e-7 of it at 512.)
+// gradient's time.  z is cut the same way over its depth, by 4e-7 of it at 512 and eight times
+// that at 4096, so deeper logits of float32 are added in chunks too (DEEP below).
 constexpr int kChunk = 8;
 
 // Units of one pair.  kStats and kPiece: a contiguous share of the (row tile,
@@ -320,7 +336,7 @@ struct Units {
   }
   __device__ __forceinline__ bool get(Unit &u) {
     if (!CHUNKS) {
-      u.first = true;
+      u.first = u.last = true;
       return get_tile(u);
     }
     if (depth >= tile.nkb) {
@@ -332,6 +348,7 @@ struct Units {
     u.nkb = min(kChunk, tile.nkb - depth);
     u.first = depth == 0;
     depth += u.nkb;
+    u.last = depth >= tile.nkb;
     return true;
   }
   __device__ __forceinline__ bool get_tile(Unit &u) {
@@ -456,7 +473,12 @@ __device__ __forceinline__ void db_columns(const MmaArgs &a, int count, int etid
 //
 // HELD (kStats, kPiece with one piece per element and dim <= 512): the row tile of x stays in
 // shared memory while the pair walks along the vocabulary, and the ring carries W only.
-template <int MODE, typename T, bool HELD>
+//
+// DEEP (kStats, kPiece in float32 with dim > 512): the chunks of a tile's depth are added in
+// float32.  The first stays in its accumulator, the later ones pass one by one through the
+// other, and the epilogue adds each to the first in tensor memory; the next tile starts in
+// the one that is free first.  It costs 1% of loss and gradients at 2048 x 50257 x 1024 (2.6 ms).
+template <int MODE, typename T, bool HELD, bool DEEP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ce_mma_kernel(const __grid_constant__ Maps maps, const MmaArgs a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -516,8 +538,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int products = a.planes == 1 ? 1 : 3;
   const int bn = MODE == kProducts ? a.bn : kTileN;  // columns of a tile; either CTA loads half
   constexpr bool kChunks = MODE == kProducts && sizeof(T) == 4;
-  Units<MODE, kChunks> units(a, count);
-  Unit u;
+  Units<MODE, kChunks || DEEP> units(a, count);
+  Unit u{};
+  // The accumulator that a unit goes to, and how often that was used before: in turn, or as
+  // DEEP has it.
+  int unit_no = 0, side = 1, used0 = 0, used1 = 0;
+  auto place = [&](int &acc, int &use) {
+    if constexpr (DEEP) {
+      if (u.first) side ^= 1;
+      acc = u.first ? side : side ^ 1;
+      use = acc ? used1++ : used0++;
+    } else {
+      acc = unit_no & 1;
+      use = unit_no >> 1;
+    }
+    ++unit_no;
+  };
 
   if (warp == 0) {
     if (elect_one()) {  // ---------------- loads
@@ -574,15 +610,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {  // ---------------- MMAs
       uint32_t s = 0, turn = 0;
-      int j = 0, gen = -1, last_m = -1;
+      int gen = -1, last_m = -1;
       bool ok = true;
-      for (; ok && units.get(u); ++j) {
-        const int acc = j & 1;
+      while (ok && units.get(u)) {
+        int acc, use;
+        place(acc, use);
         const bool fresh = HELD && u.m != last_m;
         const bool leaving = HELD && (u.n == a.tiles_n - 1 || units.next >= units.end);  // last tile of these rows
         if (fresh) ++gen;
         last_m = u.m;
-        if (j >= 2 && !wait_bounded(&tempty[acc], ((j >> 1) - 1) & 1)) { ok = false; break; }
+        if (use > 0 && !wait_bounded(&tempty[acc], (use - 1) & 1)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         // rows by 64: 128-byte rows, 8-row groups 1024 apart; columns by 64: blocks of 64
         // columns 8192 apart, 8-row groups 1024 apart
@@ -620,7 +657,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16);
     Boxes<kBoxesPerWarp> box{boxes + (warp - 2) * kBoxesPerWarp * kBoxBytes};
     const int etid = tid - 64;
-    int j = 0, last_m = -1;
+    int last_m = -1;
     float run_m = -INFINITY, run_s = 0.f;  // kStats: this row's statistics over the pair's tiles
     float lse = 0.f;
     int32_t tgt = -1;
@@ -641,9 +678,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       a.stats[(slot * 2 + half) * kTileM + rank * 128 + q * 32 + lane] = make_float2(run_m, run_s);
     };
     bool dead = false;  // a wait ran out: keep the barriers below in step, touch nothing
-    for (; units.get(u); ++j) {
-      const int acc = j & 1;
-      const float *sb = sbias + acc * kTileN;
+    while (units.get(u)) {
+      const int turn = unit_no & 1;  // of the buffers of a tile's bias
+      int acc, use;
+      place(acc, use);
+      const float *sb = sbias + turn * kTileN;
       uint32_t some_out = 0;
       if (MODE != kProducts) {
         // this tile's bias (-Inf behind the vocabulary); the buffer's last reader passed
@@ -651,8 +690,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int v = a.v0 + u.n * kTileN + etid;
         float b = -INFINITY;
         if (v < a.vocab) b = a.bias ? op_load<T>(static_cast<const T *>(a.bias)[v]) : 0.f;
-        sbias[acc * kTileN + etid] = b;
-        if (sizeof(T) == 4) sfac[acc * kTileN + etid] = v < a.vocab ? (uint8_t)(__float_as_uint(a.winv[v]) >> 23) : 127;
+        sbias[turn * kTileN + etid] = b;
+        if (sizeof(T) == 4) sfac[turn * kTileN + etid] = v < a.vocab ? (uint8_t)(__float_as_uint(a.winv[v]) >> 23) : 127;
         // (and whether a bias of -Inf or the vocabulary's end takes some columns out)
         asm volatile(
             "{\n\t.reg .pred p, q;\n\t"
@@ -676,7 +715,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           last_m = u.m;
         }
       }
-      if (!dead && (!wait_bounded(&tfull[acc], (j >> 1) & 1) || *(volatile uint32_t *)err)) {
+      if (!dead && (!wait_bounded(&tfull[acc], use & 1) || *(volatile uint32_t *)err)) {
         atomicExch(err, 1u);
         dead = true;
       }
@@ -686,24 +725,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int hcols = bn / 2;  // this warp's columns
-      const uint32_t t0 = lane_addr + (uint32_t)(acc * kTileN + half * hcols);
-      const int row0 = u.m * kTileM + (int)rank * 128 + q * 32;
-      auto release = [&]() {  // the accumulator has been read: hand it back
+      auto release = [&](int which) {  // the accumulator has been read: hand it back
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (elect_one()) remote_arrive(leader_addr(&tempty[acc]));
+        if (elect_one()) remote_arrive(leader_addr(&tempty[which]));
       };
+      if constexpr (DEEP) {
+        if (u.first) continue;  // stays
+        const uint32_t from = lane_addr + (uint32_t)(acc * kTileN + half * hcols);
+        const uint32_t to = lane_addr + (uint32_t)((acc ^ 1) * kTileN + half * hcols);
+#pragma unroll 1
+        for (int c = 0; c < kTileN / 2; c += 32) {
+          float v[32], w[32];
+          tmem_load32(from + c, v);
+          if (c + 32 == kTileN / 2) release(acc);
+          tmem_load32(to + c, w);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += w[i];
+          tmem_store32(to + c, v);
+        }
+        if (!u.last) continue;
+        acc ^= 1;
+      }
+      const uint32_t t0 = lane_addr + (uint32_t)(acc * kTileN + half * hcols);
+      const int row0 = u.m * kTileM + (int)rank * 128 + q * 32;
       // 32 of this warp's columns; `last`: the accumulator is not read again
       auto fetch = [&](int c, float (&v)[32], bool last) {
         tmem_load32(t0 + c, v);
-        if (last) release();
+        if (last) release(acc);
       };
       // Which of 32 columns are taken out, whatever their logits are: an overflow to +Inf would
       // make them NaN.
       auto masked = [&](int c) { return __ballot_sync(0xffffffffu, sb[half * hcols + c + lane] == -INFINITY); };
       // float32: z of columns c.. c + 3 (of this warp's, c a multiple of 4) from their accumulators
       auto unscale4 = [&](float *v, int c) {
-        const uint32_t e = reinterpret_cast<const uint32_t *>(sfac + acc * kTileN + half * hcols)[c >> 2];
+        const uint32_t e = reinterpret_cast<const uint32_t *>(sfac + turn * kTileN + half * hcols)[c >> 2];
         const float2 f[2] = {make_float2(__uint_as_float(e << 23 & 0x7f800000u), __uint_as_float(e << 15 & 0x7f800000u)),
                              make_float2(__uint_as_float(e << 7 & 0x7f800000u), __uint_as_float(e >> 1 & 0x7f800000u))};
 #pragma unroll
@@ -1657,7 +1713,7 @@ int row_width(uint32_t dim, const void *p, int64_t ld, size_t el) {
   return el == 2 && dim % 2 == 0 && ld % 2 == 0 && op_aligned(p, 4) ? 2 : 1;
 }
 
-template <int MODE, typename T, bool HELD>
+template <int MODE, typename T, bool HELD, bool DEEP>
 cudaError_t launch_as(const Plan &p, const Maps &maps, MmaArgs a, cudaStream_t st) {
   const int held = HELD ? (a.dim + kBlockK - 1) / kBlockK : 0;
   const int boxes = kEpiWarps * (MODE == kStats ? 0 : HELD ? 1 : 2) * kBoxBytes;
@@ -1666,7 +1722,7 @@ cudaError_t launch_as(const Plan &p, const Maps &maps, MmaArgs a, cudaStream_t s
   a.stages = (kSmemLimit - fixed - boxes - held * kHalfBytes) / stage;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   const int smem = held * kHalfBytes + a.stages * stage + boxes + fixed;
-  auto kernel = ce_mma_kernel<MODE, T, HELD>;
+  auto kernel = ce_mma_kernel<MODE, T, HELD, DEEP>;
   // the attribute belongs to the kernel, not to the call: always the same value, or a call
   // of another thread could lower it between here and the launch
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
@@ -1676,9 +1732,12 @@ cudaError_t launch_as(const Plan &p, const Maps &maps, MmaArgs a, cudaStream_t s
 template <int MODE, typename T>
 cudaError_t launch_mma(const Plan &p, const Maps &maps, const MmaArgs &a, cudaStream_t st) {
   if constexpr (MODE != kProducts && sizeof(T) == 2) {
-    if (a.dim <= kMaxHeld * kBlockK) return launch_as<MODE, T, true>(p, maps, a, st);
+    if (a.dim <= kMaxHeld * kBlockK) return launch_as<MODE, T, true, false>(p, maps, a, st);
   }
-  return launch_as<MODE, T, false>(p, maps, a, st);
+  if constexpr (MODE != kProducts && sizeof(T) == 4) {
+    if (a.dim > kChunk * kBlockK) return launch_as<MODE, T, false, true>(p, maps, a, st);
+  }
+  return launch_as<MODE, T, false, false>(p, maps, a, st);
 }
 
 template <typename T>

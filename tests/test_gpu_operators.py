@@ -694,6 +694,32 @@ def test_linear_ce_gradients_in_float32_at_the_ends_of_the_range(power, dloss):
     assert torch.equal(dw * far, dw2) and torch.equal(dx / far, dx2)
 
 
+@pytest.mark.parametrize("rows,dim", [(40, 16384), (300, 16390), (513, 4097), (300, 577), (9, 513)])
+def test_linear_ce_of_deep_rows_in_float32(rows, dim):
+    """Logits of positive terms, where every cut of the tensor cores has the same sign: over 512
+    of dim 32 steps of 2 U32 each at most, 12 U32 for 22-bit operands and their two smaller
+    products, and one rounding for each 512 of dim.  No term grows with dim but the last."""
+    g = gen(dim)
+    x = rand(g, rows, dim).abs()
+    w = rand(g, 300, dim, std=157.0 / dim).abs()  # logits about 100
+    tg = torch.randint(0, 300, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    _, row_loss, lse = K.linear_ce(x, w, tg)
+    z = x.double() @ w.double().t()
+    eps = (64 + 12 + dim // 512 + 1) * U32
+    want = torch.logsumexp(z, 1)
+    elz = eps * z.amax(1) + 600 * U32 + 4 * U32 * want
+    close(lse, want, elz)
+    zt = z.gather(1, tg.long()[:, None])[:, 0]
+    close(row_loss, want - zt, elz + (dim // 32 + 16) * U32 * zt)  # the target's logit: a float32 sum by 32 lanes
+    dx, dw, _ = K.linear_ce_grad(x, w, tg, lse)
+    G = (z - lse.double()[:, None]).exp()  # by the lse that it gets
+    eG = G * torch.expm1(eps * z + 2 * U32 * z + 16 * U32) + 2 * U32
+    G[torch.arange(rows, device="cuda"), tg.long()] -= 1
+    G, eG = G / rows, eG / rows
+    for got, p, e, m in ((dx, G, eG, w.double()), (dw, G.t(), eG.t(), x.double())):
+        close(got, p @ m, e @ m + (64 + 12 + 8 + p.shape[1] // 512) * U32 * (p.abs() @ m) + TINY[F32])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_ce_peaked_rows(dtype):
     """Large logits: the softmax is all but one-hot, the loss near zero or large."""
