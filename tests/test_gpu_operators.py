@@ -6,13 +6,14 @@ operation counts: U32 = 2^-24 is half a step of float32, U[t] of the stored
 type, TINY[t] half of the smallest number it can hold, and a float32 sum of k
 terms is off by at most k U32 sum |terms| (2 k U32 where the tensor cores add,
 which may cut instead of round)."""
+import ctypes as C
 import threading
 
 import pytest
 import torch
 
 from aideen_b200 import operators as K
-from aideen_b200.backend import AideenError
+from aideen_b200.backend import AideenError, LinearCeArgs, load_library
 
 pytestmark = pytest.mark.gpu
 
@@ -418,6 +419,36 @@ def test_linear_ce_few_rows(dtype, rows, dim, vocab, pad):
 def test_linear_ce_at_the_training_vocabulary(dtype):
     x, w, b, tg = ce_inputs(3, 200, 512, 50257, dtype, True, 0.1)
     ce_check(x, w, b, tg, reduction="sum", dloss=0.25 if dtype != F16 else 8.0)
+
+
+@pytest.mark.parametrize("dtype,rows,dim,vocab,ignored", [
+    (F32, 2048, 512, 50257, 0.0),    # 3 pieces of 68, 68 and 61 tiles of 256 entries (on 148 SMs)
+    (BF16, 2048, 512, 50257, 0.0),   # 160 + 37
+    (BF16, 5000, 512, 50257, 0.3),   # 3 x 54 + 35
+    (F32, 4500, 136, 50257, 0.1),    # 5 x 37 + 12
+    (F16, 9000, 256, 20011, 0.5),    # 2 x 36 + 7
+    (F32, 4200, 520, 20011, 0.6),    # 2 x 34 + 11
+    (BF16, 5000, 200, 50257, 0.93)])
+def test_linear_ce_gradient_over_several_pieces(dtype, rows, dim, vocab, ignored):
+    """Every piece of the vocabulary adds to dx, the shorter last one too."""
+    x, w, b, tg = ce_inputs(rows + dim, rows, dim, vocab, dtype, True, ignored)
+    size = C.c_size_t()
+    a = LinearCeArgs(TYPES.index(dtype), rows, dim, vocab, 0, dim, dim, dim, dim)
+    assert load_library().aideen_linear_ce_workspace(C.byref(a), None, C.byref(size)) == 0
+    # without x's layouts, W's in float32 and three slabs of dx (there are at least that many)
+    # there is not room for softmax - onehot of all entries at once
+    planes, m = 2 if dtype == F32 else 1, -(-rows // 256) * 256
+    others = 3 * m * dim * 4 + planes * planes * 2 * m * dim + (2 * vocab * dim * 4 if dtype == F32 else 0)
+    assert size.value - others < m * -(-vocab // 256) * 256 * 2 * planes
+    dloss = 1024.0 if dtype == F16 else 1.0
+    _, _, lse, dx, _, _ = ce_check(x, w, b, tg, dloss=dloss)
+    # that bound is tight enough to miss any tenth of the vocabulary
+    want, e = ce_reference(x, w, b, tg, "mean", dloss, dtype)["dx"]
+    keep = ((tg >= 0) & (tg < vocab)).nonzero()[:, 0]
+    for part in torch.arange(vocab, device="cuda").split(-(-vocab // 10)):
+        p = (x[keep].double() @ w[part].double().t() + b[part].double() - lse[keep].double()[:, None]).exp()
+        share = dloss / keep.numel() * (p @ w[part].double())
+        assert bool((share.abs() > 2 * (e[keep] + U[dtype] * (want[keep].abs() + e[keep]) + TINY[dtype])).any())
 
 
 @pytest.mark.parametrize("dtype", TYPES)
