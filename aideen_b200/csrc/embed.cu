@@ -534,7 +534,8 @@ extern "C" int aideen_embed_grad(const aideen_embed_args *args, const int32_t *i
     s.flat = s.row_bytes == s.ld_bytes && op_aligned(table_grad, 16);
     s.clear16 = s.flat || (s.row_bytes % 16 == 0 && op_vec16(table_grad, args->table_ld, el));
     // several CTAs per SM, so that uneven placement of the clusters evens out
-    const size_t ctas = (s.row_bytes / (s.clear16 ? 16 : 2) * s.vocab + kSortThreads - 1) / kSortThreads;
+    const size_t stores = s.flat ? s.row_bytes * s.vocab / 16 + 1 : s.row_bytes / (s.clear16 ? 16 : 2) * s.vocab;
+    const size_t ctas = (stores + kSortThreads - 1) / kSortThreads;
     const size_t most = op_round(4 * (size_t)op_sm_count(), s.ctas), want = op_round(ctas, s.ctas);
     grid += (unsigned)(want < most ? want : most);
   }

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from aideen_b200 import operators as K
-from aideen_b200.backend import AideenError, LinearCeArgs, load_library
+from aideen_b200.backend import AideenError, EmbedArgs, LinearCeArgs, load_library
 
 pytestmark = pytest.mark.gpu
 
@@ -118,6 +118,27 @@ def test_embed_grad(dtype, n, dim, vocab, kind, into):
     close(got, want, sums + U[dtype] * (want.abs() + sums) + TINY[dtype])
     if not into:
         assert torch.equal(got, K.embed_grad(ids, dout, vocab, scale=scale))  # the same bits
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,dim,vocab,pad", [(1, 1, 450, 0), (5, 3, 5851, 0), (2, 7, 33, 0), (40, 5, 20011, 0), (3, 1, 7, 2),
+                                             (0, 3, 100, 0), (0, 6, 9, 2), (2, 12, 4097, 0), (1, 4, 1, 0), (6, 2, 900, 6)])
+def test_embed_grad_writes_every_row(dtype, n, dim, vocab, pad):
+    """Whatever the memory held, also where a row is shorter than 16 bytes."""
+    g = gen(n + dim + vocab)
+    ids = torch.randint(0, vocab, (n,), generator=g, device="cuda", dtype=torch.int32)
+    dout = rand(g, n, dim, dtype=dtype)
+    old = torch.full((vocab, dim + pad), 7.0, dtype=dtype, device="cuda")
+    a, size = EmbedArgs(TYPES.index(dtype), n, dim, vocab, 1.0, 0, dim + pad, dim), C.c_size_t()
+    lib = load_library()
+    assert lib.aideen_embed_grad_workspace(C.byref(a), C.byref(size)) == 0
+    ws = torch.empty(size.value + 256, dtype=torch.uint8, device="cuda")
+    assert lib.aideen_embed_grad(C.byref(a), ids.data_ptr(), dout.data_ptr(), old.data_ptr(), ws.data_ptr(), size.value,
+                                 torch.cuda.current_stream().cuda_stream) == 0
+    want, mag, count = embed_grad_reference(ids, dout, vocab, 1.0)
+    sums = (count[:, None] + 2) * U32 * mag
+    close(old[:, :dim], want, sums + U[dtype] * (want.abs() + sums) + TINY[dtype])
+    assert bool((old[:, dim:] == 7).all())
 
 
 def test_embed_grad_strides_and_shapes():
