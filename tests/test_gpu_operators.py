@@ -929,6 +929,35 @@ def test_streams_and_captured_graphs():
         assert all(torch.equal(p, q) for p, q in zip(outs[k], want[k + 1]))
 
 
+@pytest.mark.parametrize("dim", [72, 640])
+def test_captured_loss_and_gradient_in_float32(dim):
+    """Replayed with inputs of another magnitude and another outlying masked row than at capture
+    (the scales are found anew), the same bits as called."""
+    sets = [ce_inputs(50 + k, 300, dim, 700, F32, True, 0.2) for k in range(3)]
+    for k, (x, w, b, tg) in enumerate(sets):
+        x.mul_(4.0 ** k), w.mul_(0.25 ** k)
+        w[10 * k] *= 1e20
+        b[10 * k] = -float("inf")
+        tg[tg == 10 * k] = 5
+
+    def work(x, w, b, tg):
+        loss, row_loss, lse = K.linear_ce(x, w, tg, bias=b)
+        return (loss, row_loss, lse) + K.linear_ce_grad(x, w, tg, lse, bias=b)
+    want = [work(*s) for s in sets]
+    live = [t.clone() for t in sets[0]]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(*live)
+    for k in (1, 2, 0):
+        for dst, src in zip(live, sets[k]):
+            dst.copy_(src)
+        graph.replay()
+        assert all(torch.equal(p, q) for p, q in zip(got, want[k]))
+        assert bool(torch.isfinite(want[k][0]))
+    K.check()
+
+
 def test_calls_of_several_host_threads():
     """Threads that call at once, each on its own stream and at its own sizes (so with other
     amounts of shared memory), get what they get alone."""
