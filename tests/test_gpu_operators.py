@@ -593,6 +593,23 @@ def test_linear_ce_masked_logits_that_overflow(dtype, rows):
     assert bool(torch.isfinite(lse).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [4, 140])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_linear_ce_masked_entries_that_hold_no_numbers(dtype, rows, value):
+    """A bias of -Inf takes an entry out of the loss, dW and dbias whatever its row of W holds."""
+    x, w, b, tg = ce_inputs(rows, rows, 40, 300, dtype, True)
+    b[[7, 290]] = -float("inf")
+    tg[(tg == 7) | (tg == 290)] = 1
+    loss, row_loss, lse = K.linear_ce(x, w, tg, b)
+    _, dw, db = K.linear_ce_grad(x, w, tg, lse, b, want=("weight", "bias"))
+    w[7], w[290, 3] = value, value
+    for p, q in zip(K.linear_ce(x, w, tg, b), (loss, row_loss, lse)):
+        assert torch.equal(p, q) and bool(torch.isfinite(p).all())
+    got = K.linear_ce_grad(x, w, tg, lse, b, want=("weight", "bias"))
+    assert torch.equal(got[1], dw) and torch.equal(got[2], db) and bool(torch.isfinite(dw).all())
+
+
 def test_linear_ce_nonfinite_rows_spoil_only_themselves():
     x, w, b, tg = ce_inputs(8, 64, 32, 100, F32, True)
     x[5, 3], x[9, 1] = float("nan"), float("inf")
