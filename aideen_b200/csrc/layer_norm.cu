@@ -11,12 +11,15 @@
 // gradient, whose column sums need the registers); longer ones are walked in memory.
 // 32768 x 1024 bf16 forward: 26 us, 5.1 TB/s (a device copy of the same bytes: 22-24 us).
 // 32749 x 1000 f16 gradient with dw and db: 48 us, 4.1 TB/s, where an elementwise sum of
-// the same bytes takes 30 us: the 20 operations per element and the row's reduction
-// stand between the loads, and the column sums take the registers that more rows in
-// flight would need (one row at a time with three CTAs per SM: 55 us).  2048 x 512 f32
-// gradient: 7 us.
-// Rows that do not start on 16 bytes cost 1.5 to 2.2 times as much (32768 x 1001 bf16:
-// 58 us and 104 us; element by element 78 and 190).
+// the same bytes takes 30 us.  Neither issue (42%) nor DRAM (43%) is busy: a row's loads, its
+// reduction and its stores follow each other, and the column sums take the registers that
+// more rows in flight would need (one row at a time with three CTAs per SM: 55 us).  2048 x
+// 512 f32 gradient: 7 us.
+// Rows that do not start on 16 bytes cost 1.5 to 2.2 times as much, 3 to 4.4 times what their
+// bytes need (32768 x 1001 bf16: 58 us and 104 us; element by element 78 and 190): the
+// instructions that cut 16 bytes out of two blocks bound them.
+// Rows longer than the registers hold are walked element by element, one CTA per row: 1000 x
+// 20000 f32 from a cold cache 92 us and 137 us (bytes: 24 and 37 us).
 #include <type_traits>
 
 #include "common.cuh"

@@ -29,14 +29,21 @@
 // its largest magnitude (G: 1) to 2^14..2^15 and written as high + low float16 pieces;
 // high x high + high x low + low x high leave out 2^-22 of a product, three passes where
 // bfloat16 pieces would take six (training shard 50257 x 512, 2048 rows, loss and gradient:
-// 2.23 ms with those, 1.43 ms this way).  For the logits every row of x and of W has its own
+// 2.23 ms with those, 1.45 ms this way).  For the logits every row of x and of W has its own
 // scale, so that a row of W that dwarfs the others costs them nothing: with one scale, a
 // masked row 10^8 times the others put lse off by 1e-3.  The products with G add up over
 // rows, so there x and W have one scale each, in a second layout of the gradient, where what
 // lies below 2^-40 of the largest magnitude is rounded off.
+//
+// 16 bits: G is rounded to the type before the two products, as the tensor cores take it.  The
+// gradients of the large bf16 batch below are then 1.68e-3 from 64 bits in the 2-norm, where
+// rounding the results alone gives 1.66e-3 (f16, 1021 x 4999 x 250: 2.2e-4 and 2.1e-4); a second
+// piece of G would take the products, 525 us of that batch's 1370, twice.  db needs no product and
+// adds up the float32 values.
+//
 // Bound: the tensor cores (2 N V d for the loss, 6 N V d for the gradient, z being
 // formed twice), and behind them the power limit: 8192 rows, nine in ten counted, 50257 x 512
-// bf16, loss and gradient take 1.35 ms, 1.12 PFLOP/s, at clocks that the limit holds at 1.3-1.5 GHz.
+// bf16, loss and gradient take 1.37 ms, 1.10 PFLOP/s, at clocks that the limit holds at 1.3-1.5 GHz.
 //
 // Every wait is bounded; a wait that runs out sets an error word, issues nothing
 // further, lets its copies land, frees the tensor memory and returns.
@@ -467,9 +474,9 @@ __device__ __forceinline__ void db_columns(const MmaArgs &a, int count, int etid
 }
 
 // 8192 x 50257 x 512 bf16, a tenth of the rows not counted, one launch at a time: kStats
-// 231 us (1.64 PFLOP/s), the five kPiece launches 314 us (1.21; G goes out to L2 and HBM
-// meanwhile), the five kProducts 525 us (1.45; G comes back for either product).  2048
-// rows in float32, three products each: 206 us (1.54), 257 us and 532 us.
+// 235 us (1.62 PFLOP/s), the five kPiece launches 318 us (1.19; G goes out to L2 and HBM
+// meanwhile), the five kProducts 529 us (1.43; G comes back for either product).  2048
+// rows in float32, three products each: 211 us (1.50), 257 us and 542 us.
 //
 // HELD (kStats, kPiece with one piece per element and dim <= 512): the row tile of x stays in
 // shared memory while the pair walks along the vocabulary, and the ring carries W only.
@@ -1466,7 +1473,7 @@ __global__ void __launch_bounds__(32 * kFewRows) ce_few_join_kernel(const FewArg
 
 // dx: the slabs added in order, scaled, back to the rows' places.  A CTA takes
 // `per_cta` rows, 8 / per_cta warps each; BATCH slabs are in flight at a time (behind the
-// last, the last again, not added).  8192 x 512 bf16: 23 us.
+// last, the last again, not added).  8192 x 512 bf16: 17 us.
 template <typename T, int BATCH>
 __global__ void __launch_bounds__(256) ce_dx_kernel(const float *slab, size_t slab_stride, int pitch, const MmaArgs a,
                                                     const int32_t *slot, long rows, int per_cta, int vec, T *dx,

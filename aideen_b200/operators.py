@@ -8,7 +8,12 @@ bfloat16 or float16.  Every call goes through `libaideen_b200.so`
 there is no CPU fallback.  Work is queued on torch's current stream of the
 tensors' device, outputs and scratch memory come from torch's allocator, and
 nothing waits, so every call can be captured into a CUDA graph.  Arguments that
-cannot be served raise `AideenError` before anything is launched.
+cannot be served raise `AideenError` before anything is launched.  No call looks
+for a bounded device-side wait that ran out: `check` does, and waits.
+
+The calls are outside autograd: inputs that require gradients are read like any
+others, outputs carry no history, and the backward pass is the caller's chain of
+the `_grad` calls (a `torch.autograd.Function` can wrap a pair of them).
 
 A matrix may have any row stride as long as its last dimension is contiguous
 and its leading dimensions share one stride; 16-byte aligned rows are fastest.
@@ -312,7 +317,12 @@ def _ce_args(what, x, weight, targets, bias, reduction):
 def linear_ce(x, weight, targets, bias=None, reduction: str = "mean"):
     """(loss [1], row_loss, lse) of the cross entropy of `x @ weight.T + bias`
     against int32 targets; the logits are not kept.  Rows whose target lies
-    outside [0, vocab) are not counted (row_loss and lse 0)."""
+    outside [0, vocab) are not counted (row_loss and lse 0).  A bias of -Inf
+    takes an entry out, whatever its row of weight holds.
+
+    In float32, past 8 rows, x and weight enter the products with 22 bits of a
+    value; what lies below 2^-39 of its own row's largest magnitude is rounded
+    off."""
     what = "linear_ce"
     a, weight, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)
     lib, size, r = load_library(), C.c_size_t(), C.byref(a)
@@ -334,7 +344,13 @@ def linear_ce_grad(x, weight, targets, lse, bias=None, dloss=None, reduction: st
     """(dx, dweight, dbias) of `dloss * loss` from `linear_ce`'s lse (same bias
     and reduction); dloss is a float32 tensor of one element or None (1).
     `want` names the gradients to form; the others, and dbias without a bias,
-    are None."""
+    are None.
+
+    In 16 bits, softmax - onehot is rounded to the type before its products with
+    weight and x (not before dbias's sum).  In float32, weight and x have one scale
+    each there: an entry or a row of x 2^17 times all others takes digits from
+    theirs, and what lies below 2^-39 of the largest magnitude is rounded off
+    (entries that a bias of -Inf masks do not count)."""
     what = "linear_ce_grad"
     want = _wanted(want, what)
     a, weight, tp, bp = _ce_args(what, x, weight, targets, bias, reduction)

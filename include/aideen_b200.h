@@ -445,8 +445,14 @@ int aideen_linear_ce(const aideen_linear_ce_args *args, const void *x, const voi
  * products with softmax - onehot, what lies below 2^-39 of the tensor's (of W
  * without the rows that a bias of -Inf masks, unless they are targets).  An
  * infinite x or W makes its logits infinite in the loss and NaN in dx or dW.
- * An entry whose bias is -Inf has probability 0, also where its logit without the
- * bias would overflow. */
+ * An entry whose bias is -Inf has probability 0, whatever its row of W holds (where
+ * that is not finite, dx is NaN).
+ * Logits add up in float32: in the tensor cores, which cut towards zero, over 512 of
+ * dim at most in float32 (off by 4e-7 where all terms have one sign), over all of dim
+ * in 16 bits, and a 16-bit dW over all rows (2e-5 of it at 16384, growing with them;
+ * its own rounding is 5e-4 in float16 and 4e-3 in bfloat16).
+ * Probabilities are exp(z - lse) with lse as stored, so they carry its rounding,
+ * half a unit of float32's last place. */
 int aideen_linear_ce_grad(const aideen_linear_ce_args *args, const void *x, const void *w, const void *bias,
                           const int32_t *targets, const float *lse, const float *dloss, void *dx, void *dw,
                           void *dbias, void *workspace, size_t workspace_bytes, void *stream);
